@@ -10,21 +10,29 @@ from . import _lib
 from ._lib import FagqError, load as load_library, load_probe as load_probe_library
 from .dsa_topk import dsa_topk_page_table_transform
 from .gemm import fp8_block_scaled_gemm, gemm_route
+from .kv_cache import empty_kv_cache, kv_cache_read, kv_cache_write, paged_attention
 from .mla_bwd import mla_bwd_nope_dkdv
 from .ops import (empty_scales, fused_add_rmsnorm_group_quant, fused_add_rmsnorm_group_quant_fn,
                   fused_reduce_add_rmsnorm_group_quant, route_for)
+from .qk_rope import qk_norm_rope, qk_norm_rope_bwd
 
 __all__ = [
     "FagqError",
     "dsa_topk_page_table_transform",
+    "empty_kv_cache",
     "empty_scales",
     "fp8_block_scaled_gemm",
     "fused_add_rmsnorm_group_quant",
     "fused_add_rmsnorm_group_quant_fn",
     "fused_reduce_add_rmsnorm_group_quant",
     "gemm_route",
+    "kv_cache_read",
+    "kv_cache_write",
     "load_library",
     "load_probe_library",
     "mla_bwd_nope_dkdv",
+    "paged_attention",
+    "qk_norm_rope",
+    "qk_norm_rope_bwd",
     "route_for",
 ]

@@ -1,6 +1,6 @@
 """ctypes binding of libfagq.so (the C ABI declared in include/fagq.h,
-include/fagq_gemm.h, include/fagq_dsa.h, include/fagq_mla.h and
-include/fagq_diag.h) and of libfagq_probe.so (include/fagq_probe.h, the
+include/fagq_gemm.h, include/fagq_dsa.h, include/fagq_mla.h,
+include/fagq_rope.h, include/fagq_cache.h and include/fagq_diag.h) and of libfagq_probe.so (include/fagq_probe.h, the
 measurement probes, loaded only when asked for).
 
 The library is loaded after ``import torch`` so that its libamdhip64.so.7
@@ -72,6 +72,7 @@ SIGNATURES = {
     "fagq_version": ([], _I),
     "fagq_diag_encode": ([_P, _P, _I64, _I, _I, _I, _P], _I),
     "fagq_diag_scale_offsets": ([_I64, _I64, _I64, _I, _I, _I, _I64, _P, _I64], _I),
+    "fagq_diag_cache_slots": ([_P, _P, _I64, _I64, _I64, _I64, _P, _I64], _I),
     "fagq_dsa_topk_launch": ([_P, _I, _P, _P, _P, _I, _P, _P] + [_I64] * 6 + [_P], _I),
     "fagq_gemm_launch": ([_P] * 5 + [_I64, _I64, _I64, _I, _I, _I, _P], _I),
     "fagq_gemm_launch_mapped": ([_P] * 5 + [_I64, _I64, _I64, _I, _I, _I, _I, _P], _I),
@@ -80,6 +81,13 @@ SIGNATURES = {
     "fagq_mla_bwd_query_route": ([_I64] * 4 + [_I, _I64, ctypes.POINTER(MlaRoute)], _I),
     "fagq_mla_bwd_launch": ([_P] * 8 + [_I64] * 5 + [_F, _I, _I, _P], _I),
     "fagq_mla_bwd_launch_noalloc": ([_P] * 7 + [_I64] * 4 + [_F, _I, _I, _P], _I),
+    "fagq_qk_norm_rope_launch": ([_P] * 10 + [_I64] * 6 + [_F, _I, _I, _I, _P], _I),
+    "fagq_qk_norm_rope_bwd_workspace_bytes": ([_I64] * 4, _I64),
+    "fagq_qk_norm_rope_bwd_launch": ([_P] * 14 + [_I64, _P] + [_I64] * 6 + [_F, _I, _I, _I, _P], _I),
+    "fagq_kv_cache_write_launch": ([_P] * 8 + [_I64] * 6 + [_I] * 4 + [_P], _I),
+    "fagq_kv_cache_read_launch": ([_P] * 8 + [_I64] * 8 + [_I] * 3 + [_P], _I),
+    "fagq_paged_attention_workspace_bytes": ([_I64] * 7, _I64),
+    "fagq_paged_attention_launch": ([_P] * 10 + [_I64, _P] + [_I64] * 10 + [_F, _I, _I, _I, _I, _P], _I),
 }
 
 

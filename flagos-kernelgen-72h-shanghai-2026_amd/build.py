@@ -22,7 +22,8 @@ INCLUDE = REPO_DIR / "include"
 OBJ_DIR = PKG_DIR / "_build"
 LIB_PATH = PKG_DIR / "libfagq.so"
 PROBE_LIB_PATH = PKG_DIR / "libfagq_probe.so"
-LIB_UNITS = ("fagq_api", "fagq_device", "fagq_gemm", "dsa_topk", "mla_bwd")
+LIB_UNITS = ("fagq_api", "fagq_device", "fagq_gemm", "dsa_topk", "mla_bwd", "qk_rope", "kv_cache",
+             "paged_attn")
 PROBE_UNITS = ("fagq_probe", "fagq_device")
 
 ARCH = "gfx950"

@@ -1,0 +1,611 @@
+// qk_rope.hip - RMS norm of each query and key head with the rotation by position in
+// the same pass, and the gradients (include/fagq_rope.h).
+//
+// y = R(p) (x rstd w), rstd = 1 / sqrt(mean(x^2) + eps).  R(p) is orthogonal, so the
+// gradient of the normed row is dy rotated back, and with a = dn w
+//   dx = rstd (a - x rstd^2 mean(a x)),   dw = sum over rows of dn x rstd.
+// rstd is recomputed from x, which the backward reads anyway.
+//
+// Both directions are bound by HBM: 2 (3) tensors at one read or write each.  A row of D
+// elements belongs to LPR = D / 16 lanes (a power of two, 4 to 32), 16 elements each in two
+// chunks of 8: for pairs (i, i + R / 2) lane l holds elements 8 l.. and R / 2 + 8 l.., for
+// adjacent pairs 16 l.. and 16 l + 8.., so that both halves of every pair are in one lane
+// and every access is 16 bytes.  A wave walks the heads of one token, 64 / LPR at a time
+// (a "pass"), and holds the token's cos and sin and both weights in registers.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "fagq.h"
+#include "fagq_dispatch.hpp"
+#include "fagq_rope.h"
+
+namespace fagq {
+namespace rope {
+namespace {
+
+constexpr int kWaves = 4;             // waves per workgroup
+constexpr int kMaxBwdGroups = 512;    // workgroups of the backward (two per CU), each with its
+                                      // own sums of the weight gradients
+constexpr int kSumRows = 64;          // partial sums that a column's threads share out
+
+struct Args {
+  const void* q;
+  const void* k;
+  const void* qw;
+  const void* kw;
+  const float* cos;
+  const float* sin;
+  const void* pos;
+  void* qo;          // forward: q_out; backward: dq
+  void* ko;
+  const void* dq;    // backward: dq_out, dk_out
+  const void* dk;
+  float* sums;       // backward: [workgroups][2][D]
+  int64_t table_rows;
+  int32_t qs[2], ks[2], qos[2], kos[2], dqs[2], dks[2];   // {token, head} strides, elements
+  int32_t T, Hq, Hk, D, R;
+  int32_t splits;    // waves per token
+  int32_t per_wave;  // passes per wave
+  int32_t idx64;
+  float eps;
+};
+
+template <int E> struct Elem { using type = uint16_t; };
+template <> struct Elem<ET_F32> { using type = float; };
+
+// Eight consecutive elements as fp32, and back (one rounding to nearest even).
+template <int E>
+struct Raw8 {
+  u32x4 v[E == ET_F32 ? 2 : 1];
+};
+template <int E>
+__device__ __forceinline__ Raw8<E> load8(const typename Elem<E>::type* p) {
+  Raw8<E> r;
+  r.v[0] = *reinterpret_cast<const u32x4*>(p);
+  if constexpr (E == ET_F32) r.v[1] = *reinterpret_cast<const u32x4*>(p + 4);
+  return r;
+}
+template <int E>
+__device__ __forceinline__ Raw8<E> zero8() {
+  Raw8<E> r;
+  r.v[0] = u32x4{0, 0, 0, 0};
+  if constexpr (E == ET_F32) r.v[1] = u32x4{0, 0, 0, 0};
+  return r;
+}
+template <int E>
+__device__ __forceinline__ void unpack8(const Raw8<E>& r, float* f) {
+  if constexpr (E == ET_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r.v[i / 4][i % 4]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = lo16<E>(r.v[0][i]);
+      f[2 * i + 1] = hi16<E>(r.v[0][i]);
+    }
+  }
+}
+template <int E>
+__device__ __forceinline__ void store8(typename Elem<E>::type* p, const float* f) {
+  if constexpr (E == ET_F32) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(f[4 * h + i]);
+      *reinterpret_cast<u32x4*>(p + 4 * h) = v;
+    }
+  } else {
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pack16<E>(f[2 * i], f[2 * i + 1]);
+    *reinterpret_cast<u32x4*>(p) = v;
+  }
+}
+
+// Sum over the LPR lanes of a row; every lane receives the same value.
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {
+  v += __uint_as_float(dpp_u32<0xB1>(__float_as_uint(v)));    // quad_perm [1,0,3,2]
+  v += __uint_as_float(dpp_u32<0x4E>(__float_as_uint(v)));    // quad_perm [2,3,0,1]
+  if constexpr (LPR >= 8) v += __uint_as_float(dpp_u32<0x141>(__float_as_uint(v)));
+  if constexpr (LPR >= 16) v += __uint_as_float(dpp_u32<0x140>(__float_as_uint(v)));
+  if constexpr (LPR >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+
+// What a lane knows of every row: where its two chunks are, and its pairs' angles.
+struct Lane {
+  int sub;        // lane within the row
+  int row;        // row within a pass
+  int c0, c1;     // first elements of its chunks
+  bool on;        // the lane holds elements
+};
+
+template <int LPR, bool INTER>
+__device__ __forceinline__ Lane lane_of(int lane, int D, int R) {
+  Lane l;
+  l.sub = lane & (LPR - 1);
+  l.row = lane / LPR;
+  l.on = 16 * l.sub < D;
+  const bool pairs_apart = !INTER && 16 * l.sub < R;
+  l.c0 = pairs_apart ? 8 * l.sub : 16 * l.sub;
+  l.c1 = pairs_apart ? R / 2 + 8 * l.sub : 16 * l.sub + 8;
+  return l;
+}
+
+// cos and sin of the lane's eight pairs (1 and 0 where its elements are not rotated).
+struct Turn {
+  float c[8], s[8];
+};
+__device__ __forceinline__ Turn load_turn(const Args& a, const Lane& l, int64_t pos, bool real) {
+  Turn t;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    t.c[i] = 1.0f;
+    t.s[i] = 0.0f;
+  }
+  if (real && 16 * l.sub < a.R) {      // padding may have no table row to read
+    const int64_t at = pos * (a.R / 2) + 8 * l.sub;
+    unpack8<ET_F32>(load8<ET_F32>(a.cos + at), t.c);
+    unpack8<ET_F32>(load8<ET_F32>(a.sin + at), t.s);
+  }
+  return t;
+}
+
+// Rotates the lane's 16 elements (chunk 0, chunk 1) in place; BACK: the other way.
+template <bool INTER, bool BACK>
+__device__ __forceinline__ void rotate(float (&n)[16], const Turn& t) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int ia = INTER ? 2 * i : i, ib = INTER ? 2 * i + 1 : i + 8;
+    const float x = n[ia], y = n[ib], s = BACK ? -t.s[i] : t.s[i];
+    n[ia] = __builtin_fmaf(x, t.c[i], -(y * s));
+    n[ib] = __builtin_fmaf(y, t.c[i], x * s);
+  }
+}
+
+__device__ __forceinline__ float rstd_of(float ss, int D, float eps) {
+  return 1.0f / __builtin_sqrtf(ss / (float)D + eps);
+}
+
+__device__ __forceinline__ int64_t position(const Args& a, int t) {
+  return a.idx64 ? static_cast<const int64_t*>(a.pos)[t]
+                 : (int64_t) static_cast<const int32_t*>(a.pos)[t];
+}
+
+template <int E, int LPR, bool INTER>
+__global__ __launch_bounds__(64 * kWaves) void qk_norm_rope_fwd(Args a) {
+  using T = typename Elem<E>::type;
+  constexpr int kRows = 64 / LPR;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * kWaves + threadIdx.x / 64));
+  const int t = wave / a.splits;
+  if (t >= a.T) return;
+  const Lane l = lane_of<LPR, INTER>(threadIdx.x & 63, a.D, a.R);
+  const int pq = (a.Hq + kRows - 1) / kRows, passes = pq + (a.Hk + kRows - 1) / kRows;
+  const int p0 = (wave - t * a.splits) * a.per_wave;
+  const int p1 = p0 + a.per_wave < passes ? p0 + a.per_wave : passes;
+  const int64_t pos = position(a, t);
+  const bool real = pos >= 0 && pos < a.table_rows;
+  const Turn turn = load_turn(a, l, pos, real);
+  for (int p = p0; p < p1; ++p) {
+    const bool isq = p < pq;
+    const int h = (isq ? p : p - pq) * kRows + l.row;
+    const bool on = l.on && h < (isq ? a.Hq : a.Hk);
+    const T* x = static_cast<const T*>(isq ? a.q : a.k) +
+                 ((int64_t)t * (isq ? a.qs[0] : a.ks[0]) + (int64_t)h * (isq ? a.qs[1] : a.ks[1]));
+    T* y = static_cast<T*>(isq ? a.qo : a.ko) +
+           ((int64_t)t * (isq ? a.qos[0] : a.kos[0]) + (int64_t)h * (isq ? a.qos[1] : a.kos[1]));
+    const T* w = static_cast<const T*>(isq ? a.qw : a.kw);
+    Raw8<E> x0 = zero8<E>(), x1 = zero8<E>(), w0 = zero8<E>(), w1 = zero8<E>();
+    if (on) {
+      x0 = load8<E>(x + l.c0);
+      x1 = load8<E>(x + l.c1);
+      w0 = load8<E>(w + l.c0);
+      w1 = load8<E>(w + l.c1);
+    }
+    float n[16], g[16];
+    unpack8<E>(x0, n);
+    unpack8<E>(x1, n + 8);
+    unpack8<E>(w0, g);
+    unpack8<E>(w1, g + 8);
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ss = __builtin_fmaf(n[i], n[i], ss);
+    const float rstd = rstd_of(row_sum<LPR>(ss), a.D, a.eps);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) n[i] = n[i] * rstd * g[i];
+    rotate<INTER, false>(n, turn);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) n[i] = real ? n[i] : 0.0f;
+    if (on) {
+      store8<E>(y + l.c0, n);
+      store8<E>(y + l.c1, n + 8);
+    }
+  }
+}
+
+template <int E, int LPR, bool INTER>
+__global__ __launch_bounds__(64 * kWaves) void qk_norm_rope_bwd(Args a) {
+  using T = typename Elem<E>::type;
+  constexpr int kRows = 64 / LPR;
+  extern __shared__ float sums[];               // [waves][2][D]
+  const int wg_wave = threadIdx.x / 64;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * kWaves + wg_wave));
+  const int waves = gridDim.x * kWaves;
+  const Lane l = lane_of<LPR, INTER>(threadIdx.x & 63, a.D, a.R);
+  const int pq = (a.Hq + kRows - 1) / kRows, passes = pq + (a.Hk + kRows - 1) / kRows;
+  float dw[2][16] = {};                         // of q's and k's weight
+  for (int64_t item = wave; item < (int64_t)a.T * a.splits; item += waves) {
+    const int t = (int)(item / a.splits);
+    const int p0 = (int)(item - (int64_t)t * a.splits) * a.per_wave;
+    const int p1 = p0 + a.per_wave < passes ? p0 + a.per_wave : passes;
+    const int64_t pos = position(a, t);
+    const bool real = pos >= 0 && pos < a.table_rows;
+    const Turn turn = load_turn(a, l, pos, real);
+    auto pass = [&](int p, bool isq, float (&acc)[16]) {
+      const int h = (isq ? p : p - pq) * kRows + l.row;
+      const bool on = l.on && h < (isq ? a.Hq : a.Hk);
+      const int64_t st = isq ? a.qs[0] : a.ks[0], sh = isq ? a.qs[1] : a.ks[1];
+      const int64_t dt = isq ? a.dqs[0] : a.dks[0], dh = isq ? a.dqs[1] : a.dks[1];
+      const int64_t ot = isq ? a.qos[0] : a.kos[0], oh = isq ? a.qos[1] : a.kos[1];
+      const T* x = static_cast<const T*>(isq ? a.q : a.k) + (t * st + h * sh);
+      const T* dy = static_cast<const T*>(isq ? a.dq : a.dk) + (t * dt + h * dh);
+      T* dx = static_cast<T*>(isq ? a.qo : a.ko) + (t * ot + h * oh);
+      const T* w = static_cast<const T*>(isq ? a.qw : a.kw);
+      Raw8<E> x0 = zero8<E>(), x1 = zero8<E>(), w0 = zero8<E>(), w1 = zero8<E>();
+      Raw8<E> d0 = zero8<E>(), d1 = zero8<E>();
+      if (on) {
+        x0 = load8<E>(x + l.c0);
+        x1 = load8<E>(x + l.c1);
+        d0 = load8<E>(dy + l.c0);
+        d1 = load8<E>(dy + l.c1);
+        w0 = load8<E>(w + l.c0);
+        w1 = load8<E>(w + l.c1);
+      }
+      float n[16], d[16], g[16];
+      unpack8<E>(x0, n);
+      unpack8<E>(x1, n + 8);
+      unpack8<E>(d0, d);
+      unpack8<E>(d1, d + 8);
+      unpack8<E>(w0, g);
+      unpack8<E>(w1, g + 8);
+      rotate<INTER, true>(d, turn);
+      float ss = 0.0f, ax = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        ss = __builtin_fmaf(n[i], n[i], ss);
+        ax = __builtin_fmaf(d[i] * g[i], n[i], ax);
+      }
+      const float rstd = rstd_of(row_sum<LPR>(ss), a.D, a.eps);
+      const float back = row_sum<LPR>(ax) / (float)a.D * rstd * rstd;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        // Rows past the last head hold zeros and add nothing; padding adds nothing either.
+        const float gx = d[i] * (n[i] * rstd);
+        acc[i] += real && on ? gx : 0.0f;
+        n[i] = real ? rstd * __builtin_fmaf(-n[i], back, d[i] * g[i]) : 0.0f;
+      }
+      if (on) {
+        store8<E>(dx + l.c0, n);
+        store8<E>(dx + l.c1, n + 8);
+      }
+    };
+    int p = p0;
+    for (; p < p1 && p < pq; ++p) pass(p, true, dw[0]);
+    for (; p < p1; ++p) pass(p, false, dw[1]);
+  }
+#pragma unroll
+  for (int o = 0; o < 2; ++o)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+#pragma unroll
+      for (int m = LPR; m < 64; m *= 2) dw[o][i] += __shfl_xor(dw[o][i], m);
+    }
+  if ((threadIdx.x & 63) < LPR && l.on) {
+#pragma unroll
+    for (int o = 0; o < 2; ++o)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        sums[(wg_wave * 2 + o) * a.D + l.c0 + i] = dw[o][i];
+        sums[(wg_wave * 2 + o) * a.D + l.c1 + i] = dw[o][8 + i];
+      }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * a.D; i += 64 * kWaves) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) s += sums[w * 2 * a.D + i];
+    a.sums[(int64_t)blockIdx.x * 2 * a.D + i] = s;
+  }
+}
+
+struct SumArgs {
+  const float* sums;    // [n][2 * D]
+  float* dqw;
+  float* dkw;
+  int32_t n, D;
+};
+
+// The workgroups' sums of 16 columns: 64 threads of each column take every 64th one, then
+// add their own in LDS in a fixed order.
+__global__ __launch_bounds__(16 * kSumRows) void weight_sums(SumArgs a) {
+  __shared__ float part[kSumRows][17];
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + c;          // 2 D is a multiple of 32
+  float s = 0.0f;
+#pragma unroll 8
+  for (int i = r; i < a.n; i += kSumRows) s += a.sums[(int64_t)i * 2 * a.D + col];
+  part[r][c] = s;
+  __syncthreads();
+  for (int half = kSumRows / 2; half > 0; half /= 2) {
+    if (r < half) part[r][c] += part[r + half][c];
+    __syncthreads();
+  }
+  if (r == 0) (col < a.D ? a.dqw[col] : a.dkw[col - a.D]) = part[0][c];
+}
+
+// ---------------------------------------------------------------------------------- host
+
+bool aligned(const void* p, uintptr_t a) {
+  return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
+}
+
+// Rows of D elements at token and head strides.
+struct Rows {
+  const void* p;
+  int64_t H, st, sh;
+};
+
+int64_t span(const Rows& r, int64_t T, int64_t D) {
+  return (T - 1) * r.st + (r.H - 1) * r.sh + D;
+}
+
+// Whether two sets of rows share an element (told exactly for heads that lie within a token's
+// stride, as views of one fused buffer do; otherwise by their ranges).
+bool overlap(const Rows& a, const Rows& b, int64_t T, int64_t D, int64_t es) {
+  const intptr_t pa = reinterpret_cast<intptr_t>(a.p), pb = reinterpret_cast<intptr_t>(b.p);
+  if (pa + span(a, T, D) * es <= pb || pb + span(b, T, D) * es <= pa) return false;
+  const int64_t wa = ((a.H - 1) * a.sh + D) * es, wb = ((b.H - 1) * b.sh + D) * es;
+  const int64_t s = a.st * es;
+  if (a.st != b.st || T < 2 || wa > s || wb > s) return true;
+  const int64_t off = ((pb - pa) % s + s) % s;       // b's heads start here in a's token
+  return off < wa || (off != 0 && s - off < wb);
+}
+
+bool overlap_range(const Rows& a, int64_t T, int64_t D, int64_t es, const void* p, int64_t n) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(a.p), q = reinterpret_cast<uintptr_t>(p);
+  return lo < q + (uintptr_t)n && q < lo + (uintptr_t)(span(a, T, D) * es);
+}
+
+// Rows that are written must not share an element among themselves.
+bool self_overlap(const Rows& r, int64_t T, int64_t D) {
+  const bool heads = r.H < 2 || r.sh >= D, tokens = T < 2 || r.st >= D;
+  if (!heads || !tokens) return true;
+  if (r.H < 2 || T < 2) return false;
+  return r.st < (r.H - 1) * r.sh + D && r.sh < (T - 1) * r.st + D;
+}
+
+bool same(const Rows& a, const Rows& b) { return a.p == b.p && a.st == b.st && a.sh == b.sh; }
+
+int check_sizes(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t R, int64_t table_rows) {
+  if (T < 0 || Hq < 1 || Hk < 1 || D < 16 || D % 16 != 0 || R < 16 || R > D || R % 16 != 0 ||
+      table_rows < 0)
+    return FAGQ_E_SHAPE;
+  if (D > FAGQ_ROPE_MAX_D || T > (1ll << 24) || Hq > 4096 || Hk > 4096 || table_rows > (1ll << 31))
+    return FAGQ_E_TOO_LARGE;
+  return FAGQ_OK;
+}
+
+int lanes_per_row(int64_t D) { return D <= 64 ? 4 : D <= 128 ? 8 : D <= 256 ? 16 : 32; }
+
+template <int E, int LPR>
+const void* kernel_for(bool inter, bool bwd) {
+  if (bwd)
+    return inter ? reinterpret_cast<const void*>(&qk_norm_rope_bwd<E, LPR, true>)
+                 : reinterpret_cast<const void*>(&qk_norm_rope_bwd<E, LPR, false>);
+  return inter ? reinterpret_cast<const void*>(&qk_norm_rope_fwd<E, LPR, true>)
+               : reinterpret_cast<const void*>(&qk_norm_rope_fwd<E, LPR, false>);
+}
+template <int E>
+const void* kernel_for(int lpr, bool inter, bool bwd) {
+  switch (lpr) {
+    case 4: return kernel_for<E, 4>(inter, bwd);
+    case 8: return kernel_for<E, 8>(inter, bwd);
+    case 16: return kernel_for<E, 16>(inter, bwd);
+    default: return kernel_for<E, 32>(inter, bwd);
+  }
+}
+const void* kernel_for(int dtype, int lpr, bool inter, bool bwd) {
+  return dtype == FAGQ_DT_BF16  ? kernel_for<ET_BF16>(lpr, inter, bwd)
+         : dtype == FAGQ_DT_F16 ? kernel_for<ET_F16>(lpr, inter, bwd)
+                                : kernel_for<ET_F32>(lpr, inter, bwd);
+}
+
+// How the heads of a token are shared out over waves.
+struct Split {
+  int64_t splits, per_wave;
+};
+Split split_for(int64_t T, int64_t Hq, int64_t Hk, int64_t D) {
+  const int64_t rows = 64 / lanes_per_row(D);
+  const int64_t passes = (Hq + rows - 1) / rows + (Hk + rows - 1) / rows;
+  // A wave takes a whole token where that fills the GPU (8 waves on each of 256 CUs, twice).
+  int64_t per = passes * T / 4096;
+  per = per < 1 ? 1 : per > passes ? passes : per;
+  return {(passes + per - 1) / per, per};
+}
+
+int64_t bwd_groups(int64_t T, int64_t Hq, int64_t Hk, int64_t D) {
+  const int64_t n = (T * split_for(T, Hq, Hk, D).splits + kWaves - 1) / kWaves;
+  return n > kMaxBwdGroups ? kMaxBwdGroups : n;
+}
+
+int check_common(const void* const* ptrs, int n, const int64_t* strides, int nstrides, int64_t T,
+                 int64_t Hq, int64_t Hk, int64_t D, int64_t R, int64_t table_rows, float eps,
+                 int dtype, int index_dtype, const void* positions) {
+  for (int i = 0; i < n; ++i)
+    if (!ptrs[i]) return FAGQ_E_NULL;
+  if (!positions || !strides) return FAGQ_E_NULL;
+  if (dtype != FAGQ_DT_BF16 && dtype != FAGQ_DT_F16 && dtype != FAGQ_DT_F32) return FAGQ_E_FORMAT;
+  if (index_dtype != FAGQ_IDX_I32 && index_dtype != FAGQ_IDX_I64) return FAGQ_E_FORMAT;
+  if (!(eps >= 0.0f) || eps > 3.0e38f) return FAGQ_E_EPS;
+  const int sizes = check_sizes(T, Hq, Hk, D, R, table_rows);
+  if (sizes != FAGQ_OK) return sizes;
+  const int64_t unit = dtype == FAGQ_DT_F32 ? 4 : 8;
+  for (int i = 0; i < nstrides; ++i) {
+    if (strides[i] < 0) return FAGQ_E_SHAPE;
+    if (strides[i] >= (1ll << 31)) return FAGQ_E_TOO_LARGE;
+    if (strides[i] % unit != 0) return FAGQ_E_ALIGN;
+  }
+  for (int i = 0; i < n; ++i)
+    if (!aligned(ptrs[i], 16)) return FAGQ_E_ALIGN;
+  if (!aligned(positions, index_dtype == FAGQ_IDX_I64 ? 8 : 4)) return FAGQ_E_ALIGN;
+  return FAGQ_OK;
+}
+
+void set_strides(int32_t (&to)[2], const int64_t* from) {
+  to[0] = (int32_t)from[0];
+  to[1] = (int32_t)from[1];
+}
+
+}  // namespace
+}  // namespace rope
+}  // namespace fagq
+
+extern "C" {
+
+FAGQ_API int fagq_qk_norm_rope_launch(const void* q, const void* k, const void* q_weight,
+                                      const void* k_weight, const float* cos, const float* sin,
+                                      const void* positions, void* q_out, void* k_out,
+                                      const int64_t* strides, int64_t T, int64_t Hq, int64_t Hk,
+                                      int64_t D, int64_t R, int64_t table_rows, float eps,
+                                      int interleaved, int dtype, int index_dtype, void* stream) {
+  using namespace fagq;
+  using namespace fagq::rope;
+  const void* ptrs[] = {q, k, q_weight, k_weight, cos, sin, q_out, k_out};
+  const int v = check_common(ptrs, 8, strides, 8, T, Hq, Hk, D, R, table_rows, eps, dtype,
+                             index_dtype, positions);
+  if (v != FAGQ_OK) return v;
+  if (T == 0) return FAGQ_OK;
+  const int64_t es = dtype == FAGQ_DT_F32 ? 4 : 2;
+  const Rows in[2] = {{q, Hq, strides[0], strides[1]}, {k, Hk, strides[2], strides[3]}};
+  const Rows out[2] = {{q_out, Hq, strides[4], strides[5]}, {k_out, Hk, strides[6], strides[7]}};
+  const void* rest[] = {q_weight, k_weight, cos, sin, positions};
+  const int64_t nrest[] = {D * es, D * es, table_rows * R * 2, table_rows * R * 2,
+                           T * (index_dtype == FAGQ_IDX_I64 ? 8 : 4)};
+  if (overlap(out[0], out[1], T, D, es)) return FAGQ_E_ALIAS;
+  for (int i = 0; i < 2; ++i) {
+    if (self_overlap(out[i], T, D)) return FAGQ_E_ALIAS;
+    for (int j = 0; j < 2; ++j)
+      if (!(i == j && same(out[i], in[j])) && overlap(out[i], in[j], T, D, es)) return FAGQ_E_ALIAS;
+    for (int j = 0; j < 5; ++j)
+      if (overlap_range(out[i], T, D, es, rest[j], nrest[j])) return FAGQ_E_ALIAS;
+  }
+  const int dcheck = device_check();
+  if (dcheck != FAGQ_OK) return dcheck;
+  const Split s = split_for(T, Hq, Hk, D);
+  Args a = {};
+  a.q = q, a.k = k, a.qw = q_weight, a.kw = k_weight, a.cos = cos, a.sin = sin, a.pos = positions;
+  a.qo = q_out, a.ko = k_out, a.table_rows = table_rows;
+  set_strides(a.qs, strides), set_strides(a.ks, strides + 2);
+  set_strides(a.qos, strides + 4), set_strides(a.kos, strides + 6);
+  a.T = (int32_t)T, a.Hq = (int32_t)Hq, a.Hk = (int32_t)Hk, a.D = (int32_t)D, a.R = (int32_t)R;
+  a.splits = (int32_t)s.splits, a.per_wave = (int32_t)s.per_wave;
+  a.idx64 = index_dtype == FAGQ_IDX_I64, a.eps = eps;
+  void* args[] = {&a};
+  // T * splits < 2^24 * 2 when a token is split (T < 4096 then), so the grid stays below 2^31.
+  const int64_t groups = (T * s.splits + kWaves - 1) / kWaves;
+  return launch_kernel(kernel_for(dtype, lanes_per_row(D), interleaved != 0, false),
+                       dim3((unsigned)groups), dim3(64 * kWaves), args, 0,
+                       static_cast<hipStream_t>(stream));
+}
+
+FAGQ_API int64_t fagq_qk_norm_rope_bwd_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk,
+                                                       int64_t D) {
+  using namespace fagq::rope;
+  if (check_sizes(T, Hq, Hk, D, 16, 0) != FAGQ_OK) return -1;
+  return bwd_groups(T, Hq, Hk, D) * 2 * D * 4;
+}
+
+FAGQ_API int fagq_qk_norm_rope_bwd_launch(const void* dq_out, const void* dk_out, const void* q,
+                                          const void* k, const void* q_weight,
+                                          const void* k_weight, const float* cos, const float* sin,
+                                          const void* positions, void* dq, void* dk,
+                                          float* dq_weight, float* dk_weight, void* workspace,
+                                          int64_t workspace_bytes, const int64_t* strides,
+                                          int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t R,
+                                          int64_t table_rows, float eps, int interleaved,
+                                          int dtype, int index_dtype, void* stream) {
+  using namespace fagq;
+  using namespace fagq::rope;
+  const void* ptrs[] = {dq_out, dk_out, q,  k,  q_weight,  k_weight,
+                        cos,    sin,    dq, dk, dq_weight, dk_weight};
+  const int v = check_common(ptrs, 12, strides, 12, T, Hq, Hk, D, R, table_rows, eps, dtype,
+                             index_dtype, positions);
+  if (v != FAGQ_OK) return v;
+  const int64_t groups = bwd_groups(T, Hq, Hk, D), need = groups * 2 * D * 4;
+  if (need > 0 && !workspace) return FAGQ_E_NULL;
+  if (workspace_bytes < need) return FAGQ_E_SHAPE;
+  if (!aligned(workspace, 16)) return FAGQ_E_ALIGN;
+  const int64_t es = dtype == FAGQ_DT_F32 ? 4 : 2;
+  const Rows in[4] = {{dq_out, Hq, strides[0], strides[1]},
+                      {dk_out, Hk, strides[2], strides[3]},
+                      {q, Hq, strides[4], strides[5]},
+                      {k, Hk, strides[6], strides[7]}};
+  const Rows out[2] = {{dq, Hq, strides[8], strides[9]}, {dk, Hk, strides[10], strides[11]}};
+  const void* flat[] = {dq_weight, dk_weight, workspace, q_weight, k_weight, cos, sin, positions};
+  const int64_t nflat[] = {D * 4, D * 4, need, D * es, D * es, table_rows * R * 2,
+                           table_rows * R * 2, T * (index_dtype == FAGQ_IDX_I64 ? 8 : 4)};
+  if (T > 0) {
+    if (overlap(out[0], out[1], T, D, es)) return FAGQ_E_ALIAS;
+    for (int i = 0; i < 2; ++i) {
+      if (self_overlap(out[i], T, D)) return FAGQ_E_ALIAS;
+      for (int j = 0; j < 4; ++j)
+        if (overlap(out[i], in[j], T, D, es)) return FAGQ_E_ALIAS;
+      for (int j = 0; j < 8; ++j)
+        if (overlap_range(out[i], T, D, es, flat[j], nflat[j])) return FAGQ_E_ALIAS;
+    }
+    for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < 3; ++j)
+        if (overlap_range(in[i], T, D, es, flat[j], nflat[j])) return FAGQ_E_ALIAS;
+  }
+  for (int i = 0; i < 3; ++i)
+    for (int j = i + 1; j < 8; ++j) {
+      const uintptr_t x = reinterpret_cast<uintptr_t>(flat[i]), y = reinterpret_cast<uintptr_t>(flat[j]);
+      if (nflat[i] > 0 && nflat[j] > 0 && x < y + (uintptr_t)nflat[j] && y < x + (uintptr_t)nflat[i])
+        return FAGQ_E_ALIAS;
+    }
+  const int dcheck = device_check();
+  if (dcheck != FAGQ_OK) return dcheck;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (groups > 0) {
+    const Split s = split_for(T, Hq, Hk, D);
+    Args a = {};
+    a.q = q, a.k = k, a.qw = q_weight, a.kw = k_weight, a.cos = cos, a.sin = sin;
+    a.pos = positions, a.qo = dq, a.ko = dk, a.dq = dq_out, a.dk = dk_out;
+    a.sums = static_cast<float*>(workspace), a.table_rows = table_rows;
+    set_strides(a.dqs, strides), set_strides(a.dks, strides + 2);
+    set_strides(a.qs, strides + 4), set_strides(a.ks, strides + 6);
+    set_strides(a.qos, strides + 8), set_strides(a.kos, strides + 10);
+    a.T = (int32_t)T, a.Hq = (int32_t)Hq, a.Hk = (int32_t)Hk, a.D = (int32_t)D, a.R = (int32_t)R;
+    a.splits = (int32_t)s.splits, a.per_wave = (int32_t)s.per_wave;
+    a.idx64 = index_dtype == FAGQ_IDX_I64, a.eps = eps;
+    void* args[] = {&a};
+    const int ls = launch_kernel(kernel_for(dtype, lanes_per_row(D), interleaved != 0, true),
+                                 dim3((unsigned)groups), dim3(64 * kWaves), args,
+                                 (size_t)kWaves * 2 * D * 4, st);
+    if (ls != FAGQ_OK) return ls;
+  }
+  SumArgs sa = {static_cast<const float*>(workspace), dq_weight, dk_weight, (int32_t)groups,
+                (int32_t)D};
+  void* sargs[] = {&sa};
+  return launch_kernel(reinterpret_cast<const void*>(&weight_sums), dim3((unsigned)(2 * D / 16)),
+                       dim3(16 * kSumRows), sargs, 0, st);
+}
+
+}  // extern "C"

@@ -86,6 +86,14 @@ FAGQ_API int fagq_diag_scale_offsets(int64_t M, int64_t D, int64_t group_size, i
                                      int scale_layout, int waves_per_row, int64_t row,
                                      int64_t* out, int64_t cap);
 
+/* Host-side check of the paged cache's lookups, computed by the functions its
+ * kernels use, on host arrays: out[r] = the slot that row r of
+ * fagq_kv_cache_read_launch's outputs reads, -1 for a token without a page, -2
+ * for a row of no sequence.  Never touches the device. */
+FAGQ_API int fagq_diag_cache_slots(const int32_t* page_table, const int32_t* cu_seqlens, int64_t B,
+                                   int64_t table_width, int64_t num_pages, int64_t page_size,
+                                   int64_t* out, int64_t rows);
+
 #ifdef __cplusplus
 }
 #endif
