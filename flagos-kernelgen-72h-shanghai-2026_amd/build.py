@@ -31,6 +31,9 @@ ARCH = "gfx950"
 # code 0 = fp8 e4m3fn, 1 = int8 round-half-even, 2 = int8 truncate;
 # scale 0 = fp32, 1 = ue8m0.
 INST_COMBOS = [(q, s) for q in (0, 1, 2) for s in (0, 1)]
+# (element type, code format, scale format) compiled from paged_attn_inst.hip:
+# element 0 = bf16, 1 = fp16; code 0 = fp8 e4m3fn, 1 = int8; scale as above.
+ATTN_COMBOS = [(e, q, s) for e in (0, 1) for q in (0, 1) for s in (0, 1)]
 
 
 def hipcc() -> str:
@@ -106,6 +109,9 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
                       [f"-DFAGQ_QF={q}", f"-DFAGQ_SF={s}"]))
         units.append((CSRC / "fagq_inst_typed.hip", OBJ_DIR / f"fagq_inst_typed_q{q}_s{s}.o",
                       [f"-DFAGQ_QF={q}", f"-DFAGQ_SF={s}"]))
+    for e, q, s in ATTN_COMBOS:
+        units.append((CSRC / "paged_attn_inst.hip", OBJ_DIR / f"paged_attn_inst_e{e}_q{q}_s{s}.o",
+                      [f"-DFAGQ_ATTN_E={e}", f"-DFAGQ_ATTN_QF={q}", f"-DFAGQ_ATTN_SF={s}"]))
     for unit in sorted(set(LIB_UNITS) | set(PROBE_UNITS)):
         units.append((CSRC / f"{unit}.hip", OBJ_DIR / f"{unit}.o", []))
     jobs = jobs or min(len(units) + 1, max(1, min(16, os.cpu_count() or 1)))
@@ -165,6 +171,9 @@ def build_variant(name: str, *, defines: tuple[str, ...] = (), sanitize: bool = 
                       [f"-DFAGQ_QF={q}", f"-DFAGQ_SF={sf}"]))
         units.append((CSRC / "fagq_inst_typed.hip", out_dir / f"fagq_inst_typed_q{q}_s{sf}.o",
                       [f"-DFAGQ_QF={q}", f"-DFAGQ_SF={sf}"]))
+    for e, q, s in ATTN_COMBOS:
+        units.append((CSRC / "paged_attn_inst.hip", out_dir / f"paged_attn_inst_e{e}_q{q}_s{s}.o",
+                      [f"-DFAGQ_ATTN_E={e}", f"-DFAGQ_ATTN_QF={q}", f"-DFAGQ_ATTN_SF={s}"]))
     for unit in sorted(set(LIB_UNITS) | set(PROBE_UNITS)):
         units.append((CSRC / f"{unit}.hip", out_dir / f"{unit}.o", []))
     with ThreadPoolExecutor(max_workers=min(len(units), max(1, min(16, os.cpu_count() or 1)))) as ex:

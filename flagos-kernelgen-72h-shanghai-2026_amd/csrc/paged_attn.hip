@@ -1,10 +1,6 @@
-// paged_attn.hip - attention of the newest tokens of each sequence over the quantised paged
-// cache (include/fagq_cache.h).
-//
-// One pass with a running maximum m and sum l of the softmax: for key j with
-// x = q . (code_k s_k) sm_scale,  m' = max(m, x),  l = l e^(m - m') + e^(x - m'),
-// o = o e^(m - m') + e^(x - m') code_v s_v.  Parts of a row's keys have m, l and o of their
-// own and are joined by the same rule.
+// paged_attn.hip - attention over the quantised paged cache (include/fagq_cache.h): the split of
+// the work, the kernel that joins its parts, and the C entry points.  The attention itself is in
+// paged_attn_kernels.hpp.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -14,106 +10,70 @@
 #include "fagq_cache.h"
 #include "fagq_cache_index.hpp"
 #include "fagq_dispatch.hpp"
+#include "paged_attn_kernels.hpp"
 
 namespace fagq {
 namespace attn {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int64_t kGroups = 1024;      // workgroups wanted (see plan_for)
+constexpr int64_t kMinChunk = kStep * kWaves;
 
-struct Args {
-  const uint16_t* q;
-  const uint8_t* kc;
-  const uint8_t* vc;
-  const void* ks;
-  const void* vs;
-  const int32_t* table;
+struct JoinArgs {
+  const float* part;
+  const float* ml;
   const void* lens;
-  const int32_t* prefix;
   uint16_t* out;
-  int64_t num_pages;
-  int32_t qs[3];             // {sequence, token, head} strides, elements
-  int32_t S, Hq, H, group;
-  int32_t page_shift;
-  int32_t width;
-  int32_t prefix_len;
-  int32_t most;              // tokens of a sequence that are read at most
-  int32_t idx64, sf, qf;
-  float scale2;              // sm_scale * log2(e)
+  int32_t rows, S, Hq;
+  int32_t prefix_chunks, chunks, chunk, most;
+  int32_t idx64;
 };
 
-__device__ __forceinline__ float code_value(int qf, uint8_t c) {
-  return qf == QF_FP8 ? __builtin_amdgcn_cvt_f32_fp8((int)c, 0) : (float)(int8_t)c;
-}
-__device__ __forceinline__ float scale_value(int sf, const void* p, int64_t at) {
-  return sf == SF_F32 ? static_cast<const float*>(p)[at]
-                      : __builtin_ldexpf(1.0f, (int)static_cast<const uint8_t*>(p)[at] - 127);
-}
-
-// One workgroup for each query row; its waves take every fourth key, a lane D / 64 dims.
+// One wave for each query row: the chunks that hold keys of its sequence, joined by
+// o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.  A lane has D / 64 dims.
 template <int E, int D>
-__global__ __launch_bounds__(64 * kWaves) void paged_attention_rows(Args a) {
+__global__ __launch_bounds__(64 * kWaves) void paged_attention_join(JoinArgs a) {
   constexpr int N = D / 64;
-  __shared__ float part[kWaves][D + 2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = blockIdx.x;                   // (b, s, hq)
-  const int hq = row % a.Hq, s = row / a.Hq % a.S, b = row / a.Hq / a.S;
-  const int h = hq / a.group;
+  const int row = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * kWaves + threadIdx.x / 64));
+  if (row >= a.rows) return;
+  const int lane = threadIdx.x & 63;
+  const int b = row / a.Hq / a.S;
   const int64_t len = a.idx64 ? static_cast<const int64_t*>(a.lens)[b]
                               : (int64_t) static_cast<const int32_t*>(a.lens)[b];
-  const int64_t keys = a.prefix_len + cache::seen_tokens(len, a.most, a.S, s);
-  float q[N], o[N] = {}, m = -INFINITY, l = 0.0f;
+  const int own = ((int)cache::seen_tokens(len, a.most, 1, 0) + a.chunk - 1) / a.chunk;
+  const int n = a.prefix_chunks + (own > 1 ? own : 1);
+  const int64_t at = (int64_t)row * (a.prefix_chunks + a.chunks);
+  const float* ml = a.ml + 2 * at;
+  const float* part = a.part + at * D + lane * N;
+  float m = kLow;
+  for (int i = lane; i < n; i += 64) m = fmaxf(m, ml[2 * i]);
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    q[i] = lo16<E>(a.q[(int64_t)b * a.qs[0] + (int64_t)s * a.qs[1] + (int64_t)hq * a.qs[2] +
-                       lane * N + i]) * a.scale2;
-  for (int64_t j = wave; j < keys; j += kWaves) {
-    const bool front = j < a.prefix_len;
-    const int64_t t = front ? j : j - a.prefix_len;
-    const int64_t slot =
-        front ? cache::slot_of(a.prefix, ((int64_t)a.prefix_len - 1 >> a.page_shift) + 1,
-                               a.num_pages, a.page_shift, t)
-              : cache::slot_of(a.table + (int64_t)b * a.width, a.width, a.num_pages, a.page_shift, t);
-    if (slot < 0) continue;
-    const int64_t at = (((slot >> a.page_shift) * a.H + h) << a.page_shift) +
-                       (slot & ((1 << a.page_shift) - 1));
-    float x = 0.0f;
+  for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+  float o[N] = {}, l = 0.0f;
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    float w = 0.0f;
+    if (i0 + lane < n) {
+      w = __builtin_amdgcn_exp2f(ml[2 * (i0 + lane)] - m);
+      l += w * ml[2 * (i0 + lane) + 1];
+    }
+    const int stop = n - i0 < 64 ? n - i0 : 64;
+#pragma unroll 4
+    for (int i = 0; i < stop; ++i) {
+      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), i));
 #pragma unroll
-    for (int i = 0; i < N; ++i) x += q[i] * code_value(a.qf, a.kc[at * D + lane * N + i]);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
-    x *= scale_value(a.sf, a.ks, at);
-    const float top = x > m ? x : m;
-    const float keep = __builtin_amdgcn_exp2f(m - top), w = __builtin_amdgcn_exp2f(x - top);
-    const float wv = w * scale_value(a.sf, a.vs, at);
-    l = l * keep + w;
-    m = top;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      o[i] = o[i] * keep + wv * code_value(a.qf, a.vc[at * D + lane * N + i]);
+      for (int j = 0; j < N; ++j) o[j] = __builtin_fmaf(f, part[(int64_t)(i0 + i) * D + j], o[j]);
+    }
   }
 #pragma unroll
-  for (int i = 0; i < N; ++i) part[wave][lane * N + i] = o[i];
-  if (lane == 0) {
-    part[wave][D] = m;
-    part[wave][D + 1] = l;
-  }
-  __syncthreads();
-  float top = -INFINITY, total = 0.0f;
+  for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  uint16_t* out = a.out + (int64_t)row * D + lane * N;
+  if constexpr (N == 1) {
+    out[0] = (uint16_t)pack16<E>(o[0] * inv, 0.0f);
+  } else {
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = part[w][D] > top ? part[w][D] : top;
-  float f[kWaves];
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    f[w] = part[w][D] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part[w][D] - top);
-    total += f[w] * part[w][D + 1];
-  }
-  const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-  for (int d = threadIdx.x; d < D; d += 64 * kWaves) {
-    float v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) v += f[w] * part[w][d];
-    a.out[(int64_t)row * D + d] = (uint16_t)pack16<E>(v * inv, 0.0f);
+    for (int j = 0; j < N; j += 2)
+      *reinterpret_cast<uint32_t*>(out + j) = pack16<E>(o[j] * inv, o[j + 1] * inv);
   }
 }
 
@@ -145,11 +105,64 @@ int check_sizes(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t 
   return FAGQ_OK;
 }
 
+// How a call's rows and keys are cut.  A unit has 16 R rows (R = 1, 2 or 4: as few as hold the
+// rows that share their keys, so that a step's codes are widened once for all of them); keys are
+// cut into chunks so that kGroups workgroups have work, kMinChunk keys at least.
+struct Plan {
+  int R, RP;
+  int64_t tiles, prefix_tiles, chunk, prefix_chunk, chunks, prefix_chunks, items, prefix_items;
+  int64_t rows;
+};
+
+int row_tiles(int64_t rows, int64_t D) { return rows <= 16 ? 1 : rows <= 32 || D > 128 ? 2 : 4; }
+
+void cut(int64_t keys, int64_t units, int64_t* chunk, int64_t* chunks) {
+  const int64_t want = (kGroups + units - 1) / units;
+  int64_t c = (keys + want - 1) / want;
+  c = (c + kMinChunk - 1) / kMinChunk * kMinChunk;
+  *chunk = c < kMinChunk ? kMinChunk : c;
+  *chunks = (keys + *chunk - 1) / *chunk;
+}
+
+Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t prefix_len,
+              int64_t most) {
+  Plan p = {};
+  const int64_t per = S * (Hq / H);
+  p.rows = B * S * Hq;
+  p.R = row_tiles(per, D);
+  if (prefix_len > 0) {
+    p.RP = row_tiles(B * per, D);
+    if (p.R > 1) p.R = p.RP;
+    p.prefix_tiles = (B * per + 16 * p.RP - 1) / (16 * p.RP);
+    cut(prefix_len, H * p.prefix_tiles, &p.prefix_chunk, &p.prefix_chunks);
+    p.prefix_items = H * p.prefix_tiles * p.prefix_chunks;
+  }
+  p.tiles = (per + 16 * p.R - 1) / (16 * p.R);
+  cut(most, B * H * p.tiles, &p.chunk, &p.chunks);
+  if (p.chunks < 1) p.chunks = 1;       // rows without keys are written all the same
+  p.items = B * H * p.tiles * p.chunks;
+  return p;
+}
+
+int64_t workspace_bytes(const Plan& p, int64_t D) {
+  const int64_t n = p.chunks + p.prefix_chunks;
+  return n == 1 ? 0 : p.rows * n * (D + 2) * 4;
+}
+
+const void* kernel_for(int dtype, int q_format, int scale_format, int D, const Plan& p) {
+  using Lookup = const void* (*)(int, int, int);
+  static constexpr Lookup table[8] = {lookup_e0_q0_s0, lookup_e0_q0_s1, lookup_e0_q1_s0, lookup_e0_q1_s1,
+                             lookup_e1_q0_s0, lookup_e1_q0_s1, lookup_e1_q1_s0, lookup_e1_q1_s1};
+  const int e = dtype == FAGQ_DT_BF16 ? 0 : 1, q = q_format == FAGQ_Q_FP8_E4M3FN ? 0 : 1;
+  const int s = scale_format == FAGQ_SCALE_F32 ? 0 : 1;
+  return table[4 * e + 2 * q + s](D, p.R, p.RP);
+}
+
 template <int E>
-const void* kernel_for(int64_t D) {
-  return D == 64    ? reinterpret_cast<const void*>(&paged_attention_rows<E, 64>)
-         : D == 128 ? reinterpret_cast<const void*>(&paged_attention_rows<E, 128>)
-                    : reinterpret_cast<const void*>(&paged_attention_rows<E, 256>);
+const void* join_for(int64_t D) {
+  return D == 64    ? reinterpret_cast<const void*>(&paged_attention_join<E, 64>)
+         : D == 128 ? reinterpret_cast<const void*>(&paged_attention_join<E, 128>)
+                    : reinterpret_cast<const void*>(&paged_attention_join<E, 256>);
 }
 
 }  // namespace
@@ -163,7 +176,7 @@ FAGQ_API int64_t fagq_paged_attention_workspace_bytes(int64_t B, int64_t S, int6
                                                       int64_t max_kv_len) {
   using namespace fagq::attn;
   if (check_sizes(B, S, Hq, H, D, prefix_len, max_kv_len) != FAGQ_OK) return -1;
-  return 0;
+  return B == 0 ? 0 : workspace_bytes(plan_for(B, S, Hq, H, D, prefix_len, max_kv_len), D);
 }
 
 FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, const void* v_cache,
@@ -188,7 +201,7 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   if (!std::isfinite(sm_scale)) return FAGQ_E_SHAPE;
   const int sizes = check_sizes(B, S, Hq, H, D, prefix_len, max_kv_len);
   if (sizes != FAGQ_OK) return sizes;
-  if (num_pages < 0 || table_width < 0 || page_size < FAGQ_CACHE_MIN_PAGE ||
+  if (num_pages < 1 || table_width < 0 || page_size < FAGQ_CACHE_MIN_PAGE ||
       (page_size & (page_size - 1)) != 0)
     return FAGQ_E_SHAPE;
   if (page_size > FAGQ_CACHE_MAX_PAGE || num_pages > (1ll << 31) - 1 ||
@@ -202,7 +215,7 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   const int64_t ss = scale_format == FAGQ_SCALE_F32 ? 4 : 1;
   const int64_t is = index_dtype == FAGQ_IDX_I64 ? 8 : 4;
   if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) ||
-      !aligned(k_scale, 4) || !aligned(v_scale, 4) || !aligned(page_table, 4) ||
+      !aligned(k_scale, ss * 4) || !aligned(v_scale, ss * 4) || !aligned(page_table, 4) ||
       !aligned(kv_lens, is) || !aligned(prefix_pages, 4) || !aligned(out, 16))
     return FAGQ_E_ALIGN;
   const int64_t need = fagq_paged_attention_workspace_bytes(B, S, Hq, H, D, prefix_len, max_kv_len);
@@ -227,22 +240,39 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   a.kc = static_cast<const uint8_t*>(k_cache), a.vc = static_cast<const uint8_t*>(v_cache);
   a.ks = k_scale, a.vs = v_scale, a.table = page_table, a.lens = kv_lens, a.prefix = prefix_pages;
   a.out = static_cast<uint16_t*>(out);
-  a.num_pages = num_pages;
+  a.num_pages = (int32_t)num_pages;
   for (int i = 0; i < 3; ++i) a.qs[i] = (int32_t)strides[i];
-  a.S = (int32_t)S, a.Hq = (int32_t)Hq, a.H = (int32_t)H, a.group = (int32_t)(Hq / H);
+  a.B = (int32_t)B, a.S = (int32_t)S, a.Hq = (int32_t)Hq, a.H = (int32_t)H;
+  a.group = (int32_t)(Hq / H);
   a.page_shift = log2_of(page_size), a.width = (int32_t)table_width;
   a.prefix_len = (int32_t)prefix_len;
   const int64_t room = table_width > (max_kv_len >> a.page_shift) ? max_kv_len
                                                                   : table_width << a.page_shift;
   a.most = (int32_t)(room < max_kv_len ? room : max_kv_len);
   a.idx64 = index_dtype == FAGQ_IDX_I64;
-  a.sf = scale_format == FAGQ_SCALE_F32 ? SF_F32 : SF_UE8M0;
-  a.qf = q_format == FAGQ_Q_FP8_E4M3FN ? QF_FP8 : QF_I8_RNE;
   a.scale2 = sm_scale * 1.44269504088896340736f;
+  const Plan p = plan_for(B, S, Hq, H, D, prefix_len, max_kv_len);
+  a.chunk = (int32_t)p.chunk, a.chunks = (int32_t)p.chunks, a.tiles = (int32_t)p.tiles;
+  a.prefix_chunk = (int32_t)p.prefix_chunk, a.prefix_chunks = (int32_t)p.prefix_chunks;
+  a.prefix_tiles = (int32_t)p.prefix_tiles, a.prefix_items = (int32_t)p.prefix_items;
+  const int64_t n = p.chunks + p.prefix_chunks;
+  if (n > 1) {
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = a.part + p.rows * n * D;
+  }
+  // At most kGroups workgroups and one for each unit on either side: below 2^31.
   void* args[] = {&a};
-  return launch_kernel(dtype == FAGQ_DT_BF16 ? kernel_for<ET_BF16>(D) : kernel_for<ET_F16>(D),
-                       dim3((unsigned)(B * S * Hq)), dim3(64 * kWaves), args, 0,
-                       static_cast<hipStream_t>(stream));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int ls = launch_kernel(kernel_for(dtype, q_format, scale_format, (int)D, p),
+                               dim3((unsigned)(p.prefix_items + p.items)), dim3(64 * kWaves), args,
+                               0, st);
+  if (ls != FAGQ_OK || n == 1) return ls;
+  JoinArgs j = {a.part, a.part_ml, kv_lens, a.out, (int32_t)p.rows, a.S, a.Hq, a.prefix_chunks,
+                a.chunks, a.chunk, a.most, a.idx64};
+  void* jargs[] = {&j};
+  return launch_kernel(dtype == FAGQ_DT_BF16 ? join_for<ET_BF16>(D) : join_for<ET_F16>(D),
+                       dim3((unsigned)((p.rows + kWaves - 1) / kWaves)), dim3(64 * kWaves), jargs,
+                       0, st);
 }
 
 }  // extern "C"

@@ -117,8 +117,8 @@ def attention(q, kc, vc, ks, vs, table, lens, sm_scale, prefix_pages=None, prefi
 
     x = q . k errs by (D + 4) U of its terms' magnitudes X (times log2 e and the scales' two
     roundings), which moves a probability by a factor e^(2 X (D + 4) U); probabilities are
-    rounded to q's type (half a step each, and for fp16, whose weights are scaled to the
-    largest value scale, 2^-24 of that); n terms are summed in fp32 (n + 40 U)."""
+    rounded to fp16 times their value scales (half a step each, and 2^-24 of the largest scale);
+    n terms are summed in fp32 (n + 40 U)."""
     B, S, Hq, D = q.shape
     P, H, page, _ = kc.shape
     g = Hq // H
@@ -129,7 +129,7 @@ def attention(q, kc, vc, ks, vs, table, lens, sm_scale, prefix_pages=None, prefi
     most = room if most is None else min(most, room)
     out = torch.zeros(B, S, Hq, D, dtype=torch.float64)
     off = torch.zeros_like(out)
-    half = HALF[q.dtype]
+    half = HALF[torch.float16]
     front = [token_rows(t, prefix_pages.tolist() if prefix_len else [], prefix_len, P)
              for t in (kd, vd, sv)]
     for b in range(B):
@@ -151,8 +151,7 @@ def attention(q, kc, vc, ks, vs, table, lens, sm_scale, prefix_pages=None, prefi
                 spread = 2.0 ** -24 * w[:, h].amax() * (v[:, h].abs() / w[:, h].clamp_min(1e-300)).sum(0)
                 out[b, s, h * g:(h + 1) * g] = o
                 off[b, s, h * g:(h + 1) * g] = mo * (half + 4 * mx * (D + 4) * U
-                                                    + (k.shape[0] + 40) * U) + \
-                    (spread / top if q.dtype == torch.float16 else 0.0)
+                                                    + (k.shape[0] + 40) * U) + spread / top
     return out, off
 
 
