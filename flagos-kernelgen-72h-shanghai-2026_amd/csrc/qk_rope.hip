@@ -10,8 +10,7 @@
 // elements belongs to LPR = D / 16 lanes (a power of two, 4 to 32), 16 elements each in two
 // chunks of 8: for pairs (i, i + R / 2) lane l holds elements 8 l.. and R / 2 + 8 l.., for
 // adjacent pairs 16 l.. and 16 l + 8.., so that both halves of every pair are in one lane
-// and every access is 16 bytes.  A wave walks the heads of one token, 64 / LPR at a time
-// (a "pass"), and holds the token's cos and sin and both weights in registers.
+// and every access is 16 bytes.  A wave takes 64 / LPR heads of one token at a time (a "pass").
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -25,6 +24,8 @@ namespace rope {
 namespace {
 
 constexpr int kWaves = 4;             // waves per workgroup
+constexpr int kBwdAhead = 2;          // passes of a wave of the backward whose loads are under way
+                                      // at once
 constexpr int kMaxBwdGroups = 512;    // workgroups of the backward (two per CU), each with its
                                       // own sums of the weight gradients
 constexpr int kSumRows = 64;          // partial sums that a column's threads share out
@@ -45,8 +46,8 @@ struct Args {
   int64_t table_rows;
   int32_t qs[2], ks[2], qos[2], kos[2], dqs[2], dks[2];   // {token, head} strides, elements
   int32_t T, Hq, Hk, D, R;
-  int32_t splits;    // waves per token
-  int32_t per_wave;  // passes per wave
+  int32_t splits;    // backward: items of a token
+  int32_t per_wave;  // backward: passes of an item
   int32_t idx64;
   float eps;
 };
@@ -86,7 +87,13 @@ __device__ __forceinline__ void unpack8(const Raw8<E>& r, float* f) {
     }
   }
 }
-template <int E>
+// NT: streamed past the caches.
+template <bool NT>
+__device__ __forceinline__ void store_b128(void* p, u32x4 v) {
+  if constexpr (NT) __builtin_nontemporal_store(v, static_cast<u32x4*>(p));
+  else *static_cast<u32x4*>(p) = v;
+}
+template <int E, bool NT>
 __device__ __forceinline__ void store8(typename Elem<E>::type* p, const float* f) {
   if constexpr (E == ET_F32) {
 #pragma unroll
@@ -94,13 +101,13 @@ __device__ __forceinline__ void store8(typename Elem<E>::type* p, const float* f
       u32x4 v;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(f[4 * h + i]);
-      *reinterpret_cast<u32x4*>(p + 4 * h) = v;
+      store_b128<NT>(p + 4 * h, v);
     }
   } else {
     u32x4 v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = pack16<E>(f[2 * i], f[2 * i + 1]);
-    *reinterpret_cast<u32x4*>(p) = v;
+    store_b128<NT>(p, v);
   }
 }
 
@@ -170,8 +177,11 @@ __device__ __forceinline__ void rotate(float (&n)[16], const Turn& t) {
   }
 }
 
-__device__ __forceinline__ float rstd_of(float ss, int D, float eps) {
-  return 1.0f / __builtin_sqrtf(ss / (float)D + eps);
+// 1 / sqrt(v) to an ulp; v_rsq_f32 takes no subnormals.
+__device__ __forceinline__ float rsqrt_of(float v) {
+  const bool tiny = v < 0x1p-100f;
+  const float r = __builtin_amdgcn_rsqf(tiny ? v * 0x1p100f : v);
+  return tiny ? r * 0x1p50f : r;
 }
 
 __device__ __forceinline__ int64_t position(const Args& a, int t) {
@@ -179,55 +189,96 @@ __device__ __forceinline__ int64_t position(const Args& a, int t) {
                  : (int64_t) static_cast<const int32_t*>(a.pos)[t];
 }
 
+// The heads of q or of k, for one wave: where they start and how far apart.
+template <int E>
+struct Heads {
+  using T = typename Elem<E>::type;
+  const T* x;
+  const T* dy;               // backward
+  T* y;                      // forward: result; backward: dx
+  int32_t xh, dyh, yh;       // head strides
+  int32_t H;
+};
+template <int E, bool BWD>
+__device__ __forceinline__ Heads<E> heads_of(const Args& a, bool isq, int t) {
+  using T = typename Elem<E>::type;
+  Heads<E> h;
+  h.x = static_cast<const T*>(isq ? a.q : a.k) + (int64_t)t * (isq ? a.qs[0] : a.ks[0]);
+  h.y = static_cast<T*>(isq ? a.qo : a.ko) + (int64_t)t * (isq ? a.qos[0] : a.kos[0]);
+  h.xh = isq ? a.qs[1] : a.ks[1];
+  h.yh = isq ? a.qos[1] : a.kos[1];
+  h.dy = nullptr;
+  h.dyh = 0;
+  if constexpr (BWD) {
+    h.dy = static_cast<const T*>(isq ? a.dq : a.dk) + (int64_t)t * (isq ? a.dqs[0] : a.dks[0]);
+    h.dyh = isq ? a.dqs[1] : a.dks[1];
+  }
+  h.H = isq ? a.Hq : a.Hk;
+  return h;
+}
+
+// The lane's 16 elements of a row (a weight: the row at p itself).
+template <int E>
+struct Raw16 {
+  Raw8<E> a, b;
+};
+template <int E>
+__device__ __forceinline__ Raw16<E> load16(const typename Elem<E>::type* p, const Lane& l, bool on) {
+  Raw16<E> r = {zero8<E>(), zero8<E>()};
+  if (on) {
+    r.a = load8<E>(p + l.c0);
+    r.b = load8<E>(p + l.c1);
+  }
+  return r;
+}
+template <int E>
+__device__ __forceinline__ void unpack16(const Raw16<E>& r, float (&f)[16]) {
+  unpack8<E>(r.a, f);
+  unpack8<E>(r.b, f + 8);
+}
+template <int E, bool NT>
+__device__ __forceinline__ void store16(typename Elem<E>::type* p, const Lane& l, const float (&f)[16]) {
+  store8<E, NT>(p + l.c0, f);
+  store8<E, NT>(p + l.c1, f + 8);
+}
+
+// One pass for each wave, in the order of memory: waves that walk a token's heads each by
+// themselves spread the loads under way over more of HBM's pages (16384 tokens, 72 heads of 128:
+// 99 us with one pass for each wave, 102 with two, 108 with five, 115 with the whole token).
 template <int E, int LPR, bool INTER>
 __global__ __launch_bounds__(64 * kWaves) void qk_norm_rope_fwd(Args a) {
   using T = typename Elem<E>::type;
   constexpr int kRows = 64 / LPR;
   const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * kWaves + threadIdx.x / 64));
-  const int t = wave / a.splits;
-  if (t >= a.T) return;
-  const Lane l = lane_of<LPR, INTER>(threadIdx.x & 63, a.D, a.R);
   const int pq = (a.Hq + kRows - 1) / kRows, passes = pq + (a.Hk + kRows - 1) / kRows;
-  const int p0 = (wave - t * a.splits) * a.per_wave;
-  const int p1 = p0 + a.per_wave < passes ? p0 + a.per_wave : passes;
+  const int t = wave / passes;
+  if (t >= a.T) return;
+  const int p = wave - t * passes;
+  const bool isq = p < pq;
+  const Lane l = lane_of<LPR, INTER>(threadIdx.x & 63, a.D, a.R);
+  const Heads<E> s = heads_of<E, false>(a, isq, t);
+  const int h = (isq ? p : p - pq) * kRows + l.row;
+  const bool on = l.on && h < s.H;
+  const Raw16<E> raw = load16<E>(s.x + (int64_t)h * s.xh, l, on);
+  const Raw16<E> raw_w = load16<E>(static_cast<const T*>(isq ? a.qw : a.kw), l, on);
   const int64_t pos = position(a, t);
   const bool real = pos >= 0 && pos < a.table_rows;
   const Turn turn = load_turn(a, l, pos, real);
-  for (int p = p0; p < p1; ++p) {
-    const bool isq = p < pq;
-    const int h = (isq ? p : p - pq) * kRows + l.row;
-    const bool on = l.on && h < (isq ? a.Hq : a.Hk);
-    const T* x = static_cast<const T*>(isq ? a.q : a.k) +
-                 ((int64_t)t * (isq ? a.qs[0] : a.ks[0]) + (int64_t)h * (isq ? a.qs[1] : a.ks[1]));
-    T* y = static_cast<T*>(isq ? a.qo : a.ko) +
-           ((int64_t)t * (isq ? a.qos[0] : a.kos[0]) + (int64_t)h * (isq ? a.qos[1] : a.kos[1]));
-    const T* w = static_cast<const T*>(isq ? a.qw : a.kw);
-    Raw8<E> x0 = zero8<E>(), x1 = zero8<E>(), w0 = zero8<E>(), w1 = zero8<E>();
-    if (on) {
-      x0 = load8<E>(x + l.c0);
-      x1 = load8<E>(x + l.c1);
-      w0 = load8<E>(w + l.c0);
-      w1 = load8<E>(w + l.c1);
-    }
-    float n[16], g[16];
-    unpack8<E>(x0, n);
-    unpack8<E>(x1, n + 8);
-    unpack8<E>(w0, g);
-    unpack8<E>(w1, g + 8);
-    float ss = 0.0f;
+  float n[16], g[16];
+  unpack16<E>(raw, n);
+  unpack16<E>(raw_w, g);
+  float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) ss = __builtin_fmaf(n[i], n[i], ss);
-    const float rstd = rstd_of(row_sum<LPR>(ss), a.D, a.eps);
+  for (int i = 0; i < 16; ++i) ss = __builtin_fmaf(n[i], n[i], ss);
+  const float rstd = rsqrt_of(row_sum<LPR>(ss) / (float)a.D + a.eps);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) n[i] = n[i] * rstd * g[i];
-    rotate<INTER, false>(n, turn);
+  for (int i = 0; i < 16; ++i) n[i] = n[i] * rstd * g[i];
+  rotate<INTER, false>(n, turn);
+  if (!real) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) n[i] = real ? n[i] : 0.0f;
-    if (on) {
-      store8<E>(y + l.c0, n);
-      store8<E>(y + l.c1, n + 8);
-    }
+    for (int i = 0; i < 16; ++i) n[i] = 0.0f;
   }
+  if (on) store16<E, true>(s.y + (int64_t)h * s.yh, l, n);
 }
 
 template <int E, int LPR, bool INTER>
@@ -240,65 +291,63 @@ __global__ __launch_bounds__(64 * kWaves) void qk_norm_rope_bwd(Args a) {
   const int waves = gridDim.x * kWaves;
   const Lane l = lane_of<LPR, INTER>(threadIdx.x & 63, a.D, a.R);
   const int pq = (a.Hq + kRows - 1) / kRows, passes = pq + (a.Hk + kRows - 1) / kRows;
+  const Raw16<E> raw_w[2] = {load16<E>(static_cast<const T*>(a.qw), l, l.on),
+                             load16<E>(static_cast<const T*>(a.kw), l, l.on)};
+  const float inv_d = 1.0f / (float)a.D;
   float dw[2][16] = {};                         // of q's and k's weight
-  for (int64_t item = wave; item < (int64_t)a.T * a.splits; item += waves) {
-    const int t = (int)(item / a.splits);
-    const int p0 = (int)(item - (int64_t)t * a.splits) * a.per_wave;
+  for (int item = wave; item < a.T * a.splits; item += waves) {
+    const int t = item / a.splits;
+    const int p0 = (item - t * a.splits) * a.per_wave;
     const int p1 = p0 + a.per_wave < passes ? p0 + a.per_wave : passes;
     const int64_t pos = position(a, t);
     const bool real = pos >= 0 && pos < a.table_rows;
     const Turn turn = load_turn(a, l, pos, real);
-    auto pass = [&](int p, bool isq, float (&acc)[16]) {
-      const int h = (isq ? p : p - pq) * kRows + l.row;
-      const bool on = l.on && h < (isq ? a.Hq : a.Hk);
-      const int64_t st = isq ? a.qs[0] : a.ks[0], sh = isq ? a.qs[1] : a.ks[1];
-      const int64_t dt = isq ? a.dqs[0] : a.dks[0], dh = isq ? a.dqs[1] : a.dks[1];
-      const int64_t ot = isq ? a.qos[0] : a.kos[0], oh = isq ? a.qos[1] : a.kos[1];
-      const T* x = static_cast<const T*>(isq ? a.q : a.k) + (t * st + h * sh);
-      const T* dy = static_cast<const T*>(isq ? a.dq : a.dk) + (t * dt + h * dh);
-      T* dx = static_cast<T*>(isq ? a.qo : a.ko) + (t * ot + h * oh);
-      const T* w = static_cast<const T*>(isq ? a.qw : a.kw);
-      Raw8<E> x0 = zero8<E>(), x1 = zero8<E>(), w0 = zero8<E>(), w1 = zero8<E>();
-      Raw8<E> d0 = zero8<E>(), d1 = zero8<E>();
-      if (on) {
-        x0 = load8<E>(x + l.c0);
-        x1 = load8<E>(x + l.c1);
-        d0 = load8<E>(dy + l.c0);
-        d1 = load8<E>(dy + l.c1);
-        w0 = load8<E>(w + l.c0);
-        w1 = load8<E>(w + l.c1);
-      }
-      float n[16], d[16], g[16];
-      unpack8<E>(x0, n);
-      unpack8<E>(x1, n + 8);
-      unpack8<E>(d0, d);
-      unpack8<E>(d1, d + 8);
-      unpack8<E>(w0, g);
-      unpack8<E>(w1, g + 8);
-      rotate<INTER, true>(d, turn);
-      float ss = 0.0f, ax = 0.0f;
+    auto run = [&](const Heads<E>& s, const Raw16<E>& weight, float (&acc)[16], int first, int last) {
+      for (int p = first; p < last; p += kBwdAhead) {
+        Raw16<E> raw[kBwdAhead], raw_d[kBwdAhead];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        ss = __builtin_fmaf(n[i], n[i], ss);
-        ax = __builtin_fmaf(d[i] * g[i], n[i], ax);
-      }
-      const float rstd = rstd_of(row_sum<LPR>(ss), a.D, a.eps);
-      const float back = row_sum<LPR>(ax) / (float)a.D * rstd * rstd;
+        for (int u = 0; u < kBwdAhead; ++u) {
+          const int h = (p + u) * kRows + l.row;
+          const bool on = l.on && p + u < last && h < s.H;
+          raw[u] = load16<E>(s.x + (int64_t)h * s.xh, l, on);
+          raw_d[u] = load16<E>(s.dy + (int64_t)h * s.dyh, l, on);
+        }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        // Rows past the last head hold zeros and add nothing; padding adds nothing either.
-        const float gx = d[i] * (n[i] * rstd);
-        acc[i] += real && on ? gx : 0.0f;
-        n[i] = real ? rstd * __builtin_fmaf(-n[i], back, d[i] * g[i]) : 0.0f;
-      }
-      if (on) {
-        store8<E>(dx + l.c0, n);
-        store8<E>(dx + l.c1, n + 8);
+        for (int u = 0; u < kBwdAhead; ++u) {
+          if (p + u >= last) break;
+          const int h = (p + u) * kRows + l.row;
+          float n[16], d[16], g[16];
+          unpack16<E>(raw[u], n);
+          unpack16<E>(raw_d[u], d);
+          unpack16<E>(weight, g);
+          rotate<INTER, true>(d, turn);
+          float ss = 0.0f, ax = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            ss = __builtin_fmaf(n[i], n[i], ss);
+            ax = __builtin_fmaf(d[i] * g[i], n[i], ax);
+          }
+          const float rstd = rsqrt_of(row_sum<LPR>(ss) * inv_d + a.eps);
+          const float back = row_sum<LPR>(ax) * inv_d * rstd * rstd;
+          if (real) {
+            // Rows past the last head hold zeros: they add nothing, or 0 * inf where eps is 0.
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float gx = d[i] * (n[i] * rstd);
+              acc[i] += h < s.H ? gx : 0.0f;
+              n[i] = rstd * __builtin_fmaf(-n[i], back, d[i] * g[i]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) n[i] = 0.0f;
+          }
+          if (l.on && h < s.H) store16<E, false>(s.y + (int64_t)h * s.yh, l, n);
+        }
       }
     };
-    int p = p0;
-    for (; p < p1 && p < pq; ++p) pass(p, true, dw[0]);
-    for (; p < p1; ++p) pass(p, false, dw[1]);
+    if (p0 < pq) run(heads_of<E, true>(a, true, t), raw_w[0], dw[0], p0, p1 < pq ? p1 : pq);
+    if (p1 > pq)
+      run(heads_of<E, true>(a, false, t), raw_w[1], dw[1], p0 > pq ? p0 - pq : 0, p1 - pq);
   }
 #pragma unroll
   for (int o = 0; o < 2; ++o)
@@ -427,16 +476,19 @@ const void* kernel_for(int dtype, int lpr, bool inter, bool bwd) {
                                 : kernel_for<ET_F32>(lpr, inter, bwd);
 }
 
-// How the heads of a token are shared out over waves.
+int64_t passes_of(int64_t Hq, int64_t Hk, int64_t D) {
+  const int64_t rows = 64 / lanes_per_row(D);
+  return (Hq + rows - 1) / rows + (Hk + rows - 1) / rows;
+}
+
+// How the backward shares the passes of a token out over waves: kBwdAhead at a time, one where
+// that leaves waves without work (two on each of the SIMDs of 256 CUs).
 struct Split {
   int64_t splits, per_wave;
 };
 Split split_for(int64_t T, int64_t Hq, int64_t Hk, int64_t D) {
-  const int64_t rows = 64 / lanes_per_row(D);
-  const int64_t passes = (Hq + rows - 1) / rows + (Hk + rows - 1) / rows;
-  // A wave takes a whole token where that fills the GPU (8 waves on each of 256 CUs, twice).
-  int64_t per = passes * T / 4096;
-  per = per < 1 ? 1 : per > passes ? passes : per;
+  const int64_t passes = passes_of(Hq, Hk, D);
+  const int64_t per = passes * T >= 2 * 4 * 256 * kBwdAhead ? kBwdAhead : 1;
   return {(passes + per - 1) / per, per};
 }
 
@@ -508,18 +560,16 @@ FAGQ_API int fagq_qk_norm_rope_launch(const void* q, const void* k, const void* 
   }
   const int dcheck = device_check();
   if (dcheck != FAGQ_OK) return dcheck;
-  const Split s = split_for(T, Hq, Hk, D);
   Args a = {};
   a.q = q, a.k = k, a.qw = q_weight, a.kw = k_weight, a.cos = cos, a.sin = sin, a.pos = positions;
   a.qo = q_out, a.ko = k_out, a.table_rows = table_rows;
   set_strides(a.qs, strides), set_strides(a.ks, strides + 2);
   set_strides(a.qos, strides + 4), set_strides(a.kos, strides + 6);
   a.T = (int32_t)T, a.Hq = (int32_t)Hq, a.Hk = (int32_t)Hk, a.D = (int32_t)D, a.R = (int32_t)R;
-  a.splits = (int32_t)s.splits, a.per_wave = (int32_t)s.per_wave;
   a.idx64 = index_dtype == FAGQ_IDX_I64, a.eps = eps;
   void* args[] = {&a};
-  // T * splits < 2^24 * 2 when a token is split (T < 4096 then), so the grid stays below 2^31.
-  const int64_t groups = (T * s.splits + kWaves - 1) / kWaves;
+  const int64_t groups = (T * passes_of(Hq, Hk, D) + kWaves - 1) / kWaves;
+  if (groups >= (1ll << 32) / (64 * kWaves)) return FAGQ_E_TOO_LARGE;
   return launch_kernel(kernel_for(dtype, lanes_per_row(D), interleaved != 0, false),
                        dim3((unsigned)groups), dim3(64 * kWaves), args, 0,
                        static_cast<hipStream_t>(stream));
@@ -585,6 +635,7 @@ FAGQ_API int fagq_qk_norm_rope_bwd_launch(const void* dq_out, const void* dk_out
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (groups > 0) {
     const Split s = split_for(T, Hq, Hk, D);
+    if (T * s.splits >= (1ll << 31) - kWaves * kMaxBwdGroups) return FAGQ_E_TOO_LARGE;
     Args a = {};
     a.q = q, a.k = k, a.qw = q_weight, a.kw = k_weight, a.cos = cos, a.sin = sin;
     a.pos = positions, a.qo = dq, a.ko = dk, a.dq = dq_out, a.dk = dk_out;

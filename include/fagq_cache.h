@@ -39,7 +39,7 @@ extern "C" {
  *   s = max(max|x| * fp32(1 / QMAX), 1e-12),   code = encode(x * (1 / s))
  * UE8M0: s = 2^ceil(log2 s), code = encode(x / s).  fp8 (QMAX 448) and int8
  * (QMAX 127) round to nearest even.  Values are finite.
- * G in {64, 128, 256}, D % G == 0, D <= FAGQ_CACHE_MAX_D; T * H * D < 2^34.
+ * G in {64, 128, 256}, D % G == 0, D <= FAGQ_CACHE_MAX_D; T <= 2^24.
  * k, v 16-byte aligned, strides multiples of 16 bytes. */
 FAGQ_API int fagq_kv_cache_write_launch(const void* k, const void* v, const void* slots,
                                         void* k_cache, void* v_cache, void* k_scale,
@@ -54,7 +54,8 @@ FAGQ_API int fagq_kv_cache_write_launch(const void* k, const void* v, const void
  * code * scale in fp32, rounded once.  page_table int32 [B, table_width],
  * cu_seqlens int32 [B + 1], ascending from 0.  Tokens whose page lies outside the
  * table or the cache (-1: none) become zeros.  Rows behind cu_seqlens[B] are left
- * as they were; rows <= 2^31 - 1. */
+ * as they were.  rows <= 2^31 - 1, and FAGQ_E_TOO_LARGE where 2^24 workgroups do
+ * not cover them. */
 FAGQ_API int fagq_kv_cache_read_launch(const void* k_cache, const void* v_cache,
                                        const void* k_scale, const void* v_scale,
                                        const int32_t* page_table, const int32_t* cu_seqlens,

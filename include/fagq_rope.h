@@ -42,7 +42,7 @@ enum fagq_index { FAGQ_IDX_I32 = 0, FAGQ_IDX_I64 = 1 };
  * All pointers but positions 16-byte aligned, strides multiples of 16 bytes and
  * below 2^31 elements.  16 <= R <= D <= FAGQ_ROPE_MAX_D, D % 16 == 0, R % 16 == 0.
  * q_out may be q itself, and k_out k (same pointer and strides); outputs overlap
- * nothing else. */
+ * nothing else.  FAGQ_E_TOO_LARGE where 2^24 workgroups do not cover the heads. */
 FAGQ_API int fagq_qk_norm_rope_launch(const void* q, const void* k, const void* q_weight,
                                       const void* k_weight, const float* cos, const float* sin,
                                       const void* positions, void* q_out, void* k_out,

@@ -125,7 +125,7 @@ def write(lib, **kw):
     (dict(dt=3), 5), (dict(qf=2), 5), (dict(sf=2), 5), (dict(idx=2), 5),
     (dict(G=32), 3), (dict(G=512), 3), (dict(G=256), 2), (dict(H=0), 2), (dict(D=0), 2),
     (dict(page=8), 2), (dict(page=24), 2), (dict(page=131072), 7), (dict(P=-1), 2),
-    (dict(P=1 << 31), 7), (dict(D=2048), 7), (dict(T=-1), 2), (dict(T=1 << 24, D=1024), 7),
+    (dict(P=1 << 31), 7), (dict(D=2048), 7), (dict(T=-1), 2), (dict(T=(1 << 24) + 1), 7),
     (dict(st=(1028, 128, 1024, 128)), 4), (dict(st=(1024, 128, 1024, -8)), 2),
     (dict(st=(1 << 31, 128, 1024, 128)), 7), (dict(k=fake(0, 8)), 4), (dict(kc=fake(3, 8)), 4),
     (dict(ks=fake(5, 2)), 4), (dict(slots=fake(2, 4)), 4), (dict(kc=fake(0)), 9),
