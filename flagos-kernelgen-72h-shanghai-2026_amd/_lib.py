@@ -181,6 +181,14 @@ def fast_launch():
                                     (lib.fagq_launch_parts, lib.fagq_gemm_launch,
                                      lib.fagq_dsa_topk_launch, lib.fagq_mla_bwd_workspace_bytes,
                                      lib.fagq_mla_bwd_launch)])
+                _fagq_py.bind_attention(*[ctypes.cast(fn, ctypes.c_void_p).value for fn in
+                                          (lib.fagq_qk_norm_rope_launch,
+                                           lib.fagq_qk_norm_rope_bwd_workspace_bytes,
+                                           lib.fagq_qk_norm_rope_bwd_launch,
+                                           lib.fagq_kv_cache_write_launch,
+                                           lib.fagq_kv_cache_read_launch,
+                                           lib.fagq_paged_attention_workspace_bytes,
+                                           lib.fagq_paged_attention_launch)])
                 _fast = _fagq_py.launch
                 _fast_mod = _fagq_py
             except (ImportError, AttributeError):

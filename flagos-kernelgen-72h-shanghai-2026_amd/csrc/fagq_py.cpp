@@ -21,6 +21,8 @@
 //     (dsa and mla: 0), the library's status as an int where it is an error, or
 //     kArgError for any argument that the Python layer should look at: it then takes
 //     the call from the start, with the same results and its own wording of the errors.
+//   rope(...), rope_bwd(...), cache_write(...), cache_read(...), attention(...): the
+//     attention side, by the same rules.
 //     Nothing is allocated or launched before all arguments are accepted.  The
 //     allocations (which may reach hipMalloc, or wait for the device to free cached
 //     blocks) and the launch run without the GIL, as torch's and ctypes' own calls do.
@@ -38,9 +40,11 @@
 #include <vector>
 
 #include "fagq.h"
+#include "fagq_cache.h"
 #include "fagq_dsa.h"
 #include "fagq_gemm.h"
 #include "fagq_mla.h"
+#include "fagq_rope.h"
 
 namespace {
 
@@ -58,6 +62,13 @@ decltype(&fagq_gemm_launch) g_gemm = nullptr;
 decltype(&fagq_dsa_topk_launch) g_dsa = nullptr;
 decltype(&fagq_mla_bwd_workspace_bytes) g_mla_bytes = nullptr;
 decltype(&fagq_mla_bwd_launch) g_mla = nullptr;
+decltype(&fagq_qk_norm_rope_launch) g_rope = nullptr;
+decltype(&fagq_qk_norm_rope_bwd_workspace_bytes) g_rope_bytes = nullptr;
+decltype(&fagq_qk_norm_rope_bwd_launch) g_rope_bwd = nullptr;
+decltype(&fagq_kv_cache_write_launch) g_cache_write = nullptr;
+decltype(&fagq_kv_cache_read_launch) g_cache_read = nullptr;
+decltype(&fagq_paged_attention_workspace_bytes) g_attention_bytes = nullptr;
+decltype(&fagq_paged_attention_launch) g_attention = nullptr;
 
 bool is_tensor(PyObject* o) { return THPVariable_Check(o); }
 
@@ -493,6 +504,388 @@ PyObject* mla(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------ the attention side
+
+// A [T, H, D] tensor with contiguous rows; its token and head strides (0 where a dimension has
+// one element, which is never stepped over).
+bool heads_ok(const at::Tensor& t, at::IntArrayRef shape, c10::DeviceIndex dev, at::ScalarType st,
+              int64_t* strides) {
+  if (t.scalar_type() != st || t.sizes() != shape || !t.is_cuda() || t.get_device() != dev ||
+      t.stride(2) != 1)
+    return false;
+  for (int i = 0; i < 2; ++i) strides[i] = t.size(i) > 1 ? t.stride(i) : 0;
+  return true;
+}
+
+int index_code(at::ScalarType st) {
+  return st == at::kInt ? FAGQ_IDX_I32 : st == at::kLong ? FAGQ_IDX_I64 : -1;
+}
+
+bool bool_arg(PyObject* o, int* out) {
+  if (!PyBool_Check(o)) return false;
+  *out = o == Py_True;
+  return true;
+}
+
+PyObject* tuple_of(const at::Tensor* v, int n) {
+  PyObject* t = PyTuple_New(n);
+  if (!t) return nullptr;
+  for (int i = 0; i < n; ++i) {
+    PyObject* o = THPVariable_Wrap(v[i]);
+    if (!o) {
+      Py_DECREF(t);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(t, i, o);
+  }
+  return t;
+}
+
+// What both directions of the rotation take: q, k, q_weight, k_weight, cos, sin, positions, eps,
+// interleaved at args[0..8].
+struct RopeIn {
+  const at::Tensor* t[7];
+  int64_t T, Hq, Hk, D, R, table, strides[4];
+  double eps;
+  int interleaved, dtype, index;
+  c10::DeviceIndex dev;
+};
+bool rope_in(PyObject* const* args, RopeIn* r) {
+  for (int i = 0; i < 7; ++i) {
+    if (!is_plain(args[i])) return false;
+    r->t[i] = &THPVariable_Unpack(args[i]);
+  }
+  const at::Tensor &q = *r->t[0], &k = *r->t[1], &cos = *r->t[4], &pos = *r->t[6];
+  if (q.dim() != 3 || k.dim() != 3 || cos.dim() != 2 || !q.is_cuda() ||
+      !float_arg(args[7], &r->eps) || !bool_arg(args[8], &r->interleaved))
+    return false;
+  const at::ScalarType st = q.scalar_type();
+  r->dev = q.get_device();
+  r->T = q.size(0), r->Hq = q.size(1), r->Hk = k.size(1), r->D = q.size(2);
+  r->table = cos.size(0), r->R = 2 * cos.size(1);
+  r->dtype = dtype_code(st), r->index = index_code(pos.scalar_type());
+  const int64_t qs[3] = {r->T, r->Hq, r->D}, ks[3] = {r->T, r->Hk, r->D}, ws[1] = {r->D};
+  const int64_t ps[1] = {r->T};
+  return r->T > 0 && r->Hq > 0 && r->Hk > 0 && r->dtype >= 0 && r->index >= 0 && r->D % 16 == 0 &&
+         r->D >= 16 && r->D <= FAGQ_ROPE_MAX_D && r->R % 16 == 0 && r->R >= 16 && r->R <= r->D &&
+         heads_ok(q, qs, r->dev, st, r->strides) && heads_ok(k, ks, r->dev, st, r->strides + 2) &&
+         rows_ok(*r->t[2], ws, r->dev, st) && rows_ok(*r->t[3], ws, r->dev, st) &&
+         rows_ok(cos, cos.sizes(), r->dev, at::kFloat) &&
+         rows_ok(*r->t[5], cos.sizes(), r->dev, at::kFloat) &&
+         rows_ok(pos, ps, r->dev, pos.scalar_type());
+}
+
+// rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, q_out or None,
+//      k_out or None, stream) -> (q_out, k_out)
+PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 12) {
+    PyErr_SetString(PyExc_TypeError, "rope() takes 12 arguments");
+    return nullptr;
+  }
+  RopeIn r;
+  void* stream;
+  if (!g_rope || !stream_arg(args[11], &stream) || !rope_in(args, &r)) return arg_error();
+  const int64_t qs[3] = {r.T, r.Hq, r.D}, ks[3] = {r.T, r.Hk, r.D};
+  int64_t strides[8] = {r.strides[0], r.strides[1], r.strides[2], r.strides[3],
+                        r.Hq * r.D, r.D, r.Hk * r.D, r.D};
+  at::Tensor out[2];
+  for (int i = 0; i < 2; ++i) {
+    if (args[9 + i] == Py_None) continue;
+    if (!is_plain(args[9 + i])) return arg_error();
+    out[i] = THPVariable_Unpack(args[9 + i]);
+    if (!heads_ok(out[i], i ? ks : qs, r.dev, r.t[0]->scalar_type(), strides + 4 + 2 * i))
+      return arg_error();
+  }
+  const void* p[7];
+  for (int i = 0; i < 7; ++i) p[i] = r.t[i]->data_ptr();
+  const auto options = r.t[0]->options();
+  int st;
+  {
+    NoGil no_gil;
+    if (!out[0].defined()) out[0] = at::empty(qs, options);
+    if (!out[1].defined()) out[1] = at::empty(ks, options);
+    st = g_rope(p[0], p[1], p[2], p[3], static_cast<const float*>(p[4]),
+                static_cast<const float*>(p[5]), p[6], out[0].data_ptr(), out[1].data_ptr(),
+                strides, r.T, r.Hq, r.Hk, r.D, r.R, r.table, (float)r.eps, r.interleaved, r.dtype,
+                r.index, stream);
+  }
+  if (st != FAGQ_OK) return PyLong_FromLong(st);
+  return tuple_of(out, 2);
+  END_HANDLE_TH_ERRORS
+}
+
+// rope_bwd(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, dq_out, dk_out,
+//          dq or None, dk or None, stream) -> (dq, dk, dq_weight, dk_weight); the workspace is
+// allocated here.
+PyObject* rope_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 14) {
+    PyErr_SetString(PyExc_TypeError, "rope_bwd() takes 14 arguments");
+    return nullptr;
+  }
+  RopeIn r;
+  void* stream;
+  if (!g_rope_bwd || !g_rope_bytes || !stream_arg(args[13], &stream) || !is_plain(args[9]) ||
+      !is_plain(args[10]) || !rope_in(args, &r))
+    return arg_error();
+  const int64_t shape[2][3] = {{r.T, r.Hq, r.D}, {r.T, r.Hk, r.D}};
+  const at::ScalarType type = r.t[0]->scalar_type();
+  int64_t strides[12] = {0, 0, 0, 0, r.strides[0], r.strides[1], r.strides[2], r.strides[3],
+                         r.Hq * r.D, r.D, r.Hk * r.D, r.D};
+  const at::Tensor* dy[2] = {&THPVariable_Unpack(args[9]), &THPVariable_Unpack(args[10])};
+  at::Tensor out[4];
+  for (int i = 0; i < 2; ++i) {
+    if (!heads_ok(*dy[i], shape[i], r.dev, type, strides + 2 * i)) return arg_error();
+    if (args[11 + i] == Py_None) continue;
+    if (!is_plain(args[11 + i])) return arg_error();
+    out[i] = THPVariable_Unpack(args[11 + i]);
+    if (!heads_ok(out[i], shape[i], r.dev, type, strides + 8 + 2 * i)) return arg_error();
+  }
+  const int64_t need = g_rope_bytes(r.T, r.Hq, r.Hk, r.D);
+  if (need < 0) return arg_error();
+  const void* p[9];
+  for (int i = 0; i < 7; ++i) p[i] = r.t[i]->data_ptr();
+  p[7] = dy[0]->data_ptr(), p[8] = dy[1]->data_ptr();
+  const auto options = r.t[0]->options();
+  int st;
+  {
+    NoGil no_gil;
+    for (int i = 0; i < 2; ++i) {
+      if (!out[i].defined()) out[i] = at::empty(shape[i], options);
+      out[2 + i] = at::empty({r.D}, options.dtype(at::kFloat));
+    }
+    const at::Tensor ws = at::empty({std::max<int64_t>(need, 16)}, options.dtype(at::kByte));
+    st = g_rope_bwd(p[7], p[8], p[0], p[1], p[2], p[3], static_cast<const float*>(p[4]),
+                    static_cast<const float*>(p[5]), p[6], out[0].data_ptr(), out[1].data_ptr(),
+                    out[2].data_ptr<float>(), out[3].data_ptr<float>(), ws.data_ptr(), ws.numel(),
+                    strides, r.T, r.Hq, r.Hk, r.D, r.R, r.table, (float)r.eps, r.interleaved,
+                    r.dtype, r.index, stream);
+  }
+  if (st != FAGQ_OK) return PyLong_FromLong(st);
+  return tuple_of(out, 4);
+  END_HANDLE_TH_ERRORS
+}
+
+// A cache's tensors (v's may be None, together): k_cache, v_cache, k_scale, v_scale.
+struct Cache {
+  const at::Tensor* t[4];     // null where None
+  int64_t P, H, page, D, G;
+  int codes, scales;
+  c10::DeviceIndex dev;
+};
+bool cache_in(PyObject* kc, PyObject* vc, PyObject* ks, PyObject* vs, Cache* c) {
+  PyObject* o[4] = {kc, vc, ks, vs};
+  for (int i = 0; i < 4; ++i) {
+    c->t[i] = nullptr;
+    if (o[i] == Py_None && (i & 1)) continue;
+    if (!is_plain(o[i])) return false;
+    c->t[i] = &THPVariable_Unpack(o[i]);
+  }
+  if ((c->t[1] == nullptr) != (c->t[3] == nullptr)) return false;
+  const at::Tensor &codes = *c->t[0], &scales = *c->t[2];
+  if (codes.dim() != 4 || scales.dim() != 4 || !codes.is_cuda()) return false;
+  c->dev = codes.get_device();
+  c->P = codes.size(0), c->H = codes.size(1), c->page = codes.size(2), c->D = codes.size(3);
+  const int64_t groups = scales.size(2);
+  if (c->P < 1 || c->H < 1 || groups < 1 || c->D % groups != 0 || c->D > FAGQ_CACHE_MAX_D ||
+      c->page < FAGQ_CACHE_MIN_PAGE || c->page > FAGQ_CACHE_MAX_PAGE || (c->page & (c->page - 1)))
+    return false;
+  c->G = c->D / groups;
+  const at::ScalarType ct = codes.scalar_type(), st = scales.scalar_type();
+  c->codes = ct == at::kFloat8_e4m3fn ? FAGQ_Q_FP8_E4M3FN : ct == at::kChar ? FAGQ_Q_INT8 : -1;
+  c->scales = st == at::kFloat ? FAGQ_SCALE_F32 : st == at::kByte ? FAGQ_SCALE_UE8M0 : -1;
+  if (c->codes < 0 || c->scales < 0 || (c->G != 64 && c->G != 128 && c->G != 256)) return false;
+  const int64_t cs[4] = {c->P, c->H, c->page, c->D}, ss[4] = {c->P, c->H, groups, c->page};
+  for (int i = 0; i < 4; ++i)
+    if (c->t[i] && !rows_ok(*c->t[i], i < 2 ? cs : ss, c->dev, i < 2 ? ct : st)) return false;
+  return true;
+}
+void* data_or_null(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+
+// cache_write(k, v or None, slots, k_cache, v_cache or None, k_scale, v_scale or None, stream)
+// -> status
+PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 8) {
+    PyErr_SetString(PyExc_TypeError, "cache_write() takes 8 arguments");
+    return nullptr;
+  }
+  Cache c;
+  void* stream;
+  const bool has_v = args[1] != Py_None;
+  if (!g_cache_write || !stream_arg(args[7], &stream) || !is_plain(args[0]) || !is_plain(args[2]) ||
+      (has_v && !is_plain(args[1])) || !cache_in(args[3], args[4], args[5], args[6], &c) ||
+      has_v != (c.t[1] != nullptr))
+    return arg_error();
+  const at::Tensor &k = THPVariable_Unpack(args[0]), &slots = THPVariable_Unpack(args[2]);
+  const at::Tensor* v = has_v ? &THPVariable_Unpack(args[1]) : nullptr;
+  if (k.dim() != 3 || k.size(0) < 1) return arg_error();
+  const int64_t T = k.size(0), xs[3] = {T, c.H, c.D}, ss[1] = {T};
+  const at::ScalarType type = k.scalar_type();
+  const int dtype = dtype_code(type), index = index_code(slots.scalar_type());
+  int64_t strides[4] = {};
+  if (dtype < 0 || index < 0 || !heads_ok(k, xs, c.dev, type, strides) ||
+      (v && !heads_ok(*v, xs, c.dev, type, strides + 2)) ||
+      !rows_ok(slots, ss, c.dev, slots.scalar_type()))
+    return arg_error();
+  void* p[7] = {k.data_ptr(), data_or_null(v), slots.data_ptr(), c.t[0]->data_ptr(),
+                data_or_null(c.t[1]), c.t[2]->data_ptr(), data_or_null(c.t[3])};
+  int st;
+  {
+    NoGil no_gil;
+    st = g_cache_write(p[0], p[1], p[2], p[3], p[4], p[5], p[6], strides, T, c.H, c.D, c.G, c.P,
+                       c.page, dtype, c.codes, c.scales, index, stream);
+  }
+  return PyLong_FromLong(st);
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_read(k_cache, v_cache or None, k_scale, v_scale or None, page_table, cu_seqlens, k_out,
+//            v_out or None, stream) -> status
+PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 9) {
+    PyErr_SetString(PyExc_TypeError, "cache_read() takes 9 arguments");
+    return nullptr;
+  }
+  Cache c;
+  void* stream;
+  const bool has_v = args[7] != Py_None;
+  if (!g_cache_read || !stream_arg(args[8], &stream) || !is_plain(args[4]) || !is_plain(args[5]) ||
+      !is_plain(args[6]) || (has_v && !is_plain(args[7])) ||
+      !cache_in(args[0], args[1], args[2], args[3], &c) || has_v != (c.t[1] != nullptr))
+    return arg_error();
+  const at::Tensor &table = THPVariable_Unpack(args[4]), &cu = THPVariable_Unpack(args[5]);
+  const at::Tensor& ko = THPVariable_Unpack(args[6]);
+  const at::Tensor* vo = has_v ? &THPVariable_Unpack(args[7]) : nullptr;
+  if (table.dim() != 2 || ko.dim() != 3) return arg_error();
+  const int64_t B = table.size(0), width = table.size(1), rows = ko.size(0);
+  const int64_t os[3] = {rows, c.H, c.D}, cs[1] = {B + 1};
+  const at::ScalarType type = ko.scalar_type();
+  const int dtype = dtype_code(type);
+  if (B < 1 || width < 1 || rows < 1 || dtype < 0 || !rows_ok(table, table.sizes(), c.dev, at::kInt) ||
+      !rows_ok(cu, cs, c.dev, at::kInt) || !rows_ok(ko, os, c.dev, type) ||
+      (vo && !rows_ok(*vo, os, c.dev, type)))
+    return arg_error();
+  void* p[8] = {c.t[0]->data_ptr(), data_or_null(c.t[1]), c.t[2]->data_ptr(), data_or_null(c.t[3]),
+                table.data_ptr(), cu.data_ptr(), ko.data_ptr(), data_or_null(vo)};
+  int st;
+  {
+    NoGil no_gil;
+    st = g_cache_read(p[0], p[1], p[2], p[3], static_cast<const int32_t*>(p[4]),
+                      static_cast<const int32_t*>(p[5]), p[6], p[7], B, rows, c.H, c.D, c.G, c.P,
+                      c.page, width, dtype, c.codes, c.scales, stream);
+  }
+  return PyLong_FromLong(st);
+  END_HANDLE_TH_ERRORS
+}
+
+// attention(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, sm_scale,
+//           prefix_pages or None, prefix_len, max_kv_len or None, out or None, stream) -> out;
+// the workspace is allocated here.
+PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 13) {
+    PyErr_SetString(PyExc_TypeError, "attention() takes 13 arguments");
+    return nullptr;
+  }
+  Cache c;
+  void* stream;
+  double scale;
+  long long prefix_len, most = 0;
+  if (!g_attention || !g_attention_bytes || !stream_arg(args[12], &stream) || !is_plain(args[0]) ||
+      !is_plain(args[5]) || !is_plain(args[6]) || !float_arg(args[7], &scale) ||
+      !int_arg(args[9], 0, 1 << 30, &prefix_len) ||
+      (args[10] != Py_None && !int_arg(args[10], 0, INT64_MAX, &most)) ||
+      !cache_in(args[1], args[2], args[3], args[4], &c) || !c.t[1])
+    return arg_error();
+  const at::Tensor &q = THPVariable_Unpack(args[0]), &table = THPVariable_Unpack(args[5]);
+  const at::Tensor& lens = THPVariable_Unpack(args[6]);
+  const at::ScalarType type = q.scalar_type();
+  const int dtype = type == at::kBFloat16 ? FAGQ_DT_BF16 : type == at::kHalf ? FAGQ_DT_F16 : -1;
+  const int index = index_code(lens.scalar_type());
+  if (dtype < 0 || index < 0 || c.G != c.D || q.dim() != 4 || table.dim() != 2) return arg_error();
+  const int64_t B = q.size(0), S = q.size(1), Hq = q.size(2), width = table.size(1);
+  const int64_t ts[2] = {B, width}, ls[1] = {B};
+  if (B < 1 || S < 1 || Hq < 1 || Hq % c.H != 0 || q.size(3) != c.D || q.stride(3) != 1 ||
+      !q.is_cuda() || q.get_device() != c.dev || !rows_ok(table, ts, c.dev, at::kInt) ||
+      !rows_ok(lens, ls, c.dev, lens.scalar_type()))
+    return arg_error();
+  const int32_t* prefix = nullptr;
+  if (prefix_len > 0) {
+    if (!is_plain(args[8])) return arg_error();
+    const at::Tensor& t = THPVariable_Unpack(args[8]);
+    if (t.dim() != 1 || t.size(0) < (prefix_len + c.page - 1) / c.page ||
+        !rows_ok(t, t.sizes(), c.dev, at::kInt))
+      return arg_error();
+    prefix = t.data_ptr<int32_t>();
+  }
+  const int64_t room = width * c.page;
+  if (args[10] == Py_None || most > room) most = room;
+  at::Tensor out;
+  if (args[11] != Py_None) {
+    if (!is_plain(args[11])) return arg_error();
+    out = THPVariable_Unpack(args[11]);
+    if (!rows_ok(out, q.sizes(), c.dev, type)) return arg_error();
+  }
+  const int64_t need = g_attention_bytes(B, S, Hq, c.H, c.D, prefix_len, most);
+  if (need < 0) return arg_error();
+  int64_t strides[3];
+  for (int i = 0; i < 3; ++i) strides[i] = q.size(i) > 1 ? q.stride(i) : 0;
+  const void* p[7] = {q.data_ptr(), c.t[0]->data_ptr(), c.t[1]->data_ptr(), c.t[2]->data_ptr(),
+                      c.t[3]->data_ptr(), width ? table.data_ptr() : nullptr, lens.data_ptr()};
+  const auto options = q.options();
+  const int64_t os[4] = {B, S, Hq, c.D};
+  int st;
+  {
+    NoGil no_gil;
+    if (!out.defined()) out = at::empty(os, options);
+    at::Tensor ws;
+    if (need > 0) ws = at::empty({need}, options.dtype(at::kByte));
+    st = g_attention(p[0], p[1], p[2], p[3], p[4], static_cast<const int32_t*>(p[5]), p[6], prefix,
+                     out.data_ptr(), need > 0 ? ws.data_ptr() : nullptr, need, strides, B, S, Hq,
+                     c.H, c.D, c.P, c.page, width, prefix_len, most, (float)scale, dtype, c.codes,
+                     c.scales, index, stream);
+  }
+  if (st != FAGQ_OK) return PyLong_FromLong(st);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// Function addresses from Python ints; false with an error set.
+bool addresses(PyObject* const* args, Py_ssize_t nargs, Py_ssize_t n, const char* name, void** p) {
+  if (nargs != n) {
+    PyErr_Format(PyExc_TypeError, "%s() takes %zd arguments", name, n);
+    return false;
+  }
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    p[i] = PyLong_AsVoidPtr(args[i]);
+    if (PyErr_Occurred()) return false;
+    if (!p[i]) {
+      PyErr_Format(PyExc_ValueError, "%s(): null function address", name);
+      return false;
+    }
+  }
+  return true;
+}
+
+// bind_attention(addresses of fagq_qk_norm_rope_launch, fagq_qk_norm_rope_bwd_workspace_bytes,
+// fagq_qk_norm_rope_bwd_launch, fagq_kv_cache_write_launch, fagq_kv_cache_read_launch,
+// fagq_paged_attention_workspace_bytes, fagq_paged_attention_launch).
+PyObject* bind_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  void* p[7];
+  if (!addresses(args, nargs, 7, "bind_attention", p)) return nullptr;
+  g_rope = reinterpret_cast<decltype(g_rope)>(p[0]);
+  g_rope_bytes = reinterpret_cast<decltype(g_rope_bytes)>(p[1]);
+  g_rope_bwd = reinterpret_cast<decltype(g_rope_bwd)>(p[2]);
+  g_cache_write = reinterpret_cast<decltype(g_cache_write)>(p[3]);
+  g_cache_read = reinterpret_cast<decltype(g_cache_read)>(p[4]);
+  g_attention_bytes = reinterpret_cast<decltype(g_attention_bytes)>(p[5]);
+  g_attention = reinterpret_cast<decltype(g_attention)>(p[6]);
+  Py_RETURN_NONE;
+}
+
 // bind_all(addresses of fagq_launch_parts, fagq_gemm_launch,
 // fagq_dsa_topk_launch, fagq_mla_bwd_workspace_bytes, fagq_mla_bwd_launch).
 PyObject* bind_all(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -551,6 +944,18 @@ PyMethodDef kMethods[] = {
      METH_FASTCALL, "The MLA backward with a workspace of its own; returns its status."},
     {"bind_all", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&bind_all)),
      METH_FASTCALL, "Sets the addresses of the other entry points."},
+    {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&rope)),
+     METH_FASTCALL, "Norm and rotation of query and key heads: allocates and launches."},
+    {"rope_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&rope_bwd)),
+     METH_FASTCALL, "Its gradients, with outputs and a workspace of its own."},
+    {"cache_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&cache_write)),
+     METH_FASTCALL, "Quantises keys and values into cache slots; returns the status."},
+    {"cache_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&cache_read)),
+     METH_FASTCALL, "Gathers cache pages; returns the status."},
+    {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&attention)),
+     METH_FASTCALL, "Attention over the cache, with a workspace of its own."},
+    {"bind_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&bind_attention)),
+     METH_FASTCALL, "Sets the addresses of the attention side's entry points."},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fagq_py", "Per-call binding of the operators.", -1,

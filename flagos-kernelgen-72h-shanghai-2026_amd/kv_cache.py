@@ -93,6 +93,14 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor | None, slots: torch.Tensor,
     whose slot is negative or past the cache is left out; no two tokens may name one slot.  A
     cache of latents passes None for v, v_cache and v_scale.  Asynchronous on the current
     stream."""
+    mod, fast_stream = _lib.fast_module(k_cache)
+    if mod is not None:
+        st = mod.cache_write(k, v, slots, k_cache, v_cache, k_scale, v_scale, fast_stream)
+        if st == 0:
+            return
+        if st != _lib.FAST_ARG_ERROR:
+            _lib.check(st, "fagq_kv_cache_write_launch")
+        # An argument the binding leaves to the checks below.
     P, H, page, D, G, qf, sf = _check_cache(k_cache, v_cache, k_scale, v_scale)
     dev = k_cache.device
     if (v is None) != (v_cache is None):
@@ -127,6 +135,15 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor | None, k_scale: 
     [rows, H, D] contiguous, bfloat16, float16 or float32.  Tokens without a page (an entry
     outside the cache, such as -1) become zeros; rows behind cu_seqlens[B] are left as they
     were.  Returns ``(k_out, v_out)``.  Asynchronous on the current stream."""
+    mod, fast_stream = _lib.fast_module(k_cache)
+    if mod is not None:
+        st = mod.cache_read(k_cache, v_cache, k_scale, v_scale, page_table, cu_seqlens, k_out, v_out,
+                            fast_stream)
+        if st == 0:
+            return k_out, v_out
+        if st != _lib.FAST_ARG_ERROR:
+            _lib.check(st, "fagq_kv_cache_read_launch")
+        # An argument the binding leaves to the checks below.
     P, H, page, D, G, qf, sf = _check_cache(k_cache, v_cache, k_scale, v_scale)
     dev = k_cache.device
     if (v_out is None) != (v_cache is None):
@@ -195,6 +212,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     close bound gives a better split of the work.  ``workspace`` (optional): a uint8 GPU tensor
     of at least ``attention_workspace_bytes(...)`` bytes.  Returns ``out`` [B, S, Hq, D]
     (contiguous, allocated unless given), asynchronously on the current stream."""
+    mod, fast_stream = _lib.fast_module(k_cache) if workspace is None else (None, None)
+    if mod is not None:
+        r = mod.attention(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, sm_scale,
+                          prefix_pages, prefix_len, max_kv_len, out, fast_stream)
+        if type(r) is not int:
+            return r
+        if r != _lib.FAST_ARG_ERROR:
+            _lib.check(r, "fagq_paged_attention_launch")
+        # An argument the binding leaves to the checks below.
     P, H, page, D, G, qf, sf = _check_cache(k_cache, v_cache, k_scale, v_scale)
     if v_cache is None:
         raise ValueError("paged_attention needs a cache of keys and values")

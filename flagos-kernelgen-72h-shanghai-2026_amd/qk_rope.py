@@ -92,6 +92,15 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     int32 or int64.  D and R are multiples of 16.  A token with a position outside the tables
     is padding and gets zeros.  Returns ``(q_out, k_out)``, allocated unless given; they may be
     q and k themselves.  Asynchronous on the current stream."""
+    mod, fast_stream = _lib.fast_module(q)
+    if mod is not None:
+        r = mod.rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, q_out, k_out,
+                     fast_stream)
+        if type(r) is not int:
+            return r
+        if r != _lib.FAST_ARG_ERROR:
+            _lib.check(r, "fagq_qk_norm_rope_launch")
+        # An argument the binding leaves to the checks below.
     T, Hq, Hk, D, R, table, idx = _check(q, k, q_weight, k_weight, cos, sin, positions)
     dev = q.device
     if q_out is None:
@@ -132,6 +141,15 @@ def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor
     dk of q's type (allocated unless given, views of a fused gradient included), the weights'
     float32 [D].  ``workspace`` (optional): a uint8 GPU tensor of at least
     ``bwd_workspace_bytes(T, Hq, Hk, D)`` bytes.  Padding rows get zeros."""
+    mod, fast_stream = _lib.fast_module(q) if workspace is None else (None, None)
+    if mod is not None:
+        r = mod.rope_bwd(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, dq_out,
+                         dk_out, dq, dk, fast_stream)
+        if type(r) is not int:
+            return r
+        if r != _lib.FAST_ARG_ERROR:
+            _lib.check(r, "fagq_qk_norm_rope_bwd_launch")
+        # An argument the binding leaves to the checks below.
     T, Hq, Hk, D, R, table, idx = _check(q, k, q_weight, k_weight, cos, sin, positions)
     dev = q.device
     if dq is None:
