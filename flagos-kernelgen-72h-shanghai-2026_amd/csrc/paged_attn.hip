@@ -16,8 +16,10 @@ namespace fagq {
 namespace attn {
 namespace {
 
-constexpr int64_t kGroups = 1024;      // workgroups wanted (see plan_for)
-constexpr int64_t kMinChunk = kStep * kWaves;
+constexpr int64_t kCUs = 256;
+constexpr int64_t kMinChunk = kStep * kWaves;   // a step for each wave
+constexpr int64_t kFixed = 128;        // what a workgroup costs besides its keys, in keys
+constexpr int64_t kJoin = 10;          // what a chunk costs the joining kernel, in keys
 
 struct JoinArgs {
   const float* part;
@@ -29,36 +31,64 @@ struct JoinArgs {
   int32_t idx64;
 };
 
-// One wave for each query row: the chunks that hold keys of its sequence, joined by
-// o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.  A lane has D / 64 dims.
-template <int E, int D>
+// The chunks that hold keys of a row's sequence, joined by
+// o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.  W waves for each query row take every W-th chunk,
+// a lane D / 64 dims; a workgroup has kWaves / W rows.  The first kAhead chunks of a wave are
+// loaded before the length says how many count (those that do not are not used): the kernel is a
+// chain of waits, and this leaves two of them.
+constexpr int kAhead = 8;
+
+template <int E, int D, int W>
 __global__ __launch_bounds__(64 * kWaves) void paged_attention_join(JoinArgs a) {
   constexpr int N = D / 64;
-  const int row = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * kWaves + threadIdx.x / 64));
-  if (row >= a.rows) return;
+  __shared__ float joined[W > 1 ? W : 1][D];
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64));
+  const int row = (int)blockIdx.x * (kWaves / W) + wave / W, sub = wave % W;
+  if (row >= a.rows) return;                    // W > 1: no workgroup is cut
   const int lane = threadIdx.x & 63;
   const int b = row / a.Hq / a.S;
+  const int total = a.prefix_chunks + a.chunks;
+  const int64_t at = (int64_t)row * total;
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.ml) + at;
+  const float* part = a.part + at * D + lane * N;
+  float ahead[kAhead][N];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    const int i = sub + u * W;
+#pragma unroll
+    for (int j = 0; j < N; ++j) ahead[u][j] = part[(int64_t)(i < total ? i : 0) * D + j];
+  }
+  const f32x2 first = ml[lane < total ? lane : 0];
   const int64_t len = a.idx64 ? static_cast<const int64_t*>(a.lens)[b]
                               : (int64_t) static_cast<const int32_t*>(a.lens)[b];
   const int own = ((int)cache::seen_tokens(len, a.most, 1, 0) + a.chunk - 1) / a.chunk;
   const int n = a.prefix_chunks + (own > 1 ? own : 1);
-  const int64_t at = (int64_t)row * (a.prefix_chunks + a.chunks);
-  const float* ml = a.ml + 2 * at;
-  const float* part = a.part + at * D + lane * N;
-  float m = kLow;
-  for (int i = lane; i < n; i += 64) m = fmaxf(m, ml[2 * i]);
+  float m = lane < n ? first[0] : kLow;
+  for (int i = 64 + lane; i < n; i += 64) m = fmaxf(m, ml[i][0]);
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
   float o[N] = {}, l = 0.0f;
   for (int i0 = 0; i0 < n; i0 += 64) {
     float w = 0.0f;
     if (i0 + lane < n) {
-      w = __builtin_amdgcn_exp2f(ml[2 * (i0 + lane)] - m);
-      l += w * ml[2 * (i0 + lane) + 1];
+      const f32x2 v = i0 == 0 ? first : ml[i0 + lane];
+      w = __builtin_amdgcn_exp2f(v[0] - m);
+      l += w * v[1];
     }
     const int stop = n - i0 < 64 ? n - i0 : 64;
-#pragma unroll 4
-    for (int i = 0; i < stop; ++i) {
+    int i = sub;
+    if (i0 == 0) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (sub + u * W >= stop) break;
+        const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), sub + u * W));
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = __builtin_fmaf(f, ahead[u][j], o[j]);
+      }
+      i += kAhead * W;
+    }
+#pragma unroll 8
+    for (; i < stop; i += W) {
       const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), i));
 #pragma unroll
       for (int j = 0; j < N; ++j) o[j] = __builtin_fmaf(f, part[(int64_t)(i0 + i) * D + j], o[j]);
@@ -67,6 +97,16 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attention_join(JoinArgs a) 
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) joined[sub][lane * N + j] = o[j];
+    __syncthreads();
+    if (sub > 0) return;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int w = 1; w < W; ++w) o[j] += joined[w][lane * N + j];
+  }
   uint16_t* out = a.out + (int64_t)row * D + lane * N;
   if constexpr (N == 1) {
     out[0] = (uint16_t)pack16<E>(o[0] * inv, 0.0f);
@@ -105,23 +145,41 @@ int check_sizes(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t 
   return FAGQ_OK;
 }
 
-// How a call's rows and keys are cut.  A unit has 16 R rows (R = 1, 2 or 4: as few as hold the
-// rows that share their keys, so that a step's codes are widened once for all of them); keys are
-// cut into chunks so that kGroups workgroups have work, kMinChunk keys at least.
+// How a call's rows and keys are cut.  A unit has 16 R rows: as few as hold the rows that share
+// their keys, so that a step's codes are widened once for all of them, R D <= 256.
 struct Plan {
   int R, RP;
   int64_t tiles, prefix_tiles, chunk, prefix_chunk, chunks, prefix_chunks, items, prefix_items;
   int64_t rows;
 };
 
-int row_tiles(int64_t rows, int64_t D) { return rows <= 16 ? 1 : rows <= 32 || D > 128 ? 2 : 4; }
+int row_tiles(int64_t rows, int64_t D) {
+  const int R = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  return R * D <= 256 ? R : (int)(256 / D);
+}
 
+// Cuts a unit's keys into the number of chunks that takes least time where each of the `units`
+// becomes so many workgroups, the GPU runs them in rounds of two for each CU, and one takes as long
+// as its keys and kFixed.  Two workgroups for each CU fill HBM where one is not short of loads
+// under way; registers would allow three of R D <= 128, which took longer (64 sequences of 8192
+// tokens, 64 + 8 heads of 128: 185 us with one chunk each, 201 with three).
 void cut(int64_t keys, int64_t units, int64_t* chunk, int64_t* chunks) {
-  const int64_t want = (kGroups + units - 1) / units;
-  int64_t c = (keys + want - 1) / want;
-  c = (c + kMinChunk - 1) / kMinChunk * kMinChunk;
-  *chunk = c < kMinChunk ? kMinChunk : c;
-  *chunks = (keys + *chunk - 1) / *chunk;
+  const int64_t slots = 2 * kCUs;
+  const int64_t most = (keys + kMinChunk - 1) / kMinChunk;
+  int64_t best = -1;
+  *chunk = kMinChunk, *chunks = 0;
+  for (int64_t n = 1; n <= most; ++n) {
+    int64_t c = (keys + n - 1) / n;
+    c = (c + kMinChunk - 1) / kMinChunk * kMinChunk;
+    const int64_t got = (keys + c - 1) / c;
+    const int64_t cost = (units * got + slots - 1) / slots * (c + kFixed) + kJoin * got;
+    if (best < 0 || cost < best) {
+      best = cost;
+      *chunk = c;
+      *chunks = got;
+    }
+    if (units * n >= 8 * slots) break;
+  }
 }
 
 Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t prefix_len,
@@ -158,11 +216,11 @@ const void* kernel_for(int dtype, int q_format, int scale_format, int D, const P
   return table[4 * e + 2 * q + s](D, p.R, p.RP);
 }
 
-template <int E>
+template <int E, int W>
 const void* join_for(int64_t D) {
-  return D == 64    ? reinterpret_cast<const void*>(&paged_attention_join<E, 64>)
-         : D == 128 ? reinterpret_cast<const void*>(&paged_attention_join<E, 128>)
-                    : reinterpret_cast<const void*>(&paged_attention_join<E, 256>);
+  return D == 64    ? reinterpret_cast<const void*>(&paged_attention_join<E, 64, W>)
+         : D == 128 ? reinterpret_cast<const void*>(&paged_attention_join<E, 128, W>)
+                    : reinterpret_cast<const void*>(&paged_attention_join<E, 256, W>);
 }
 
 }  // namespace
@@ -255,12 +313,13 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   a.chunk = (int32_t)p.chunk, a.chunks = (int32_t)p.chunks, a.tiles = (int32_t)p.tiles;
   a.prefix_chunk = (int32_t)p.prefix_chunk, a.prefix_chunks = (int32_t)p.prefix_chunks;
   a.prefix_tiles = (int32_t)p.prefix_tiles, a.prefix_items = (int32_t)p.prefix_items;
+  a.items = (int32_t)p.items;
   const int64_t n = p.chunks + p.prefix_chunks;
   if (n > 1) {
     a.part = static_cast<float*>(workspace);
     a.part_ml = a.part + p.rows * n * D;
   }
-  // At most kGroups workgroups and one for each unit on either side: below 2^31.
+  // At most 2^24 units, and few more workgroups: below 2^31.
   void* args[] = {&a};
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int ls = launch_kernel(kernel_for(dtype, q_format, scale_format, (int)D, p),
@@ -270,9 +329,11 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   JoinArgs j = {a.part, a.part_ml, kv_lens, a.out, (int32_t)p.rows, a.S, a.Hq, a.prefix_chunks,
                 a.chunks, a.chunk, a.most, a.idx64};
   void* jargs[] = {&j};
-  return launch_kernel(dtype == FAGQ_DT_BF16 ? join_for<ET_BF16>(D) : join_for<ET_F16>(D),
-                       dim3((unsigned)((p.rows + kWaves - 1) / kWaves)), dim3(64 * kWaves), jargs,
-                       0, st);
+  const bool wide = n > kAhead;         // a workgroup for each row
+  const void* fn = dtype == FAGQ_DT_BF16 ? (wide ? join_for<ET_BF16, kWaves>(D) : join_for<ET_BF16, 1>(D))
+                                         : (wide ? join_for<ET_F16, kWaves>(D) : join_for<ET_F16, 1>(D));
+  const int64_t groups = wide ? p.rows : (p.rows + kWaves - 1) / kWaves;
+  return launch_kernel(fn, dim3((unsigned)groups), dim3(64 * kWaves), jargs, 0, st);
 }
 
 }  // extern "C"

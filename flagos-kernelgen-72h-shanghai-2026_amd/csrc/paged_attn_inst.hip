@@ -12,18 +12,20 @@ const void* kernel() {
       &paged_attention<FAGQ_ATTN_E, FAGQ_ATTN_QF, FAGQ_ATTN_SF, D, R, RP>);
 }
 
-// The pairs (R, RP) that plan_for makes: 16 rows of a sequence go with a prefix of any unit,
-// more rows with units of their own size; 256-wide heads leave no registers for R = 4.
+// The pairs (R, RP) that plan_for makes: 16 rows of a sequence go with a prefix of any unit, more
+// rows with units of their own size; R D <= 256.
 template <int D>
 const void* lookup(int R, int RP) {
-  if (R == 1) {
-    if (RP == 0) return kernel<D, 1, 0>();
-    if (RP == 1) return kernel<D, 1, 1>();
-    if (RP == 2) return kernel<D, 1, 2>();
-    if constexpr (D < 256) return kernel<D, 1, 4>();
+  if (R == 1 && RP == 0) return kernel<D, 1, 0>();
+  if (R == 1 && RP == 1) return kernel<D, 1, 1>();
+  if constexpr (D <= 128) {
+    if (R == 1 && RP == 2) return kernel<D, 1, 2>();
+    if (R == 2) return RP == 0 ? kernel<D, 2, 0>() : kernel<D, 2, 2>();
   }
-  if (R == 2) return RP == 0 ? kernel<D, 2, 0>() : kernel<D, 2, 2>();
-  if constexpr (D < 256) return RP == 0 ? kernel<D, 4, 0>() : kernel<D, 4, 4>();
+  if constexpr (D == 64) {
+    if (R == 1 && RP == 4) return kernel<D, 1, 4>();
+    if (R == 4) return RP == 0 ? kernel<D, 4, 0>() : kernel<D, 4, 4>();
+  }
   return nullptr;
 }
 

@@ -6,7 +6,9 @@
 // their own and are joined by o = sum 2^(m_i - m) o_i.
 //
 // A unit of work is 16 R query rows that read the same keys (the rows of one sequence that share
-// a cache head; for the shared prefix, those of the whole batch) times a chunk of keys.  The four
+// a cache head; for the shared prefix, those of the whole batch) times a chunk of keys.  R D <= 256:
+// with more rows the registers hold one wave on a SIMD, whose loads and products wait for each
+// other (64 rows of 64 sequences behind 32768 keys, heads of 128: R = 2 145 us, R = 4 234).  The four
 // waves of a workgroup take its steps of 32 keys in turn, each with m, l and o of its own, and are
 // joined through LDS; chunks are joined by a second kernel.
 //
@@ -66,7 +68,7 @@ struct Args {
   int32_t chunk, prefix_chunk;        // keys of a chunk, multiples of kStep * kWaves
   int32_t chunks, prefix_chunks;      // chunks of a row: its own, and of the prefix
   int32_t tiles, prefix_tiles;        // row tiles of a sequence and cache head; of the batch
-  int32_t prefix_items;               // workgroups of the prefix, ahead of the others
+  int32_t prefix_items, items;        // workgroups of the prefix, ahead of the others
   int32_t idx64;
   float scale2;                       // sm_scale * log2(e)
 };
@@ -240,104 +242,112 @@ __device__ __forceinline__ void load_values(const Args& a, int h, int lane, int3
   }
 }
 
-// The rows of a unit: each lane's query c of R tiles.
+// The rows of a unit: each lane's query c of R tiles.  One tile's queries stay in registers; more
+// of them lie in LDS in the order of the products (the waves of a workgroup have the same rows),
+// which leaves the registers for two waves on each SIMD.
 template <int E, int D, int R>
 struct Rows {
-  u32x4 q[R][D / 32];          // lane (c, g): dims 64 h + 16 g + 8 i .. of step 2 h + i
+  u32x4 q[D / 32];             // R == 1; lane (c, g): dims 64 h + 16 g + 8 i .. of step 2 h + i
+  const u32x4* lds_q;          // R > 1: [R][D / 32][64]
   f32x4 o[R][D / 16];          // dims D / 16 (4 g + r) + j at [j][r]
   float m[R], l[R];            // l: of this lane's keys
   int32_t seen[R];             // keys that the row sees
-  int32_t ve;                  // o is in units of 2^ve (see join)
+  float unit, inv_unit;        // o is in units of `unit`, a power of two (see join)
 };
 
-// Scores of one step in units of log 2.
+// Products of one step's keys with the queries.
 template <int E, int QF, int SF, int D, int R>
-__device__ __forceinline__ void scores(const Args& a, const RawKeys<D, SF>& raw, const Rows<E, D, R>& s,
+__device__ __forceinline__ void scores(int lane, const RawKeys<D, SF>& raw, const Rows<E, D, R>& s,
                                        f32x4 (&x)[R][2]) {
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int r = 0; r < R; ++r) x[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int t = 0; t < 2; ++t) x[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      const u32x4 k = widen8<E, QF>(raw.k[t][i / 2][2 * (i & 1)], raw.k[t][i / 2][2 * (i & 1) + 1]);
+  for (int i = 0; i < D / 32; ++i) {
+    u32x4 k[2];
 #pragma unroll
-      for (int r = 0; r < R; ++r) x[r][t] = mfma<E>(k, s.q[r][i], x[r][t]);
+    for (int t = 0; t < 2; ++t)
+      k[t] = widen8<E, QF>(raw.k[t][i / 2][2 * (i & 1)], raw.k[t][i / 2][2 * (i & 1) + 1]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const u32x4 q = R == 1 ? s.q[i] : s.lds_q[(r * (D / 32) + i) * 64 + lane];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) x[r][t] = mfma<E>(k[t], q, x[r][t]);
     }
   }
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float k = scale_of<SF>(raw.s[t], i) * a.scale2;
-#pragma unroll
-      for (int r = 0; r < R; ++r) x[r][t][i] *= k;
-    }
 }
 
 // The softmax and the values of one step: 32 keys from `tok` on, of which the unit's last row
-// sees those below `end`; all rows see those below `all`.
+// sees those below `end`; all rows see those below `all`.  ks: the keys' scales times scale2.
 template <int E, int QF, int SF, int D, int R>
-__device__ __forceinline__ void join(const Args& a, int lane, int32_t tok, int32_t all, int32_t end,
-                                     const Pages& pages, f32x4 (&x)[R][2], RawValues<D, SF>& raw,
-                                     Rows<E, D, R>& s) {
+__device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t end,
+                                     const Pages& pages, f32x4 (&x)[R][2], float (&ks)[8],
+                                     RawValues<D, SF>& raw, Rows<E, D, R>& s) {
   constexpr int NT = D / 16;
   const int g = lane >> 4;
   float vs[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) vs[i] = scale_of<SF>(raw.s[i / 4], i % 4);
-  const bool edge = tok + kStep > all || pages.p[0] < 0 || pages.p[1] < 0;
-  if (edge) {
-    // What no row sees may hold anything: its values and their scales become zeros here.
+  if (tok + kStep > all || pages.p[0] < 0 || pages.p[1] < 0) {
+    // What no row sees may hold anything: its values and their scales become zeros.  What a row
+    // does not see gets no weight, whatever the score and the key's scale are.
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int32_t at = tok + 16 * (i / 4) + 4 * g + i % 4;
-      const bool live = at < end && pages.p[i / 4] >= 0;
+      const bool page = pages.p[i / 4] >= 0, live = at < end && page;
       vs[i] = live ? vs[i] : 0.0f;
 #pragma unroll
       for (int w = 0; w < NT / 4; ++w) raw.v[i][w] = live ? raw.v[i][w] : 0u;
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        x[r][i / 4][i % 4] = at < s.seen[r] && pages.p[i / 4] >= 0 ? x[r][i / 4][i % 4] : -INFINITY;
+        x[r][i / 4][i % 4] = at < s.seen[r] && page ? x[r][i / 4][i % 4] * ks[i] : -INFINITY;
+      ks[i] = 1.0f;
     }
   }
-  // Probabilities times value scales have to fit fp16: they are taken in units of 2^ve, ve the
-  // exponent just above the largest value scale so far, and o with them.
-  float most = vs[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) most = fmaxf(most, vs[i]);
-  const uint32_t bits = (uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(cross_max(most)));
-  const int32_t e = (int32_t)((bits >> 23) & 255u) - 126;
-  if (e > s.ve) {
-    const float f = __builtin_ldexpf(1.0f, s.ve - e);
+  // Probabilities times value scales have to fit fp16: they are taken in units of the power of
+  // two just above the largest value scale so far, and o with them.
+  float most = fmaxf(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])),
+                     fmaxf(fmaxf(vs[4], vs[5]), fmaxf(vs[6], vs[7])));
+  if (__any(most > s.unit)) {
+    const uint32_t bits =
+        (uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(cross_max(most)));
+    int32_t e = (int32_t)(bits >> 23) - 126;
+    e = e < 127 ? e : 127;
+    const float unit = __builtin_ldexpf(1.0f, e), f = s.unit * __builtin_ldexpf(1.0f, -e);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int j = 0; j < NT; ++j) s.o[r][j] *= f;
-    s.ve = e;
+    s.unit = unit;
+    s.inv_unit = __builtin_ldexpf(1.0f, -e);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) vs[i] = __builtin_ldexpf(vs[i], -s.ve);
+  for (int i = 0; i < 8; ++i) vs[i] *= s.inv_unit;
   u32x4 p[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[r][i / 4][i % 4];
-    float top = y[0];
+    for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(x[r][i / 4][i % 4], ks[i], -s.m[r]);
+    const float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
+                            fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+    if (__any(top > kSlack)) {
+      float m = s.m[r];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, y[i]);
-    top = cross_max(top);
-    if (__any(top > s.m[r] + kSlack)) {
-      const float m = fmaxf(top, s.m[r]), f = __builtin_amdgcn_exp2f(s.m[r] - m);
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, x[r][i / 4][i % 4] * ks[i]);
+      m = cross_max(m);
+      const float f = __builtin_amdgcn_exp2f(s.m[r] - m);
       s.m[r] = m;
       s.l[r] *= f;
 #pragma unroll
       for (int j = 0; j < NT; ++j) s.o[r][j] *= f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(x[r][i / 4][i % 4], ks[i], -m);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      y[i] = __builtin_amdgcn_exp2f(y[i] - s.m[r]);
+      y[i] = __builtin_amdgcn_exp2f(y[i]);
       s.l[r] += y[i];
       y[i] *= vs[i];
     }
@@ -388,10 +398,6 @@ __device__ __forceinline__ void run_steps(const Args& a, const Keys& k, int h, i
   int32_t tok = k.begin + wave * kStep;
   constexpr int32_t kNext = kStep * kWaves;
   if (tok >= k.end) return;
-  // One set of registers each for keys and values: the next step's keys are on their way while
-  // this one's softmax and values are worked on, the next values during the next scores.
-  RawKeys<D, SF> keys;
-  RawValues<D, SF> values;
   // Table entries are read a step ahead of the loads that need them.
   auto entries = [&](int32_t t) {
     return Pages{{entry_of(k.pages, k.width, a.page_shift, t),
@@ -400,48 +406,103 @@ __device__ __forceinline__ void run_steps(const Args& a, const Keys& k, int h, i
   auto check = [&](const Pages& p) {
     return Pages{{checked(p.p[0], a.num_pages), checked(p.p[1], a.num_pages)}};
   };
-  Pages pages = check(entries(tok));
-  Pages ahead = entries(tok + kNext);
-  load_keys<D, SF>(a, h, lane, tok, pages, keys);
-  load_values<D, SF>(a, h, lane, tok, pages, values);
-  for (;;) {
-    const int32_t next = tok + kNext;
-    const bool more = next < k.end;
-    const Pages next_pages = check(ahead);
-    ahead = entries(next + kNext);
+  Pages ahead;
+  auto work = [&](RawKeys<D, SF>& keys, RawValues<D, SF>& values, const Pages& pages, auto between) {
     f32x4 x[R][2];
-    scores<E, QF, SF, D, R>(a, keys, s, x);
-    if (more) load_keys<D, SF>(a, h, lane, next, next_pages, keys);
-    join<E, QF, SF, D, R>(a, lane, tok, all, end, pages, x, values, s);
-    if (!more) return;
-    load_values<D, SF>(a, h, lane, next, next_pages, values);
-    tok = next;
-    pages = next_pages;
+    float ks[8];
+    scores<E, QF, SF, D, R>(lane, keys, s, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ks[i] = scale_of<SF>(keys.s[i / 4], i % 4) * a.scale2;
+    between();
+    join<E, QF, SF, D, R>(lane, tok, all, end, pages, x, ks, values, s);
+  };
+  if constexpr (R * D <= 128) {
+    // Bound by HBM: two sets of registers, the next step's loads all under way during this one.
+    RawKeys<D, SF> keys[2];
+    RawValues<D, SF> values[2];
+    Pages pages[2];
+    pages[0] = check(entries(tok));
+    ahead = entries(tok + kNext);
+    load_keys<D, SF>(a, h, lane, tok, pages[0], keys[0]);
+    load_values<D, SF>(a, h, lane, tok, pages[0], values[0]);
+    auto one = [&](int now, int then) {
+      const int32_t next = tok + kNext;
+      const bool more = next < k.end;
+      pages[then] = check(ahead);
+      ahead = entries(next + kNext);
+      if (more) {
+        load_keys<D, SF>(a, h, lane, next, pages[then], keys[then]);
+        load_values<D, SF>(a, h, lane, next, pages[then], values[then]);
+      }
+      work(keys[now], values[now], pages[now], [] {});
+      tok = next;
+      return more;
+    };
+    while (one(0, 1) && one(1, 0)) {
+    }
+  } else {
+    // Short of registers: one set each, the next step's keys under way during this one's softmax
+    // and values, its values during the next scores.
+    RawKeys<D, SF> keys;
+    RawValues<D, SF> values;
+    Pages pages = check(entries(tok));
+    ahead = entries(tok + kNext);
+    load_keys<D, SF>(a, h, lane, tok, pages, keys);
+    load_values<D, SF>(a, h, lane, tok, pages, values);
+    for (;;) {
+      const int32_t next = tok + kNext;
+      const bool more = next < k.end;
+      const Pages next_pages = check(ahead);
+      ahead = entries(next + kNext);
+      work(keys, values, pages, [&] {
+        if (more) load_keys<D, SF>(a, h, lane, next, next_pages, keys);
+      });
+      if (!more) return;
+      load_values<D, SF>(a, h, lane, next, next_pages, values);
+      tok = next;
+      pages = next_pages;
+    }
   }
 }
 
-// LDS of a workgroup: the waves' o of one tile of 16 rows, m and l of all of them.
+// LDS of a workgroup: the queries during the steps, then the waves' o of one tile of 16 rows; m and
+// l of all rows.
 template <int D, int R>
 struct Shared {
-  float o[kWaves][D / 4][64];
+  union {
+    u32x4 q[R > 1 ? R * (D / 32) * 64 : 1];
+    float o[kWaves][D / 4][64];
+  };
   float m[kWaves][16 * R], l[kWaves][16 * R];
 };
 
+// Which tile of which group (cache head and chunk, ...) a workgroup takes: the tiles of a group
+// read the same keys, so they go to one XCD (workgroup b runs on XCD b % 8) next to each other
+// and find them in its L2.
+struct Place {
+  int tile, group;
+};
+__device__ __forceinline__ Place place_of(int item, int items, int tiles) {
+  const int full = items / (8 * tiles) * 8 * tiles;
+  if (item >= full) return {(item - full) % tiles, (full + item - full) / tiles};
+  const int j = item >> 3;
+  return {j % tiles, j / tiles * 8 + (item & 7)};
+}
+
 // One unit and chunk.  `item`: workgroup number within its kind.
 template <int E, int QF, int SF, int D, int R, bool PREFIX>
-__device__ __forceinline__ void unit(const Args& a, int item, float* lds) {
+__device__ __forceinline__ void unit(const Args& a, int item, char* lds) {
   constexpr int NT = D / 16;
   Shared<D, R>& sh = *reinterpret_cast<Shared<D, R>*>(lds);
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int tiles = PREFIX ? a.prefix_tiles : a.tiles;
   const int chunks = PREFIX ? a.prefix_chunks : a.chunks;
-  const int tile = item % tiles;
-  item /= tiles;
-  const int chunk = item % chunks;
-  item /= chunks;
-  const int h = item % a.H;
-  const int b = item / a.H;                     // own keys: the sequence
+  const Place place = PREFIX ? place_of(item, a.prefix_items, a.prefix_tiles)
+                             : place_of(item, a.items, a.tiles);
+  const int tile = place.tile;
+  const int chunk = place.group % chunks;
+  const int h = place.group / chunks % a.H;
+  const int b = place.group / chunks / a.H;     // own keys: the sequence
   const int per = a.S * a.group;                // rows of a sequence and cache head
   const int rows = PREFIX ? a.B * per : per;
   Keys k;
@@ -472,25 +533,32 @@ __device__ __forceinline__ void unit(const Args& a, int item, float* lds) {
     r.s = PREFIX ? bs - r.b * a.S : bs;
     return r;
   };
+  auto load_q = [&](const Row& w, int j) {
+    const uint16_t* q = a.q + ((int64_t)w.b * a.qs[0] + (int64_t)w.s * a.qs[1] +
+                               (int64_t)w.hq * a.qs[2]);
+    return *reinterpret_cast<const u32x4*>(q + 64 * (j / 2) + 16 * g + 8 * (j & 1));
+  };
   Rows<E, D, R> s;
-  s.ve = -1000;
+  s.unit = 0.0f;
+  s.inv_unit = 0.0f;
   int32_t all = k.end, end = k.end;             // keys that all rows see; that the last one sees
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int i = (tile * R + r) * 16 + c;
-    const bool on = i < rows;
-    const Row w = row_of(on ? i : rows - 1);
-    const uint16_t* q = a.q + ((int64_t)w.b * a.qs[0] + (int64_t)w.s * a.qs[1] +
-                               (int64_t)w.hq * a.qs[2]);
+    const Row w = row_of(i < rows ? i : rows - 1);
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j)
-      s.q[r][j] = *reinterpret_cast<const u32x4*>(q + 64 * (j / 2) + 16 * g + 8 * (j & 1));
+    for (int j = 0; j < D / 32; ++j) {
+      if constexpr (R == 1) s.q[j] = load_q(w, j);
+      else if ((r * (D / 32) + j) % kWaves == wave) sh.q[(r * (D / 32) + j) * 64 + lane] = load_q(w, j);
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j) s.o[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     s.m[r] = kLow;
     s.l[r] = 0.0f;
     s.seen[r] = PREFIX ? k.end : (int32_t)cache::seen_tokens(len, a.most, a.S, w.s);
   }
+  s.lds_q = sh.q;
+  if constexpr (R > 1) __syncthreads();
   if constexpr (!PREFIX) {
     // Rows are in order of their tokens: the first sees least, the last most.
     all = __builtin_amdgcn_readfirstlane(s.seen[0]);
@@ -515,8 +583,7 @@ __device__ __forceinline__ void unit(const Args& a, int item, float* lds) {
     float m = kLow;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) m = fmaxf(m, sh.m[w][16 * r + c]);
-    const float f =
-        s.l[r] > 0.0f ? __builtin_ldexpf(__builtin_amdgcn_exp2f(s.m[r] - m), s.ve) : 0.0f;
+    const float f = __builtin_amdgcn_exp2f(s.m[r] - m) * s.unit;
     float l = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
@@ -563,9 +630,9 @@ __device__ __forceinline__ void unit(const Args& a, int item, float* lds) {
 
 // RP: row tiles of a unit of the prefix (0: there is none), R: of the others.
 template <int E, int QF, int SF, int D, int R, int RP>
-__global__ __launch_bounds__(64 * kWaves) void paged_attention(Args a) {
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_attention(Args a) {
   constexpr int kRows = R > RP ? R : RP;
-  __shared__ __align__(16) float lds[sizeof(Shared<D, kRows>) / 4];
+  __shared__ __align__(16) char lds[sizeof(Shared<D, kRows>)];
   const int item = (int)blockIdx.x;
   if constexpr (RP > 0) {
     if (item < a.prefix_items) {
