@@ -17,25 +17,26 @@ namespace attn {
 namespace {
 
 constexpr int64_t kCUs = 256;
-constexpr int64_t kMinChunk = kStep * kWaves;   // a step for each wave
+constexpr int64_t kSlots = 2 * kCUs;   // workgroups of a round
+constexpr int64_t kFewRounds = 8 * kSlots;      // of all units: not worth a schedule
+constexpr int64_t kCacheBytes = 256ll << 20;    // of the cache behind the XCDs' L2
 constexpr int64_t kFixed = 128;        // what a workgroup costs besides its keys, in keys
-constexpr int64_t kJoin = 10;          // what a chunk costs the joining kernel, in keys
 
 struct JoinArgs {
   const float* part;
   const float* ml;
   const void* lens;
+  const int32_t* sched;      // null: static
   uint16_t* out;
-  int32_t rows, S, Hq;
-  int32_t prefix_chunks, chunks, chunk, most;
+  int32_t B, S, Hq, H;
+  int32_t prefix_chunks, row_parts, chunk, most, height;
   int32_t idx64;
 };
 
-// The chunks that hold keys of a row's sequence, joined by
-// o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.  W waves for each query row take every W-th chunk,
-// a lane D / 64 dims; a workgroup has kWaves / W rows.  The first kAhead chunks of a wave are
-// loaded before the length says how many count (those that do not are not used): the kernel is a
-// chain of waits, and this leaves two of them.
+// The parts of a row's keys, joined by o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.  W waves for
+// each query row take every W-th part, a lane D / 64 dims; a workgroup has kWaves / W rows.  The
+// first kAhead parts of a wave are loaded at once; of static chunks before the length says how many
+// hold keys (those that do not are not used): the kernel is a chain of waits.
 constexpr int kAhead = 8;
 
 template <int E, int D, int W>
@@ -44,34 +45,60 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attention_join(JoinArgs a) 
   __shared__ float joined[W > 1 ? W : 1][D];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64));
   const int row = (int)blockIdx.x * (kWaves / W) + wave / W, sub = wave % W;
-  if (row >= a.rows) return;                    // W > 1: no workgroup is cut
+  if (row >= a.B * a.S * a.Hq) return;          // W > 1: no workgroup is cut
   const int lane = threadIdx.x & 63;
-  const int b = row / a.Hq / a.S;
-  const int total = a.prefix_chunks + a.chunks;
-  const int64_t at = (int64_t)row * total;
-  const f32x2* ml = reinterpret_cast<const f32x2*>(a.ml) + at;
-  const float* part = a.part + at * D + lane * N;
+  const int bs = row / a.Hq, hq = row - bs * a.Hq, b = bs / a.S;
+  const int32_t len = own_length(a.lens, a.idx64, a.most, b);
+  const int64_t mine = (int64_t)row * a.row_parts;
+  // Own parts: n - prefix_chunks, from index `own` on, the first one at own_first, each next one
+  // `apart` further.
+  int n, apart = 1;
+  int64_t own_first = mine + a.prefix_chunks, own = own_first;
+  if (a.sched) {
+    const int32_t rounds = rounds_of(len), q = a.sched[a.B];
+    const int group = a.Hq / a.H, h = hq / group;
+    const int32_t begin = a.sched[b] + h * rounds;
+    const int wg = begin / q, cuts = (begin + rounds - 1) / q - wg;
+    if (cuts == 0 && a.prefix_chunks == 0) return;       // written already
+    if (cuts > 0) {
+      const int i = (bs - b * a.S) * group + (hq - h * group);   // row of the unit
+      const int64_t behind = (int64_t)a.B * a.S * a.Hq * a.row_parts + i;
+      own_first = segment_at(behind, a.height, wg, 1);
+      own = segment_at(behind, a.height, wg, 0);         // + 1 workgroup: the next ones
+      apart = 2 * a.height;
+    }
+    n = a.prefix_chunks + cuts + 1;
+  } else {
+    n = a.row_parts;                            // at most; what the length says, below
+  }
+  auto index = [&](int i) {
+    const int k = i - a.prefix_chunks;
+    return k < 0 ? mine + i : k == 0 ? own_first : own + (int64_t)k * apart;
+  };
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.ml);
+  const float* part = a.part + lane * N;
   float ahead[kAhead][N];
 #pragma unroll
   for (int u = 0; u < kAhead; ++u) {
     const int i = sub + u * W;
+    const int64_t at = index(i < n ? i : 0);
 #pragma unroll
-    for (int j = 0; j < N; ++j) ahead[u][j] = part[(int64_t)(i < total ? i : 0) * D + j];
+    for (int j = 0; j < N; ++j) ahead[u][j] = part[at * D + j];
   }
-  const f32x2 first = ml[lane < total ? lane : 0];
-  const int64_t len = a.idx64 ? static_cast<const int64_t*>(a.lens)[b]
-                              : (int64_t) static_cast<const int32_t*>(a.lens)[b];
-  const int own = ((int)cache::seen_tokens(len, a.most, 1, 0) + a.chunk - 1) / a.chunk;
-  const int n = a.prefix_chunks + (own > 1 ? own : 1);
+  const f32x2 first = ml[index(lane < n ? lane : 0)];
+  if (!a.sched) {
+    const int chunks = (len + a.chunk - 1) / a.chunk;
+    n = a.prefix_chunks + (chunks > 1 ? chunks : 1);
+  }
   float m = lane < n ? first[0] : kLow;
-  for (int i = 64 + lane; i < n; i += 64) m = fmaxf(m, ml[i][0]);
+  for (int i = 64 + lane; i < n; i += 64) m = fmaxf(m, ml[index(i)][0]);
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
   float o[N] = {}, l = 0.0f;
   for (int i0 = 0; i0 < n; i0 += 64) {
     float w = 0.0f;
     if (i0 + lane < n) {
-      const f32x2 v = i0 == 0 ? first : ml[i0 + lane];
+      const f32x2 v = i0 == 0 ? first : ml[index(i0 + lane)];
       w = __builtin_amdgcn_exp2f(v[0] - m);
       l += w * v[1];
     }
@@ -91,7 +118,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attention_join(JoinArgs a) 
     for (; i < stop; i += W) {
       const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), i));
 #pragma unroll
-      for (int j = 0; j < N; ++j) o[j] = __builtin_fmaf(f, part[(int64_t)(i0 + i) * D + j], o[j]);
+      for (int j = 0; j < N; ++j) o[j] = __builtin_fmaf(f, part[index(i0 + i) * D + j], o[j]);
     }
   }
 #pragma unroll
@@ -134,23 +161,31 @@ int log2_of(int64_t v) {
   return s;
 }
 
+// Rounds that a schedule may have, at most.
+int64_t most_rounds(int64_t B, int64_t H, int64_t most) {
+  const int64_t n = (most + kRound - 1) / kRound;
+  return B * H * (n > 1 ? n : 1);
+}
+
 int check_sizes(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t prefix_len,
                 int64_t max_kv_len) {
   if (B < 0 || S < 1 || H < 1 || Hq < H || Hq % H != 0 || (D != 64 && D != 128 && D != 256) ||
       prefix_len < 0 || max_kv_len < 0)
     return FAGQ_E_SHAPE;
   if (B > 65535 || S > 65535 || Hq > 4096 || B * S * Hq > (1ll << 24) ||
-      prefix_len > (1ll << 30) || max_kv_len > (1ll << 30))
+      prefix_len > (1ll << 30) || max_kv_len > (1ll << 30) ||
+      most_rounds(B, H, max_kv_len) >= (1ll << 31))
     return FAGQ_E_TOO_LARGE;
   return FAGQ_OK;
 }
 
-// How a call's rows and keys are cut.  A unit has 16 R rows: as few as hold the rows that share
-// their keys, so that a step's codes are widened once for all of them, R D <= 256.
+// How a call's rows and keys are cut (see paged_attn_kernels.hpp).
 struct Plan {
-  int R, RP;
-  int64_t tiles, prefix_tiles, chunk, prefix_chunk, chunks, prefix_chunks, items, prefix_items;
-  int64_t rows;
+  int R, RP, form;
+  int64_t rows, tiles, prefix_tiles;
+  int64_t chunk, prefix_chunk, chunks, prefix_chunks;   // chunks: static
+  int64_t items, prefix_items;                          // workgroups
+  int64_t row_parts, parts;                             // of a row; of the workspace
 };
 
 int row_tiles(int64_t rows, int64_t D) {
@@ -159,26 +194,23 @@ int row_tiles(int64_t rows, int64_t D) {
 }
 
 // Cuts a unit's keys into the number of chunks that takes least time where each of the `units`
-// becomes so many workgroups, the GPU runs them in rounds of two for each CU, and one takes as long
-// as its keys and kFixed.  Two workgroups for each CU fill HBM where one is not short of loads
-// under way; registers would allow three of R D <= 128, which took longer (64 sequences of 8192
-// tokens, 64 + 8 heads of 128: 185 us with one chunk each, 201 with three).
+// becomes so many workgroups, the GPU runs them in rounds of kSlots, one takes as long as its keys
+// and kFixed, and each chunk costs the joining kernel kPartCost keys.
 void cut(int64_t keys, int64_t units, int64_t* chunk, int64_t* chunks) {
-  const int64_t slots = 2 * kCUs;
-  const int64_t most = (keys + kMinChunk - 1) / kMinChunk;
+  const int64_t most = (keys + kRound - 1) / kRound;
   int64_t best = -1;
-  *chunk = kMinChunk, *chunks = 0;
+  *chunk = kRound, *chunks = 0;
   for (int64_t n = 1; n <= most; ++n) {
     int64_t c = (keys + n - 1) / n;
-    c = (c + kMinChunk - 1) / kMinChunk * kMinChunk;
+    c = (c + kRound - 1) / kRound * kRound;
     const int64_t got = (keys + c - 1) / c;
-    const int64_t cost = (units * got + slots - 1) / slots * (c + kFixed) + kJoin * got;
+    const int64_t cost = (units * got + kSlots - 1) / kSlots * (c + kFixed) + (int64_t)kPartCost * got;
     if (best < 0 || cost < best) {
       best = cost;
       *chunk = c;
       *chunks = got;
     }
-    if (units * n >= 8 * slots) break;
+    if (units * n >= 8 * kSlots) break;
   }
 }
 
@@ -196,24 +228,34 @@ Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t pr
     p.prefix_items = H * p.prefix_tiles * p.prefix_chunks;
   }
   p.tiles = (per + 16 * p.R - 1) / (16 * p.R);
-  cut(most, B * H * p.tiles, &p.chunk, &p.chunks);
-  if (p.chunks < 1) p.chunks = 1;       // rows without keys are written all the same
-  p.items = B * H * p.tiles * p.chunks;
+  if (p.tiles > 1 || most_rounds(B, H, most) <= kFewRounds) {
+    p.form = kStatic;
+    cut(most, B * H * p.tiles, &p.chunk, &p.chunks);
+    if (p.chunks < 1) p.chunks = 1;     // rows without keys are written all the same
+    p.items = B * H * p.tiles * p.chunks;
+    p.row_parts = p.prefix_chunks + p.chunks;
+    p.parts = p.row_parts > 1 ? p.rows * p.row_parts : 0;
+  } else {
+    p.form = prefix_len == 0 && 2 * B * most * H * D >= kCacheBytes ? kScheduledOnce : kScheduled;
+    p.items = kSlots;
+    p.row_parts = prefix_len > 0 ? p.prefix_chunks + 1 : 0;
+    p.parts = p.rows * p.row_parts + p.items * 2 * 16 * p.R;
+  }
   return p;
 }
 
-int64_t workspace_bytes(const Plan& p, int64_t D) {
-  const int64_t n = p.chunks + p.prefix_chunks;
-  return n == 1 ? 0 : p.rows * n * (D + 2) * 4;
+// o, {m, l} of each part, and the schedule.
+int64_t workspace_bytes(const Plan& p, int64_t B, int64_t D) {
+  return p.parts * (D + 2) * 4 + (p.form == kStatic ? 0 : (B + 1) * 4);
 }
 
 const void* kernel_for(int dtype, int q_format, int scale_format, int D, const Plan& p) {
-  using Lookup = const void* (*)(int, int, int);
+  using Lookup = const void* (*)(int, int, int, int);
   static constexpr Lookup table[8] = {lookup_e0_q0_s0, lookup_e0_q0_s1, lookup_e0_q1_s0, lookup_e0_q1_s1,
-                             lookup_e1_q0_s0, lookup_e1_q0_s1, lookup_e1_q1_s0, lookup_e1_q1_s1};
+                                      lookup_e1_q0_s0, lookup_e1_q0_s1, lookup_e1_q1_s0, lookup_e1_q1_s1};
   const int e = dtype == FAGQ_DT_BF16 ? 0 : 1, q = q_format == FAGQ_Q_FP8_E4M3FN ? 0 : 1;
   const int s = scale_format == FAGQ_SCALE_F32 ? 0 : 1;
-  return table[4 * e + 2 * q + s](D, p.R, p.RP);
+  return table[4 * e + 2 * q + s](D, p.R, p.RP, p.form);
 }
 
 template <int E, int W>
@@ -234,7 +276,7 @@ FAGQ_API int64_t fagq_paged_attention_workspace_bytes(int64_t B, int64_t S, int6
                                                       int64_t max_kv_len) {
   using namespace fagq::attn;
   if (check_sizes(B, S, Hq, H, D, prefix_len, max_kv_len) != FAGQ_OK) return -1;
-  return B == 0 ? 0 : workspace_bytes(plan_for(B, S, Hq, H, D, prefix_len, max_kv_len), D);
+  return B == 0 ? 0 : workspace_bytes(plan_for(B, S, Hq, H, D, prefix_len, max_kv_len), B, D);
 }
 
 FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, const void* v_cache,
@@ -314,10 +356,11 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   a.prefix_chunk = (int32_t)p.prefix_chunk, a.prefix_chunks = (int32_t)p.prefix_chunks;
   a.prefix_tiles = (int32_t)p.prefix_tiles, a.prefix_items = (int32_t)p.prefix_items;
   a.items = (int32_t)p.items;
-  const int64_t n = p.chunks + p.prefix_chunks;
-  if (n > 1) {
+  a.row_parts = (int32_t)p.row_parts, a.slots = (int32_t)kSlots;
+  if (need > 0) {
     a.part = static_cast<float*>(workspace);
-    a.part_ml = a.part + p.rows * n * D;
+    a.part_ml = a.part + p.parts * D;
+    a.sched = p.form == kStatic ? nullptr : reinterpret_cast<int32_t*>(a.part_ml + 2 * p.parts);
   }
   // At most 2^24 units, and few more workgroups: below 2^31.
   void* args[] = {&a};
@@ -325,11 +368,17 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   const int ls = launch_kernel(kernel_for(dtype, q_format, scale_format, (int)D, p),
                                dim3((unsigned)(p.prefix_items + p.items)), dim3(64 * kWaves), args,
                                0, st);
-  if (ls != FAGQ_OK || n == 1) return ls;
-  JoinArgs j = {a.part, a.part_ml, kv_lens, a.out, (int32_t)p.rows, a.S, a.Hq, a.prefix_chunks,
-                a.chunks, a.chunk, a.most, a.idx64};
+  if (ls != FAGQ_OK || p.parts == 0) return ls;
+  JoinArgs j = {};
+  j.part = a.part, j.ml = a.part_ml, j.lens = kv_lens, j.sched = a.sched, j.out = a.out;
+  j.B = a.B, j.S = a.S, j.Hq = a.Hq, j.H = a.H;
+  j.prefix_chunks = a.prefix_chunks, j.row_parts = a.row_parts, j.chunk = a.chunk, j.most = a.most;
+  j.height = 16 * p.R, j.idx64 = a.idx64;
   void* jargs[] = {&j};
-  const bool wide = n > kAhead;         // a workgroup for each row
+  // A workgroup for each row where one may have more than kAhead parts.
+  const int64_t rounds = (max_kv_len + kRound - 1) / kRound;
+  const int64_t own = p.form == kStatic ? p.chunks : B * H >= kSlots ? 2 : rounds;
+  const bool wide = p.prefix_chunks + own > kAhead;
   const void* fn = dtype == FAGQ_DT_BF16 ? (wide ? join_for<ET_BF16, kWaves>(D) : join_for<ET_BF16, 1>(D))
                                          : (wide ? join_for<ET_F16, kWaves>(D) : join_for<ET_F16, 1>(D));
   const int64_t groups = wide ? p.rows : (p.rows + kWaves - 1) / kWaves;

@@ -6,27 +6,35 @@ namespace fagq {
 namespace attn {
 namespace {
 
-template <int D, int R, int RP>
+template <int D, int R, int RP, int FORM>
 const void* kernel() {
   return reinterpret_cast<const void*>(
-      &paged_attention<FAGQ_ATTN_E, FAGQ_ATTN_QF, FAGQ_ATTN_SF, D, R, RP>);
+      &paged_attention<FAGQ_ATTN_E, FAGQ_ATTN_QF, FAGQ_ATTN_SF, D, R, RP, FORM>);
 }
 
-// The pairs (R, RP) that plan_for makes: 16 rows of a sequence go with a prefix of any unit, more
-// rows with units of their own size; R D <= 256.
-template <int D>
-const void* lookup(int R, int RP) {
-  if (R == 1 && RP == 0) return kernel<D, 1, 0>();
-  if (R == 1 && RP == 1) return kernel<D, 1, 1>();
-  if constexpr (D <= 128) {
-    if (R == 1 && RP == 2) return kernel<D, 1, 2>();
-    if (R == 2) return RP == 0 ? kernel<D, 2, 0>() : kernel<D, 2, 2>();
-  }
-  if constexpr (D == 64) {
-    if (R == 1 && RP == 4) return kernel<D, 1, 4>();
-    if (R == 4) return RP == 0 ? kernel<D, 4, 0>() : kernel<D, 4, 4>();
+// What plan_for makes, R D <= 256: without a prefix, units of any height; with one, 16 rows go with a
+// prefix of units of any height, more rows with units of their own height.
+template <int D, int R, int RP>
+const void* lookup(int form) {
+  if constexpr (RP == 0)
+    if (form == kScheduledOnce) return kernel<D, R, RP, kScheduledOnce>();
+  return form == kStatic ? kernel<D, R, RP, kStatic>() : kernel<D, R, RP, kScheduled>();
+}
+template <int D, int R>
+const void* lookup(int RP, int form) {
+  if constexpr (R * D <= 256) {
+    if (RP == 0) return lookup<D, R, 0>(form);
+    if (RP == R) return lookup<D, R, R>(form);
+    if constexpr (R == 1 && 2 * D <= 256)
+      if (RP == 2) return lookup<D, R, 2>(form);
+    if constexpr (R == 1 && 4 * D <= 256)
+      if (RP == 4) return lookup<D, R, 4>(form);
   }
   return nullptr;
+}
+template <int D>
+const void* lookup(int R, int RP, int form) {
+  return R == 1 ? lookup<D, 1>(RP, form) : R == 2 ? lookup<D, 2>(RP, form) : lookup<D, 4>(RP, form);
 }
 
 }  // namespace
@@ -34,8 +42,10 @@ const void* lookup(int R, int RP) {
 #define FAGQ_ATTN_NAME2(e, q, s) lookup_e##e##_q##q##_s##s
 #define FAGQ_ATTN_NAME(e, q, s) FAGQ_ATTN_NAME2(e, q, s)
 
-const void* FAGQ_ATTN_NAME(FAGQ_ATTN_E, FAGQ_ATTN_QF, FAGQ_ATTN_SF)(int D, int R, int RP) {
-  return D == 64 ? lookup<64>(R, RP) : D == 128 ? lookup<128>(R, RP) : lookup<256>(R, RP);
+const void* FAGQ_ATTN_NAME(FAGQ_ATTN_E, FAGQ_ATTN_QF, FAGQ_ATTN_SF)(int D, int R, int RP, int form) {
+  return D == 64    ? lookup<64>(R, RP, form)
+         : D == 128 ? lookup<128>(R, RP, form)
+                    : lookup<256>(R, RP, form);
 }
 
 }  // namespace attn

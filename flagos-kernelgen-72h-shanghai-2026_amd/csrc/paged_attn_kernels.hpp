@@ -5,12 +5,20 @@
 // of log 2), p = 2^(x - m), l = sum p, o = sum p v; parts of a row's keys have m, l and o of
 // their own and are joined by o = sum 2^(m_i - m) o_i.
 //
-// A unit of work is 16 R query rows that read the same keys (the rows of one sequence that share
-// a cache head; for the shared prefix, those of the whole batch) times a chunk of keys.  R D <= 256:
-// with more rows the registers hold one wave on a SIMD, whose loads and products wait for each
-// other (64 rows of 64 sequences behind 32768 keys, heads of 128: R = 2 145 us, R = 4 234).  The four
-// waves of a workgroup take its steps of 32 keys in turn, each with m, l and o of its own, and are
-// joined through LDS; chunks are joined by a second kernel.
+// A unit of work is 16 R query rows that read the same keys: the rows of one sequence that share a
+// cache head, or for the shared prefix those of the whole batch.  R D <= 256: with more rows the
+// registers hold one wave on a SIMD, whose loads and products wait for each other (64 rows of 64
+// sequences behind 32768 keys, heads of 128: R = 2 145 us, R = 4 234).  A workgroup takes a range
+// of a unit's keys; its four waves take the steps of 32 keys in turn, each with m, l and o of its
+// own, and are joined through LDS.  How units are cut:
+//   scheduled  The rounds of 128 keys of all units in a row are shared out evenly, so that every
+//              workgroup reads as much as the others however the lengths differ and whatever bound
+//              on them the host knows (64 sequences of 1400 to 8192 tokens: 116 us, with chunks
+//              131).  Each workgroup works that out by itself from the lengths.
+//   static     Chunks of one size, chosen by the host: the prefix; sequences of more rows than a
+//              unit has; and calls of few rounds, where working out the shares takes longer than
+//              uneven ones (4 sequences of 1000 tokens: 8.2 us, scheduled 10.3).
+// The parts of a cut unit are joined by a second kernel.
 //
 // Keys and values go from HBM straight into the registers that feed the matrix instructions
 // (16 x 16 x 32), with no LDS and no shuffle on the way:
@@ -41,10 +49,17 @@ namespace attn {
 
 constexpr int kWaves = 4;
 constexpr int kStep = 32;            // keys of a wave's step
+constexpr int kRound = kStep * kWaves;
 constexpr float kLow = -3.0e38f;     // running maximum before the first key
 // The running maximum follows a row's scores only where they pass it by this much (p <= 2^8 then,
 // which neither the sums nor fp16 probabilities mind), so that o is rarely multiplied.
 constexpr float kSlack = 8.0f;
+constexpr float kPartCost = 15.0f;   // what a part costs the joining kernel, in keys of a workgroup
+
+// kScheduledOnce: the codes are read past the caches (64 sequences of 8192 tokens, 64 + 8 heads of
+// 128, 1.07 GB: 172 against 186 us); calls whose cache may still hold what the last one read
+// lose by it (8 of 4000 tokens, 32 heads, 131 MB: 46 against 36 us).
+enum Form { kStatic = 0, kScheduled = 1, kScheduledOnce = 2 };
 
 struct Args {
   const uint16_t* q;
@@ -55,9 +70,13 @@ struct Args {
   const int32_t* table;
   const void* lens;
   const int32_t* prefix;
-  uint16_t* out;             // one chunk for each row: the result itself
-  float* part;               // else [rows][chunks][D], then m and l [rows][chunks][2]
+  uint16_t* out;
+  // Parts of cut units: o [index][D], then {m, l} [index][2].  Index: row * row_parts + i (i: chunk
+  // of the prefix, then a chunk of its own keys or all of them), behind those
+  // segment_at(workgroup, slot) + row of the unit.
+  float* part;
   float* part_ml;
+  int32_t* sched;            // scheduled: each sequence's first round, then the rounds of a workgroup
   int32_t num_pages;
   int32_t qs[3];             // {sequence, token, head} strides, elements
   int32_t B, S, Hq, H, group;
@@ -65,10 +84,12 @@ struct Args {
   int32_t width;             // pages of a row of the table
   int32_t prefix_len;
   int32_t most;              // tokens of a sequence that are read at most
-  int32_t chunk, prefix_chunk;        // keys of a chunk, multiples of kStep * kWaves
-  int32_t chunks, prefix_chunks;      // chunks of a row: its own, and of the prefix
+  int32_t chunk, prefix_chunk;        // keys of a chunk, multiples of kRound
+  int32_t chunks, prefix_chunks;      // chunks of a row: its own (static), and of the prefix
+  int32_t row_parts;
   int32_t tiles, prefix_tiles;        // row tiles of a sequence and cache head; of the batch
   int32_t prefix_items, items;        // workgroups of the prefix, ahead of the others
+  int32_t slots;                      // workgroups that the schedule fills
   int32_t idx64;
   float scale2;                       // sm_scale * log2(e)
 };
@@ -125,6 +146,23 @@ __device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi) {
   return u32x4{a[0], a[1], b[0], b[1]};
 }
 
+// Rounds of a sequence's units: one for a sequence without keys, whose rows are written too.
+__device__ __forceinline__ int32_t own_length(const void* lens, int idx64, int32_t most, int b) {
+  const int64_t n = idx64 ? static_cast<const int64_t*>(lens)[b]
+                          : (int64_t) static_cast<const int32_t*>(lens)[b];
+  return (int32_t)cache::seen_tokens(n, most, 1, 0);
+}
+__device__ __forceinline__ int32_t rounds_of(int32_t len) {
+  const int32_t n = (len + kRound - 1) / kRound;
+  return n > 1 ? n : 1;
+}
+
+// First index of the parts that a workgroup leaves of units of `height` rows: slot 1 of the unit
+// that it began and did not finish, slot 0 of the one that it did not begin.
+__device__ __forceinline__ int64_t segment_at(int64_t first, int height, int wg, int slot) {
+  return first + ((int64_t)wg * 2 + slot) * height;
+}
+
 // Maximum (sum) over the four lanes c, c + 16, c + 32, c + 48; every one of them receives it.
 __device__ __forceinline__ float cross_max(float v) {
   const uint32_t u = __float_as_uint(v);
@@ -148,25 +186,34 @@ struct Pages {
   int32_t p[2];
 };
 
-template <int NT>
+// ONCE: the codes are read once and are too many to be found in a cache by the next call.
+template <bool ONCE, typename T>
+__device__ __forceinline__ T load_codes(const uint8_t* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  else return *reinterpret_cast<const T*>(p);
+}
+template <int NT, bool ONCE>
 __device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t (&v)[NT / 4]) {
   if constexpr (NT == 4) {
-    v[0] = *reinterpret_cast<const uint32_t*>(p);
+    v[0] = load_codes<ONCE, uint32_t>(p);
   } else if constexpr (NT == 8) {
-    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+    const u32x2 x = load_codes<ONCE, u32x2>(p);
     v[0] = x[0], v[1] = x[1];
   } else {
-    const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+    const u32x4 x = load_codes<ONCE, u32x4>(p);
     v[0] = x[0], v[1] = x[1], v[2] = x[2], v[3] = x[3];
   }
 }
 
 // The table's entry for the tile of 16 keys at `tok`, past its end -1; not checked yet, so that
-// nothing waits for it until `checked`.
+// nothing waits for it until `checked`.  A scalar load (the table is constant during the kernel,
+// which the compiler cannot know of a kernel that stores): a vector load would stand in line with
+// the codes' and be waited for with them.
 __device__ __forceinline__ int32_t entry_of(const int32_t* pages, int32_t width, int shift,
                                             int32_t tok) {
+  using Constant = const __attribute__((address_space(4))) int32_t;
   const int32_t p = tok >> shift;
-  return p < width ? pages[p] : -1;
+  return p < width ? reinterpret_cast<Constant*>(reinterpret_cast<uintptr_t>(pages))[p] : -1;
 }
 __device__ __forceinline__ int32_t checked(int32_t page, int32_t num_pages) {
   return page < num_pages ? page : -1;          // negative: no page
@@ -211,7 +258,7 @@ struct RawValues {
   typename Scales<SF>::type s[2];
 };
 
-template <int D, int SF>
+template <int D, int SF, bool ONCE>
 __device__ __forceinline__ void load_keys(const Args& a, int h, int lane, int32_t tok,
                                           const Pages& pages, RawKeys<D, SF>& r) {
   const int c = lane & 15, g = lane >> 4;
@@ -221,12 +268,12 @@ __device__ __forceinline__ void load_keys(const Args& a, int h, int lane, int32_
     const uint8_t* k = a.kc + row * D;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i)
-      r.k[t][i] = *reinterpret_cast<const u32x4*>(k + (uint32_t)(c * D + 16 * g + 64 * i));
+      r.k[t][i] = load_codes<ONCE, u32x4>(k + (uint32_t)(c * D + 16 * g + 64 * i));
     r.s[t] = load_scales<SF>(a.ks, row + 4 * g);
   }
 }
 
-template <int D, int SF>
+template <int D, int SF, bool ONCE>
 __device__ __forceinline__ void load_values(const Args& a, int h, int lane, int32_t tok,
                                             const Pages& pages, RawValues<D, SF>& r) {
   constexpr int NT = D / 16;
@@ -237,7 +284,7 @@ __device__ __forceinline__ void load_values(const Args& a, int h, int lane, int3
     const uint8_t* v = a.vc + row * D;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      load_bytes<NT>(v + (uint32_t)((4 * g + i) * D + c * NT), r.v[4 * t + i]);
+      load_bytes<NT, ONCE>(v + (uint32_t)((4 * g + i) * D + c * NT), r.v[4 * t + i]);
     r.s[t] = load_scales<SF>(a.vs, row + 4 * g);
   }
 }
@@ -392,11 +439,10 @@ struct Keys {
   int32_t begin, end;          // of this workgroup
 };
 
-template <int E, int QF, int SF, int D, int R>
+template <int E, int QF, int SF, int D, int R, bool ONCE>
 __device__ __forceinline__ void run_steps(const Args& a, const Keys& k, int h, int lane, int wave,
                                           int32_t all, int32_t end, Rows<E, D, R>& s) {
   int32_t tok = k.begin + wave * kStep;
-  constexpr int32_t kNext = kStep * kWaves;
   if (tok >= k.end) return;
   // Table entries are read a step ahead of the loads that need them.
   auto entries = [&](int32_t t) {
@@ -406,62 +452,31 @@ __device__ __forceinline__ void run_steps(const Args& a, const Keys& k, int h, i
   auto check = [&](const Pages& p) {
     return Pages{{checked(p.p[0], a.num_pages), checked(p.p[1], a.num_pages)}};
   };
-  Pages ahead;
-  auto work = [&](RawKeys<D, SF>& keys, RawValues<D, SF>& values, const Pages& pages, auto between) {
+  // One set of registers each: the next step's keys are under way during this one's softmax and
+  // values, its values during the next scores.  (A second set, with both under way during all of a
+  // step, changed nothing where HBM bounds: 187 against 186 us.)
+  RawKeys<D, SF> keys;
+  RawValues<D, SF> values;
+  Pages pages = check(entries(tok));
+  Pages ahead = entries(tok + kRound);
+  load_keys<D, SF, ONCE>(a, h, lane, tok, pages, keys);
+  load_values<D, SF, ONCE>(a, h, lane, tok, pages, values);
+  for (;;) {
+    const int32_t next = tok + kRound;
+    const bool more = next < k.end;
+    const Pages next_pages = check(ahead);
+    ahead = entries(next + kRound);
     f32x4 x[R][2];
     float ks[8];
     scores<E, QF, SF, D, R>(lane, keys, s, x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) ks[i] = scale_of<SF>(keys.s[i / 4], i % 4) * a.scale2;
-    between();
+    if (more) load_keys<D, SF, ONCE>(a, h, lane, next, next_pages, keys);
     join<E, QF, SF, D, R>(lane, tok, all, end, pages, x, ks, values, s);
-  };
-  if constexpr (R * D <= 128) {
-    // Bound by HBM: two sets of registers, the next step's loads all under way during this one.
-    RawKeys<D, SF> keys[2];
-    RawValues<D, SF> values[2];
-    Pages pages[2];
-    pages[0] = check(entries(tok));
-    ahead = entries(tok + kNext);
-    load_keys<D, SF>(a, h, lane, tok, pages[0], keys[0]);
-    load_values<D, SF>(a, h, lane, tok, pages[0], values[0]);
-    auto one = [&](int now, int then) {
-      const int32_t next = tok + kNext;
-      const bool more = next < k.end;
-      pages[then] = check(ahead);
-      ahead = entries(next + kNext);
-      if (more) {
-        load_keys<D, SF>(a, h, lane, next, pages[then], keys[then]);
-        load_values<D, SF>(a, h, lane, next, pages[then], values[then]);
-      }
-      work(keys[now], values[now], pages[now], [] {});
-      tok = next;
-      return more;
-    };
-    while (one(0, 1) && one(1, 0)) {
-    }
-  } else {
-    // Short of registers: one set each, the next step's keys under way during this one's softmax
-    // and values, its values during the next scores.
-    RawKeys<D, SF> keys;
-    RawValues<D, SF> values;
-    Pages pages = check(entries(tok));
-    ahead = entries(tok + kNext);
-    load_keys<D, SF>(a, h, lane, tok, pages, keys);
-    load_values<D, SF>(a, h, lane, tok, pages, values);
-    for (;;) {
-      const int32_t next = tok + kNext;
-      const bool more = next < k.end;
-      const Pages next_pages = check(ahead);
-      ahead = entries(next + kNext);
-      work(keys, values, pages, [&] {
-        if (more) load_keys<D, SF>(a, h, lane, next, next_pages, keys);
-      });
-      if (!more) return;
-      load_values<D, SF>(a, h, lane, next, next_pages, values);
-      tok = next;
-      pages = next_pages;
-    }
+    if (!more) return;
+    load_values<D, SF, ONCE>(a, h, lane, next, next_pages, values);
+    tok = next;
+    pages = next_pages;
   }
 }
 
@@ -489,41 +504,30 @@ __device__ __forceinline__ Place place_of(int item, int items, int tiles) {
   return {j % tiles, j / tiles * 8 + (item & 7)};
 }
 
-// One unit and chunk.  `item`: workgroup number within its kind.
-template <int E, int QF, int SF, int D, int R, bool PREFIX>
-__device__ __forceinline__ void unit(const Args& a, int item, char* lds) {
+// What a workgroup does at a time: a range of one unit's keys.
+struct Segment {
+  int b, h, tile;            // sequence (own keys), cache head, row tile
+  int32_t len;               // own keys of the sequence
+  Keys keys;
+  int64_t to;                // index of row 0 of its part; kRowParts: of each row's own; kOut
+  int row_part;              // kRowParts: which of a row's parts
+};
+constexpr int64_t kOut = -1;          // the result itself
+constexpr int64_t kRowParts = -2;
+
+template <int E, int QF, int SF, int D, int R, bool PREFIX, bool ONCE>
+__device__ __forceinline__ void run_segment(const Args& a, const Segment& seg, Shared<D, R>& sh) {
   constexpr int NT = D / 16;
-  Shared<D, R>& sh = *reinterpret_cast<Shared<D, R>*>(lds);
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  int lane = threadIdx.x & 63;
+  // Opaque, so that what a segment derives from it is not kept in registers from one to the next.
+  asm volatile("" : "+v"(lane));
+  const int c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int chunks = PREFIX ? a.prefix_chunks : a.chunks;
-  const Place place = PREFIX ? place_of(item, a.prefix_items, a.prefix_tiles)
-                             : place_of(item, a.items, a.tiles);
-  const int tile = place.tile;
-  const int chunk = place.group % chunks;
-  const int h = place.group / chunks % a.H;
-  const int b = place.group / chunks / a.H;     // own keys: the sequence
+  const int h = seg.h, b = seg.b, tile = seg.tile;
+  const int32_t len = seg.len;
   const int per = a.S * a.group;                // rows of a sequence and cache head
   const int rows = PREFIX ? a.B * per : per;
-  Keys k;
-  int32_t len = 0;                              // a sequence's own keys
-  if constexpr (PREFIX) {
-    k.pages = a.prefix;
-    k.width = ((a.prefix_len - 1) >> a.page_shift) + 1;
-    k.begin = chunk * a.prefix_chunk;
-    k.end = k.begin + a.prefix_chunk < a.prefix_len ? k.begin + a.prefix_chunk : a.prefix_len;
-  } else {
-    const int64_t n = a.idx64 ? static_cast<const int64_t*>(a.lens)[b]
-                              : (int64_t) static_cast<const int32_t*>(a.lens)[b];
-    len = (int32_t)cache::seen_tokens(n, a.most, 1, 0);
-    k.pages = a.table + (int64_t)b * a.width;
-    k.width = a.width;
-    k.begin = chunk * a.chunk;
-    k.end = k.begin + a.chunk < len ? k.begin + a.chunk : len;
-    // The joining kernel reads as many chunks as the length has.  The first one is always
-    // written, for rows without keys.
-    if (k.begin >= len && chunk > 0) return;
-  }
+  Keys k = seg.keys;
   // Row i of the unit: i = (b,) s, query head of the group.
   auto row_of = [&](int i) {
     Row r;
@@ -566,7 +570,7 @@ __device__ __forceinline__ void unit(const Args& a, int item, char* lds) {
     end = (int32_t)cache::seen_tokens(len, a.most, a.S, row_of(last < rows ? last : rows - 1).s);
     if (k.end > end) k.end = end;
   }
-  run_steps<E, QF, SF, D, R>(a, k, h, lane, wave, all, end, s);
+  run_steps<E, QF, SF, D, R, ONCE>(a, k, h, lane, wave, all, end, s);
 
   // Join the waves.
 #pragma unroll
@@ -607,14 +611,13 @@ __device__ __forceinline__ void unit(const Args& a, int item, char* lds) {
       const Row w = row_of(i);
       const int64_t row = ((int64_t)w.b * a.S + w.s) * a.Hq + w.hq;
       const int d = NT * (4 * g + wave);
-      const int n = a.prefix_chunks + a.chunks;
-      if (n == 1) {
+      if (seg.to == kOut) {
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
         uint32_t* to = reinterpret_cast<uint32_t*>(a.out + row * D + d);
 #pragma unroll
         for (int j = 0; j < NT; j += 2) to[j / 2] = pack16<E>(o[j] * inv, o[j + 1] * inv);
       } else {
-        const int64_t at = row * n + (PREFIX ? chunk : a.prefix_chunks + chunk);
+        const int64_t at = seg.to == kRowParts ? row * a.row_parts + seg.row_part : seg.to + i;
         float* to = a.part + at * D + d;
 #pragma unroll
         for (int j = 0; j < NT; j += 4)
@@ -628,31 +631,229 @@ __device__ __forceinline__ void unit(const Args& a, int item, char* lds) {
   }
 }
 
-// RP: row tiles of a unit of the prefix (0: there is none), R: of the others.
-template <int E, int QF, int SF, int D, int R, int RP>
+// One chunk of the prefix or (static) of a sequence's own keys.  `item`: workgroup number within
+// its kind.
+template <int E, int QF, int SF, int D, int R, bool PREFIX>
+__device__ __forceinline__ void run_chunk(const Args& a, int item, Shared<D, R>& sh) {
+  const int chunks = PREFIX ? a.prefix_chunks : a.chunks;
+  const Place place = PREFIX ? place_of(item, a.prefix_items, a.prefix_tiles)
+                             : place_of(item, a.items, a.tiles);
+  Segment s;
+  s.tile = place.tile;
+  const int chunk = place.group % chunks;
+  s.h = place.group / chunks % a.H;
+  s.b = place.group / chunks / a.H;
+  s.len = 0;
+  s.row_part = PREFIX ? chunk : a.prefix_chunks + chunk;
+  s.to = a.row_parts > 1 ? kRowParts : kOut;
+  if constexpr (PREFIX) {
+    s.keys.pages = a.prefix;
+    s.keys.width = ((a.prefix_len - 1) >> a.page_shift) + 1;
+    s.keys.begin = chunk * a.prefix_chunk;
+    s.keys.end = s.keys.begin + a.prefix_chunk < a.prefix_len ? s.keys.begin + a.prefix_chunk
+                                                              : a.prefix_len;
+  } else {
+    s.len = own_length(a.lens, a.idx64, a.most, s.b);
+    s.keys.pages = a.table + (int64_t)s.b * a.width;
+    s.keys.width = a.width;
+    s.keys.begin = chunk * a.chunk;
+    s.keys.end = s.keys.begin + a.chunk < s.len ? s.keys.begin + a.chunk : s.len;
+    // The joining kernel reads as many chunks as the length has.  The first one is always
+    // written, for rows without keys.
+    if (s.keys.begin >= s.len && chunk > 0) return;
+  }
+  run_segment<E, QF, SF, D, R, PREFIX, false>(a, s, sh);
+}
+
+// LDS of the schedule.
+struct Schedule {
+  int32_t sum[kWaves], most[kWaves];
+  int32_t b, first;
+};
+
+// A workgroup's share of all units' rounds in a row (sequence, then head): [lo, hi), and the
+// sequence of round lo with its first round.
+struct Share {
+  int32_t lo, hi, b, first;
+};
+
+// q rounds for each workgroup.  Few rounds for each leave many parts for each row to join: a part
+// costs as much as kPartCost keys, so n rounds are best cut into parts of sqrt(n kPartCost / kRound).
+__device__ __forceinline__ int32_t rounds_each(int32_t total, int32_t most, int32_t slots) {
+  const int32_t q = (total + slots - 1) / slots;
+  const int32_t least = (int32_t)(__builtin_sqrtf((float)most * (kPartCost / kRound)) + 0.5f);
+  return q > least ? q : least > 1 ? least : 1;
+}
+__device__ __forceinline__ void cut_out(int wg, int32_t q, int32_t total, Share& s) {
+  const int64_t lo = (int64_t)wg * q;
+  s.lo = lo < total ? (int32_t)lo : total;
+  s.hi = total - s.lo > q ? s.lo + q : total;
+}
+__device__ __forceinline__ int32_t scan64(int32_t v, int lane) {     // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int32_t o = __shfl_up(v, d);
+    v += lane >= d ? o : 0;
+  }
+  return v;
+}
+__device__ __forceinline__ int32_t max64(int32_t v) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int32_t o = __shfl_xor(v, d);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+// Up to 64 sequences, one for each lane: every wave by itself.
+__device__ __forceinline__ Share share_of_few(const Args& a, int wg, int32_t len) {
+  const int lane = threadIdx.x & 63;
+  const int32_t n = lane < a.B ? rounds_of(len) * a.H : 0;
+  const int32_t upto = scan64(n, lane), first = upto - n;
+  const int32_t total = __builtin_amdgcn_readlane(upto, 63);
+  const int32_t q = rounds_each(total, max64(n) / a.H, a.slots);
+  Share s;
+  cut_out(wg, q, total, s);
+  const uint64_t here = __ballot(s.lo >= first && s.lo < upto);
+  s.b = here ? (int)__builtin_ctzll(here) : 0;
+  s.first = __builtin_amdgcn_readlane(first, s.b);
+  if (wg == 0 && threadIdx.x < 64) {
+    if (lane < a.B) a.sched[lane] = first;
+    if (lane == 0) a.sched[a.B] = q;
+  }
+  return s;
+}
+
+// Any number of sequences: the workgroup's threads together, twice over the lengths.
+__device__ __forceinline__ Share share_of_many(const Args& a, int wg, Schedule& sc) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int32_t sum = 0, most = 0;
+  for (int b = tid; b < a.B; b += 64 * kWaves) {
+    const int32_t n = rounds_of(own_length(a.lens, a.idx64, a.most, b));
+    sum += n;
+    most = n > most ? n : most;
+  }
+  sum = scan64(sum, lane);
+  most = max64(most);
+  if (lane == 63) {
+    sc.sum[wave] = sum;
+    sc.most[wave] = most;
+  }
+  if (tid == 0) {
+    sc.b = 0;
+    sc.first = 0;
+  }
+  __syncthreads();
+  int32_t total = 0;
+  most = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    total += sc.sum[w];
+    most = sc.most[w] > most ? sc.most[w] : most;
+  }
+  total *= a.H;
+  const int32_t q = rounds_each(total, most, a.slots);
+  Share s;
+  cut_out(wg, q, total, s);
+  // The sequence that holds round lo; workgroup 0 writes all sequences' first rounds down.
+  int32_t base = 0;
+  for (int b0 = 0; b0 < a.B && (wg == 0 || base <= s.lo); b0 += 64 * kWaves) {
+    const int b = b0 + tid;
+    const int32_t n = b < a.B ? rounds_of(own_length(a.lens, a.idx64, a.most, b)) * a.H : 0;
+    const int32_t upto = scan64(n, lane);
+    __syncthreads();                            // the sums of before have been read
+    if (lane == 63) sc.sum[wave] = upto;
+    __syncthreads();
+    int32_t first = base + upto - n;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      first += w < wave ? sc.sum[w] : 0;
+      base += sc.sum[w];
+    }
+    if (b < a.B) {
+      if (wg == 0) a.sched[b] = first;
+      if (s.lo >= first && s.lo < first + n) {
+        sc.b = b;
+        sc.first = first;
+      }
+    }
+  }
+  if (wg == 0 && tid == 0) a.sched[a.B] = q;
+  __syncthreads();
+  s.b = __builtin_amdgcn_readfirstlane(sc.b);
+  s.first = __builtin_amdgcn_readfirstlane(sc.first);
+  return s;
+}
+
+template <int E, int QF, int SF, int D, int R, bool ONCE>
+__device__ __forceinline__ void run_share(const Args& a, int wg, Shared<D, R>& sh, Schedule& sc) {
+  const int lane = threadIdx.x & 63;
+  const bool few = a.B <= 64;
+  const int32_t lens = few ? own_length(a.lens, a.idx64, a.most, lane < a.B ? lane : 0) : 0;
+  const Share share = few ? share_of_few(a, wg, lens) : share_of_many(a, wg, sc);
+  const int32_t lo = share.lo, hi = share.hi;
+  int b = share.b;
+  int32_t first = share.first;
+  for (int32_t pos = lo; pos < hi;) {
+    Segment s;
+    s.b = b;
+    s.tile = 0;
+    s.len = few ? __builtin_amdgcn_readlane(lens, b)
+                : __builtin_amdgcn_readfirstlane(own_length(a.lens, a.idx64, a.most, b));
+    const int32_t n = rounds_of(s.len);
+    s.h = (pos - first) / n;
+    const int32_t r0 = pos - first - s.h * n;
+    const int32_t r1 = n - r0 < hi - pos ? n : r0 + (hi - pos);
+    s.keys.pages = a.table + (int64_t)b * a.width;
+    s.keys.width = a.width;
+    s.keys.begin = r0 * kRound;
+    s.keys.end = r1 == n ? s.len : r1 * kRound;
+    s.row_part = a.prefix_chunks;
+    s.to = r0 > 0 || r1 < n
+               ? segment_at((int64_t)a.B * a.S * a.Hq * a.row_parts, 16 * R, wg, r0 > 0 ? 0 : 1)
+           : a.prefix_len > 0 ? kRowParts
+                              : kOut;
+    if (pos > lo) __syncthreads();              // the last segment's LDS has been read
+    run_segment<E, QF, SF, D, R, false, ONCE>(a, s, sh);
+    pos += r1 - r0;
+    if (r1 == n && s.h == a.H - 1) {
+      first += n * a.H;
+      ++b;
+    }
+  }
+}
+
+// R: row tiles of a unit of the sequences' own keys, RP: of the prefix (0: there is none).
+template <int E, int QF, int SF, int D, int R, int RP, int FORM>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention(Args a) {
   constexpr int kRows = R > RP ? R : RP;
   __shared__ __align__(16) char lds[sizeof(Shared<D, kRows>)];
+  __shared__ Schedule sc;
   const int item = (int)blockIdx.x;
   if constexpr (RP > 0) {
     if (item < a.prefix_items) {
-      unit<E, QF, SF, D, RP, true>(a, item, lds);
+      run_chunk<E, QF, SF, D, RP, true>(a, item, *reinterpret_cast<Shared<D, RP>*>(lds));
       return;
     }
   }
-  unit<E, QF, SF, D, R, false>(a, item - a.prefix_items, lds);
+  Shared<D, R>& sh = *reinterpret_cast<Shared<D, R>*>(lds);
+  if constexpr (FORM == kStatic)
+    run_chunk<E, QF, SF, D, R, false>(a, item - a.prefix_items, sh);
+  else
+    run_share<E, QF, SF, D, R, FORM == kScheduledOnce>(a, item - a.prefix_items, sh, sc);
 }
 
 // Kernels for an element type (ET_BF16, ET_F16), code format (QF_FP8, QF_I8_RNE) and scale format:
 // lookup_e<E>_q<QF>_s<SF>, one for each instantiation unit.
-const void* lookup_e0_q0_s0(int D, int R, int RP);
-const void* lookup_e0_q0_s1(int D, int R, int RP);
-const void* lookup_e0_q1_s0(int D, int R, int RP);
-const void* lookup_e0_q1_s1(int D, int R, int RP);
-const void* lookup_e1_q0_s0(int D, int R, int RP);
-const void* lookup_e1_q0_s1(int D, int R, int RP);
-const void* lookup_e1_q1_s0(int D, int R, int RP);
-const void* lookup_e1_q1_s1(int D, int R, int RP);
+const void* lookup_e0_q0_s0(int D, int R, int RP, int form);
+const void* lookup_e0_q0_s1(int D, int R, int RP, int form);
+const void* lookup_e0_q1_s0(int D, int R, int RP, int form);
+const void* lookup_e0_q1_s1(int D, int R, int RP, int form);
+const void* lookup_e1_q0_s0(int D, int R, int RP, int form);
+const void* lookup_e1_q0_s1(int D, int R, int RP, int form);
+const void* lookup_e1_q1_s0(int D, int R, int RP, int form);
+const void* lookup_e1_q1_s1(int D, int R, int RP, int form);
 
 }  // namespace attn
 }  // namespace fagq
