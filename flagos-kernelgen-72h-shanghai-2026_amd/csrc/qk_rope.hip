@@ -24,10 +24,8 @@ namespace rope {
 namespace {
 
 constexpr int kWaves = 4;             // waves per workgroup
-constexpr int kBwdAhead = 2;          // passes of a wave of the backward whose loads are under way
-                                      // at once
-constexpr int kMaxBwdGroups = 512;    // workgroups of the backward (two per CU), each with its
-                                      // own sums of the weight gradients
+constexpr int kMaxBwdGroups = 768;    // workgroups of the backward (three per CU), each with its
+                                      // own sum of a weight's gradient
 constexpr int kSumRows = 64;          // partial sums that a column's threads share out
 
 struct Args {
@@ -42,12 +40,11 @@ struct Args {
   void* ko;
   const void* dq;    // backward: dq_out, dk_out
   const void* dk;
-  float* sums;       // backward: [workgroups][2][D]
+  float* sums;       // backward: [workgroups][D]
   int64_t table_rows;
   int32_t qs[2], ks[2], qos[2], kos[2], dqs[2], dks[2];   // {token, head} strides, elements
   int32_t T, Hq, Hk, D, R;
-  int32_t splits;    // backward: items of a token
-  int32_t per_wave;  // backward: passes of an item
+  int32_t gq;        // backward: workgroups of q
   int32_t idx64;
   float eps;
 };
@@ -184,9 +181,13 @@ __device__ __forceinline__ float rsqrt_of(float v) {
   return tiny ? r * 0x1p50f : r;
 }
 
+// A scalar load: positions are constant during the kernel, which the compiler cannot know of one
+// that stores.
 __device__ __forceinline__ int64_t position(const Args& a, int t) {
-  return a.idx64 ? static_cast<const int64_t*>(a.pos)[t]
-                 : (int64_t) static_cast<const int32_t*>(a.pos)[t];
+  using C64 = const __attribute__((address_space(4))) int64_t;
+  using C32 = const __attribute__((address_space(4))) int32_t;
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a.pos);
+  return a.idx64 ? reinterpret_cast<C64*>(p)[t] : (int64_t) reinterpret_cast<C32*>(p)[t];
 }
 
 // The heads of q or of k, for one wave: where they start and how far apart.
@@ -281,122 +282,111 @@ __global__ __launch_bounds__(64 * kWaves) void qk_norm_rope_fwd(Args a) {
   if (on) store16<E, true>(s.y + (int64_t)h * s.yh, l, n);
 }
 
+// A workgroup works on q (the first a.gq of them) or on k, so that it holds one weight and one sum:
+// its waves walk the passes of that side in the order of memory, each pass's position read one
+// ahead (its angles would wait for it otherwise).
 template <int E, int LPR, bool INTER>
-__global__ __launch_bounds__(64 * kWaves) void qk_norm_rope_bwd(Args a) {
+__global__ __launch_bounds__(64 * kWaves, 3) void qk_norm_rope_bwd(Args a) {
   using T = typename Elem<E>::type;
   constexpr int kRows = 64 / LPR;
-  extern __shared__ float sums[];               // [waves][2][D]
+  extern __shared__ float sums[];               // [waves][D]
+  const bool isq = (int)blockIdx.x < a.gq;
   const int wg_wave = threadIdx.x / 64;
-  const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * kWaves + wg_wave));
-  const int waves = gridDim.x * kWaves;
+  const int group = isq ? (int)blockIdx.x : (int)blockIdx.x - a.gq;
+  const int wave = __builtin_amdgcn_readfirstlane(group * kWaves + wg_wave);
+  const int waves = (isq ? a.gq : (int)gridDim.x - a.gq) * kWaves;
   const Lane l = lane_of<LPR, INTER>(threadIdx.x & 63, a.D, a.R);
-  const int pq = (a.Hq + kRows - 1) / kRows, passes = pq + (a.Hk + kRows - 1) / kRows;
-  const Raw16<E> raw_w[2] = {load16<E>(static_cast<const T*>(a.qw), l, l.on),
-                             load16<E>(static_cast<const T*>(a.kw), l, l.on)};
+  const int passes = ((isq ? a.Hq : a.Hk) + kRows - 1) / kRows;
+  const Raw16<E> weight = load16<E>(static_cast<const T*>(isq ? a.qw : a.kw), l, l.on);
   const float inv_d = 1.0f / (float)a.D;
-  float dw[2][16] = {};                         // of q's and k's weight
-  for (int item = wave; item < a.T * a.splits; item += waves) {
-    const int t = item / a.splits;
-    const int p0 = (item - t * a.splits) * a.per_wave;
-    const int p1 = p0 + a.per_wave < passes ? p0 + a.per_wave : passes;
-    const int64_t pos = position(a, t);
+  float dw[16] = {};
+  const int items = a.T * passes;
+  int64_t next_pos = wave < items ? position(a, wave / passes) : 0;
+  for (int item = wave; item < items; item += waves) {
+    const int t = item / passes;
+    const Heads<E> s = heads_of<E, true>(a, isq, t);
+    const int h = (item - t * passes) * kRows + l.row;
+    const bool on = l.on && h < s.H;
+    const Raw16<E> raw = load16<E>(s.x + (int64_t)h * s.xh, l, on);
+    const Raw16<E> raw_d = load16<E>(s.dy + (int64_t)h * s.dyh, l, on);
+    const int64_t pos = next_pos;
     const bool real = pos >= 0 && pos < a.table_rows;
     const Turn turn = load_turn(a, l, pos, real);
-    auto run = [&](const Heads<E>& s, const Raw16<E>& weight, float (&acc)[16], int first, int last) {
-      for (int p = first; p < last; p += kBwdAhead) {
-        Raw16<E> raw[kBwdAhead], raw_d[kBwdAhead];
-#pragma unroll
-        for (int u = 0; u < kBwdAhead; ++u) {
-          const int h = (p + u) * kRows + l.row;
-          const bool on = l.on && p + u < last && h < s.H;
-          raw[u] = load16<E>(s.x + (int64_t)h * s.xh, l, on);
-          raw_d[u] = load16<E>(s.dy + (int64_t)h * s.dyh, l, on);
-        }
-#pragma unroll
-        for (int u = 0; u < kBwdAhead; ++u) {
-          if (p + u >= last) break;
-          const int h = (p + u) * kRows + l.row;
-          float n[16], d[16], g[16];
-          unpack16<E>(raw[u], n);
-          unpack16<E>(raw_d[u], d);
-          unpack16<E>(weight, g);
-          rotate<INTER, true>(d, turn);
-          float ss = 0.0f, ax = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            ss = __builtin_fmaf(n[i], n[i], ss);
-            ax = __builtin_fmaf(d[i] * g[i], n[i], ax);
-          }
-          const float rstd = rsqrt_of(row_sum<LPR>(ss) * inv_d + a.eps);
-          const float back = row_sum<LPR>(ax) * inv_d * rstd * rstd;
-          if (real) {
-            // Rows past the last head hold zeros: they add nothing, or 0 * inf where eps is 0.
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float gx = d[i] * (n[i] * rstd);
-              acc[i] += h < s.H ? gx : 0.0f;
-              n[i] = rstd * __builtin_fmaf(-n[i], back, d[i] * g[i]);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) n[i] = 0.0f;
-          }
-          if (l.on && h < s.H) store16<E, false>(s.y + (int64_t)h * s.yh, l, n);
-        }
-      }
-    };
-    if (p0 < pq) run(heads_of<E, true>(a, true, t), raw_w[0], dw[0], p0, p1 < pq ? p1 : pq);
-    if (p1 > pq)
-      run(heads_of<E, true>(a, false, t), raw_w[1], dw[1], p0 > pq ? p0 - pq : 0, p1 - pq);
-  }
-#pragma unroll
-  for (int o = 0; o < 2; ++o)
+    if (item + waves < items) next_pos = position(a, (item + waves) / passes);
+    float n[16], d[16], g[16];
+    unpack16<E>(raw, n);
+    unpack16<E>(raw_d, d);
+    unpack16<E>(weight, g);
+    rotate<INTER, true>(d, turn);
+    float ss = 0.0f, ax = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-#pragma unroll
-      for (int m = LPR; m < 64; m *= 2) dw[o][i] += __shfl_xor(dw[o][i], m);
+      ss = __builtin_fmaf(n[i], n[i], ss);
+      ax = __builtin_fmaf(d[i] * g[i], n[i], ax);
     }
+    const float rstd = rsqrt_of(row_sum<LPR>(ss) * inv_d + a.eps);
+    const float back = row_sum<LPR>(ax) * inv_d * rstd * rstd;
+    if (real) {
+      // Rows past the last head hold zeros: they add nothing, or 0 * inf where eps is 0.
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float gx = d[i] * (n[i] * rstd);
+        dw[i] += h < s.H ? gx : 0.0f;
+        n[i] = rstd * __builtin_fmaf(-n[i], back, d[i] * g[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) n[i] = 0.0f;
+    }
+    if (on) store16<E, false>(s.y + (int64_t)h * s.yh, l, n);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+#pragma unroll
+    for (int m = LPR; m < 64; m *= 2) dw[i] += __shfl_xor(dw[i], m);
+  }
   if ((threadIdx.x & 63) < LPR && l.on) {
 #pragma unroll
-    for (int o = 0; o < 2; ++o)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sums[(wg_wave * 2 + o) * a.D + l.c0 + i] = dw[o][i];
-        sums[(wg_wave * 2 + o) * a.D + l.c1 + i] = dw[o][8 + i];
-      }
+    for (int i = 0; i < 8; ++i) {
+      sums[wg_wave * a.D + l.c0 + i] = dw[i];
+      sums[wg_wave * a.D + l.c1 + i] = dw[8 + i];
+    }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * a.D; i += 64 * kWaves) {
+  for (int i = threadIdx.x; i < a.D; i += 64 * kWaves) {
     float s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) s += sums[w * 2 * a.D + i];
-    a.sums[(int64_t)blockIdx.x * 2 * a.D + i] = s;
+    for (int w = 0; w < kWaves; ++w) s += sums[w * a.D + i];
+    a.sums[(int64_t)blockIdx.x * a.D + i] = s;
   }
 }
 
 struct SumArgs {
-  const float* sums;    // [n][2 * D]
+  const float* sums;    // [gq + gk][D]
   float* dqw;
   float* dkw;
-  int32_t n, D;
+  int32_t gq, gk, D;
 };
 
 // The workgroups' sums of 16 columns: 64 threads of each column take every 64th one, then
-// add their own in LDS in a fixed order.
+// add their own in LDS in a fixed order.  blockIdx.y: q or k.
 __global__ __launch_bounds__(16 * kSumRows) void weight_sums(SumArgs a) {
   __shared__ float part[kSumRows][17];
   const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
-  const int col = blockIdx.x * 16 + c;          // 2 D is a multiple of 32
+  const int col = blockIdx.x * 16 + c;          // D is a multiple of 16
+  const bool isq = blockIdx.y == 0;
+  const int n = isq ? a.gq : a.gk;
+  const float* sums = a.sums + (isq ? 0 : (int64_t)a.gq * a.D) + col;
   float s = 0.0f;
 #pragma unroll 8
-  for (int i = r; i < a.n; i += kSumRows) s += a.sums[(int64_t)i * 2 * a.D + col];
+  for (int i = r; i < n; i += kSumRows) s += sums[(int64_t)i * a.D];
   part[r][c] = s;
   __syncthreads();
   for (int half = kSumRows / 2; half > 0; half /= 2) {
     if (r < half) part[r][c] += part[r + half][c];
     __syncthreads();
   }
-  if (r == 0) (col < a.D ? a.dqw[col] : a.dkw[col - a.D]) = part[0][c];
+  if (r == 0) (isq ? a.dqw : a.dkw)[col] = part[0][c];
 }
 
 // ---------------------------------------------------------------------------------- host
@@ -481,21 +471,21 @@ int64_t passes_of(int64_t Hq, int64_t Hk, int64_t D) {
   return (Hq + rows - 1) / rows + (Hk + rows - 1) / rows;
 }
 
-// How the backward shares the passes of a token out over waves: kBwdAhead at a time, one where
-// that leaves waves without work (two on each of the SIMDs of 256 CUs).
+// The backward's workgroups of q and of k, in proportion to their passes.
 struct Split {
-  int64_t splits, per_wave;
+  int64_t gq, gk;
 };
 Split split_for(int64_t T, int64_t Hq, int64_t Hk, int64_t D) {
-  const int64_t passes = passes_of(Hq, Hk, D);
-  const int64_t per = passes * T >= 2 * 4 * 256 * kBwdAhead ? kBwdAhead : 1;
-  return {(passes + per - 1) / per, per};
+  const int64_t rows = 64 / lanes_per_row(D);
+  const int64_t pq = (Hq + rows - 1) / rows, pk = (Hk + rows - 1) / rows;
+  int64_t gq = (kMaxBwdGroups * pq + (pq + pk) / 2) / (pq + pk);
+  gq = gq < 1 ? 1 : gq > kMaxBwdGroups - 1 ? kMaxBwdGroups - 1 : gq;
+  const int64_t gk = kMaxBwdGroups - gq;
+  const int64_t nq = (T * pq + kWaves - 1) / kWaves, nk = (T * pk + kWaves - 1) / kWaves;
+  return {nq < gq ? nq : gq, nk < gk ? nk : gk};
 }
 
-int64_t bwd_groups(int64_t T, int64_t Hq, int64_t Hk, int64_t D) {
-  const int64_t n = (T * split_for(T, Hq, Hk, D).splits + kWaves - 1) / kWaves;
-  return n > kMaxBwdGroups ? kMaxBwdGroups : n;
-}
+int64_t bwd_bytes(const Split& s, int64_t D) { return (s.gq + s.gk) * D * 4; }
 
 int check_common(const void* const* ptrs, int n, const int64_t* strides, int nstrides, int64_t T,
                  int64_t Hq, int64_t Hk, int64_t D, int64_t R, int64_t table_rows, float eps,
@@ -579,7 +569,7 @@ FAGQ_API int64_t fagq_qk_norm_rope_bwd_workspace_bytes(int64_t T, int64_t Hq, in
                                                        int64_t D) {
   using namespace fagq::rope;
   if (check_sizes(T, Hq, Hk, D, 16, 0) != FAGQ_OK) return -1;
-  return bwd_groups(T, Hq, Hk, D) * 2 * D * 4;
+  return bwd_bytes(split_for(T, Hq, Hk, D), D);
 }
 
 FAGQ_API int fagq_qk_norm_rope_bwd_launch(const void* dq_out, const void* dk_out, const void* q,
@@ -598,7 +588,8 @@ FAGQ_API int fagq_qk_norm_rope_bwd_launch(const void* dq_out, const void* dk_out
   const int v = check_common(ptrs, 12, strides, 12, T, Hq, Hk, D, R, table_rows, eps, dtype,
                              index_dtype, positions);
   if (v != FAGQ_OK) return v;
-  const int64_t groups = bwd_groups(T, Hq, Hk, D), need = groups * 2 * D * 4;
+  const Split s = split_for(T, Hq, Hk, D);
+  const int64_t need = bwd_bytes(s, D);
   if (need > 0 && !workspace) return FAGQ_E_NULL;
   if (workspace_bytes < need) return FAGQ_E_SHAPE;
   if (!aligned(workspace, 16)) return FAGQ_E_ALIGN;
@@ -633,9 +624,8 @@ FAGQ_API int fagq_qk_norm_rope_bwd_launch(const void* dq_out, const void* dk_out
   const int dcheck = device_check();
   if (dcheck != FAGQ_OK) return dcheck;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (groups > 0) {
-    const Split s = split_for(T, Hq, Hk, D);
-    if (T * s.splits >= (1ll << 31) - kWaves * kMaxBwdGroups) return FAGQ_E_TOO_LARGE;
+  if (T > 0) {
+    if (T * passes_of(Hq, Hk, D) >= (1ll << 31) - kWaves * kMaxBwdGroups) return FAGQ_E_TOO_LARGE;
     Args a = {};
     a.q = q, a.k = k, a.qw = q_weight, a.kw = k_weight, a.cos = cos, a.sin = sin;
     a.pos = positions, a.qo = dq, a.ko = dk, a.dq = dq_out, a.dk = dk_out;
@@ -644,18 +634,18 @@ FAGQ_API int fagq_qk_norm_rope_bwd_launch(const void* dq_out, const void* dk_out
     set_strides(a.qs, strides + 4), set_strides(a.ks, strides + 6);
     set_strides(a.qos, strides + 8), set_strides(a.kos, strides + 10);
     a.T = (int32_t)T, a.Hq = (int32_t)Hq, a.Hk = (int32_t)Hk, a.D = (int32_t)D, a.R = (int32_t)R;
-    a.splits = (int32_t)s.splits, a.per_wave = (int32_t)s.per_wave;
+    a.gq = (int32_t)s.gq;
     a.idx64 = index_dtype == FAGQ_IDX_I64, a.eps = eps;
     void* args[] = {&a};
     const int ls = launch_kernel(kernel_for(dtype, lanes_per_row(D), interleaved != 0, true),
-                                 dim3((unsigned)groups), dim3(64 * kWaves), args,
-                                 (size_t)kWaves * 2 * D * 4, st);
+                                 dim3((unsigned)(s.gq + s.gk)), dim3(64 * kWaves), args,
+                                 (size_t)kWaves * D * 4, st);
     if (ls != FAGQ_OK) return ls;
   }
-  SumArgs sa = {static_cast<const float*>(workspace), dq_weight, dk_weight, (int32_t)groups,
-                (int32_t)D};
+  SumArgs sa = {static_cast<const float*>(workspace), dq_weight, dk_weight, (int32_t)s.gq,
+                (int32_t)s.gk, (int32_t)D};
   void* sargs[] = {&sa};
-  return launch_kernel(reinterpret_cast<const void*>(&weight_sums), dim3((unsigned)(2 * D / 16)),
+  return launch_kernel(reinterpret_cast<const void*>(&weight_sums), dim3((unsigned)(D / 16), 2),
                        dim3(16 * kSumRows), sargs, 0, st);
 }
 

@@ -101,7 +101,7 @@ def test_rope_workspace(lib):
     assert f(0, 4, 2, 128) == 0
     for T in (1, 7, 4096, 1 << 24):
         n = f(T, 32, 8, 128)
-        assert 0 < n <= 512 * 2 * 128 * 4 and n % (2 * 128 * 4) == 0
+        assert 0 < n <= 768 * 128 * 4 and n % (128 * 4) == 0
     assert f(-1, 4, 2, 128) == -1 and f(4, 0, 2, 128) == -1 and f(4, 4, 2, 100) == -1
     assert f(4, 4, 2, 1024) == -1
 
