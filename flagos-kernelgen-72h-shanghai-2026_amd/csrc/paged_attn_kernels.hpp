@@ -258,34 +258,40 @@ struct RawValues {
   typename Scales<SF>::type s[2];
 };
 
+// Where a step's two tiles are.
+struct Rows2 {
+  int64_t row[2];
+};
+__device__ __forceinline__ Rows2 rows_at(const Args& a, int h, const Pages& pages, int32_t tok) {
+  return {{first_row(a, h, pages.p[0], tok), first_row(a, h, pages.p[1], tok + 16)}};
+}
+
 template <int D, int SF, bool ONCE>
-__device__ __forceinline__ void load_keys(const Args& a, int h, int lane, int32_t tok,
-                                          const Pages& pages, RawKeys<D, SF>& r) {
+__device__ __forceinline__ void load_keys(const Args& a, int lane, const Rows2& at,
+                                          RawKeys<D, SF>& r) {
   const int c = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int64_t row = first_row(a, h, pages.p[t], tok + 16 * t);
-    const uint8_t* k = a.kc + row * D;
+    const uint8_t* k = a.kc + at.row[t] * D;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i)
       r.k[t][i] = load_codes<ONCE, u32x4>(k + (uint32_t)(c * D + 16 * g + 64 * i));
-    r.s[t] = load_scales<SF>(a.ks, row + 4 * g);
+    r.s[t] = load_scales<SF>(a.ks, at.row[t] + 4 * g);
   }
 }
 
 template <int D, int SF, bool ONCE>
-__device__ __forceinline__ void load_values(const Args& a, int h, int lane, int32_t tok,
-                                            const Pages& pages, RawValues<D, SF>& r) {
+__device__ __forceinline__ void load_values(const Args& a, int lane, const Rows2& at,
+                                            RawValues<D, SF>& r) {
   constexpr int NT = D / 16;
   const int c = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int64_t row = first_row(a, h, pages.p[t], tok + 16 * t);
-    const uint8_t* v = a.vc + row * D;
+    const uint8_t* v = a.vc + at.row[t] * D;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       load_bytes<NT, ONCE>(v + (uint32_t)((4 * g + i) * D + c * NT), r.v[4 * t + i]);
-    r.s[t] = load_scales<SF>(a.vs, row + 4 * g);
+    r.s[t] = load_scales<SF>(a.vs, at.row[t] + 4 * g);
   }
 }
 
@@ -299,7 +305,7 @@ struct Rows {
   f32x4 o[R][D / 16];          // dims D / 16 (4 g + r) + j at [j][r]
   float m[R], l[R];            // l: of this lane's keys
   int32_t seen[R];             // keys that the row sees
-  float unit, inv_unit;        // o is in units of `unit`, a power of two (see join)
+  float unit, inv_unit;        // o is in units of `unit` (see join)
 };
 
 // Products of one step's keys with the queries.
@@ -352,22 +358,20 @@ __device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t
       ks[i] = 1.0f;
     }
   }
-  // Probabilities times value scales have to fit fp16: they are taken in units of the power of
-  // two just above the largest value scale so far, and o with them.
-  float most = fmaxf(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])),
-                     fmaxf(fmaxf(vs[4], vs[5]), fmaxf(vs[6], vs[7])));
+  // Probabilities times value scales have to fit fp16: they are taken in units of the largest value
+  // scale so far, and o with them.  (Where one key has all the weight, its product is exact.)
+  const float most = fmaxf(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])),
+                           fmaxf(fmaxf(vs[4], vs[5]), fmaxf(vs[6], vs[7])));
   if (__any(most > s.unit)) {
-    const uint32_t bits =
-        (uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(cross_max(most)));
-    int32_t e = (int32_t)(bits >> 23) - 126;
-    e = e < 127 ? e : 127;
-    const float unit = __builtin_ldexpf(1.0f, e), f = s.unit * __builtin_ldexpf(1.0f, -e);
+    const float unit = fmaxf(__uint_as_float(__builtin_amdgcn_readfirstlane(
+                                 __float_as_uint(cross_max(most)))), 0x1p-100f);
+    const float inv = 1.0f / unit, f = s.unit * inv;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int j = 0; j < NT; ++j) s.o[r][j] *= f;
     s.unit = unit;
-    s.inv_unit = __builtin_ldexpf(1.0f, -e);
+    s.inv_unit = inv;
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) vs[i] *= s.inv_unit;
@@ -459,22 +463,27 @@ __device__ __forceinline__ void run_steps(const Args& a, const Keys& k, int h, i
   RawValues<D, SF> values;
   Pages pages = check(entries(tok));
   Pages ahead = entries(tok + kRound);
-  load_keys<D, SF, ONCE>(a, h, lane, tok, pages, keys);
-  load_values<D, SF, ONCE>(a, h, lane, tok, pages, values);
+  Rows2 at = rows_at(a, h, pages, tok);
+  load_keys<D, SF, ONCE>(a, lane, at, keys);
+  load_values<D, SF, ONCE>(a, lane, at, values);
   for (;;) {
     const int32_t next = tok + kRound;
     const bool more = next < k.end;
     const Pages next_pages = check(ahead);
-    ahead = entries(next + kRound);
+    // Behind the last step its own rows are loaded again: loads that are under way on one path only
+    // would have every wait for older ones wait for them too.
+    if (more) at = rows_at(a, h, next_pages, next);
     f32x4 x[R][2];
     float ks[8];
     scores<E, QF, SF, D, R>(lane, keys, s, x);
+    // Behind the scores: their LDS reads would wait for a scalar load under way.
+    ahead = entries(next + kRound);
 #pragma unroll
     for (int i = 0; i < 8; ++i) ks[i] = scale_of<SF>(keys.s[i / 4], i % 4) * a.scale2;
-    if (more) load_keys<D, SF, ONCE>(a, h, lane, next, next_pages, keys);
+    load_keys<D, SF, ONCE>(a, lane, at, keys);
     join<E, QF, SF, D, R>(lane, tok, all, end, pages, x, ks, values, s);
     if (!more) return;
-    load_values<D, SF, ONCE>(a, h, lane, next, next_pages, values);
+    load_values<D, SF, ONCE>(a, lane, at, values);
     tok = next;
     pages = next_pages;
   }
