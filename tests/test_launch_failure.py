@@ -106,3 +106,24 @@ def test_python_layer_raises_on_it(seam):
     with pytest.raises(_lib.FagqError) as e:
         _lib.check(st)
     assert e.value.status == -HIP_ERROR_LAUNCH_FAILURE and "HIP error" in str(e.value)
+
+
+def test_the_attention_side_reports_it(seam):
+    i64 = lambda *v: (ctypes.c_int64 * len(v))(*v)
+    st = seam.fagq_qk_norm_rope_launch(*[fake(i) for i in range(9)], i64(512, 128, 256, 128, 512, 128, 256, 128), 5, 4, 2,
+                                       128, 128, 64, 1e-6, 0, 0, 1, None)
+    assert st == -HIP_ERROR_LAUNCH_FAILURE
+    need = seam.fagq_qk_norm_rope_bwd_workspace_bytes(5, 4, 2, 128)
+    st = seam.fagq_qk_norm_rope_bwd_launch(*[fake(i) for i in range(14)], need, i64(*(512, 128, 256, 128) * 3), 5, 4, 2,
+                                           128, 128, 64, 1e-6, 0, 0, 1, None)
+    assert st == -HIP_ERROR_LAUNCH_FAILURE
+    st = seam.fagq_kv_cache_write_launch(*[fake(i) for i in range(7)], i64(256, 128, 256, 128), 5, 2, 128, 128, 9, 16, 0,
+                                         1, 0, 1, None)
+    assert st == -HIP_ERROR_LAUNCH_FAILURE
+    st = seam.fagq_kv_cache_read_launch(*[fake(i) for i in range(8)], 3, 50, 2, 128, 128, 9, 16, 4, 0, 1, 0, None)
+    assert st == -HIP_ERROR_LAUNCH_FAILURE
+    for S, prefix, most in ((1, 0, 64), (1, 20, 64), (40, 0, 64), (1, 0, 1 << 20)):
+        need = seam.fagq_paged_attention_workspace_bytes(3, S, 8, 2, 128, prefix, most)
+        st = seam.fagq_paged_attention_launch(*[fake(i) for i in range(10)], need, i64(1024 * S, 1024, 128), 3, S, 8, 2,
+                                              128, 9, 16, 1 << 16, prefix, most, 0.1, 0, 1, 0, 0, None)
+        assert st == -HIP_ERROR_LAUNCH_FAILURE, (S, prefix, most)
