@@ -21,6 +21,7 @@ constexpr int64_t kSlots = 2 * kCUs;   // workgroups of a round
 constexpr int64_t kFewRounds = 8 * kSlots;      // of all units: not worth a schedule
 constexpr int64_t kCacheBytes = 256ll << 20;    // of the cache behind the XCDs' L2
 constexpr int64_t kFixed = 128;        // what a workgroup costs besides its keys, in keys
+constexpr int64_t kTallKeys = 1024;    // of a workgroup, from which on tall units pay (see row_tiles)
 
 struct JoinArgs {
   const float* part;
@@ -188,7 +189,22 @@ struct Plan {
   int64_t row_parts, parts;                             // of a row; of the workspace
 };
 
-int row_tiles(int64_t rows, int64_t D) {
+// Rows of a unit.
+int64_t height(int R, int64_t D) { return R == kTall ? kWaves * 16 * (256 / D) : 16 * R; }
+
+// The row tiles of a unit, for so many rows that see so many keys, in each of `lists` lists of keys:
+// as few as hold them.  Tall units for heads of 128 and 256 where at least two thirds of their rows
+// are used and where each of the kSlots workgroups has kTallKeys keys: fewer leave four times as many
+// parts to join (shared prefix, 8 heads of 128, us short / tall: 512 rows of 32768 keys 122 / 115, of
+// 4096 35 / 45, 192 rows of 32768 57 / 65; 16 sequences of 4096 keys, 8 heads of 128: 64 rows 47 /
+// 60, 96 rows 76 / 65, 128 rows 68 / 72, 256 rows 126 / 116, 2 heads of 256, 128 rows: 94 / 76).  Heads of 64 are bound
+// by the softmax, which is the same in both forms (8 sequences of 256 tokens, 32 + 8 heads, 4096
+// keys: 113 / 133).
+int row_tiles(int64_t rows, int64_t D, int64_t lists, int64_t keys) {
+  if (D >= 128) {
+    const int64_t tall = height(kTall, D), tiles = (rows + tall - 1) / tall;
+    if (3 * rows >= 2 * tiles * tall && lists * tiles * keys >= kSlots * kTallKeys) return kTall;
+  }
   const int R = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   return R * D <= 256 ? R : (int)(256 / D);
 }
@@ -219,16 +235,16 @@ Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t pr
   Plan p = {};
   const int64_t per = S * (Hq / H);
   p.rows = B * S * Hq;
-  p.R = row_tiles(per, D);
+  p.R = row_tiles(per, D, B * H, most);
   if (prefix_len > 0) {
-    p.RP = row_tiles(B * per, D);
-    if (p.R > 1) p.R = p.RP;
-    p.prefix_tiles = (B * per + 16 * p.RP - 1) / (16 * p.RP);
+    p.RP = row_tiles(B * per, D, H, prefix_len);
+    if (p.R > 1 && p.RP != kTall) p.R = p.RP;
+    p.prefix_tiles = (B * per + height(p.RP, D) - 1) / height(p.RP, D);
     cut(prefix_len, H * p.prefix_tiles, &p.prefix_chunk, &p.prefix_chunks);
     p.prefix_items = H * p.prefix_tiles * p.prefix_chunks;
   }
-  p.tiles = (per + 16 * p.R - 1) / (16 * p.R);
-  if (p.tiles > 1 || most_rounds(B, H, most) <= kFewRounds) {
+  p.tiles = (per + height(p.R, D) - 1) / height(p.R, D);
+  if (p.tiles > 1 || p.R == kTall || most_rounds(B, H, most) <= kFewRounds) {
     p.form = kStatic;
     cut(most, B * H * p.tiles, &p.chunk, &p.chunks);
     if (p.chunks < 1) p.chunks = 1;     // rows without keys are written all the same

@@ -12,19 +12,27 @@ const void* kernel() {
       &paged_attention<FAGQ_ATTN_E, FAGQ_ATTN_QF, FAGQ_ATTN_SF, D, R, RP, FORM>);
 }
 
-// What plan_for makes, R D <= 256: without a prefix, units of any height; with one, 16 rows go with a
-// prefix of units of any height, more rows with units of their own height.
+// What plan_for makes, R D <= 256 or, for heads of 128 and 256, tall units: without a prefix, units
+// of any height; with one, 16 rows go with a prefix of units of any height, more rows with units of
+// their own height or tall ones, tall ones with tall ones.
 template <int D, int R, int RP>
 const void* lookup(int form) {
-  if constexpr (RP == 0)
-    if (form == kScheduledOnce) return kernel<D, R, RP, kScheduledOnce>();
-  return form == kStatic ? kernel<D, R, RP, kStatic>() : kernel<D, R, RP, kScheduled>();
+  if constexpr (R == kTall) {
+    return kernel<D, R, RP, kStatic>();
+  } else {
+    if constexpr (RP == 0)
+      if (form == kScheduledOnce) return kernel<D, R, RP, kScheduledOnce>();
+    return form == kStatic ? kernel<D, R, RP, kStatic>() : kernel<D, R, RP, kScheduled>();
+  }
 }
 template <int D, int R>
 const void* lookup(int RP, int form) {
-  if constexpr (R * D <= 256) {
+  if constexpr (R == kTall ? D >= 128 : R * D <= 256) {
     if (RP == 0) return lookup<D, R, 0>(form);
-    if (RP == R) return lookup<D, R, R>(form);
+    if constexpr (D >= 128)
+      if (RP == kTall) return lookup<D, R, kTall>(form);
+    if constexpr (R != kTall)
+      if (RP == R) return lookup<D, R, R>(form);
     if constexpr (R == 1 && 2 * D <= 256)
       if (RP == 2) return lookup<D, R, 2>(form);
     if constexpr (R == 1 && 4 * D <= 256)
@@ -34,7 +42,10 @@ const void* lookup(int RP, int form) {
 }
 template <int D>
 const void* lookup(int R, int RP, int form) {
-  return R == 1 ? lookup<D, 1>(RP, form) : R == 2 ? lookup<D, 2>(RP, form) : lookup<D, 4>(RP, form);
+  return R == 1   ? lookup<D, 1>(RP, form)
+         : R == 2 ? lookup<D, 2>(RP, form)
+         : R == 4 ? lookup<D, 4>(RP, form)
+                  : lookup<D, kTall>(RP, form);
 }
 
 }  // namespace

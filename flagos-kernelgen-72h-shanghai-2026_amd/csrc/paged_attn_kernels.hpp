@@ -10,7 +10,8 @@
 // registers hold one wave on a SIMD, whose loads and products wait for each other (64 rows of 64
 // sequences behind 32768 keys, heads of 128: R = 2 145 us, R = 4 234).  A workgroup takes a range
 // of a unit's keys; its four waves take the steps of 32 keys in turn, each with m, l and o of its
-// own, and are joined through LDS.  How units are cut:
+// own, and are joined through LDS.  Units of many rows of heads of 128 and 256 are tall ones: four
+// times as many rows, a quarter for each wave (see Tall).  How units are cut:
 //   scheduled  The rounds of 128 keys of all units in a row are shared out evenly, so that every
 //              workgroup reads as much as the others however the lengths differ and whatever bound
 //              on them the host knows (64 sequences of 1400 to 8192 tokens: 116 us, with chunks
@@ -144,6 +145,19 @@ template <int E, int QF>
 __device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi) {
   const u32x2 a = widen4<E, QF>(lo), b = widen4<E, QF>(hi);
   return u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// Bytes of 4 keys x 4 dims -> 4 dims x 4 keys.
+__device__ __forceinline__ void transpose4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                           uint32_t (&d)[4]) {
+  const uint32_t e0 = __builtin_amdgcn_perm(a1, a0, 0x05010400u);   // dims 0, 1 of keys 0, 1
+  const uint32_t e1 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);   // dims 2, 3
+  const uint32_t f0 = __builtin_amdgcn_perm(a3, a2, 0x05010400u);
+  const uint32_t f1 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
+  d[0] = __builtin_amdgcn_perm(f0, e0, 0x05040100u);
+  d[1] = __builtin_amdgcn_perm(f0, e0, 0x07060302u);
+  d[2] = __builtin_amdgcn_perm(f1, e1, 0x05040100u);
+  d[3] = __builtin_amdgcn_perm(f1, e1, 0x07060302u);
 }
 
 // Rounds of a sequence's units: one for a sequence without keys, whose rows are written too.
@@ -331,30 +345,24 @@ __device__ __forceinline__ void scores(int lane, const RawKeys<D, SF>& raw, cons
   }
 }
 
-// The softmax and the values of one step: 32 keys from `tok` on, of which the unit's last row
-// sees those below `end`; all rows see those below `all`.  ks: the keys' scales times scale2.
-template <int E, int QF, int SF, int D, int R>
-__device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t end,
-                                     const Pages& pages, f32x4 (&x)[R][2], float (&ks)[8],
-                                     RawValues<D, SF>& raw, Rows<E, D, R>& s) {
+// The softmax of one step: 32 keys from `tok` on, of which all rows see those below `all`.  From the
+// products x, the keys' scales times scale2 and the values' scales (zeros for what no row sees) to
+// the probabilities times value scales, in units of s.unit, as fp16 operands of the next product.
+template <int E, int D, int R>
+__device__ __forceinline__ void softmax(int lane, int32_t tok, int32_t all, const Pages& pages,
+                                        f32x4 (&x)[R][2], float (&ks)[8], float (&vs)[8],
+                                        Rows<E, D, R>& s, u32x4 (&p)[R]) {
   constexpr int NT = D / 16;
   const int g = lane >> 4;
-  float vs[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) vs[i] = scale_of<SF>(raw.s[i / 4], i % 4);
   if (tok + kStep > all || pages.p[0] < 0 || pages.p[1] < 0) {
-    // What no row sees may hold anything: its values and their scales become zeros.  What a row
-    // does not see gets no weight, whatever the score and the key's scale are.
+    // What a row does not see gets no weight, whatever the score and the key's scale are.
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int32_t at = tok + 16 * (i / 4) + 4 * g + i % 4;
-      const bool page = pages.p[i / 4] >= 0, live = at < end && page;
-      vs[i] = live ? vs[i] : 0.0f;
-#pragma unroll
-      for (int w = 0; w < NT / 4; ++w) raw.v[i][w] = live ? raw.v[i][w] : 0u;
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        x[r][i / 4][i % 4] = at < s.seen[r] && page ? x[r][i / 4][i % 4] * ks[i] : -INFINITY;
+        x[r][i / 4][i % 4] =
+            at < s.seen[r] && pages.p[i / 4] >= 0 ? x[r][i / 4][i % 4] * ks[i] : -INFINITY;
       ks[i] = 1.0f;
     }
   }
@@ -375,7 +383,6 @@ __device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) vs[i] *= s.inv_unit;
-  u32x4 p[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     float y[8];
@@ -405,26 +412,39 @@ __device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t
 #pragma unroll
     for (int i = 0; i < 4; ++i) p[r][i] = pack16<ET_F16>(y[2 * i], y[2 * i + 1]);
   }
+}
+
+// One step of keys in registers, `end`: the unit's last row sees the keys below it.
+template <int E, int QF, int SF, int D, int R>
+__device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t end,
+                                     const Pages& pages, f32x4 (&x)[R][2], float (&ks)[8],
+                                     RawValues<D, SF>& raw, Rows<E, D, R>& s) {
+  constexpr int NT = D / 16;
+  const int g = lane >> 4;
+  float vs[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) vs[i] = scale_of<SF>(raw.s[i / 4], i % 4);
+  if (tok + kStep > end || pages.p[0] < 0 || pages.p[1] < 0) {
+    // What no row sees may hold anything: its values and their scales become zeros.
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool live = tok + 16 * (i / 4) + 4 * g + i % 4 < end && pages.p[i / 4] >= 0;
+      vs[i] = live ? vs[i] : 0.0f;
+#pragma unroll
+      for (int w = 0; w < NT / 4; ++w) raw.v[i][w] = live ? raw.v[i][w] : 0u;
+    }
+  }
+  u32x4 p[R];
+  softmax<E, D, R>(lane, tok, all, pages, x, ks, vs, s, p);
 #pragma unroll
   for (int w = 0; w < NT / 4; ++w) {
-    // Bytes of 8 keys x 4 dims -> 4 dims x 8 keys.
-    uint32_t d[4][2];
+    uint32_t d[2][4];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint32_t a0 = raw.v[4 * t][w], a1 = raw.v[4 * t + 1][w];
-      const uint32_t a2 = raw.v[4 * t + 2][w], a3 = raw.v[4 * t + 3][w];
-      const uint32_t e0 = __builtin_amdgcn_perm(a1, a0, 0x05010400u);   // dims 0, 1 of keys 0, 1
-      const uint32_t e1 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);   // dims 2, 3
-      const uint32_t f0 = __builtin_amdgcn_perm(a3, a2, 0x05010400u);
-      const uint32_t f1 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
-      d[0][t] = __builtin_amdgcn_perm(f0, e0, 0x05040100u);
-      d[1][t] = __builtin_amdgcn_perm(f0, e0, 0x07060302u);
-      d[2][t] = __builtin_amdgcn_perm(f1, e1, 0x05040100u);
-      d[3][t] = __builtin_amdgcn_perm(f1, e1, 0x07060302u);
-    }
+    for (int t = 0; t < 2; ++t)
+      transpose4(raw.v[4 * t][w], raw.v[4 * t + 1][w], raw.v[4 * t + 2][w], raw.v[4 * t + 3][w], d[t]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const u32x4 v = widen8<ET_F16, QF>(d[i][0], d[i][1]);
+      const u32x4 v = widen8<ET_F16, QF>(d[0][i], d[1][i]);
 #pragma unroll
       for (int r = 0; r < R; ++r) s.o[r][4 * w + i] = mfma<ET_F16>(v, p[r], s.o[r][4 * w + i]);
     }
@@ -640,10 +660,277 @@ __device__ __forceinline__ void run_segment(const Args& a, const Segment& seg, S
   }
 }
 
+// ------------------------------------------------------------------------- many rows
+
+// Tall units: each wave has 16 R rows of its own (R D = 256), and the four waves see the same keys.
+// A step's codes are widened once for all of them, a quarter by each wave, and handed on through LDS
+// in the order of the products; the next steps' are staged while these are worked on.  The shorter
+// units widen as much for 16 R rows as these do for 64 R, which is a third of their instructions.
+// V's tile (h, i) of the product has the dims 64 h + 4 c + i.
+template <int D>
+struct Tall {
+  static constexpr int R = 256 / D;
+  // Steps between two barriers, as far as two workgroups' LDS fits a CU (heads of 128: one step
+  // 188 us, two 181; heads of 256: 223, two 388).
+  static constexpr int kSteps = 256 / D;
+  static constexpr int kPieces = D / 32;        // 16-byte pieces of a step's keys; 4-key tiles of
+                                                // 64 dims of its values
+  static constexpr int kEach = kPieces / kWaves;
+  static_assert(kPieces % kWaves == 0, "heads of 128 and 256");
+  struct Lds {
+    u32x4 k[2][kSteps][2 * (D / 32)][64];
+    u32x4 v[2][kSteps][D / 16][64];
+    float ks[2][kSteps][kStep], vs[2][kSteps][kStep];
+  };
+  struct Raw {
+    u32x4 k[kEach];
+    uint32_t v[kEach][4];
+    float scale;               // wave 0: of key lane % 32, keys' below lane 32, values' above
+    Pages pages;
+    int32_t tok;
+  };
+  static __device__ __forceinline__ int piece(int wave, int n) { return wave + n * kWaves; }
+};
+
+template <int SF, int D>
+__device__ __forceinline__ void load_tall(const Args& a, int h, int lane, int wave, int32_t tok,
+                                          const Pages& pages, typename Tall<D>::Raw& r) {
+  const int c = lane & 15, g = lane >> 4;
+  const Rows2 at = rows_at(a, h, pages, tok);
+  r.pages = pages;
+  r.tok = tok;
+#pragma unroll
+  for (int n = 0; n < Tall<D>::kEach; ++n) {
+    const int p = Tall<D>::piece(wave, n);
+    r.k[n] = *reinterpret_cast<const u32x4*>(
+        a.kc + (p < D / 64 ? at.row[0] : at.row[1]) * D +
+        (uint32_t)(c * D + 16 * g + 64 * (p % (D / 64))));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r.v[n][i] = *reinterpret_cast<const uint32_t*>(
+          a.vc + (p & 1 ? at.row[1] : at.row[0]) * D +
+          (uint32_t)((4 * g + i) * D + 64 * (p >> 1) + 4 * c));
+  }
+  if (wave == 0) {
+    const void* s = lane < kStep ? a.ks : a.vs;
+    const int64_t row = (lane & 16 ? at.row[1] : at.row[0]) + c;
+    r.scale = SF == SF_UE8M0
+                  ? __uint_as_float((uint32_t) static_cast<const uint8_t*>(s)[row] << 23)
+                  : static_cast<const float*>(s)[row];
+  }
+}
+
+template <int E, int QF, int D>
+__device__ __forceinline__ void stage_tall(const Args& a, int lane, int wave, int32_t end,
+                                           const typename Tall<D>::Raw& r,
+                                           typename Tall<D>::Lds& sh, int buf, int step) {
+  const int c = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int n = 0; n < Tall<D>::kEach; ++n) {
+    const int p = Tall<D>::piece(wave, n);
+    const int at = p / (D / 64) * (D / 32) + 2 * (p % (D / 64));
+    sh.k[buf][step][at][lane] = widen8<E, QF>(r.k[n][0], r.k[n][1]);
+    sh.k[buf][step][at + 1][lane] = widen8<E, QF>(r.k[n][2], r.k[n][3]);
+    const int t = p & 1;
+    const bool page = (t ? r.pages.p[1] : r.pages.p[0]) >= 0;
+    uint32_t v[4], d[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = r.v[n][i];
+    if (r.tok + kStep > end || !page) {
+      // What no row sees may hold anything: it becomes zeros.
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = r.tok + 16 * t + 4 * g + i < end && page ? v[i] : 0u;
+    }
+    transpose4(v[0], v[1], v[2], v[3], d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<u32x2*>(&sh.v[buf][step][4 * (p >> 1) + i][lane])[t] =
+          widen4<ET_F16, QF>(d[i]);
+  }
+  if (wave == 0) {
+    const int t = (lane >> 4) & 1;
+    if (lane < kStep) {
+      sh.ks[buf][step][lane] = r.scale * a.scale2;
+    } else {
+      const bool live = r.tok + 16 * t + c < end && (t ? r.pages.p[1] : r.pages.p[0]) >= 0;
+      sh.vs[buf][step][lane - kStep] = live ? r.scale : 0.0f;
+    }
+  }
+}
+
+template <int E, int QF, int SF, int D, bool PREFIX>
+__device__ __forceinline__ void run_tall(const Args& a, const Segment& seg,
+                                         typename Tall<D>::Lds& sh) {
+  constexpr int R = Tall<D>::R, NT = D / 16;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int per = a.S * a.group;
+  const int rows = PREFIX ? a.B * per : per;
+  const int first_row = (seg.tile * kWaves + wave) * 16 * R;
+  Keys k = seg.keys;
+  auto row_of = [&](int i) {
+    Row r;
+    const int bs = i / a.group;
+    r.hq = seg.h * a.group + (i - bs * a.group);
+    r.b = PREFIX ? bs / a.S : seg.b;
+    r.s = PREFIX ? bs - r.b * a.S : bs;
+    return r;
+  };
+  Rows<E, D, R> s;
+  u32x4 q[R][D / 32];
+  s.unit = 0.0f;
+  s.inv_unit = 0.0f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = first_row + 16 * r + c;
+    const Row w = row_of(i < rows ? i : rows - 1);
+    const uint16_t* at = a.q + ((int64_t)w.b * a.qs[0] + (int64_t)w.s * a.qs[1] +
+                                (int64_t)w.hq * a.qs[2]);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+      q[r][j] = *reinterpret_cast<const u32x4*>(at + 64 * (j / 2) + 16 * g + 8 * (j & 1));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) s.o[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    s.m[r] = kLow;
+    s.l[r] = 0.0f;
+    s.seen[r] = PREFIX ? k.end : (int32_t)cache::seen_tokens(seg.len, a.most, a.S, w.s);
+  }
+  int32_t all = k.end;                          // keys that all rows of this wave see
+  if constexpr (!PREFIX) {
+    // Rows are in order of their tokens: the last one of the workgroup sees most.
+    all = __builtin_amdgcn_readfirstlane(s.seen[0]);
+    const int last = (seg.tile + 1) * kWaves * 16 * R - 1;
+    const int32_t end =
+        (int32_t)cache::seen_tokens(seg.len, a.most, a.S, row_of(last < rows ? last : rows - 1).s);
+    if (k.end > end) k.end = end;
+  }
+  if (k.begin < k.end) {
+    auto entries = [&](int32_t t) {
+      return Pages{{entry_of(k.pages, k.width, a.page_shift, t),
+                    entry_of(k.pages, k.width, a.page_shift, t + 16)}};
+    };
+    auto check = [&](const Pages& p) {
+      return Pages{{checked(p.p[0], a.num_pages), checked(p.p[1], a.num_pages)}};
+    };
+    constexpr int kSteps = Tall<D>::kSteps, kKeys = kSteps * kStep;
+    typename Tall<D>::Raw raw[kSteps];
+    int32_t tok = k.begin;
+    Pages pages[kSteps], next_pages[kSteps], ahead[kSteps];
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) {
+      pages[u] = check(entries(tok + u * kStep));
+      next_pages[u] = check(entries(tok + kKeys + u * kStep));
+      ahead[u] = entries(tok + 2 * kKeys + u * kStep);
+    }
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u)
+      load_tall<SF, D>(a, seg.h, lane, wave, tok + u * kStep, pages[u], raw[u]);
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u)
+      stage_tall<E, QF, D>(a, lane, wave, k.end, raw[u], sh, 0, u);
+    // Behind the last steps codes are loaded again: see run_steps.
+    if (tok + kKeys < k.end) {
+#pragma unroll
+      for (int u = 0; u < kSteps; ++u)
+        load_tall<SF, D>(a, seg.h, lane, wave, tok + kKeys + u * kStep, next_pages[u], raw[u]);
+    }
+    // The queries are waited for here: in the loop their first use would wait for all loads under
+    // way, every time (heads of 128: 200 us, so 188).
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) asm volatile("" : "+v"(q[r][j]));
+    for (int buf = 0;; buf ^= 1) {
+      const bool more = tok + kKeys < k.end, far = tok + 2 * kKeys < k.end;
+      lds_barrier();                            // these steps are staged, the last ones done with
+      if (more) {
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u)
+          stage_tall<E, QF, D>(a, lane, wave, k.end, raw[u], sh, buf ^ 1, u);
+      }
+      Pages now[kSteps];
+#pragma unroll
+      for (int u = 0; u < kSteps; ++u) {
+        now[u] = pages[u];
+        pages[u] = next_pages[u];
+        next_pages[u] = check(ahead[u]);
+        load_tall<SF, D>(a, seg.h, lane, wave, (far ? tok + 2 * kKeys : tok) + u * kStep,
+                         far ? next_pages[u] : now[u], raw[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kSteps; ++u) {
+        f32x4 x[R][2];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) x[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const u32x4 k0 = sh.k[buf][u][i][lane], k1 = sh.k[buf][u][D / 32 + i][lane];
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            x[r][0] = mfma<E>(k0, q[r][i], x[r][0]);
+            x[r][1] = mfma<E>(k1, q[r][i], x[r][1]);
+          }
+        }
+        float ks[8], vs[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          ks[i] = sh.ks[buf][u][16 * (i / 4) + 4 * g + i % 4];
+          vs[i] = sh.vs[buf][u][16 * (i / 4) + 4 * g + i % 4];
+        }
+        u32x4 p[R];
+        softmax<E, D, R>(lane, tok + u * kStep, all, now[u], x, ks, vs, s, p);
+        if (u == kSteps - 1) {
+#pragma unroll
+          for (int w = 0; w < kSteps; ++w) ahead[w] = entries(tok + 3 * kKeys + w * kStep);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const u32x4 v = sh.v[buf][u][j][lane];
+#pragma unroll
+          for (int r = 0; r < R; ++r) s.o[r][j] = mfma<ET_F16>(v, p[r], s.o[r][j]);
+        }
+      }
+      if (!more) break;
+      tok += kKeys;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float l = cross_sum(s.l[r]);
+    const int i = first_row + 16 * r + c;
+    if (i >= rows) continue;
+    const Row w = row_of(i);
+    const int64_t row = ((int64_t)w.b * a.S + w.s) * a.Hq + w.hq;
+    const bool whole = seg.to == kOut;
+    const int64_t at = whole ? 0 : row * a.row_parts + seg.row_part;
+    const float f = whole ? (l > 0.0f ? s.unit / l : 0.0f) : s.unit;
+#pragma unroll
+    for (int hh = 0; hh < D / 64; ++hh) {       // dims 64 hh + 16 g + 4 r + i
+      const int d = 64 * hh + 16 * g;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 o = {s.o[r][4 * hh][e] * f, s.o[r][4 * hh + 1][e] * f,
+                         s.o[r][4 * hh + 2][e] * f, s.o[r][4 * hh + 3][e] * f};
+        if (whole)
+          *reinterpret_cast<u32x2*>(a.out + row * D + d + 4 * e) =
+              u32x2{pack16<E>(o[0], o[1]), pack16<E>(o[2], o[3])};
+        else
+          *reinterpret_cast<f32x4*>(a.part + at * D + d + 4 * e) = o;
+      }
+    }
+    if (!whole && g == 0) {
+      a.part_ml[2 * at] = s.m[r];
+      a.part_ml[2 * at + 1] = l;
+    }
+  }
+}
+
 // One chunk of the prefix or (static) of a sequence's own keys.  `item`: workgroup number within
 // its kind.
-template <int E, int QF, int SF, int D, int R, bool PREFIX>
-__device__ __forceinline__ void run_chunk(const Args& a, int item, Shared<D, R>& sh) {
+template <int E, int QF, int SF, int D, int R, bool PREFIX, bool TALL>
+__device__ __forceinline__ void run_chunk(const Args& a, int item, char* lds) {
   const int chunks = PREFIX ? a.prefix_chunks : a.chunks;
   const Place place = PREFIX ? place_of(item, a.prefix_items, a.prefix_tiles)
                              : place_of(item, a.items, a.tiles);
@@ -671,7 +958,10 @@ __device__ __forceinline__ void run_chunk(const Args& a, int item, Shared<D, R>&
     // written, for rows without keys.
     if (s.keys.begin >= s.len && chunk > 0) return;
   }
-  run_segment<E, QF, SF, D, R, PREFIX, false>(a, s, sh);
+  if constexpr (TALL)
+    run_tall<E, QF, SF, D, PREFIX>(a, s, *reinterpret_cast<typename Tall<D>::Lds*>(lds));
+  else
+    run_segment<E, QF, SF, D, R, PREFIX, false>(a, s, *reinterpret_cast<Shared<D, R>*>(lds));
 }
 
 // LDS of the schedule.
@@ -833,24 +1123,34 @@ __device__ __forceinline__ void run_share(const Args& a, int wg, Shared<D, R>& s
   }
 }
 
-// R: row tiles of a unit of the sequences' own keys, RP: of the prefix (0: there is none).
+// R: row tiles of a unit of the sequences' own keys, RP: of the prefix (0: there is none); kTall:
+// tall units.
+constexpr int kTall = 8;
+template <int D, int R>
+constexpr int lds_of() {
+  if constexpr (R == 0) return 0;
+  else if constexpr (R == kTall) return sizeof(typename Tall<D>::Lds);
+  else return sizeof(Shared<D, R>);
+}
+
 template <int E, int QF, int SF, int D, int R, int RP, int FORM>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention(Args a) {
-  constexpr int kRows = R > RP ? R : RP;
-  __shared__ __align__(16) char lds[sizeof(Shared<D, kRows>)];
-  __shared__ Schedule sc;
+  constexpr int kLds = lds_of<D, R>() > lds_of<D, RP>() ? lds_of<D, R>() : lds_of<D, RP>();
+  __shared__ __align__(16) char lds[kLds];
   const int item = (int)blockIdx.x;
   if constexpr (RP > 0) {
     if (item < a.prefix_items) {
-      run_chunk<E, QF, SF, D, RP, true>(a, item, *reinterpret_cast<Shared<D, RP>*>(lds));
+      run_chunk<E, QF, SF, D, RP == kTall ? 1 : RP, true, RP == kTall>(a, item, lds);
       return;
     }
   }
-  Shared<D, R>& sh = *reinterpret_cast<Shared<D, R>*>(lds);
-  if constexpr (FORM == kStatic)
-    run_chunk<E, QF, SF, D, R, false>(a, item - a.prefix_items, sh);
-  else
-    run_share<E, QF, SF, D, R, FORM == kScheduledOnce>(a, item - a.prefix_items, sh, sc);
+  if constexpr (FORM == kStatic) {
+    run_chunk<E, QF, SF, D, R == kTall ? 1 : R, false, R == kTall>(a, item - a.prefix_items, lds);
+  } else {
+    __shared__ Schedule sc;
+    run_share<E, QF, SF, D, R, FORM == kScheduledOnce>(
+        a, item - a.prefix_items, *reinterpret_cast<Shared<D, R>*>(lds), sc);
+  }
 }
 
 // Kernels for an element type (ET_BF16, ET_F16), code format (QF_FP8, QF_I8_RNE) and scale format:
