@@ -47,7 +47,8 @@ __host__ __device__ inline int64_t gathered_slot(const int32_t* cu, const int32_
 // How many of its own tokens query s of the newest S of a sequence of kv_len tokens sees, where
 // no more than `most` of them are read.
 __host__ __device__ inline int64_t seen_tokens(int64_t kv_len, int64_t most, int S, int s) {
-  const int64_t n = (kv_len < most ? kv_len : most) - S + s + 1;
+  const int64_t read = kv_len < 0 ? 0 : kv_len < most ? kv_len : most;
+  const int64_t n = read - S + s + 1;
   return n > 0 ? n : 0;
 }
 

@@ -173,9 +173,10 @@ int check_sizes(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t 
   if (B < 0 || S < 1 || H < 1 || Hq < H || Hq % H != 0 || (D != 64 && D != 128 && D != 256) ||
       prefix_len < 0 || max_kv_len < 0)
     return FAGQ_E_SHAPE;
-  if (B > 65535 || S > 65535 || Hq > 4096 || B * S * Hq > (1ll << 24) ||
+  // A grid of 2^32 threads is one too many: the joining kernel may have a workgroup for each row.
+  if (B > 65535 || S > 65535 || Hq > 4096 || B * S * Hq >= (1ll << 32) / (64 * kWaves) ||
       prefix_len > (1ll << 30) || max_kv_len > (1ll << 30) ||
-      most_rounds(B, H, max_kv_len) >= (1ll << 31))
+      most_rounds(B, H, max_kv_len) >= (1ll << 31) - kSlots)
     return FAGQ_E_TOO_LARGE;
   return FAGQ_OK;
 }
@@ -211,12 +212,16 @@ int row_tiles(int64_t rows, int64_t D, int64_t lists, int64_t keys) {
 
 // Cuts a unit's keys into the number of chunks that takes least time where each of the `units`
 // becomes so many workgroups, the GPU runs them in rounds of kSlots, one takes as long as its keys
-// and kFixed, and each chunk costs the joining kernel kPartCost keys.
+// and kFixed, and each chunk costs the joining kernel kPartCost keys.  With w rounds, n chunks cost
+// w (keys / n + kFixed) + kPartCost n, least at sqrt(w keys / kPartCost): tried for each w, as far
+// as w rounds go (all n cost the host 19 us for one unit of 524288 keys).
 void cut(int64_t keys, int64_t units, int64_t* chunk, int64_t* chunks) {
   const int64_t most = (keys + kRound - 1) / kRound;
   int64_t best = -1;
   *chunk = kRound, *chunks = 0;
-  for (int64_t n = 1; n <= most; ++n) {
+  auto consider = [&](int64_t n) {
+    n = n < most ? n : most;
+    if (n < 1) return;
     int64_t c = (keys + n - 1) / n;
     c = (c + kRound - 1) / kRound * kRound;
     const int64_t got = (keys + c - 1) / c;
@@ -226,7 +231,14 @@ void cut(int64_t keys, int64_t units, int64_t* chunk, int64_t* chunks) {
       *chunk = c;
       *chunks = got;
     }
-    if (units * n >= 8 * kSlots) break;
+  };
+  consider(1);
+  for (int64_t w = 1; w <= 16; ++w) {
+    const int64_t fit = w * kSlots / units;
+    if (fit == 0) continue;
+    const int64_t n = (int64_t)std::sqrt((double)(w * keys) / kPartCost);
+    consider(n < fit ? n : fit);
+    consider(n + 1 < fit ? n + 1 : fit);
   }
 }
 
@@ -261,7 +273,7 @@ Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t pr
 }
 
 // o, {m, l} of each part, and the schedule.
-int64_t workspace_bytes(const Plan& p, int64_t B, int64_t D) {
+int64_t bytes_of(const Plan& p, int64_t B, int64_t D) {
   return p.parts * (D + 2) * 4 + (p.form == kStatic ? 0 : (B + 1) * 4);
 }
 
@@ -292,7 +304,8 @@ FAGQ_API int64_t fagq_paged_attention_workspace_bytes(int64_t B, int64_t S, int6
                                                       int64_t max_kv_len) {
   using namespace fagq::attn;
   if (check_sizes(B, S, Hq, H, D, prefix_len, max_kv_len) != FAGQ_OK) return -1;
-  return B == 0 ? 0 : workspace_bytes(plan_for(B, S, Hq, H, D, prefix_len, max_kv_len), B, D);
+  if (B == 0) return 0;
+  return bytes_of(plan_for(B, S, Hq, H, D, prefix_len, max_kv_len), B, D);
 }
 
 FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, const void* v_cache,
@@ -334,7 +347,8 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
       !aligned(k_scale, ss * 4) || !aligned(v_scale, ss * 4) || !aligned(page_table, 4) ||
       !aligned(kv_lens, is) || !aligned(prefix_pages, 4) || !aligned(out, 16))
     return FAGQ_E_ALIGN;
-  const int64_t need = fagq_paged_attention_workspace_bytes(B, S, Hq, H, D, prefix_len, max_kv_len);
+  const Plan p = B > 0 ? plan_for(B, S, Hq, H, D, prefix_len, max_kv_len) : Plan{};
+  const int64_t need = B > 0 ? bytes_of(p, B, D) : 0;
   if (need > 0 && !workspace) return FAGQ_E_NULL;
   if (workspace_bytes < need) return FAGQ_E_SHAPE;
   if (!aligned(workspace, 16)) return FAGQ_E_ALIGN;
@@ -367,7 +381,6 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   a.most = (int32_t)(room < max_kv_len ? room : max_kv_len);
   a.idx64 = index_dtype == FAGQ_IDX_I64;
   a.scale2 = sm_scale * 1.44269504088896340736f;
-  const Plan p = plan_for(B, S, Hq, H, D, prefix_len, max_kv_len);
   a.chunk = (int32_t)p.chunk, a.chunks = (int32_t)p.chunks, a.tiles = (int32_t)p.tiles;
   a.prefix_chunk = (int32_t)p.prefix_chunk, a.prefix_chunks = (int32_t)p.prefix_chunks;
   a.prefix_tiles = (int32_t)p.prefix_tiles, a.prefix_items = (int32_t)p.prefix_items;
@@ -378,7 +391,6 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
     a.part_ml = a.part + p.parts * D;
     a.sched = p.form == kStatic ? nullptr : reinterpret_cast<int32_t*>(a.part_ml + 2 * p.parts);
   }
-  // At most 2^24 units, and few more workgroups: below 2^31.
   void* args[] = {&a};
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int ls = launch_kernel(kernel_for(dtype, q_format, scale_format, (int)D, p),

@@ -44,6 +44,8 @@ def empty_kv_cache(num_pages: int, heads: int, page_size: int, head_dim: int,
     G = head_dim if group_size is None else group_size
     if G not in GROUPS or head_dim % G:
         raise ValueError(f"group size must be one of {GROUPS} and divide {head_dim}, got {G}")
+    if dtype not in _CODES:
+        raise TypeError(f"a cache's codes are float8_e4m3fn or int8, got {dtype}")
     codes = torch.empty(num_pages, heads, page_size, head_dim, dtype=dtype, device=device)
     scales = torch.empty(num_pages, heads, head_dim // G, page_size, device=device,
                          dtype=torch.uint8 if scale_ue8m0 else torch.float32)
@@ -210,7 +212,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     ``max_kv_len`` (default: the table's capacity) bounds kv_lens; longer ones are cut to it.  A
     close bound gives a better split of the work.  ``workspace`` (optional): a uint8 GPU tensor
-    of at least ``attention_workspace_bytes(...)`` bytes.  Returns ``out`` [B, S, Hq, D]
+    of at least ``attention_workspace_bytes(...)`` bytes, which calls that may overlap do not
+    share.  Codes and scales of the tokens that are seen are finite.  Returns ``out`` [B, S, Hq, D]
     (contiguous, allocated unless given), asynchronously on the current stream."""
     mod, fast_stream = _lib.fast_module(k_cache) if workspace is None else (None, None)
     if mod is not None:

@@ -140,7 +140,8 @@ def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor
     outputs, the other arguments its inputs.  Returns ``(dq, dk, dq_weight, dk_weight)``: dq and
     dk of q's type (allocated unless given, views of a fused gradient included), the weights'
     float32 [D].  ``workspace`` (optional): a uint8 GPU tensor of at least
-    ``bwd_workspace_bytes(T, Hq, Hk, D)`` bytes.  Padding rows get zeros."""
+    ``bwd_workspace_bytes(T, Hq, Hk, D)`` bytes, which calls that may overlap do not share.
+    Padding rows get zeros."""
     mod, fast_stream = _lib.fast_module(q) if workspace is None else (None, None)
     if mod is not None:
         r = mod.rope_bwd(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, dq_out,

@@ -77,12 +77,16 @@ FAGQ_API int fagq_kv_cache_read_launch(const void* k_cache, const void* v_cache,
  * One scale for each token and head (G == D), D in {64, 128, 256}.  strides
  * (host memory, in elements): {sequence, token, head} of q, multiples of 8, below
  * 2^31; out is contiguous.  page_table int32 [B, table_width], null if the
- * width is 0; kv_lens [B] (index_dtype); prefix_pages int32 [ceil(prefix_len / page_size)], null without.
+ * width is 0; kv_lens [B] (index_dtype); prefix_pages int32
+ * [ceil(prefix_len / page_size)], null without.
  * max_kv_len: no kv_lens[b] is larger (it sizes the work split; longer ones are
  * cut to it).  Sums and softmax are in fp32; the probabilities, times their value
  * scales, are rounded to fp16 (relative to the largest) for the product with the
  * codes.  Codes and scales of the tokens that a sequence reads are finite; what
- * lies in other slots does not matter. */
+ * lies in other slots does not matter.  A UE8M0 scale of 0 (2^-127) counts as 0.
+ * The workspace (16-byte aligned) belongs to this call until it has run: calls that
+ * may overlap need one each.  FAGQ_E_TOO_LARGE (workspace: -1) for 2^24 rows
+ * and more. */
 FAGQ_API int64_t fagq_paged_attention_workspace_bytes(int64_t B, int64_t S, int64_t Hq, int64_t H,
                                                       int64_t D, int64_t prefix_len,
                                                       int64_t max_kv_len);

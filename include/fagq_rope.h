@@ -57,7 +57,8 @@ FAGQ_API int64_t fagq_qk_norm_rope_bwd_workspace_bytes(int64_t T, int64_t Hq, in
 
 /* dq_out, dk_out: gradients of q_out and k_out.  Writes dq, dk (dtype) and
  * dq_weight, dk_weight [D] (fp32).  strides: {token, head} of dq_out, dk_out, q,
- * k, dq, dk.  workspace: 16-byte aligned, overwritten.  Outputs overlap nothing.
+ * k, dq, dk.  workspace: 16-byte aligned, overwritten; calls that may overlap need
+ * one each.  Outputs overlap nothing.
  * The sums are added in an order that depends on the sizes alone. */
 FAGQ_API int fagq_qk_norm_rope_bwd_launch(const void* dq_out, const void* dk_out, const void* q,
                                           const void* k, const void* q_weight,

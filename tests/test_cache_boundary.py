@@ -206,6 +206,23 @@ def test_attention_workspace_is_checked(lib):
         assert attend(lib, ws=fake(2)) == 9
 
 
+def test_attention_refuses_what_no_grid_holds(lib):
+    # The largest grid is below 2^24 workgroups, and the joining kernel may have one for each row.
+    f = lib.fagq_paged_attention_workspace_bytes
+    assert f(65535, 1, 256, 256, 128, 0, 64) >= 0
+    assert f(4096, 1, 4096, 4096, 128, 0, 64) == -1
+    assert attend(lib, B=4096, Hq=4096, H=4096, prefix=0) == 7
+
+
+def test_attention_workspace_of_any_size_is_moderate(lib):
+    # A row has few parts, however its keys are cut: rows x parts of (D + 2) floats.
+    f = lib.fagq_paged_attention_workspace_bytes
+    for B, S, H in ((1, 1, 1), (1, 1, 8), (3, 1, 5), (1, 512, 1), (64, 1, 8), (700, 2, 3)):
+        for prefix, most in ((0, 1), (0, 100000), (0, 1 << 22), (1 << 20, 64), (5000, 5000)):
+            need = f(B, S, 8 * H, H, 128, prefix, most)
+            assert 0 <= need <= (B * S * 8 * H * 1100 + 512 * 2 * 64) * 130 * 4 + 4 * (B + 1)
+
+
 # ------------------------------------------------------------------------------------ lookups
 
 def slots(lib, table, cu, pages, page, rows):
@@ -287,3 +304,8 @@ def test_empty_kv_cache_formats(pkg):
     for D, G in ((512, None), (96, None), (128, 256), (128, 32)):
         with pytest.raises(ValueError):
             pkg.empty_kv_cache(3, 1, 64, D, G, device="cpu")
+
+
+def test_empty_kv_cache_refuses_codes_that_no_operator_takes(pkg):
+    with pytest.raises(TypeError, match="float8_e4m3fn or int8"):
+        pkg.empty_kv_cache(2, 2, 16, 64, dtype=torch.bfloat16, device="cpu")

@@ -152,6 +152,16 @@ def test_lengths_past_the_table_and_the_bound(pkg, gpu):
     assert bool((run(pkg, gpu, (q, caches, table, none, pp)) == 0).all())
 
 
+@pytest.mark.parametrize("S", [1, 5])
+def test_lengths_of_any_value(pkg, gpu, S):
+    note(f"attention with lengths of any value, S {S}")
+    low, high = torch.iinfo(torch.int64).min, torch.iinfo(torch.int64).max
+    made = make(12, [40] * 6, S, 4, 2, 64, 16)
+    table = made[2][:, :3].contiguous()
+    lens = torch.tensor([low, low + S, -1, high, high - S, 40], dtype=torch.int64)
+    check(pkg, gpu, (made[0], made[1], table, lens, None), most=40)
+
+
 def test_strided_queries_int64_lengths_and_a_given_output(pkg, gpu):
     made = make(8, [50, 3], 3, 6, 2, 128, 32)
     q, ((kc, ks), (vc, vs)), table, lens, _ = made
