@@ -198,9 +198,9 @@ int64_t height(int R, int64_t D) { return R == kTall ? kWaves * 16 * (256 / D) :
 // are used and where each of the kSlots workgroups has kTallKeys keys: fewer leave four times as many
 // parts to join (shared prefix, 8 heads of 128, us short / tall: 512 rows of 32768 keys 122 / 115, of
 // 4096 35 / 45, 192 rows of 32768 57 / 65; 16 sequences of 4096 keys, 8 heads of 128: 64 rows 47 /
-// 60, 96 rows 76 / 65, 128 rows 68 / 72, 256 rows 126 / 116, 2 heads of 256, 128 rows: 94 / 76).  Heads of 64 are bound
-// by the softmax, which is the same in both forms (8 sequences of 256 tokens, 32 + 8 heads, 4096
-// keys: 113 / 133).
+// 60, 96 rows 76 / 65, 128 rows 68 / 72, 256 rows 126 / 116, 4 heads of 256, 128 rows: 94 / 76).
+// Heads of 64 are bound by the softmax, which is the same in both forms (8 sequences of 256 tokens,
+// 32 + 8 heads, 4096 keys: 113 / 133).
 int row_tiles(int64_t rows, int64_t D, int64_t lists, int64_t keys) {
   if (D >= 128) {
     const int64_t tall = height(kTall, D), tiles = (rows + tall - 1) / tall;

@@ -14,7 +14,7 @@
 // times as many rows, a quarter for each wave (see Tall).  How units are cut:
 //   scheduled  The rounds of 128 keys of all units in a row are shared out evenly, so that every
 //              workgroup reads as much as the others however the lengths differ and whatever bound
-//              on them the host knows (64 sequences of 1400 to 8192 tokens: 116 us, with chunks
+//              on them the host knows (64 sequences of 1400 to 8192 tokens: 115 us, with chunks
 //              131).  Each workgroup works that out by itself from the lengths.
 //   static     Chunks of one size, chosen by the host: the prefix; sequences of more rows than a
 //              unit has; and calls of few rounds, where working out the shares takes longer than
@@ -36,6 +36,12 @@
 // fp32.  Probabilities times value scales are rounded to fp16 whatever q's type is: half a step
 // of 2^-11 of each, where bf16's 2^-8 would be as large an error as the result's own rounding
 // (measured against 64 bits: 2.4e-3 with bf16, 1.7e-3 with fp16, 1.7e-3 for the rounding alone).
+//
+// Bound: decode batches by HBM (64 sequences of 8192 tokens, 64 + 8 heads of 128: 174 us, 6.4 TB/s);
+// many rows by the softmax, whose VALU instructions take as many cycles as the products and are
+// overlapped with them in part (64 sequences behind 32768 shared tokens 116 us, 600 TFLOP/s; 4 of
+// 512 new tokens over 4096 keys, 32 + 8 heads of 128, 179 us, 720); small calls by two dependent
+// launches (4 sequences of 1000 tokens 9.2 us).
 #pragma once
 
 #include <hip/hip_runtime.h>

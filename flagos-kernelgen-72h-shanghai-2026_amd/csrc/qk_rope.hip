@@ -6,7 +6,9 @@
 //   dx = rstd (a - x rstd^2 mean(a x)),   dw = sum over rows of dn x rstd.
 // rstd is recomputed from x, which the backward reads anyway.
 //
-// Both directions are bound by HBM: 2 (3) tensors at one read or write each.  A row of D
+// Both directions are bound by HBM: 2 (3) tensors at one read or write each (16384 tokens, 64 + 8
+// heads of 128, bf16: 98.5 us, 6.2 TB/s; backward, 8192 tokens, 32 + 8: 43.6 us, 5.9 TB/s, and 4.8
+// for the sums of the weights' gradients).  A row of D
 // elements belongs to LPR = D / 16 lanes (a power of two, 4 to 32), 16 elements each in two
 // chunks of 8: for pairs (i, i + R / 2) lane l holds elements 8 l.. and R / 2 + 8 l.., for
 // adjacent pairs 16 l.. and 16 l + 8.., so that both halves of every pair are in one lane
