@@ -58,9 +58,10 @@ constexpr int kWaves = 4;
 constexpr int kStep = 32;            // keys of a wave's step
 constexpr int kRound = kStep * kWaves;
 constexpr float kLow = -3.0e38f;     // running maximum before the first key
-// The running maximum follows a row's scores only where they pass it by this much (p <= 2^8 then,
-// which neither the sums nor fp16 probabilities mind), so that o is rarely multiplied.
+// The running maximum follows a row's scores only where a weight (probability times value scale)
+// could pass 2^kSlack, which neither the sums nor fp16 minds, so that o is rarely multiplied.
 constexpr float kSlack = 8.0f;
+constexpr float kLeastScale = 0x1p-100f;   // smaller value scales count as this: p stays finite
 constexpr float kPartCost = 15.0f;   // what a part costs the joining kernel, in keys of a workgroup
 
 // kScheduledOnce: the codes are read past the caches (64 sequences of 8192 tokens, 64 + 8 heads of
@@ -325,7 +326,6 @@ struct Rows {
   f32x4 o[R][D / 16];          // dims D / 16 (4 g + r) + j at [j][r]
   float m[R], l[R];            // l: of this lane's keys
   int32_t seen[R];             // keys that the row sees
-  float unit, inv_unit;        // o is in units of `unit` (see join)
 };
 
 // Products of one step's keys with the queries.
@@ -353,10 +353,14 @@ __device__ __forceinline__ void scores(int lane, const RawKeys<D, SF>& raw, cons
 
 // The softmax of one step: 32 keys from `tok` on, of which all rows see those below `all`.  From the
 // products x, the keys' scales times scale2 and the values' scales (zeros for what no row sees) to
-// the probabilities times value scales, in units of s.unit, as fp16 operands of the next product.
+// the probabilities times value scales, as fp16 operands of the next product.
+//
+// m is the running maximum of score + log2(value scale), not of the score: p = 2^(x - m) times its
+// value scale is at most 2^kSlack then, which fits fp16, and what fp16 loses of a small one is lost
+// relative to the largest contribution to the row, however far apart the value scales are.
 template <int E, int D, int R>
 __device__ __forceinline__ void softmax(int lane, int32_t tok, int32_t all, const Pages& pages,
-                                        f32x4 (&x)[R][2], float (&ks)[8], float (&vs)[8],
+                                        f32x4 (&x)[R][2], float (&ks)[8], const float (&vs)[8],
                                         Rows<E, D, R>& s, u32x4 (&p)[R]) {
   constexpr int NT = D / 16;
   const int g = lane >> 4;
@@ -372,23 +376,9 @@ __device__ __forceinline__ void softmax(int lane, int32_t tok, int32_t all, cons
       ks[i] = 1.0f;
     }
   }
-  // Probabilities times value scales have to fit fp16: they are taken in units of the largest value
-  // scale so far, and o with them.  (Where one key has all the weight, its product is exact.)
   const float most = fmaxf(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])),
                            fmaxf(fmaxf(vs[4], vs[5]), fmaxf(vs[6], vs[7])));
-  if (__any(most > s.unit)) {
-    const float unit = fmaxf(__uint_as_float(__builtin_amdgcn_readfirstlane(
-                                 __float_as_uint(cross_max(most)))), 0x1p-100f);
-    const float inv = 1.0f / unit, f = s.unit * inv;
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) s.o[r][j] *= f;
-    s.unit = unit;
-    s.inv_unit = inv;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) vs[i] *= s.inv_unit;
+  const float room = kSlack - __builtin_amdgcn_logf(fmaxf(most, kLeastScale));
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     float y[8];
@@ -396,10 +386,12 @@ __device__ __forceinline__ void softmax(int lane, int32_t tok, int32_t all, cons
     for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(x[r][i / 4][i % 4], ks[i], -s.m[r]);
     const float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
                             fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-    if (__any(top > kSlack)) {
+    if (__any(!(top <= room))) {
       float m = s.m[r];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, x[r][i / 4][i % 4] * ks[i]);
+      for (int i = 0; i < 8; ++i)
+        m = fmaxf(m, __builtin_fmaf(x[r][i / 4][i % 4], ks[i],
+                                    __builtin_amdgcn_logf(fmaxf(vs[i], kLeastScale))));
       m = cross_max(m);
       const float f = __builtin_amdgcn_exp2f(s.m[r] - m);
       s.m[r] = m;
@@ -429,7 +421,7 @@ __device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t
   const int g = lane >> 4;
   float vs[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) vs[i] = scale_of<SF>(raw.s[i / 4], i % 4);
+  for (int i = 0; i < 8; ++i) vs[i] = fmaxf(scale_of<SF>(raw.s[i / 4], i % 4), kLeastScale);
   if (tok + kStep > end || pages.p[0] < 0 || pages.p[1] < 0) {
     // What no row sees may hold anything: its values and their scales become zeros.
 #pragma unroll
@@ -578,8 +570,6 @@ __device__ __forceinline__ void run_segment(const Args& a, const Segment& seg, S
     return *reinterpret_cast<const u32x4*>(q + 64 * (j / 2) + 16 * g + 8 * (j & 1));
   };
   Rows<E, D, R> s;
-  s.unit = 0.0f;
-  s.inv_unit = 0.0f;
   int32_t all = k.end, end = k.end;             // keys that all rows see; that the last one sees
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -622,7 +612,7 @@ __device__ __forceinline__ void run_segment(const Args& a, const Segment& seg, S
     float m = kLow;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) m = fmaxf(m, sh.m[w][16 * r + c]);
-    const float f = __builtin_amdgcn_exp2f(s.m[r] - m) * s.unit;
+    const float f = __builtin_amdgcn_exp2f(s.m[r] - m);
     float l = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
@@ -759,7 +749,7 @@ __device__ __forceinline__ void stage_tall(const Args& a, int lane, int wave, in
       sh.ks[buf][step][lane] = r.scale * a.scale2;
     } else {
       const bool live = r.tok + 16 * t + c < end && (t ? r.pages.p[1] : r.pages.p[0]) >= 0;
-      sh.vs[buf][step][lane - kStep] = live ? r.scale : 0.0f;
+      sh.vs[buf][step][lane - kStep] = live ? fmaxf(r.scale, kLeastScale) : 0.0f;
     }
   }
 }
@@ -784,8 +774,6 @@ __device__ __forceinline__ void run_tall(const Args& a, const Segment& seg,
   };
   Rows<E, D, R> s;
   u32x4 q[R][D / 32];
-  s.unit = 0.0f;
-  s.inv_unit = 0.0f;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int i = first_row + 16 * r + c;
@@ -911,7 +899,7 @@ __device__ __forceinline__ void run_tall(const Args& a, const Segment& seg,
     const int64_t row = ((int64_t)w.b * a.S + w.s) * a.Hq + w.hq;
     const bool whole = seg.to == kOut;
     const int64_t at = whole ? 0 : row * a.row_parts + seg.row_part;
-    const float f = whole ? (l > 0.0f ? s.unit / l : 0.0f) : s.unit;
+    const float f = whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
 #pragma unroll
     for (int hh = 0; hh < D / 64; ++hh) {       // dims 64 hh + 16 g + 4 r + i
       const int d = 64 * hh + 16 * g;

@@ -81,9 +81,10 @@ FAGQ_API int fagq_kv_cache_read_launch(const void* k_cache, const void* v_cache,
  * [ceil(prefix_len / page_size)], null without.
  * max_kv_len: no kv_lens[b] is larger (it sizes the work split; longer ones are
  * cut to it).  Sums and softmax are in fp32; the probabilities, times their value
- * scales, are rounded to fp16 (relative to the largest) for the product with the
- * codes.  Codes and scales of the tokens that a sequence reads are finite; what
- * lies in other slots does not matter.  A UE8M0 scale of 0 (2^-127) counts as 0.
+ * scales, are rounded to fp16 (relative to the row's largest) for the product with
+ * the codes.  Codes and scales of the tokens that a sequence reads are finite, value
+ * scales at most 2^100 (those below 2^-100 count as 2^-100, key scales of UE8M0 0 as
+ * 0); what lies in other slots does not matter.
  * The workspace (16-byte aligned) belongs to this call until it has run: calls that
  * may overlap need one each.  FAGQ_E_TOO_LARGE (workspace: -1) for 2^24 rows
  * and more. */
