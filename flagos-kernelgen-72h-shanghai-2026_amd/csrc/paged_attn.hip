@@ -20,8 +20,6 @@ constexpr int64_t kCUs = 256;
 constexpr int64_t kSlots = 2 * kCUs;   // workgroups of a round
 constexpr int64_t kFewRounds = 8 * kSlots;      // of all units: not worth a schedule
 constexpr int64_t kCacheBytes = 256ll << 20;    // of the cache behind the XCDs' L2
-constexpr int64_t kFixed = 128;        // what a workgroup costs besides its keys, in keys
-constexpr int64_t kTallKeys = 1024;    // of a workgroup, from which on tall units pay (see row_tiles)
 
 struct JoinArgs {
   const float* part;
@@ -193,29 +191,23 @@ struct Plan {
 // Rows of a unit.
 int64_t height(int R, int64_t D) { return R == kTall ? kWaves * 16 * (256 / D) : 16 * R; }
 
-// The row tiles of a unit, for so many rows that see so many keys, in each of `lists` lists of keys:
-// as few as hold them.  Tall units for heads of 128 and 256 where at least two thirds of their rows
-// are used and where each of the kSlots workgroups has kTallKeys keys: fewer leave four times as many
-// parts to join (shared prefix, 8 heads of 128, us short / tall: 512 rows of 32768 keys 122 / 115, of
-// 4096 35 / 45, 192 rows of 32768 57 / 65; 16 sequences of 4096 keys, 8 heads of 128: 64 rows 47 /
-// 60, 96 rows 76 / 65, 128 rows 68 / 72, 256 rows 126 / 116, 4 heads of 256, 128 rows: 94 / 76).
-// Heads of 64 are bound by the softmax, which is the same in both forms (8 sequences of 256 tokens,
-// 32 + 8 heads, 4096 keys: 113 / 133).
-int row_tiles(int64_t rows, int64_t D, int64_t lists, int64_t keys) {
-  if (D >= 128) {
-    const int64_t tall = height(kTall, D), tiles = (rows + tall - 1) / tall;
-    if (3 * rows >= 2 * tiles * tall && lists * tiles * keys >= kSlots * kTallKeys) return kTall;
-  }
-  const int R = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  return R * D <= 256 ? R : (int)(256 / D);
+// What a workgroup's keys cost, in keys of a short unit's workgroup / 5, and what it costs besides.
+constexpr int64_t kShortKey = 5, kTallKey = 14, kFixed = 5 * 128;
+
+int64_t key_cost(int R) { return R == kTall ? kTallKey : kShortKey; }
+
+// What one more part of each of so many rows costs the joining kernel: a step of its chain, or its
+// bytes, of which HBM moves 35 KB in the time of a key.
+int64_t part_cost(int64_t rows, int64_t D) {
+  const int64_t bytes = rows * D * 5 / (68 * 128);
+  return bytes > 5 * (int64_t)kPartCost ? bytes : 5 * (int64_t)kPartCost;
 }
 
 // Cuts a unit's keys into the number of chunks that takes least time where each of the `units`
-// becomes so many workgroups, the GPU runs them in rounds of kSlots, one takes as long as its keys
-// and kFixed, and each chunk costs the joining kernel kPartCost keys.  With w rounds, n chunks cost
-// w (keys / n + kFixed) + kPartCost n, least at sqrt(w keys / kPartCost): tried for each w, as far
-// as w rounds go (all n cost the host 19 us for one unit of 524288 keys).
-void cut(int64_t keys, int64_t units, int64_t* chunk, int64_t* chunks) {
+// becomes so many workgroups and the GPU runs them in rounds of kSlots; returns that time.  With w
+// rounds, n chunks cost w (key keys / n + kFixed) + part n, least at sqrt(w key keys / part): tried for
+// each w, as far as w rounds go (all n cost the host 19 us for one unit of 524288 keys).
+int64_t cut(int64_t keys, int64_t units, int64_t key, int64_t part, int64_t* chunk, int64_t* chunks) {
   const int64_t most = (keys + kRound - 1) / kRound;
   int64_t best = -1;
   *chunk = kRound, *chunks = 0;
@@ -225,9 +217,10 @@ void cut(int64_t keys, int64_t units, int64_t* chunk, int64_t* chunks) {
     int64_t c = (keys + n - 1) / n;
     c = (c + kRound - 1) / kRound * kRound;
     const int64_t got = (keys + c - 1) / c;
-    const int64_t cost = (units * got + kSlots - 1) / kSlots * (c + kFixed) + (int64_t)kPartCost * got;
-    if (best < 0 || cost < best) {
-      best = cost;
+    const int64_t time =
+        (units * got + kSlots - 1) / kSlots * (c * key + kFixed) + part * got;
+    if (best < 0 || time < best) {
+      best = time;
       *chunk = c;
       *chunks = got;
     }
@@ -236,10 +229,31 @@ void cut(int64_t keys, int64_t units, int64_t* chunk, int64_t* chunks) {
   for (int64_t w = 1; w <= 16; ++w) {
     const int64_t fit = w * kSlots / units;
     if (fit == 0) continue;
-    const int64_t n = (int64_t)std::sqrt((double)(w * keys) / kPartCost);
+    const int64_t n = (int64_t)std::sqrt((double)(w * keys * key) / (double)part);
     consider(n < fit ? n : fit);
     consider(n + 1 < fit ? n + 1 : fit);
   }
+  return best;
+}
+
+// The units of so many rows that see the same keys, in each of `lists` lists of so many: short ones, of
+// as few row tiles as hold the rows, or for heads of 128 and 256 tall ones where that takes less time.
+// (Heads of 64 are bound by the softmax, which is the same in both: 8 sequences of 256 tokens, 32 + 8
+// heads, 4096 keys 113 us short, 133 tall.)  Tall units read and widen codes once for four times as
+// many rows, but leave four times as many parts where workgroups are few, and waste more of their
+// last rows.  Short / tall, us: 16 sequences of 4096 keys, 8 heads of 128: 64 rows 47 / 60, 96 rows
+// 76 / 65, 256 rows 126 / 116; 4 heads of 256: 32 rows 38 / 43, 96 rows 95 / 74; 2 sequences, 8
+// heads of 128, 256 rows 28 / 37; a prefix, 8 heads of 128: 512 rows of 32768 keys 122 / 114, of
+// 4096 35 / 45.  The costs were fitted to 73 such pairs: over them the choice is 0.4 % off the best.
+int row_tiles(int64_t rows, int64_t D, int64_t lists, int64_t keys) {
+  int R = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  R = R * D <= 256 ? R : (int)(256 / D);
+  if (D == 64) return R;
+  int64_t chunk, chunks;
+  auto units = [&](int r) { return lists * ((rows + height(r, D) - 1) / height(r, D)); };
+  const int64_t part = part_cost(lists * rows, D);
+  const int64_t tall = cut(keys, units(kTall), key_cost(kTall), part, &chunk, &chunks);
+  return tall < cut(keys, units(R), key_cost(R), part, &chunk, &chunks) ? kTall : R;
 }
 
 Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t prefix_len,
@@ -252,13 +266,14 @@ Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t pr
     p.RP = row_tiles(B * per, D, H, prefix_len);
     if (p.R > 1 && p.RP != kTall) p.R = p.RP;
     p.prefix_tiles = (B * per + height(p.RP, D) - 1) / height(p.RP, D);
-    cut(prefix_len, H * p.prefix_tiles, &p.prefix_chunk, &p.prefix_chunks);
+    cut(prefix_len, H * p.prefix_tiles, key_cost(p.RP), part_cost(p.rows, D), &p.prefix_chunk,
+        &p.prefix_chunks);
     p.prefix_items = H * p.prefix_tiles * p.prefix_chunks;
   }
   p.tiles = (per + height(p.R, D) - 1) / height(p.R, D);
   if (p.tiles > 1 || p.R == kTall || most_rounds(B, H, most) <= kFewRounds) {
     p.form = kStatic;
-    cut(most, B * H * p.tiles, &p.chunk, &p.chunks);
+    cut(most, B * H * p.tiles, key_cost(p.R), part_cost(p.rows, D), &p.chunk, &p.chunks);
     if (p.chunks < 1) p.chunks = 1;     // rows without keys are written all the same
     p.items = B * H * p.tiles * p.chunks;
     p.row_parts = p.prefix_chunks + p.chunks;
