@@ -28,7 +28,7 @@ struct JoinArgs {
   const int32_t* sched;      // null: static
   uint16_t* out;
   int32_t B, S, Hq, H;
-  int32_t prefix_chunks, row_parts, chunk, most, height;
+  int32_t prefix_chunks, row_parts, chunk, most;
   int32_t idx64;
 };
 
@@ -62,9 +62,9 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attention_join(JoinArgs a) 
     if (cuts > 0) {
       const int i = (bs - b * a.S) * group + (hq - h * group);   // row of the unit
       const int64_t behind = (int64_t)a.B * a.S * a.Hq * a.row_parts + i;
-      own_first = segment_at(behind, a.height, wg, 1);
-      own = segment_at(behind, a.height, wg, 0);         // + 1 workgroup: the next ones
-      apart = 2 * a.height;
+      own_first = segment_at(behind, wg, 1);
+      own = segment_at(behind, wg, 0);         // + 1 workgroup: the next ones
+      apart = 2 * kSegmentRows;
     }
     n = a.prefix_chunks + cuts + 1;
   } else {
@@ -271,7 +271,7 @@ Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t pr
     p.prefix_items = H * p.prefix_tiles * p.prefix_chunks;
   }
   p.tiles = (per + height(p.R, D) - 1) / height(p.R, D);
-  if (p.tiles > 1 || p.R == kTall || most_rounds(B, H, most) <= kFewRounds) {
+  if (p.tiles > 1 || p.R > 1 || most_rounds(B, H, most) <= kFewRounds) {
     p.form = kStatic;
     cut(most, B * H * p.tiles, key_cost(p.R), part_cost(p.rows, D), &p.chunk, &p.chunks);
     if (p.chunks < 1) p.chunks = 1;     // rows without keys are written all the same
@@ -282,7 +282,7 @@ Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t pr
     p.form = prefix_len == 0 && 2 * B * most * H * D >= kCacheBytes ? kScheduledOnce : kScheduled;
     p.items = kSlots;
     p.row_parts = prefix_len > 0 ? p.prefix_chunks + 1 : 0;
-    p.parts = p.rows * p.row_parts + p.items * 2 * 16 * p.R;
+    p.parts = p.rows * p.row_parts + p.items * 2 * kSegmentRows;
   }
   return p;
 }
@@ -416,7 +416,7 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   j.part = a.part, j.ml = a.part_ml, j.lens = kv_lens, j.sched = a.sched, j.out = a.out;
   j.B = a.B, j.S = a.S, j.Hq = a.Hq, j.H = a.H;
   j.prefix_chunks = a.prefix_chunks, j.row_parts = a.row_parts, j.chunk = a.chunk, j.most = a.most;
-  j.height = 16 * p.R, j.idx64 = a.idx64;
+  j.idx64 = a.idx64;
   void* jargs[] = {&j};
   // A workgroup for each row where one may have more than kAhead parts.
   const int64_t rounds = (max_kv_len + kRound - 1) / kRound;

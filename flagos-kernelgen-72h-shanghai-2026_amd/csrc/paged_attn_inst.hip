@@ -14,16 +14,15 @@ const void* kernel() {
 
 // What plan_for makes, R D <= 256 or, for heads of 128 and 256, tall units: without a prefix, units
 // of any height; with one, 16 rows go with a prefix of units of any height, more rows with units of
-// their own height or tall ones, tall ones with tall ones.
+// their own height or tall ones, tall ones with tall ones.  Units of 16 rows may be scheduled.
 template <int D, int R, int RP>
 const void* lookup(int form) {
-  if constexpr (R == kTall) {
-    return kernel<D, R, RP, kStatic>();
-  } else {
+  if constexpr (R == 1) {
     if constexpr (RP == 0)
       if (form == kScheduledOnce) return kernel<D, R, RP, kScheduledOnce>();
-    return form == kStatic ? kernel<D, R, RP, kStatic>() : kernel<D, R, RP, kScheduled>();
+    if (form != kStatic) return kernel<D, R, RP, kScheduled>();
   }
+  return kernel<D, R, RP, kStatic>();
 }
 template <int D, int R>
 const void* lookup(int RP, int form) {

@@ -16,9 +16,11 @@
 //              workgroup reads as much as the others however the lengths differ and whatever bound
 //              on them the host knows (64 sequences of 1400 to 8192 tokens: 115 us, with chunks
 //              131).  Each workgroup works that out by itself from the lengths.
-//   static     Chunks of one size, chosen by the host: the prefix; sequences of more rows than a
-//              unit has; and calls of few rounds, where working out the shares takes longer than
-//              uneven ones (4 sequences of 1000 tokens: 8.2 us, scheduled 10.3).
+//   static     Chunks of one size, chosen by the host: the prefix; sequences of more than 16 rows,
+//              whose units cost more to begin and to end in the middle (64 of 1500 tokens, 8 heads of
+//              128, 32 rows: 43 us, scheduled 51; 16 of 4096, 16 heads of 64, 64 rows: 48, 80); and
+//              calls of few rounds, where working out the shares takes longer than uneven ones (4
+//              sequences of 1000 tokens: 8.2 us, scheduled 10.3).
 // The parts of a cut unit are joined by a second kernel.
 //
 // Keys and values go from HBM straight into the registers that feed the matrix instructions
@@ -178,10 +180,11 @@ __device__ __forceinline__ int32_t rounds_of(int32_t len) {
   return n > 1 ? n : 1;
 }
 
-// First index of the parts that a workgroup leaves of units of `height` rows: slot 1 of the unit
-// that it began and did not finish, slot 0 of the one that it did not begin.
-__device__ __forceinline__ int64_t segment_at(int64_t first, int height, int wg, int slot) {
-  return first + ((int64_t)wg * 2 + slot) * height;
+// First index of the parts that a workgroup leaves of units of 16 rows: slot 1 of the unit that it
+// began and did not finish, slot 0 of the one that it did not begin.
+constexpr int kSegmentRows = 16;
+__device__ __forceinline__ int64_t segment_at(int64_t first, int wg, int slot) {
+  return first + ((int64_t)wg * 2 + slot) * kSegmentRows;
 }
 
 // Maximum (sum) over the four lanes c, c + 16, c + 32, c + 48; every one of them receives it.
@@ -1079,8 +1082,8 @@ __device__ __forceinline__ Share share_of_many(const Args& a, int wg, Schedule& 
   return s;
 }
 
-template <int E, int QF, int SF, int D, int R, bool ONCE>
-__device__ __forceinline__ void run_share(const Args& a, int wg, Shared<D, R>& sh, Schedule& sc) {
+template <int E, int QF, int SF, int D, bool ONCE>
+__device__ __forceinline__ void run_share(const Args& a, int wg, Shared<D, 1>& sh, Schedule& sc) {
   const int lane = threadIdx.x & 63;
   const bool few = a.B <= 64;
   const int32_t lens = few ? own_length(a.lens, a.idx64, a.most, lane < a.B ? lane : 0) : 0;
@@ -1104,11 +1107,11 @@ __device__ __forceinline__ void run_share(const Args& a, int wg, Shared<D, R>& s
     s.keys.end = r1 == n ? s.len : r1 * kRound;
     s.row_part = a.prefix_chunks;
     s.to = r0 > 0 || r1 < n
-               ? segment_at((int64_t)a.B * a.S * a.Hq * a.row_parts, 16 * R, wg, r0 > 0 ? 0 : 1)
+               ? segment_at((int64_t)a.B * a.S * a.Hq * a.row_parts, wg, r0 > 0 ? 0 : 1)
            : a.prefix_len > 0 ? kRowParts
                               : kOut;
     if (pos > lo) __syncthreads();              // the last segment's LDS has been read
-    run_segment<E, QF, SF, D, R, false, ONCE>(a, s, sh);
+    run_segment<E, QF, SF, D, 1, false, ONCE>(a, s, sh);
     pos += r1 - r0;
     if (r1 == n && s.h == a.H - 1) {
       first += n * a.H;
@@ -1142,8 +1145,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention(Args a) {
     run_chunk<E, QF, SF, D, R == kTall ? 1 : R, false, R == kTall>(a, item - a.prefix_items, lds);
   } else {
     __shared__ Schedule sc;
-    run_share<E, QF, SF, D, R, FORM == kScheduledOnce>(
-        a, item - a.prefix_items, *reinterpret_cast<Shared<D, R>*>(lds), sc);
+    static_assert(R == 1, "units of 16 rows");
+    run_share<E, QF, SF, D, FORM == kScheduledOnce>(
+        a, item - a.prefix_items, *reinterpret_cast<Shared<D, 1>*>(lds), sc);
   }
 }
 
