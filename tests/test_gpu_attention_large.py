@@ -44,7 +44,7 @@ def test_cache_of_more_than_4_gib(pkg, gpu, S, group):
         vc, vs = pkg.empty_kv_cache(pages, H, page, D, device=gpu)
         slots = (where[:, None] * page + torch.arange(page, device=gpu)).reshape(-1)
         pkg.kv_cache_write(k, v, slots, kc, vc, ks, vs)
-        for most in (192, 1 << 19):      # rows on few keys, and as many as tall units take
+        for most in (192, 1 << 22):      # rows on few keys, and as many as tall units take
             t = torch.full((B, most // page), -1, dtype=torch.int32, device=gpu)
             t[:, :3] = table
             results.append(pkg.paged_attention(q, kc, vc, ks, vs, t, lens, D ** -0.5))

@@ -67,8 +67,8 @@ def put(made, prefix, token, b, score, factor):
 FORMS = [
     # lens, S, Hq, H, D, prefix, tokens that the table has room for
     ([200, 33], 1, 8, 2, 128, 0, None), ([300], 1, 8, 1, 64, 0, 1 << 20), ([260, 90], 1, 2, 2, 256, 0, None),
-    ([140, 150], 20, 4, 2, 64, 0, None), ([150, 120], 24, 4, 1, 128, 0, None), ([260, 190], 100, 2, 1, 128, 0, 1 << 18),
-    ([190], 64, 2, 1, 256, 0, 1 << 18), ([40, 90, 0], 1, 8, 2, 64, 150, None), ([70] * 9, 2, 4, 1, 128, 150, None),
+    ([140, 150], 20, 4, 2, 64, 0, None), ([150, 120], 24, 4, 1, 128, 0, None), ([260, 190], 100, 2, 1, 128, 0, 1 << 24),
+    ([190], 64, 2, 1, 256, 0, 1 << 24), ([40, 90, 0], 1, 8, 2, 64, 150, None), ([70] * 9, 2, 4, 1, 128, 150, None),
 ]
 
 

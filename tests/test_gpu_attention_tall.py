@@ -1,7 +1,7 @@
 """paged_attention's tall units (64 or 128 query rows that see the same keys, for heads of 256 and
 128): long chunks of new tokens and prefixes of large batches, against the softmax in 64 bits, at
-row counts about the border where they are taken and lengths that end anywhere.  They are taken where
-the bound on the keys is large; what is really there may be little."""
+row counts about the borders of units and lengths that end anywhere.  They are taken where the bound
+on the keys is large; what is really there may be little."""
 import random
 
 import pytest
@@ -15,7 +15,7 @@ from tests.test_gpu_paged_attention import BF16, F16, FP8, INT8, check, clean, m
 pytestmark = pytest.mark.gpu
 
 FORMATS = [(FP8, False, BF16), (FP8, True, F16), (INT8, False, F16), (INT8, True, BF16)]
-KEYS = 1 << 19                     # of all units' lists together, from which on units are tall
+KEYS = 1 << 25                     # of all units' lists together: so many that units are tall
 
 CASES = [
     # lens, S, Hq, H, D, page
@@ -84,8 +84,9 @@ def test_border_of_row_counts(pkg, gpu, rows):
     check_spread(pkg, gpu, make(rows, [2] * rows, 1, 1, 1, 128, 16, 70), 70, KEYS)
 
 
-@pytest.mark.parametrize("keys", [KEYS // 2 - 16, KEYS // 2, KEYS - 16, KEYS])
-def test_border_of_keys(pkg, gpu, keys):
+@pytest.mark.parametrize("keys", [KEYS >> i for i in range(12)])
+def test_number_of_keys(pkg, gpu, keys):
+    """Few keys leave short units, many take tall ones."""
     note(f"tall keys {keys}")
     check(pkg, gpu, widened(make(5, [200, 90], 96, 1, 1, 128, 16), keys // 2, 16))
     check_spread(pkg, gpu, make(6, [2] * 100, 1, 1, 1, 128, 16, 70), 70, keys)
@@ -105,7 +106,7 @@ def test_prefix_beside_shares(pkg, gpu, tokens):
     note(f"tall prefix beside shares, {tokens}")
     lens = [900, 3, 0, 260] * 30
     made = make(2, lens, 1, 4, 2, 128, 16, 300)
-    check_spread(pkg, gpu, widened(made, tokens, 16), 300, KEYS // 2)
+    check_spread(pkg, gpu, widened(made, tokens, 16), 300, KEYS)
 
 
 def test_short_prefix_beside_many_rows(pkg, gpu):
