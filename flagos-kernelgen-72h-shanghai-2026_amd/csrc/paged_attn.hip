@@ -18,7 +18,14 @@ namespace {
 
 constexpr int64_t kCUs = 256;
 constexpr int64_t kSlots = 2 * kCUs;   // workgroups of a round
-constexpr int64_t kFewRounds = 8 * kSlots;      // of all units: not worth a schedule
+// Shares are for long lists of keys: with short ones a workgroup has several units, one after the
+// other, that chunks give to as many workgroups at once (chunks / shares, us: 8 heads of 128, 64
+// sequences of 4096 keys 102 / 97, of 3000 77 / 74, 256 of 2048 199 / 205, ragged 79 / 71, 56 / 58 and
+// 136 / 164; 2 heads of 128, 512 ragged ones of 300: 53 / 105; 8 heads of 64, 64 of 6000 77 / 73, of
+// 4096 54 / 54, 16 heads, 16 of 4096: 28 / 32), and for many rounds altogether (8 heads of 128, 4 of
+// 32768 keys 57 / 55, 8 of 8192 28.7 / 30.2).
+constexpr int64_t kLongUnit = 32, kLongUnit64 = 40;   // rounds; of heads of 64
+constexpr int64_t kFewRounds = 8 * kSlots;            // of all units
 constexpr int64_t kCacheBytes = 256ll << 20;    // of the cache behind the XCDs' L2
 
 struct JoinArgs {
@@ -271,7 +278,8 @@ Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t pr
     p.prefix_items = H * p.prefix_tiles * p.prefix_chunks;
   }
   p.tiles = (per + height(p.R, D) - 1) / height(p.R, D);
-  if (p.tiles > 1 || p.R > 1 || most_rounds(B, H, most) <= kFewRounds) {
+  if (p.tiles > 1 || p.R > 1 || most_rounds(1, 1, most) < (D == 64 ? kLongUnit64 : kLongUnit) ||
+      most_rounds(B, H, most) <= kFewRounds) {
     p.form = kStatic;
     cut(most, B * H * p.tiles, key_cost(p.R), part_cost(p.rows, D), &p.chunk, &p.chunks);
     if (p.chunks < 1) p.chunks = 1;     // rows without keys are written all the same

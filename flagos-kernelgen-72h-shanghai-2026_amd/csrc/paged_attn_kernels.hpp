@@ -18,9 +18,9 @@
 //              131).  Each workgroup works that out by itself from the lengths.
 //   static     Chunks of one size, chosen by the host: the prefix; sequences of more than 16 rows,
 //              whose units cost more to begin and to end in the middle (64 of 1500 tokens, 8 heads of
-//              128, 32 rows: 43 us, scheduled 51; 16 of 4096, 16 heads of 64, 64 rows: 48, 80); and
-//              calls of few rounds, where working out the shares takes longer than uneven ones (4
-//              sequences of 1000 tokens: 8.2 us, scheduled 10.3).
+//              128, 32 rows: 43 us, scheduled 51; 16 of 4096, 16 heads of 64, 64 rows: 48, 80); short
+//              sequences; and calls of few rounds, where working out the shares takes longer than
+//              uneven ones (4 sequences of 1000 tokens: 8.2 us, scheduled 10.3).
 // The parts of a cut unit are joined by a second kernel.
 //
 // Keys and values go from HBM straight into the registers that feed the matrix instructions

@@ -105,3 +105,22 @@ def test_workspace_of_shares(pkg, gpu, tokens, prefix):
         buf[:need] = fill
         got = run(pkg, gpu, made, prefix, workspace=buf[:need])
         assert torch.equal(got, want) and bool((buf[need:] == 0xA5).all())
+
+
+@pytest.mark.parametrize("B,idx,D", [(64, torch.int32, 64), (65, torch.int64, 128), (257, torch.int32, 64), (700, torch.int64, 256)])
+def test_many_sequences_in_shares(pkg, gpu, B, idx, D):
+    """As above, with room for sequences so long that they are cut into shares."""
+    rng = random.Random(B)
+    lens = [rng.choice([0, 1, rng.randint(1, 300)]) for _ in range(B)]
+    lens[B // 2], lens[-1] = 1700, 900
+    note(f"schedule {B} sequences in shares, D {D}")
+    q, caches, table, n, pp = make(B, lens, 1, 4, 2, D, 16)
+    check(pkg, gpu, widened((q, caches, table, n.to(idx), pp), 128 * 48, 16))
+
+
+def test_full_shares_of_long_sequences(pkg, gpu):
+    rng = random.Random(10)
+    lens = [rng.randint(1, 1500) for _ in range(40)]
+    note("schedule, full shares of long sequences")
+    check(pkg, gpu, widened(make(5, lens, 1, 32, 16, 64, 64), 128 * 48, 64))
+    check(pkg, gpu, widened(make(6, lens, 1, 32, 16, 128, 64, 70), 128 * 48, 64), 70)
