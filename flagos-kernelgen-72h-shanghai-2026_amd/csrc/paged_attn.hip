@@ -21,12 +21,14 @@ constexpr int64_t kSlots = 2 * kCUs;   // workgroups of a round
 // Shares are for long lists of keys: with short ones a workgroup has several units, one after the
 // other, that chunks give to as many workgroups at once (chunks / shares, us: 8 heads of 128, 64
 // sequences of 4096 keys 102 / 97, of 3000 77 / 74, 256 of 2048 199 / 205, ragged 79 / 71, 56 / 58 and
-// 136 / 164; 2 heads of 128, 512 ragged ones of 300: 53 / 105; 8 heads of 64, 64 of 6000 77 / 73, of
+// 136 / 164, 512 ragged ones of 300 53 / 105; 8 heads of 64, 64 of 6000 77 / 73, of
 // 4096 54 / 54, 16 heads, 16 of 4096: 28 / 32), and for many rounds altogether (8 heads of 128, 4 of
 // 32768 keys 57 / 55, 8 of 8192 28.7 / 30.2).
 constexpr int64_t kLongUnit = 32, kLongUnit64 = 40;   // rounds; of heads of 64
 constexpr int64_t kFewRounds = 8 * kSlots;            // of all units
 constexpr int64_t kCacheBytes = 256ll << 20;    // of the cache behind the XCDs' L2
+
+constexpr int64_t kMostGroups = (1ll << 32) / (64 * kWaves);   // a grid of 2^32 threads is too large
 
 struct JoinArgs {
   const float* part;
@@ -178,8 +180,8 @@ int check_sizes(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t 
   if (B < 0 || S < 1 || H < 1 || Hq < H || Hq % H != 0 || (D != 64 && D != 128 && D != 256) ||
       prefix_len < 0 || max_kv_len < 0)
     return FAGQ_E_SHAPE;
-  // A grid of 2^32 threads is one too many: the joining kernel may have a workgroup for each row.
-  if (B > 65535 || S > 65535 || Hq > 4096 || B * S * Hq >= (1ll << 32) / (64 * kWaves) ||
+  // The joining kernel may have a workgroup for each row.
+  if (B > 65535 || S > 65535 || Hq > 4096 || B * S * Hq >= kMostGroups ||
       prefix_len > (1ll << 30) || max_kv_len > (1ll << 30) ||
       most_rounds(B, H, max_kv_len) >= (1ll << 31) - kSlots)
     return FAGQ_E_TOO_LARGE;
@@ -255,9 +257,10 @@ int64_t cut(int64_t keys, int64_t units, int64_t key, int64_t part, int64_t* chu
 int row_tiles(int64_t rows, int64_t D, int64_t lists, int64_t keys) {
   int R = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   R = R * D <= 256 ? R : (int)(256 / D);
-  if (D == 64) return R;
-  int64_t chunk, chunks;
   auto units = [&](int r) { return lists * ((rows + height(r, D) - 1) / height(r, D)); };
+  // A tall unit never takes less time than two short ones.
+  if (D == 64 || units(R) <= 2 * units(kTall)) return R;
+  int64_t chunk, chunks;
   const int64_t part = part_cost(lists * rows, D);
   const int64_t tall = cut(keys, units(kTall), key_cost(kTall), part, &chunk, &chunks);
   return tall < cut(keys, units(R), key_cost(R), part, &chunk, &chunks) ? kTall : R;
@@ -328,7 +331,8 @@ FAGQ_API int64_t fagq_paged_attention_workspace_bytes(int64_t B, int64_t S, int6
   using namespace fagq::attn;
   if (check_sizes(B, S, Hq, H, D, prefix_len, max_kv_len) != FAGQ_OK) return -1;
   if (B == 0) return 0;
-  return bytes_of(plan_for(B, S, Hq, H, D, prefix_len, max_kv_len), B, D);
+  const Plan p = plan_for(B, S, Hq, H, D, prefix_len, max_kv_len);
+  return p.prefix_items + p.items < kMostGroups ? bytes_of(p, B, D) : -1;
 }
 
 FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, const void* v_cache,
@@ -371,6 +375,7 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
       !aligned(kv_lens, is) || !aligned(prefix_pages, 4) || !aligned(out, 16))
     return FAGQ_E_ALIGN;
   const Plan p = B > 0 ? plan_for(B, S, Hq, H, D, prefix_len, max_kv_len) : Plan{};
+  if (p.prefix_items + p.items >= kMostGroups) return FAGQ_E_TOO_LARGE;
   const int64_t need = B > 0 ? bytes_of(p, B, D) : 0;
   if (need > 0 && !workspace) return FAGQ_E_NULL;
   if (workspace_bytes < need) return FAGQ_E_SHAPE;

@@ -43,7 +43,7 @@
 // many rows by the softmax, whose VALU instructions take as many cycles as the products and are
 // overlapped with them in part (64 sequences behind 32768 shared tokens 116 us, 600 TFLOP/s; 4 of
 // 512 new tokens over 4096 keys, 32 + 8 heads of 128, 179 us, 720); small calls by two dependent
-// launches (4 sequences of 1000 tokens 9.2 us).
+// launches (4 sequences of 1000 tokens 9.6 us).
 #pragma once
 
 #include <hip/hip_runtime.h>

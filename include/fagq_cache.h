@@ -87,7 +87,7 @@ FAGQ_API int fagq_kv_cache_read_launch(const void* k_cache, const void* v_cache,
  * 0); what lies in other slots does not matter.
  * The workspace (16-byte aligned) belongs to this call until it has run: calls that
  * may overlap need one each.  FAGQ_E_TOO_LARGE (workspace: -1) for 2^24 rows
- * and more. */
+ * or workgroups and more. */
 FAGQ_API int64_t fagq_paged_attention_workspace_bytes(int64_t B, int64_t S, int64_t Hq, int64_t H,
                                                       int64_t D, int64_t prefix_len,
                                                       int64_t max_kv_len);

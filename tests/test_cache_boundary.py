@@ -212,6 +212,9 @@ def test_attention_refuses_what_no_grid_holds(lib):
     assert f(65535, 1, 256, 256, 128, 0, 64) >= 0
     assert f(4096, 1, 4096, 4096, 128, 0, 64) == -1
     assert attend(lib, B=4096, Hq=4096, H=4096, prefix=0) == 7
+    # 65535 * 256 units of own keys, and those of the prefix ahead of them.
+    assert f(65535, 1, 256, 256, 128, 64, 64) == -1
+    assert attend(lib, B=65535, Hq=256, H=256, prefix=64) == 7
 
 
 def test_attention_workspace_of_any_size_is_moderate(lib):
