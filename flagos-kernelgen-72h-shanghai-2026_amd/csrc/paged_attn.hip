@@ -107,8 +107,9 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attention_join(JoinArgs a) 
     float w = 0.0f;
     if (i0 + lane < n) {
       const f32x2 v = i0 == 0 ? first : ml[index(i0 + lane)];
-      w = __builtin_amdgcn_exp2f(v[0] - m);
-      l += w * v[1];
+      const Power f = power_of(v[0] - m);
+      w = f.a * f.b;
+      l = __builtin_fmaf(v[1] * f.b, f.a, l);
     }
     const int stop = n - i0 < 64 ? n - i0 : 64;
     int i = sub;

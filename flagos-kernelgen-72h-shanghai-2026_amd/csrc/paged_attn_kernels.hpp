@@ -63,7 +63,9 @@ constexpr float kLow = -3.0e38f;     // running maximum before the first key
 // The running maximum follows a row's scores only where a weight (probability times value scale)
 // could pass 2^kSlack, which neither the sums nor fp16 minds, so that o is rarely multiplied.
 constexpr float kSlack = 8.0f;
-constexpr float kLeastScale = 0x1p-100f;   // smaller value scales count as this: p stays finite
+// Value scales lie in [0, 2^64]; smaller ones than this count as this in the running maximum, so that p
+// is at most 2^(64 + kSlack).  See softmax for what the two bounds are for.
+constexpr float kLeastScale = 0x1p-64f;
 constexpr float kPartCost = 15.0f;   // what a part costs the joining kernel, in keys of a workgroup
 
 // kScheduledOnce: the codes are read past the caches (64 sequences of 8192 tokens, 64 + 8 heads of
@@ -203,6 +205,15 @@ __device__ __forceinline__ float cross_sum(float v) {
   const uint32_t w = __float_as_uint(m);
   const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// 2^d for d <= 0 as a product: what 2^d alone is too small for in fp32 keeps its value if it is multiplied
+// by b, then by a.  b is 1 for d >= -64.
+struct Power {
+  float a, b;
+};
+__device__ __forceinline__ Power power_of(float d) {
+  return {__builtin_amdgcn_exp2f(fmaxf(d, -64.0f)), __builtin_amdgcn_exp2f(fminf(d + 64.0f, 0.0f))};
 }
 
 // The pages of a step's two tiles, -1: none.
@@ -360,7 +371,12 @@ __device__ __forceinline__ void scores(int lane, const RawKeys<D, SF>& raw, cons
 //
 // m is the running maximum of score + log2(value scale), not of the score: p = 2^(x - m) times its
 // value scale is at most 2^kSlack then, which fits fp16, and what fp16 loses of a small one is lost
-// relative to the largest contribution to the row, however far apart the value scales are.
+// relative to the largest contribution to the row, however far apart the value scales are.  l is in the
+// same units, so the bounds of the value scales keep it in fp32's range: m <= largest score + 64, so the
+// largest score's p is 2^-64 or more and what is flushed below 2^-126 is 2^-62 of it; and p <= 2^72, so
+// 2^31 keys add up to at most 2^103.  But from one m to the next l may fall by more than 2^-126 (keys of
+// scale 0, then one of 2^64: 2^-128 at equal scores), where o, whose terms fall with it, may become 0
+// and l may not: it takes the factor in two.
 template <int E, int D, int R>
 __device__ __forceinline__ void softmax(int lane, int32_t tok, int32_t all, const Pages& pages,
                                         f32x4 (&x)[R][2], float (&ks)[8], const float (&vs)[8],
@@ -396,11 +412,11 @@ __device__ __forceinline__ void softmax(int lane, int32_t tok, int32_t all, cons
         m = fmaxf(m, __builtin_fmaf(x[r][i / 4][i % 4], ks[i],
                                     __builtin_amdgcn_logf(fmaxf(vs[i], kLeastScale))));
       m = cross_max(m);
-      const float f = __builtin_amdgcn_exp2f(s.m[r] - m);
+      const Power f = power_of(s.m[r] - m);
       s.m[r] = m;
-      s.l[r] *= f;
+      s.l[r] = s.l[r] * f.b * f.a;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) s.o[r][j] *= f;
+      for (int j = 0; j < NT; ++j) s.o[r][j] *= f.a * f.b;
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(x[r][i / 4][i % 4], ks[i], -m);
     }
@@ -424,7 +440,7 @@ __device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t
   const int g = lane >> 4;
   float vs[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) vs[i] = fmaxf(scale_of<SF>(raw.s[i / 4], i % 4), kLeastScale);
+  for (int i = 0; i < 8; ++i) vs[i] = scale_of<SF>(raw.s[i / 4], i % 4);
   if (tok + kStep > end || pages.p[0] < 0 || pages.p[1] < 0) {
     // What no row sees may hold anything: its values and their scales become zeros.
 #pragma unroll
@@ -618,8 +634,10 @@ __device__ __forceinline__ void run_segment(const Args& a, const Segment& seg, S
     const float f = __builtin_amdgcn_exp2f(s.m[r] - m);
     float l = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-      l += sh.l[w][16 * r + c] * __builtin_amdgcn_exp2f(sh.m[w][16 * r + c] - m);
+    for (int w = 0; w < kWaves; ++w) {
+      const Power g = power_of(sh.m[w][16 * r + c] - m);
+      l = __builtin_fmaf(sh.l[w][16 * r + c] * g.b, g.a, l);
+    }
     if (r > 0) __syncthreads();                 // the last tile's o has been read
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -752,7 +770,7 @@ __device__ __forceinline__ void stage_tall(const Args& a, int lane, int wave, in
       sh.ks[buf][step][lane] = r.scale * a.scale2;
     } else {
       const bool live = r.tok + 16 * t + c < end && (t ? r.pages.p[1] : r.pages.p[0]) >= 0;
-      sh.vs[buf][step][lane - kStep] = live ? fmaxf(r.scale, kLeastScale) : 0.0f;
+      sh.vs[buf][step][lane - kStep] = live ? r.scale : 0.0f;
     }
   }
 }

@@ -214,8 +214,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     close bound gives a better split of the work.  ``workspace`` (optional): a uint8 GPU tensor
     of at least ``attention_workspace_bytes(...)`` bytes, which calls that may overlap do not
     share.  Codes and scales of the tokens that are seen are finite, value
-    scales at most 2^100.  Returns ``out`` [B, S, Hq, D]
-    (contiguous, allocated unless given), asynchronously on the current stream."""
+    scales 0 to 2^64.  Returns ``out`` [B, S, Hq, D] (contiguous, allocated unless given),
+    asynchronously on the current stream."""
     mod, fast_stream = _lib.fast_module(k_cache) if workspace is None else (None, None)
     if mod is not None:
         r = mod.attention(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, sm_scale,

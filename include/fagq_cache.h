@@ -83,8 +83,8 @@ FAGQ_API int fagq_kv_cache_read_launch(const void* k_cache, const void* v_cache,
  * cut to it).  Sums and softmax are in fp32; the probabilities, times their value
  * scales, are rounded to fp16 (relative to the row's largest) for the product with
  * the codes.  Codes and scales of the tokens that a sequence reads are finite, value
- * scales at most 2^100 (those below 2^-100 count as 2^-100, key scales of UE8M0 0 as
- * 0); what lies in other slots does not matter.
+ * scales 0 to 2^64 (below 2^-64 what a key adds is exact to 2^-88 of its codes only;
+ * UE8M0 0 counts as 0); what lies in other slots does not matter.
  * The workspace (16-byte aligned) belongs to this call until it has run: calls that
  * may overlap need one each.  FAGQ_E_TOO_LARGE (workspace: -1) for 2^24 rows
  * or workgroups and more. */
