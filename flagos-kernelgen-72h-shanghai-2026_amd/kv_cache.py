@@ -186,6 +186,10 @@ def _check_table(page_table: torch.Tensor, dev: torch.device) -> tuple[int, int]
 
 def attention_workspace_bytes(B: int, S: int, Hq: int, H: int, D: int, prefix_len: int,
                               max_kv_len: int) -> int:
+    """Workspace bytes of a ``paged_attention`` of exactly these sizes, where max_kv_len is the
+    smaller of its argument and the page table's capacity.  Not monotone: a smaller batch or bound
+    is cut into more parts and may need more, so a workspace that serves several calls is as large
+    as the largest of theirs."""
     n = _lib.load().fagq_paged_attention_workspace_bytes(B, S, Hq, H, D, prefix_len, max_kv_len)
     if n < 0:
         raise ValueError(f"no workspace size for B={B}, S={S}, Hq={Hq}, H={H}, D={D}, "
@@ -212,8 +216,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     ``max_kv_len`` (default: the table's capacity) bounds kv_lens; longer ones are cut to it.  A
     close bound gives a better split of the work.  ``workspace`` (optional): a uint8 GPU tensor
-    of at least ``attention_workspace_bytes(...)`` bytes, which calls that may overlap do not
-    share.  Codes and scales of the tokens that are seen are finite, value
+    of at least ``attention_workspace_bytes(...)`` bytes for these sizes (a smaller call may need
+    more), which calls that may overlap do not share.  Codes and scales of the tokens that are seen are finite, value
     scales 0 to 2^64.  Returns ``out`` [B, S, Hq, D] (contiguous, allocated unless given),
     asynchronously on the current stream."""
     mod, fast_stream = _lib.fast_module(k_cache) if workspace is None else (None, None)

@@ -86,7 +86,10 @@ FAGQ_API int fagq_kv_cache_read_launch(const void* k_cache, const void* v_cache,
  * scales 0 to 2^64 (below 2^-64 what a key adds is exact to 2^-88 of its codes only;
  * UE8M0 0 counts as 0); what lies in other slots does not matter.
  * The workspace (16-byte aligned) belongs to this call until it has run: calls that
- * may overlap need one each.  FAGQ_E_TOO_LARGE (workspace: -1) for 2^24 rows
+ * may overlap need one each.  Its size is that of exactly these B ... max_kv_len: fewer
+ * sequences or a smaller bound are cut into more parts and may need more (B 16 2.1 MB where
+ * B 64 needs none), so one that serves several calls is as large as the largest of theirs.
+ * FAGQ_E_TOO_LARGE (workspace: -1) for 2^24 rows
  * or workgroups and more. */
 FAGQ_API int64_t fagq_paged_attention_workspace_bytes(int64_t B, int64_t S, int64_t Hq, int64_t H,
                                                       int64_t D, int64_t prefix_len,

@@ -206,6 +206,22 @@ def test_attention_workspace_is_checked(lib):
         assert attend(lib, ws=fake(2)) == 9
 
 
+@pytest.mark.parametrize("large,small", [
+    (dict(B=64, S=1, Hq=64, H=8, D=128, most=1024), dict(B=16)),
+    (dict(B=112, S=16, Hq=32, H=8, D=256, most=9409), dict(most=8190)),
+    (dict(B=83, S=16, Hq=64, H=8, D=256, most=2574), dict(B=41)),
+])
+def test_a_smaller_call_may_need_a_larger_workspace(lib, large, small):
+    # As documented: the larger call's workspace is refused then, before any device work.
+    small = {**large, **small}
+    size = lambda c: lib.fagq_paged_attention_workspace_bytes(c["B"], c["S"], c["Hq"], c["H"], c["D"], 0, c["most"])
+    call = lambda c, n: attend(lib, **c, width=1 << 10, prefix=0, wsb=n, ws=fake(9),
+                               st=(c["S"] * c["Hq"] * c["D"], c["Hq"] * c["D"], c["D"]))
+    assert 0 <= size(large) < size(small)
+    assert call(small, size(large)) == 2
+    assert call(small, size(small) - 1) == 2
+
+
 def test_attention_refuses_what_no_grid_holds(lib):
     # The largest grid is below 2^24 workgroups, and the joining kernel may have one for each row.
     f = lib.fagq_paged_attention_workspace_bytes
