@@ -18,6 +18,9 @@ namespace {
 
 constexpr int64_t kCUs = 256;
 constexpr int64_t kSlots = 2 * kCUs;   // workgroups of a round
+// Which way is taken goes by `most`, the caller's bound on the lengths: a loose one takes the way of the
+// lengths that it allows (512 ragged sequences of 300 tokens, 32 + 8 heads of 128: 43 us with a close
+// bound, 95 with room for 32768 tokens; 4 sequences of 2000, 4 tokens, 64 + 8 heads: 16.5, 39.5).
 // Shares are for long lists of keys: with short ones a workgroup has several units, one after the
 // other, that chunks give to as many workgroups at once (chunks / shares, us: 8 heads of 128, 64
 // sequences of 4096 keys 102 / 97, of 3000 77 / 74, 256 of 2048 199 / 205, ragged 79 / 71, 56 / 58 and

@@ -11,11 +11,12 @@
 // sequences behind 32768 keys, heads of 128: R = 2 145 us, R = 4 234).  A workgroup takes a range
 // of a unit's keys; its four waves take the steps of 32 keys in turn, each with m, l and o of its
 // own, and are joined through LDS.  Units of many rows of heads of 128 and 256 are tall ones: four
-// times as many rows, a quarter for each wave (see Tall).  How units are cut:
+// times as many rows, a quarter for each wave (see Tall).  How units are cut goes by the host's
+// bound on the lengths (plan_for), which knows nothing of the lengths themselves:
 //   scheduled  The rounds of 128 keys of all units in a row are shared out evenly, so that every
-//              workgroup reads as much as the others however the lengths differ and whatever bound
-//              on them the host knows (64 sequences of 1400 to 8192 tokens: 115 us, with chunks
-//              131).  Each workgroup works that out by itself from the lengths.
+//              workgroup reads as much as the others however the lengths differ (64 sequences of
+//              1400 to 8192 tokens: 115 us, with chunks 131).  Each workgroup works that out by
+//              itself from the lengths.
 //   static     Chunks of one size, chosen by the host: the prefix; sequences of more than 16 rows,
 //              whose units cost more to begin and to end in the middle (64 of 1500 tokens, 8 heads of
 //              128, 32 rows: 43 us, scheduled 51; 16 of 4096, 16 heads of 64, 64 rows: 48, 80); short
@@ -70,7 +71,8 @@ constexpr float kPartCost = 15.0f;   // what a part costs the joining kernel, in
 
 // kScheduledOnce: the codes are read past the caches (64 sequences of 8192 tokens, 64 + 8 heads of
 // 128, 1.07 GB: 172 against 186 us); calls whose cache may still hold what the last one read
-// lose by it (8 of 4000 tokens, 32 heads, 131 MB: 46 against 36 us).
+// lose by it (8 of 4000 tokens, 32 heads, 131 MB: 46 against 36 us).  It is taken by the bytes of
+// the bound on the lengths, which a wide table makes larger than what is read.
 enum Form { kStatic = 0, kScheduled = 1, kScheduledOnce = 2 };
 
 struct Args {

@@ -79,8 +79,8 @@ FAGQ_API int fagq_kv_cache_read_launch(const void* k_cache, const void* v_cache,
  * 2^31; out is contiguous.  page_table int32 [B, table_width], null if the
  * width is 0; kv_lens [B] (index_dtype); prefix_pages int32
  * [ceil(prefix_len / page_size)], null without.
- * max_kv_len: no kv_lens[b] is larger (it sizes the work split; longer ones are
- * cut to it).  Sums and softmax are in fp32; the probabilities, times their value
+ * max_kv_len: no kv_lens[b] is larger (it alone chooses the work split and
+ * whether codes are read past the caches; longer ones are cut to it).  Sums and softmax are in fp32; the probabilities, times their value
  * scales, are rounded to fp16 (relative to the row's largest) for the product with
  * the codes.  Codes and scales of the tokens that a sequence reads are finite, value
  * scales 0 to 2^64 (below 2^-64 what a key adds is exact to 2^-88 of its codes only;
