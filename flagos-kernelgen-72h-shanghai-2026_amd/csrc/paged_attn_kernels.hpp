@@ -41,9 +41,10 @@
 // (measured against 64 bits: 2.4e-3 with bf16, 1.7e-3 with fp16, 1.7e-3 for the rounding alone).
 //
 // Bound: decode batches by HBM (64 sequences of 8192 tokens, 64 + 8 heads of 128: 174 us, 6.4 TB/s);
-// many rows by the softmax, whose VALU instructions take as many cycles as the products and are
-// overlapped with them in part (64 sequences behind 32768 shared tokens 116 us, 600 TFLOP/s; 4 of
-// 512 new tokens over 4096 keys, 32 + 8 heads of 128, 179 us, 720); small calls by two dependent
+// many rows by no one unit: VALU instructions (the softmax) take 43 % of a SIMD's cycles, products 26 %,
+// LDS 26 %, and its one or two waves wait for loads, LDS and barriers a quarter of theirs (64
+// sequences behind 32768 shared tokens 116 us, 600 TFLOP/s; 4 of 512 new tokens over 4096 keys,
+// 32 + 8 heads of 128, 179 us, 720); small calls by two dependent
 // launches (4 sequences of 1000 tokens 9.6 us).
 #pragma once
 
