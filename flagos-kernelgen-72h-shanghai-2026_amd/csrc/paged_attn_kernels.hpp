@@ -21,7 +21,7 @@
 //              whose units cost more to begin and to end in the middle (64 of 1500 tokens, 8 heads of
 //              128, 32 rows: 43 us, scheduled 51; 16 of 4096, 16 heads of 64, 64 rows: 48, 80); short
 //              sequences; and calls of few rounds, where working out the shares takes longer than
-//              uneven ones (4 sequences of 1000 tokens: 8.2 us, scheduled 10.3).
+//              uneven ones (a call of 4 sequences of 1000 tokens: 9.0 us, scheduled 9.9).
 // The parts of a cut unit are joined by a second kernel.
 //
 // Keys and values go from HBM straight into the registers that feed the matrix instructions
@@ -45,7 +45,7 @@
 // LDS 26 %, and its one or two waves wait for loads, LDS and barriers a quarter of theirs (64
 // sequences behind 32768 shared tokens 116 us, 600 TFLOP/s; 4 of 512 new tokens over 4096 keys,
 // 32 + 8 heads of 128, 179 us, 720); small calls by two dependent
-// launches (4 sequences of 1000 tokens 9.6 us).
+// launches (4 sequences of 1000 tokens 9.0 us, of which the kernels are 5.7 and 3.6).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -174,12 +174,13 @@ __device__ __forceinline__ void transpose4(uint32_t a0, uint32_t a1, uint32_t a2
   d[3] = __builtin_amdgcn_perm(f1, e1, 0x07060302u);
 }
 
-// Rounds of a sequence's units: one for a sequence without keys, whose rows are written too.
+// Own keys of a sequence: its length, as far as `most` of them are read.
 __device__ __forceinline__ int32_t own_length(const void* lens, int idx64, int32_t most, int b) {
   const int64_t n = idx64 ? static_cast<const int64_t*>(lens)[b]
                           : (int64_t) static_cast<const int32_t*>(lens)[b];
   return (int32_t)cache::seen_tokens(n, most, 1, 0);
 }
+// Rounds of a sequence's units: one for a sequence without keys, whose rows are written too.
 __device__ __forceinline__ int32_t rounds_of(int32_t len) {
   const int32_t n = (len + kRound - 1) / kRound;
   return n > 1 ? n : 1;
