@@ -8,7 +8,9 @@ pass, and its gradients.
 in fp32 with one rounding, from the views of a fused projection as they are;
 ``qk_norm_rope_bwd`` the gradients of q, k and both weights.  The kernels are
 libfagq.so's ``fagq_qk_norm_rope_launch`` and ``fagq_qk_norm_rope_bwd_launch``
-(include/fagq_rope.h); there is no fallback.
+(include/fagq_rope.h); there is no fallback.  Neither records anything for autograd: their results
+carry no gradient, and a training program calls the backward from a ``torch.autograd.Function``
+of its own.
 
 No counterpart in the reference repository: its RMSNorm
 (src/task01_fused_add_rmsnorm_group_quant.py:88-100) is over hidden rows.
@@ -91,7 +93,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     rotated in pairs (i, i + R / 2), or (2 i, 2 i + 1) if ``interleaved``; positions [T]:
     int32 or int64.  D and R are multiples of 16.  A token with a position outside the tables
     is padding and gets zeros.  Returns ``(q_out, k_out)``, allocated unless given; they may be
-    q and k themselves.  Asynchronous on the current stream."""
+    q and k themselves.  Autograd does not see the call (``qk_norm_rope_bwd`` has the
+    gradients).  Asynchronous on the current stream."""
     mod, fast_stream = _lib.fast_module(q)
     if mod is not None:
         r = mod.rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, q_out, k_out,
