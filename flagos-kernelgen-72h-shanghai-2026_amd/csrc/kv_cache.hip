@@ -392,9 +392,13 @@ FAGQ_API int fagq_kv_cache_read_launch(const void* k_cache, const void* v_cache,
                                        int q_format, int scale_format, void* stream) {
   using namespace fagq;
   using namespace fagq::cache;
-  if (!k_cache || !k_scale || !page_table || !cu_seqlens || !k_out) return FAGQ_E_NULL;
-  const int n = v_cache ? 2 : 1;
-  if ((v_cache == nullptr) != (v_scale == nullptr) || (v_cache == nullptr) != (v_out == nullptr))
+  // A cache of no pages and a table of no width have nothing to point to, and are never read.
+  if ((num_pages > 0 && (!k_cache || !k_scale)) || (table_width > 0 && !page_table) || !cu_seqlens ||
+      !k_out)
+    return FAGQ_E_NULL;
+  const int n = v_out ? 2 : 1;
+  if (num_pages > 0 &&
+      ((v_cache == nullptr) != (v_out == nullptr) || (v_scale == nullptr) != (v_out == nullptr)))
     return FAGQ_E_NULL;
   const int layout = check_layout(H, D, G, num_pages, page_size, dtype, q_format, scale_format);
   if (layout != FAGQ_OK) return layout;

@@ -164,8 +164,6 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor | None, k_scale: 
         raise ValueError(f"cu_seqlens must be a contiguous int32 tensor of shape ({B + 1},) on {dev}")
     if B == 0 or rows == 0 or H == 0:
         return k_out, v_out
-    if P == 0 or width == 0:
-        raise ValueError("the cache and the page table must not be empty")
     lib = _lib.load()
     with torch.cuda.device(dev):
         stream = torch.cuda.current_stream(dev).cuda_stream

@@ -54,7 +54,8 @@ FAGQ_API int fagq_kv_cache_write_launch(const void* k, const void* v, const void
  * code * scale in fp32, rounded once.  page_table int32 [B, table_width],
  * cu_seqlens int32 [B + 1], ascending from 0.  Tokens whose page lies outside the
  * table or the cache (-1: none) become zeros.  Rows behind cu_seqlens[B] are left
- * as they were.  rows <= 2^31 - 1, and FAGQ_E_TOO_LARGE where 2^24 workgroups do
+ * as they were.  The cache may be null where num_pages is 0, page_table where the
+ * width is 0: all tokens are zeros then.  rows <= 2^31 - 1, and FAGQ_E_TOO_LARGE where 2^24 workgroups do
  * not cover them. */
 FAGQ_API int fagq_kv_cache_read_launch(const void* k_cache, const void* v_cache,
                                        const void* k_scale, const void* v_scale,

@@ -160,6 +160,19 @@ def test_read_validation(lib, kw, status):
     assert read(lib, **kw) == status
 
 
+@pytest.mark.parametrize("kw", [
+    dict(pt=None, width=0), dict(kc=None, vc=None, ks=None, vs=None, P=0),
+    dict(kc=None, vc=None, ks=None, vs=None, P=0, pt=None, width=0), dict(kc=None, ks=None, vo=None, vc=None, vs=None, P=0),
+])
+def test_read_takes_tables_and_caches_of_nothing(lib, kw):
+    # Every token is one without a page; without a GPU the call ends at the device check.
+    if torch.cuda.is_available():
+        pytest.skip("the pointers are made up")
+    ok = read(lib)
+    assert (ok < 0 or ok == 8) and read(lib, **kw) == ok
+    assert read(lib, **kw, cu=None) == 1 and read(lib, **kw, ko=None) == 1
+
+
 def attend(lib, **kw):
     a = dict(q=fake(0), kc=fake(1), vc=fake(2), ks=fake(3), vs=fake(4), pt=fake(5), lens=fake(6),
              pp=fake(7), out=fake(8), ws=fake(9), wsb=1 << 31, st=(1024, 1024, 128), B=3, S=1, Hq=8,

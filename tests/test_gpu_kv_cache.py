@@ -226,3 +226,20 @@ def test_refusals(pkg, gpu):
                 dict(v_out=x), dict(k_out=x.transpose(0, 1)), dict(page_table=t.cpu())):
         with pytest.raises(ValueError):
             pkg.kv_cache_read(**{**ok, **bad})
+
+
+@pytest.mark.parametrize("pages,width", [(0, 2), (3, 0), (0, 0)])
+def test_read_without_pages_or_table(pkg, gpu, pages, width):
+    """All tokens are without a page then: zeros, and the rows behind the last sequence stay."""
+    note(f"read of {pages} pages, table of {width}")
+    (kc, ks), (vc, vs) = (pkg.empty_kv_cache(pages, 2, 16, 64, device=gpu) for _ in range(2))
+    table = torch.zeros(3, width, dtype=torch.int32, device=gpu)
+    cu = torch.tensor([0, 5, 5, 9], dtype=torch.int32, device=gpu)
+    outs = [torch.full((11, 2, 64), 5.0, dtype=BF16, device=gpu) for _ in range(2)]
+    got = pkg.kv_cache_read(kc, vc, ks, vs, table, cu, *outs)
+    assert got[0] is outs[0] and got[1] is outs[1]
+    for o in outs:
+        assert bool((o[:9] == 0).all()) and bool((o[9:] == 5.0).all())
+    alone = torch.full((11, 2, 64), 5.0, dtype=BF16, device=gpu)
+    pkg.kv_cache_read(kc, None, ks, None, table, cu, alone, None)
+    assert torch.equal(alone, outs[0])
