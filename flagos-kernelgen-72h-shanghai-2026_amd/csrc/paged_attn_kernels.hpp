@@ -21,7 +21,7 @@
 //              whose units cost more to begin and to end in the middle (64 of 1500 tokens, 8 heads of
 //              128, 32 rows: 43 us, scheduled 51; 16 of 4096, 16 heads of 64, 64 rows: 48, 80); short
 //              sequences; and calls of few rounds, where working out the shares takes longer than
-//              uneven ones (a call of 4 sequences of 1000 tokens: 9.0 us, scheduled 9.9).
+//              uneven ones (a call of 4 sequences of 1000 tokens: 0.9 us longer).
 // The parts of a cut unit are joined by a second kernel.
 //
 // Keys and values go from HBM straight into the registers that feed the matrix instructions
@@ -45,7 +45,7 @@
 // LDS 26 %, and its one or two waves wait for loads, LDS and barriers a quarter of theirs (64
 // sequences behind 32768 shared tokens 116 us, 600 TFLOP/s; 4 of 512 new tokens over 4096 keys,
 // 32 + 8 heads of 128, 179 us, 720); small calls by two dependent
-// launches (4 sequences of 1000 tokens 9.0 us, of which the kernels are 5.7 and 3.6).
+// launches (4 sequences of 1000 tokens 9.2 us, of which the kernels are 5.8 and 3.6).
 #pragma once
 
 #include <hip/hip_runtime.h>
