@@ -44,8 +44,8 @@
 // many rows by no one unit: VALU instructions (the softmax) take 43 % of a SIMD's cycles, products 26 %,
 // LDS 26 %, and its one or two waves wait for loads, LDS and barriers a quarter of theirs (64
 // sequences behind 32768 shared tokens 116 us, 600 TFLOP/s; 4 of 512 new tokens over 4096 keys,
-// 32 + 8 heads of 128, 179 us, 720); small calls by two dependent
-// launches (4 sequences of 1000 tokens 9.2 us, of which the kernels are 5.8 and 3.6).
+// 32 + 8 heads of 128, 179 us, 720); small calls by two dependent launches (4 sequences of 1000
+// tokens 9.2 us, of which the kernels are 5.8 and 3.6).
 #pragma once
 
 #include <hip/hip_runtime.h>

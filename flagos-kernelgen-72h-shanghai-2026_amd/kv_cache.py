@@ -92,9 +92,9 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor | None, slots: torch.Tensor,
                    v_scale: torch.Tensor | None) -> None:
     """Quantises k and v [T, H, D] (bfloat16, float16 or float32, contiguous rows at any 16-byte
     aligned token and head strides) into the slots [T] (int32 or int64) of the cache.  A token
-    whose slot is negative or past the cache is left out; no two tokens may name one slot.  A
-    cache of latents passes None for v, v_cache and v_scale.  Asynchronous on the current
-    stream."""
+    whose slot is negative or past the cache is left out; no two tokens may name one slot.
+    Values are finite (others spoil their own group, no other).  A cache of latents passes None
+    for v, v_cache and v_scale.  Asynchronous on the current stream."""
     mod, fast_stream = _lib.fast_module(k_cache)
     if mod is not None:
         st = mod.cache_write(k, v, slots, k_cache, v_cache, k_scale, v_scale, fast_stream)
@@ -214,11 +214,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     ``max_kv_len`` (default: the table's capacity) bounds kv_lens; longer ones are cut to it.  The
     split of the work and whether codes are read past the caches go by it and not by kv_lens: give
-    a close one where the table is wide (up to 2.4 times as fast).  ``workspace`` (optional): a uint8 GPU tensor
-    of at least ``attention_workspace_bytes(...)`` bytes for these sizes (a smaller call may need
-    more), which calls that may overlap do not share.  Codes and scales of the tokens that are seen are finite, value
-    scales 0 to 2^64.  Returns ``out`` [B, S, Hq, D] (contiguous, allocated unless given),
-    asynchronously on the current stream."""
+    a close one where the table is wide (up to 2.4 times as fast).  ``workspace`` (optional): a
+    uint8 GPU tensor of at least ``attention_workspace_bytes(...)`` bytes for these sizes (a
+    smaller call may need more), which calls that may overlap do not share.  Codes and scales of
+    the tokens that are seen are finite, value scales 0 to 2^64.  Returns ``out`` [B, S, Hq, D]
+    (contiguous, allocated unless given), asynchronously on the current stream."""
     mod, fast_stream = _lib.fast_module(k_cache) if workspace is None else (None, None)
     if mod is not None:
         r = mod.attention(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, sm_scale,

@@ -55,8 +55,8 @@ FAGQ_API int fagq_kv_cache_write_launch(const void* k, const void* v, const void
  * cu_seqlens int32 [B + 1], ascending from 0.  Tokens whose page lies outside the
  * table or the cache (-1: none) become zeros.  Rows behind cu_seqlens[B] are left
  * as they were.  The cache may be null where num_pages is 0, page_table where the
- * width is 0: all tokens are zeros then.  rows <= 2^31 - 1, and FAGQ_E_TOO_LARGE where 2^24 workgroups do
- * not cover them. */
+ * width is 0: all tokens are zeros then.  rows <= 2^31 - 1, and FAGQ_E_TOO_LARGE
+ * where 2^24 workgroups do not cover them. */
 FAGQ_API int fagq_kv_cache_read_launch(const void* k_cache, const void* v_cache,
                                        const void* k_scale, const void* v_scale,
                                        const int32_t* page_table, const int32_t* cu_seqlens,
@@ -80,18 +80,19 @@ FAGQ_API int fagq_kv_cache_read_launch(const void* k_cache, const void* v_cache,
  * 2^31; out is contiguous.  page_table int32 [B, table_width], null if the
  * width is 0; kv_lens [B] (index_dtype); prefix_pages int32
  * [ceil(prefix_len / page_size)], null without.
- * max_kv_len: no kv_lens[b] is larger (it alone chooses the work split and
- * whether codes are read past the caches; longer ones are cut to it).  Sums and softmax are in fp32; the probabilities, times their value
- * scales, are rounded to fp16 (relative to the row's largest) for the product with
- * the codes.  Codes and scales of the tokens that a sequence reads are finite, value
- * scales 0 to 2^64 (below 2^-64 what a key adds is exact to 2^-88 of its codes only;
- * UE8M0 0 counts as 0); what lies in other slots does not matter.
+ * max_kv_len: no kv_lens[b] is larger; longer ones are cut to it.  It, and not the
+ * lengths, decides how the work is split and whether codes are read past the caches.
+ * Sums and softmax are in fp32; the probabilities, times their value scales, are
+ * rounded to fp16 (relative to the row's largest) for the product with the codes.
+ * Codes and scales of the tokens that a sequence reads are finite, value scales 0 to
+ * 2^64 (below 2^-64 what a key adds is exact to 2^-88 of its codes only; UE8M0 0
+ * counts as 0); what lies in other slots does not matter.
  * The workspace (16-byte aligned) belongs to this call until it has run: calls that
- * may overlap need one each.  Its size is that of exactly these B ... max_kv_len: fewer
- * sequences or a smaller bound are cut into more parts and may need more (B 16 2.1 MB where
- * B 64 needs none), so one that serves several calls is as large as the largest of theirs.
- * FAGQ_E_TOO_LARGE (workspace: -1) for 2^24 rows
- * or workgroups and more. */
+ * may overlap need one each.  Its size is that of exactly these B ... max_kv_len:
+ * fewer sequences or a smaller bound are cut into more parts and may need more (1024
+ * keys, 64 + 8 heads of 128: B 16 2.1 MB, B 64 none), so one that serves several
+ * calls is as large as the largest of theirs.
+ * FAGQ_E_TOO_LARGE (workspace: -1) for 2^24 rows or workgroups and more. */
 FAGQ_API int64_t fagq_paged_attention_workspace_bytes(int64_t B, int64_t S, int64_t Hq, int64_t H,
                                                       int64_t D, int64_t prefix_len,
                                                       int64_t max_kv_len);

@@ -10,7 +10,7 @@
  *          (a, b) -> (a cos[p, i] - b sin[p, i], b cos[p, i] + a sin[p, i]),
  *          pair i of R / 2: (n[i], n[i + R / 2]), or (n[2 i], n[2 i + 1]) if interleaved
  *
- * all in fp32, rounded once to the element type.  A token whose position lies
+ * all in fp32 (squares too: values lie below 2^59), rounded once to the element type.  A token whose position lies
  * outside [0, table_rows) is padding: its rows of y are zeros, and so are its
  * gradients.  The backward takes the same inputs and dy:
  *
