@@ -1,6 +1,7 @@
 """ctypes binding of libfagq.so (the C ABI declared in include/fagq.h,
 include/fagq_gemm.h, include/fagq_dsa.h, include/fagq_mla.h,
-include/fagq_rope.h, include/fagq_cache.h and include/fagq_diag.h) and of libfagq_probe.so (include/fagq_probe.h, the
+include/fagq_rope.h, include/fagq_cache.h, include/fagq_prompt.h and
+include/fagq_diag.h) and of libfagq_probe.so (include/fagq_probe.h, the
 measurement probes, loaded only when asked for).
 
 The library is loaded after ``import torch`` so that its libamdhip64.so.7
@@ -88,6 +89,14 @@ SIGNATURES = {
     "fagq_kv_cache_read_launch": ([_P] * 8 + [_I64] * 8 + [_I] * 3 + [_P], _I),
     "fagq_paged_attention_workspace_bytes": ([_I64] * 7, _I64),
     "fagq_paged_attention_launch": ([_P] * 10 + [_I64, _P] + [_I64] * 10 + [_F, _I, _I, _I, _I, _P], _I),
+    "fagq_paged_tree_attention_workspace_bytes": ([_I64] * 7, _I64),
+    "fagq_paged_tree_attention_launch": ([_P] * 9 + [_I, _P, _P, _I64, _P] + [_I64] * 10 +
+                                         [_F, _I, _I, _I, _I, _P], _I),
+    "fagq_batch_tables_launch": ([_P] * 11 + [_I64] * 5 + [_I, _P], _I),
+    "fagq_prompt_attention_workspace_bytes": ([_I64] * 6, _I64),
+    "fagq_prompt_attention_launch": ([_P] * 8 + [_I64, _P] + [_I64] * 6 + [_F, _I, _I, _P], _I),
+    "fagq_prompt_attention_bwd_workspace_bytes": ([_I64] * 6, _I64),
+    "fagq_prompt_attention_bwd_launch": ([_P] * 12 + [_I64, _P] + [_I64] * 6 + [_F, _I, _I, _P], _I),
 }
 
 

@@ -23,7 +23,7 @@ OBJ_DIR = PKG_DIR / "_build"
 LIB_PATH = PKG_DIR / "libfagq.so"
 PROBE_LIB_PATH = PKG_DIR / "libfagq_probe.so"
 LIB_UNITS = ("fagq_api", "fagq_device", "fagq_gemm", "dsa_topk", "mla_bwd", "qk_rope", "kv_cache",
-             "paged_attn")
+             "paged_attn", "prompt_attn", "prompt_attn_bwd", "batch_tables")
 PROBE_UNITS = ("fagq_probe", "fagq_device")
 
 ARCH = "gfx950"

@@ -180,14 +180,14 @@ int64_t most_rounds(int64_t B, int64_t H, int64_t most) {
 }
 
 int check_sizes(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t prefix_len,
-                int64_t max_kv_len) {
+                int64_t max_kv_len, bool tree) {
   if (B < 0 || S < 1 || H < 1 || Hq < H || Hq % H != 0 || (D != 64 && D != 128 && D != 256) ||
       prefix_len < 0 || max_kv_len < 0)
     return FAGQ_E_SHAPE;
   // The joining kernel may have a workgroup for each row.
   if (B > 65535 || S > 65535 || Hq > 4096 || B * S * Hq >= kMostGroups ||
       prefix_len > (1ll << 30) || max_kv_len > (1ll << 30) ||
-      most_rounds(B, H, max_kv_len) >= (1ll << 31) - kSlots)
+      most_rounds(B, H, max_kv_len) >= (1ll << 31) - kSlots || (tree && S > FAGQ_TREE_MAX_S))
     return FAGQ_E_TOO_LARGE;
   return FAGQ_OK;
 }
@@ -271,7 +271,7 @@ int row_tiles(int64_t rows, int64_t D, int64_t lists, int64_t keys) {
 }
 
 Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t prefix_len,
-              int64_t most) {
+              int64_t most, bool tree) {
   Plan p = {};
   const int64_t per = S * (Hq / H);
   p.rows = B * S * Hq;
@@ -285,7 +285,7 @@ Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t pr
     p.prefix_items = H * p.prefix_tiles * p.prefix_chunks;
   }
   p.tiles = (per + height(p.R, D) - 1) / height(p.R, D);
-  if (p.tiles > 1 || p.R > 1 || most_rounds(1, 1, most) < (D == 64 ? kLongUnit64 : kLongUnit) ||
+  if (tree || p.tiles > 1 || p.R > 1 || most_rounds(1, 1, most) < (D == 64 ? kLongUnit64 : kLongUnit) ||
       most_rounds(B, H, most) <= kFewRounds) {
     p.form = kStatic;
     cut(most, B * H * p.tiles, key_cost(p.R), part_cost(p.rows, D), &p.chunk, &p.chunks);
@@ -307,13 +307,13 @@ int64_t bytes_of(const Plan& p, int64_t B, int64_t D) {
   return p.parts * (D + 2) * 4 + (p.form == kStatic ? 0 : (B + 1) * 4);
 }
 
-const void* kernel_for(int dtype, int q_format, int scale_format, int D, const Plan& p) {
-  using Lookup = const void* (*)(int, int, int, int);
+const void* kernel_for(int dtype, int q_format, int scale_format, int D, const Plan& p, bool tree) {
+  using Lookup = const void* (*)(int, int, int, int, bool);
   static constexpr Lookup table[8] = {lookup_e0_q0_s0, lookup_e0_q0_s1, lookup_e0_q1_s0, lookup_e0_q1_s1,
                                       lookup_e1_q0_s0, lookup_e1_q0_s1, lookup_e1_q1_s0, lookup_e1_q1_s1};
   const int e = dtype == FAGQ_DT_BF16 ? 0 : 1, q = q_format == FAGQ_Q_FP8_E4M3FN ? 0 : 1;
   const int s = scale_format == FAGQ_SCALE_F32 ? 0 : 1;
-  return table[4 * e + 2 * q + s](D, p.R, p.RP, p.form);
+  return table[4 * e + 2 * q + s](D, p.R, p.RP, p.form, tree);
 }
 
 template <int E, int W>
@@ -323,43 +323,37 @@ const void* join_for(int64_t D) {
                     : reinterpret_cast<const void*>(&paged_attention_join<E, 256, W>);
 }
 
-}  // namespace
-}  // namespace attn
-}  // namespace fagq
-
-extern "C" {
-
-FAGQ_API int64_t fagq_paged_attention_workspace_bytes(int64_t B, int64_t S, int64_t Hq, int64_t H,
-                                                      int64_t D, int64_t prefix_len,
-                                                      int64_t max_kv_len) {
-  using namespace fagq::attn;
-  if (check_sizes(B, S, Hq, H, D, prefix_len, max_kv_len) != FAGQ_OK) return -1;
+int64_t workspace_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t prefix_len,
+                      int64_t max_kv_len, bool tree) {
+  if (check_sizes(B, S, Hq, H, D, prefix_len, max_kv_len, tree) != FAGQ_OK) return -1;
   if (B == 0) return 0;
-  const Plan p = plan_for(B, S, Hq, H, D, prefix_len, max_kv_len);
+  const Plan p = plan_for(B, S, Hq, H, D, prefix_len, max_kv_len, tree);
   return p.prefix_items + p.items < kMostGroups ? bytes_of(p, B, D) : -1;
 }
 
-FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, const void* v_cache,
-                                         const void* k_scale, const void* v_scale,
-                                         const int32_t* page_table, const void* kv_lens,
-                                         const int32_t* prefix_pages, void* out, void* workspace,
-                                         int64_t workspace_bytes, const int64_t* strides,
-                                         int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D,
-                                         int64_t num_pages, int64_t page_size, int64_t table_width,
-                                         int64_t prefix_len, int64_t max_kv_len, float sm_scale,
-                                         int dtype, int q_format, int scale_format,
-                                         int index_dtype, void* stream) {
-  using namespace fagq;
-  using namespace fagq::attn;
+// The masks of drafted trees.
+struct Drafts {
+  const uint8_t* mask;
+  bool shared;                 // one for all sequences
+};
+
+// Attention of the newest tokens, one after the other or (`tree` given) drafts.
+int launch(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
+           const void* v_scale, const int32_t* page_table, const void* kv_lens,
+           const int32_t* prefix_pages, const Drafts* tree, void* out, void* workspace,
+           int64_t workspace_bytes, const int64_t* strides, int64_t B, int64_t S, int64_t Hq, int64_t H,
+           int64_t D, int64_t num_pages, int64_t page_size, int64_t table_width, int64_t prefix_len,
+           int64_t max_kv_len, float sm_scale, int dtype, int q_format, int scale_format,
+           int index_dtype, void* stream) {
   if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !kv_lens || !out || !strides ||
-      (table_width > 0 && !page_table) || (prefix_len > 0 && !prefix_pages))
+      (table_width > 0 && !page_table) || (prefix_len > 0 && !prefix_pages) || (tree && !tree->mask))
     return FAGQ_E_NULL;
   if (dtype != FAGQ_DT_BF16 && dtype != FAGQ_DT_F16) return FAGQ_E_FORMAT;
   if (q_format != FAGQ_Q_FP8_E4M3FN && q_format != FAGQ_Q_INT8) return FAGQ_E_FORMAT;
   if (scale_format != FAGQ_SCALE_F32 && scale_format != FAGQ_SCALE_UE8M0) return FAGQ_E_FORMAT;
   if (index_dtype != FAGQ_IDX_I32 && index_dtype != FAGQ_IDX_I64) return FAGQ_E_FORMAT;
   if (!std::isfinite(sm_scale)) return FAGQ_E_SHAPE;
-  const int sizes = check_sizes(B, S, Hq, H, D, prefix_len, max_kv_len);
+  const int sizes = check_sizes(B, S, Hq, H, D, prefix_len, max_kv_len, tree != nullptr);
   if (sizes != FAGQ_OK) return sizes;
   if (num_pages < 1 || table_width < 0 || page_size < FAGQ_CACHE_MIN_PAGE ||
       (page_size & (page_size - 1)) != 0)
@@ -378,7 +372,7 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
       !aligned(k_scale, ss * 4) || !aligned(v_scale, ss * 4) || !aligned(page_table, 4) ||
       !aligned(kv_lens, is) || !aligned(prefix_pages, 4) || !aligned(out, 16))
     return FAGQ_E_ALIGN;
-  const Plan p = B > 0 ? plan_for(B, S, Hq, H, D, prefix_len, max_kv_len) : Plan{};
+  const Plan p = B > 0 ? plan_for(B, S, Hq, H, D, prefix_len, max_kv_len, tree != nullptr) : Plan{};
   if (p.prefix_items + p.items >= kMostGroups) return FAGQ_E_TOO_LARGE;
   const int64_t need = B > 0 ? bytes_of(p, B, D) : 0;
   if (need > 0 && !workspace) return FAGQ_E_NULL;
@@ -386,12 +380,14 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   if (!aligned(workspace, 16)) return FAGQ_E_ALIGN;
   if (B == 0) return FAGQ_OK;
   const int64_t ncodes = num_pages * page_size * H * D, nscales = num_pages * page_size * H * ss;
-  const void* ins[8] = {q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, prefix_pages};
-  const int64_t nin[8] = {((B - 1) * strides[0] + (S - 1) * strides[1] + (Hq - 1) * strides[2] + D) * 2,
+  const void* ins[9] = {q,          k_cache, v_cache,      k_scale, v_scale,
+                        page_table, kv_lens, prefix_pages, tree ? tree->mask : nullptr};
+  const int64_t nin[9] = {((B - 1) * strides[0] + (S - 1) * strides[1] + (Hq - 1) * strides[2] + D) * 2,
                           ncodes, ncodes, nscales, nscales, B * table_width * 4, B * is,
-                          (prefix_len + page_size - 1) / page_size * 4};
+                          (prefix_len + page_size - 1) / page_size * 4,
+                          tree ? (tree->shared ? 1 : B) * S * S : 0};
   const int64_t nout = B * S * Hq * D * 2;
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 9; ++i)
     if (overlap(out, nout, ins[i], nin[i]) || overlap(workspace, need, ins[i], nin[i]))
       return FAGQ_E_ALIAS;
   if (overlap(out, nout, workspace, need)) return FAGQ_E_ALIAS;
@@ -413,6 +409,7 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   a.most = (int32_t)(room < max_kv_len ? room : max_kv_len);
   a.idx64 = index_dtype == FAGQ_IDX_I64;
   a.scale2 = sm_scale * 1.44269504088896340736f;
+  if (tree) a.tree = tree->mask, a.tree_next = tree->shared ? 0 : S * S;
   a.chunk = (int32_t)p.chunk, a.chunks = (int32_t)p.chunks, a.tiles = (int32_t)p.tiles;
   a.prefix_chunk = (int32_t)p.prefix_chunk, a.prefix_chunks = (int32_t)p.prefix_chunks;
   a.prefix_tiles = (int32_t)p.prefix_tiles, a.prefix_items = (int32_t)p.prefix_items;
@@ -425,7 +422,7 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
   }
   void* args[] = {&a};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int ls = launch_kernel(kernel_for(dtype, q_format, scale_format, (int)D, p),
+  const int ls = launch_kernel(kernel_for(dtype, q_format, scale_format, (int)D, p, tree != nullptr),
                                dim3((unsigned)(p.prefix_items + p.items)), dim3(64 * kWaves), args,
                                0, st);
   if (ls != FAGQ_OK || p.parts == 0) return ls;
@@ -443,6 +440,56 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
                                          : (wide ? join_for<ET_F16, kWaves>(D) : join_for<ET_F16, 1>(D));
   const int64_t groups = wide ? p.rows : (p.rows + kWaves - 1) / kWaves;
   return launch_kernel(fn, dim3((unsigned)groups), dim3(64 * kWaves), jargs, 0, st);
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace fagq
+
+extern "C" {
+
+FAGQ_API int64_t fagq_paged_attention_workspace_bytes(int64_t B, int64_t S, int64_t Hq, int64_t H,
+                                                      int64_t D, int64_t prefix_len,
+                                                      int64_t max_kv_len) {
+  return fagq::attn::workspace_for(B, S, Hq, H, D, prefix_len, max_kv_len, false);
+}
+
+FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, const void* v_cache,
+                                         const void* k_scale, const void* v_scale,
+                                         const int32_t* page_table, const void* kv_lens,
+                                         const int32_t* prefix_pages, void* out, void* workspace,
+                                         int64_t workspace_bytes, const int64_t* strides,
+                                         int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D,
+                                         int64_t num_pages, int64_t page_size, int64_t table_width,
+                                         int64_t prefix_len, int64_t max_kv_len, float sm_scale,
+                                         int dtype, int q_format, int scale_format,
+                                         int index_dtype, void* stream) {
+  return fagq::attn::launch(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, prefix_pages,
+                            nullptr, out, workspace, workspace_bytes, strides, B, S, Hq, H, D,
+                            num_pages, page_size, table_width, prefix_len, max_kv_len, sm_scale, dtype,
+                            q_format, scale_format, index_dtype, stream);
+}
+
+FAGQ_API int64_t fagq_paged_tree_attention_workspace_bytes(int64_t B, int64_t S, int64_t Hq,
+                                                           int64_t H, int64_t D,
+                                                           int64_t prefix_len,
+                                                           int64_t max_kv_len) {
+  return fagq::attn::workspace_for(B, S, Hq, H, D, prefix_len, max_kv_len, true);
+}
+
+FAGQ_API int fagq_paged_tree_attention_launch(
+    const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
+    const void* v_scale, const int32_t* page_table, const void* kv_lens,
+    const int32_t* prefix_pages, const uint8_t* tree_mask, int shared_mask, void* out,
+    void* workspace, int64_t workspace_bytes, const int64_t* strides, int64_t B, int64_t S,
+    int64_t Hq, int64_t H, int64_t D, int64_t num_pages, int64_t page_size, int64_t table_width,
+    int64_t prefix_len, int64_t max_kv_len, float sm_scale, int dtype, int q_format,
+    int scale_format, int index_dtype, void* stream) {
+  const fagq::attn::Drafts tree = {tree_mask, shared_mask != 0};
+  return fagq::attn::launch(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, prefix_pages,
+                            &tree, out, workspace, workspace_bytes, strides, B, S, Hq, H, D,
+                            num_pages, page_size, table_width, prefix_len, max_kv_len, sm_scale, dtype,
+                            q_format, scale_format, index_dtype, stream);
 }
 
 }  // extern "C"

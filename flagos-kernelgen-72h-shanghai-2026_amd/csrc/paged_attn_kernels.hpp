@@ -107,6 +107,8 @@ struct Args {
   int32_t slots;                      // workgroups that the schedule fills
   int32_t idx64;
   float scale2;                       // sm_scale * log2(e)
+  const uint8_t* tree;                // [S][S] of each sequence, tree_next bytes apart (see Tree)
+  int64_t tree_next;
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -346,6 +348,21 @@ struct Rows {
   int32_t seen[R];             // keys that the row sees
 };
 
+// TREE: the newest S tokens are drafts.  Query s sees the len - S tokens before them and the drafts t
+// (token len - S + t) whose byte [s][t] of the mask is not 0.  Rows::seen then is s S, where the
+// row's bytes begin.
+struct Tree {
+  const uint8_t* mask;
+  int32_t context, len;
+};
+template <bool TREE>
+__device__ __forceinline__ bool sees(int32_t seen, const Tree& tree, int32_t at) {
+  if constexpr (TREE)
+    return at < tree.context || (at < tree.len && tree.mask[seen + (at - tree.context)] != 0);
+  else
+    return at < seen;
+}
+
 // Products of one step's keys with the queries.
 template <int E, int QF, int SF, int D, int R>
 __device__ __forceinline__ void scores(int lane, const RawKeys<D, SF>& raw, const Rows<E, D, R>& s,
@@ -381,10 +398,10 @@ __device__ __forceinline__ void scores(int lane, const RawKeys<D, SF>& raw, cons
 // 2^31 keys add up to at most 2^103.  But from one m to the next l may fall by more than 2^-126 (keys of
 // scale 0, then one of 2^64: 2^-128 at equal scores), where o, whose terms fall with it, may become 0
 // and l may not: it takes the factor in two.
-template <int E, int D, int R>
+template <int E, int D, int R, bool TREE>
 __device__ __forceinline__ void softmax(int lane, int32_t tok, int32_t all, const Pages& pages,
                                         f32x4 (&x)[R][2], float (&ks)[8], const float (&vs)[8],
-                                        Rows<E, D, R>& s, u32x4 (&p)[R]) {
+                                        const Tree& tree, Rows<E, D, R>& s, u32x4 (&p)[R]) {
   constexpr int NT = D / 16;
   const int g = lane >> 4;
   if (tok + kStep > all || pages.p[0] < 0 || pages.p[1] < 0) {
@@ -395,7 +412,7 @@ __device__ __forceinline__ void softmax(int lane, int32_t tok, int32_t all, cons
 #pragma unroll
       for (int r = 0; r < R; ++r)
         x[r][i / 4][i % 4] =
-            at < s.seen[r] && pages.p[i / 4] >= 0 ? x[r][i / 4][i % 4] * ks[i] : -INFINITY;
+            sees<TREE>(s.seen[r], tree, at) && pages.p[i / 4] >= 0 ? x[r][i / 4][i % 4] * ks[i] : -INFINITY;
       ks[i] = 1.0f;
     }
   }
@@ -436,10 +453,10 @@ __device__ __forceinline__ void softmax(int lane, int32_t tok, int32_t all, cons
 }
 
 // One step of keys in registers, `end`: the unit's last row sees the keys below it.
-template <int E, int QF, int SF, int D, int R>
+template <int E, int QF, int SF, int D, int R, bool TREE>
 __device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t end,
                                      const Pages& pages, f32x4 (&x)[R][2], float (&ks)[8],
-                                     RawValues<D, SF>& raw, Rows<E, D, R>& s) {
+                                     RawValues<D, SF>& raw, const Tree& tree, Rows<E, D, R>& s) {
   constexpr int NT = D / 16;
   const int g = lane >> 4;
   float vs[8];
@@ -456,7 +473,7 @@ __device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t
     }
   }
   u32x4 p[R];
-  softmax<E, D, R>(lane, tok, all, pages, x, ks, vs, s, p);
+  softmax<E, D, R, TREE>(lane, tok, all, pages, x, ks, vs, tree, s, p);
 #pragma unroll
   for (int w = 0; w < NT / 4; ++w) {
     uint32_t d[2][4];
@@ -484,9 +501,10 @@ struct Keys {
   int32_t begin, end;          // of this workgroup
 };
 
-template <int E, int QF, int SF, int D, int R, bool ONCE>
+template <int E, int QF, int SF, int D, int R, bool ONCE, bool TREE>
 __device__ __forceinline__ void run_steps(const Args& a, const Keys& k, int h, int lane, int wave,
-                                          int32_t all, int32_t end, Rows<E, D, R>& s) {
+                                          int32_t all, int32_t end, const Tree& tree,
+                                          Rows<E, D, R>& s) {
   int32_t tok = k.begin + wave * kStep;
   if (tok >= k.end) return;
   // Table entries are read a step ahead of the loads that need them.
@@ -522,7 +540,7 @@ __device__ __forceinline__ void run_steps(const Args& a, const Keys& k, int h, i
 #pragma unroll
     for (int i = 0; i < 8; ++i) ks[i] = scale_of<SF>(keys.s[i / 4], i % 4) * a.scale2;
     load_keys<D, SF, ONCE>(a, lane, at, keys);
-    join<E, QF, SF, D, R>(lane, tok, all, end, pages, x, ks, values, s);
+    join<E, QF, SF, D, R, TREE>(lane, tok, all, end, pages, x, ks, values, tree, s);
     if (!more) return;
     load_values<D, SF, ONCE>(a, lane, at, values);
     tok = next;
@@ -565,7 +583,13 @@ struct Segment {
 constexpr int64_t kOut = -1;          // the result itself
 constexpr int64_t kRowParts = -2;
 
-template <int E, int QF, int SF, int D, int R, bool PREFIX, bool ONCE>
+template <bool TREE>
+__device__ __forceinline__ Tree tree_of(const Args& a, int b, int32_t len) {
+  if constexpr (TREE) return {a.tree + b * a.tree_next, len - a.S, len};
+  else return {};
+}
+
+template <int E, int QF, int SF, int D, int R, bool PREFIX, bool ONCE, bool TREE>
 __device__ __forceinline__ void run_segment(const Args& a, const Segment& seg, Shared<D, R>& sh) {
   constexpr int NT = D / 16;
   int lane = threadIdx.x & 63;
@@ -607,18 +631,22 @@ __device__ __forceinline__ void run_segment(const Args& a, const Segment& seg, S
     for (int j = 0; j < NT; ++j) s.o[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     s.m[r] = kLow;
     s.l[r] = 0.0f;
-    s.seen[r] = PREFIX ? k.end : (int32_t)cache::seen_tokens(len, a.most, a.S, w.s);
+    s.seen[r] = PREFIX ? k.end : TREE ? w.s * a.S : (int32_t)cache::seen_tokens(len, a.most, a.S, w.s);
   }
   s.lds_q = sh.q;
   if constexpr (R > 1) __syncthreads();
-  if constexpr (!PREFIX) {
+  const Tree tree = tree_of<TREE>(a, b, len);
+  if constexpr (TREE) {
+    all = tree.context;
+    end = len;
+  } else if constexpr (!PREFIX) {
     // Rows are in order of their tokens: the first sees least, the last most.
     all = __builtin_amdgcn_readfirstlane(s.seen[0]);
     const int last = tile * R * 16 + 16 * R - 1;
     end = (int32_t)cache::seen_tokens(len, a.most, a.S, row_of(last < rows ? last : rows - 1).s);
     if (k.end > end) k.end = end;
   }
-  run_steps<E, QF, SF, D, R, ONCE>(a, k, h, lane, wave, all, end, s);
+  run_steps<E, QF, SF, D, R, ONCE, TREE>(a, k, h, lane, wave, all, end, tree, s);
 
   // Join the waves.
 #pragma unroll
@@ -779,7 +807,7 @@ __device__ __forceinline__ void stage_tall(const Args& a, int lane, int wave, in
   }
 }
 
-template <int E, int QF, int SF, int D, bool PREFIX>
+template <int E, int QF, int SF, int D, bool PREFIX, bool TREE>
 __device__ __forceinline__ void run_tall(const Args& a, const Segment& seg,
                                          typename Tall<D>::Lds& sh) {
   constexpr int R = Tall<D>::R, NT = D / 16;
@@ -812,10 +840,15 @@ __device__ __forceinline__ void run_tall(const Args& a, const Segment& seg,
     for (int j = 0; j < NT; ++j) s.o[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     s.m[r] = kLow;
     s.l[r] = 0.0f;
-    s.seen[r] = PREFIX ? k.end : (int32_t)cache::seen_tokens(seg.len, a.most, a.S, w.s);
+    s.seen[r] = PREFIX ? k.end
+                : TREE ? w.s * a.S
+                       : (int32_t)cache::seen_tokens(seg.len, a.most, a.S, w.s);
   }
   int32_t all = k.end;                          // keys that all rows of this wave see
-  if constexpr (!PREFIX) {
+  const Tree tree = tree_of<TREE>(a, seg.b, seg.len);
+  if constexpr (TREE) {
+    all = tree.context;
+  } else if constexpr (!PREFIX) {
     // Rows are in order of their tokens: the last one of the workgroup sees most.
     all = __builtin_amdgcn_readfirstlane(s.seen[0]);
     const int last = (seg.tile + 1) * kWaves * 16 * R - 1;
@@ -899,7 +932,7 @@ __device__ __forceinline__ void run_tall(const Args& a, const Segment& seg,
           vs[i] = sh.vs[buf][u][16 * (i / 4) + 4 * g + i % 4];
         }
         u32x4 p[R];
-        softmax<E, D, R>(lane, tok + u * kStep, all, now[u], x, ks, vs, s, p);
+        softmax<E, D, R, TREE>(lane, tok + u * kStep, all, now[u], x, ks, vs, tree, s, p);
         if (u == kSteps - 1) {
 #pragma unroll
           for (int w = 0; w < kSteps; ++w) ahead[w] = entries(tok + 3 * kKeys + w * kStep);
@@ -948,7 +981,7 @@ __device__ __forceinline__ void run_tall(const Args& a, const Segment& seg,
 
 // One chunk of the prefix or (static) of a sequence's own keys.  `item`: workgroup number within
 // its kind.
-template <int E, int QF, int SF, int D, int R, bool PREFIX, bool TALL>
+template <int E, int QF, int SF, int D, int R, bool PREFIX, bool TALL, bool TREE>
 __device__ __forceinline__ void run_chunk(const Args& a, int item, char* lds) {
   const int chunks = PREFIX ? a.prefix_chunks : a.chunks;
   const Place place = PREFIX ? place_of(item, a.prefix_items, a.prefix_tiles)
@@ -978,9 +1011,9 @@ __device__ __forceinline__ void run_chunk(const Args& a, int item, char* lds) {
     if (s.keys.begin >= s.len && chunk > 0) return;
   }
   if constexpr (TALL)
-    run_tall<E, QF, SF, D, PREFIX>(a, s, *reinterpret_cast<typename Tall<D>::Lds*>(lds));
+    run_tall<E, QF, SF, D, PREFIX, TREE>(a, s, *reinterpret_cast<typename Tall<D>::Lds*>(lds));
   else
-    run_segment<E, QF, SF, D, R, PREFIX, false>(a, s, *reinterpret_cast<Shared<D, R>*>(lds));
+    run_segment<E, QF, SF, D, R, PREFIX, false, TREE>(a, s, *reinterpret_cast<Shared<D, R>*>(lds));
 }
 
 // LDS of the schedule.
@@ -1133,7 +1166,7 @@ __device__ __forceinline__ void run_share(const Args& a, int wg, Shared<D, 1>& s
            : a.prefix_len > 0 ? kRowParts
                               : kOut;
     if (pos > lo) __syncthreads();              // the last segment's LDS has been read
-    run_segment<E, QF, SF, D, 1, false, ONCE>(a, s, sh);
+    run_segment<E, QF, SF, D, 1, false, ONCE, false>(a, s, sh);
     pos += r1 - r0;
     if (r1 == n && s.h == a.H - 1) {
       first += n * a.H;
@@ -1152,37 +1185,37 @@ constexpr int lds_of() {
   else return sizeof(Shared<D, R>);
 }
 
-template <int E, int QF, int SF, int D, int R, int RP, int FORM>
+template <int E, int QF, int SF, int D, int R, int RP, int FORM, bool TREE>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention(Args a) {
   constexpr int kLds = lds_of<D, R>() > lds_of<D, RP>() ? lds_of<D, R>() : lds_of<D, RP>();
   __shared__ __align__(16) char lds[kLds];
   const int item = (int)blockIdx.x;
   if constexpr (RP > 0) {
     if (item < a.prefix_items) {
-      run_chunk<E, QF, SF, D, RP == kTall ? 1 : RP, true, RP == kTall>(a, item, lds);
+      run_chunk<E, QF, SF, D, RP == kTall ? 1 : RP, true, RP == kTall, false>(a, item, lds);
       return;
     }
   }
   if constexpr (FORM == kStatic) {
-    run_chunk<E, QF, SF, D, R == kTall ? 1 : R, false, R == kTall>(a, item - a.prefix_items, lds);
+    run_chunk<E, QF, SF, D, R == kTall ? 1 : R, false, R == kTall, TREE>(a, item - a.prefix_items, lds);
   } else {
     __shared__ Schedule sc;
-    static_assert(R == 1, "units of 16 rows");
+    static_assert(R == 1 && !TREE, "units of 16 rows, no trees");
     run_share<E, QF, SF, D, FORM == kScheduledOnce>(
         a, item - a.prefix_items, *reinterpret_cast<Shared<D, 1>*>(lds), sc);
   }
 }
 
 // Kernels for an element type (ET_BF16, ET_F16), code format (QF_FP8, QF_I8_RNE) and scale format:
-// lookup_e<E>_q<QF>_s<SF>, one for each instantiation unit.
-const void* lookup_e0_q0_s0(int D, int R, int RP, int form);
-const void* lookup_e0_q0_s1(int D, int R, int RP, int form);
-const void* lookup_e0_q1_s0(int D, int R, int RP, int form);
-const void* lookup_e0_q1_s1(int D, int R, int RP, int form);
-const void* lookup_e1_q0_s0(int D, int R, int RP, int form);
-const void* lookup_e1_q0_s1(int D, int R, int RP, int form);
-const void* lookup_e1_q1_s0(int D, int R, int RP, int form);
-const void* lookup_e1_q1_s1(int D, int R, int RP, int form);
+// lookup_e<E>_q<QF>_s<SF>, one for each instantiation unit.  tree: of drafted trees, static.
+const void* lookup_e0_q0_s0(int D, int R, int RP, int form, bool tree);
+const void* lookup_e0_q0_s1(int D, int R, int RP, int form, bool tree);
+const void* lookup_e0_q1_s0(int D, int R, int RP, int form, bool tree);
+const void* lookup_e0_q1_s1(int D, int R, int RP, int form, bool tree);
+const void* lookup_e1_q0_s0(int D, int R, int RP, int form, bool tree);
+const void* lookup_e1_q0_s1(int D, int R, int RP, int form, bool tree);
+const void* lookup_e1_q1_s0(int D, int R, int RP, int form, bool tree);
+const void* lookup_e1_q1_s1(int D, int R, int RP, int form, bool tree);
 
 }  // namespace attn
 }  // namespace fagq

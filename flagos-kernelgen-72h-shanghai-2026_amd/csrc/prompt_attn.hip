@@ -1,0 +1,227 @@
+// prompt_attn.hip - causal attention of packed prompts (include/fagq_prompt.h).
+//
+// One pass with a running maximum m and sum l of the softmax: for key j with score x (in units of
+// log 2), p = 2^(x - m), l = sum p, o = sum p v.  A workgroup takes 128 queries of one head, each
+// wave 32; keys and values come through LDS in tiles of 64, the next ones under way while these
+// are worked on.
+//   scores   S^T = K Q^T: lane (c, h) has query c's scores of half of the keys.
+//   output   O^T = V^T P^T: the packed probabilities are its B operand as they are.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "fagq.h"
+#include "fagq_dispatch.hpp"
+#include "fagq_prompt.h"
+#include "prompt_attn.hpp"
+
+namespace fagq {
+namespace prompt {
+namespace {
+
+constexpr float kLow = -3.0e38f;     // running maximum before the first key
+// The running maximum follows a row's scores only where p could pass 2^kSlack, which neither the
+// sums nor 16 bits mind, so that o is rarely multiplied.
+constexpr float kSlack = 8.0f;
+
+struct Args {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  Sequences seq;
+  uint16_t* out;
+  float* lse;
+  int64_t qs[2], ks[2], vs[2];       // {token, head} strides, elements
+  int32_t Hq, H, group, fill;
+  float scale2;                      // |sm_scale| log2(e), not 0
+  uint32_t flip;                     // signs of a pair of queries' values, where sm_scale < 0
+};
+
+// Rows behind the last sequence.
+template <int D>
+__device__ __forceinline__ void fill_tail(const Args& a, const Place& p, int hq) {
+  const int64_t first = (int64_t)p.end + (int64_t)p.tile * kTile;
+  for (int i = threadIdx.x; i < kTile * (D / 8); i += 64 * kWaves) {
+    const int64_t row = first + i / (D / 8);
+    if (row >= a.seq.T) break;
+    if (a.fill & FAGQ_FILL_OUT)
+      *reinterpret_cast<u32x4*>(a.out + (row * a.Hq + hq) * D + i % (D / 8) * 8) = u32x4{0, 0, 0, 0};
+    if (a.lse && (a.fill & FAGQ_FILL_LSE) && i % (D / 8) == 0) a.lse[(int64_t)hq * a.seq.T + row] = -INFINITY;
+  }
+}
+
+template <int E, int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention(Args a) {
+  using L = Tile<D>;
+  __shared__ __align__(16) char lds[2][2][L::kBytes];
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int wave = scalar((int)(threadIdx.x >> 6));
+  // Workgroup b runs on XCD b % 8: heads that share keys stay on one.
+  const int item = (int)blockIdx.x, kvh = item % a.H, rest = item / a.H;
+  const int hq = kvh * a.group + rest % a.group;
+  const Place p = place_of<true>(a.seq, rest / a.group);
+  if (p.b < 0) {
+    if (a.fill) fill_tail<D>(a, p, hq);
+    return;
+  }
+  const int32_t ahead = p.m - p.n;               // query i sees the keys up to i + ahead
+  const int32_t q0 = p.tile * kTile, mine = q0 + wave * kRows;
+  const int32_t i = mine + c;
+  auto seen_by = [&](int32_t query) {
+    const int32_t n = query + ahead + 1;
+    return n < 0 ? 0 : n < p.m ? n : p.m;
+  };
+  const int32_t seen = i < p.n ? seen_by(i) : 0;
+  const int32_t all = seen_by(mine);             // keys that every query of the wave sees
+  const int32_t last = mine + kRows <= p.n ? mine + kRows - 1 : p.n - 1;
+  const int32_t end = mine < p.n ? seen_by(last) : 0;                    // that one of them sees
+  const int32_t stop = seen_by(q0 + kTile <= p.n ? q0 + kTile - 1 : p.n - 1);
+
+  Copier<D> ck, cv;
+  ck.init(a.k, (int64_t)p.other * a.ks[0] + (int64_t)kvh * a.ks[1], a.ks[0], lane, wave);
+  cv.init(a.v, (int64_t)p.other * a.vs[0] + (int64_t)kvh * a.vs[1], a.vs[0], lane, wave);
+  if (stop > 0) {
+    ck.issue(lds[0][0], wave, 0, p.m - 1);
+    cv.issue(lds[0][1], wave, 0, p.m - 1);
+  }
+  u32x4 q[D / 16];
+  load_row<D>(a.q + (int64_t)(p.row + (i < p.n ? i : p.n - 1)) * a.qs[0] + (int64_t)hq * a.qs[1], h, q);
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) q[j] ^= a.flip;
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) o[d] = splat(0.0f);
+  float m = kLow, l = 0.0f;
+
+  int buf = 0;
+  for (int32_t tok = 0; tok < stop; tok += kStep, buf ^= 1) {
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);         // this step's tiles have landed, of this wave
+    lds_barrier();                               // of all; the last step's are done with
+    if (tok + kStep < stop) {
+      ck.issue(lds[buf ^ 1][0], wave, tok + kStep, p.m - 1);
+      cv.issue(lds[buf ^ 1][1], wave, tok + kStep, p.m - 1);
+    }
+    if (tok >= end) continue;
+    f32x16 x[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      x[t] = splat(0.0f);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) x[t] = mfma<E>(row_frag<D>(lds[buf][0], lane, t, j), q[j], x[t]);
+    }
+    if (tok + kStep > all) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          x[t][r] = tok + 32 * t + row_of(r, h) < seen ? x[t][r] : -INFINITY;
+    }
+    float top = x[0][0];
+#pragma unroll
+    for (int r = 1; r < 32; ++r) top = fmaxf(top, x[r / 16][r % 16]);
+    if (__any(__builtin_fmaf(top, a.scale2, -m) > kSlack)) {
+      const float next = fmaxf(m, cross_max(top) * a.scale2);
+      const float f = __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= f;
+    }
+    u32x4 w[4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        x[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][r], a.scale2, -m));
+        l += x[t][r];
+      }
+      w[2 * t] = pack8<E>(x[t], 0);
+      w[2 * t + 1] = pack8<E>(x[t], 1);
+    }
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) o[d] = mfma<E>(col_frag<D>(lds[buf][1], lane, d, t), w[t], o[d]);
+  }
+  l = cross_sum(l);
+  const int64_t row = p.row + i;
+  store_row<E, D>(a.out + (row * a.Hq + hq) * D, h, o, l > 0.0f ? 1.0f / l : 0.0f, i < p.n);
+  if (a.lse && h == 0 && i < p.n)
+    a.lse[(int64_t)hq * a.seq.T + row] =
+        l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * (1.0f / kLog2e) : -INFINITY;
+}
+
+template <int E>
+const void* kernel_for(int64_t D) {
+  return D == 64    ? reinterpret_cast<const void*>(&prompt_attention<E, 64>)
+         : D == 128 ? reinterpret_cast<const void*>(&prompt_attention<E, 128>)
+                    : reinterpret_cast<const void*>(&prompt_attention<E, 256>);
+}
+
+}  // namespace
+}  // namespace prompt
+}  // namespace fagq
+
+extern "C" {
+
+FAGQ_API int64_t fagq_prompt_attention_workspace_bytes(int64_t B, int64_t T, int64_t Tk,
+                                                       int64_t Hq, int64_t H, int64_t D) {
+  return fagq::prompt::check_sizes(B, T, Tk, Hq, H, D) == FAGQ_OK ? 0 : -1;
+}
+
+FAGQ_API int fagq_prompt_attention_launch(const void* q, const void* k, const void* v,
+                                          const int32_t* cu_seqlens, const int32_t* cu_seqlens_k,
+                                          void* out, float* lse, void* workspace,
+                                          int64_t workspace_bytes, const int64_t* strides,
+                                          int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H,
+                                          int64_t D, float sm_scale, int dtype, int fill,
+                                          void* stream) {
+  using namespace fagq;
+  using namespace fagq::prompt;
+  (void)workspace, (void)workspace_bytes;
+  if (!q || (Tk > 0 && (!k || !v)) || !cu_seqlens || !out || !strides) return FAGQ_E_NULL;
+  if (dtype != FAGQ_DT_BF16 && dtype != FAGQ_DT_F16) return FAGQ_E_FORMAT;
+  if (fill & ~(FAGQ_FILL_OUT | FAGQ_FILL_LSE)) return FAGQ_E_FORMAT;
+  if (!std::isfinite(sm_scale)) return FAGQ_E_SHAPE;
+  const int sizes = check_sizes(B, T, Tk, Hq, H, D);
+  if (sizes != FAGQ_OK) return sizes;
+  if (!cu_seqlens_k && T != Tk) return FAGQ_E_SHAPE;
+  const int st = check_strides(strides, 6);
+  if (st != FAGQ_OK) return st;
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(lse, 4) ||
+      !aligned(cu_seqlens, 4) || !aligned(cu_seqlens_k, 4))
+    return FAGQ_E_ALIGN;
+  if (T == 0) return FAGQ_OK;
+  const Rows rows[3] = {{q, T, Hq, D, strides[0], strides[1]},
+                        {k, Tk, H, D, strides[2], strides[3]},
+                        {v, Tk, H, D, strides[4], strides[5]}};
+  const void* ins[5] = {q, k, v, cu_seqlens, cu_seqlens_k};
+  const int64_t nin[5] = {rows[0].bytes(), rows[1].bytes(), rows[2].bytes(), (B + 1) * 4,
+                          cu_seqlens_k ? (B + 1) * 4 : 0};
+  const int64_t nout = T * Hq * D * 2, nlse = lse ? T * Hq * 4 : 0;
+  for (int i = 0; i < 5; ++i)
+    if (overlap(out, nout, ins[i], nin[i]) || overlap(lse, nlse, ins[i], nin[i])) return FAGQ_E_ALIAS;
+  if (overlap(out, nout, lse, nlse)) return FAGQ_E_ALIAS;
+  const int dcheck = device_check();
+  if (dcheck != FAGQ_OK) return dcheck;
+  Args a = {};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
+  a.seq = {cu_seqlens, cu_seqlens_k ? cu_seqlens_k : cu_seqlens, (int32_t)B, (int32_t)T, (int32_t)Tk};
+  a.out = static_cast<uint16_t*>(out), a.lse = lse;
+  for (int i = 0; i < 2; ++i) a.qs[i] = strides[i], a.ks[i] = strides[2 + i], a.vs[i] = strides[4 + i];
+  a.Hq = (int32_t)Hq, a.H = (int32_t)H, a.group = (int32_t)(Hq / H);
+  a.fill = fill;
+  // What a query does not see has the score -inf, which times 0 would be no number.
+  a.scale2 = std::fmax(std::fabs(sm_scale) * kLog2e, 0x1p-126f);
+  a.flip = sm_scale < 0.0f ? 0x80008000u : 0u;
+  void* args[] = {&a};
+  return launch_kernel(dtype == FAGQ_DT_BF16 ? kernel_for<ET_BF16>(D) : kernel_for<ET_F16>(D),
+                       dim3((unsigned)(tile_slots(T, B) * Hq)), dim3(64 * kWaves), args, 0,
+                       static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

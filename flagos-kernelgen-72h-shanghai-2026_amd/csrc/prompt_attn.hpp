@@ -1,0 +1,327 @@
+// prompt_attn.hpp - device code shared by the attention of prompts and its gradients
+// (include/fagq_prompt.h): which rows a workgroup takes, tiles in LDS, operands of the matrix
+// instructions, and the host's checks.
+//
+// Matrix instructions are 32 x 32 x 16.  Lane (c, h), c = lane % 32, h = lane / 32:
+//   A, B     row (column) c, places 8 h .. 8 h + 7 of the sum over 16
+//   C        column c, rows (r % 4) + 8 (r / 4) + 4 h at register r
+// A product's result therefore is the B operand of the next one as it stands: registers 8 t .. of
+// a lane are 8 of 16 places of the sum over the result's rows, and the A operand only has to have
+// the same rows there, 4 h + 0..3 and 8 + 4 h + 0..3 of each 16.  A tile that lies in LDS row by
+// row gives both kinds of operand: rows as they are (16-byte reads), columns by the transposed
+// 8-byte read (a lane receives 4 rows of its column).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "fagq.h"
+#include "fagq_dispatch.hpp"
+
+namespace fagq {
+namespace prompt {
+
+constexpr int kWaves = 4;
+constexpr int kRows = 32;                       // of a wave
+constexpr int kTile = kRows * kWaves;           // of a workgroup
+constexpr int kStep = 64;                       // rows of the other side that are in LDS at a time
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int64_t kMostGroups = 1ll << 24;      // a grid of 2^32 threads is too large
+constexpr int kVmcnt0 = 0x0F70;                 // s_waitcnt vmcnt(0), other counters not waited
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+template <int E>
+__device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (E == ET_BF16) {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a),
+                                                   __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  } else {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a),
+                                                  __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+}
+
+__device__ __forceinline__ f32x16 splat(float v) {
+  f32x16 r;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = v;
+  return r;
+}
+
+// Row of a 32 x 32 result at register r.
+__device__ __forceinline__ int row_of(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
+
+// Maximum (sum) over the lanes c and c + 32; both receive it.
+__device__ __forceinline__ float cross_max(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float cross_sum(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// ------------------------------------------------------------------------- tiles in LDS
+
+// A tile of kStep rows of D elements, row by row, in 16-byte chunks; chunk c of row r lies at chunk
+// c ^ swizzle(r) of it.  256 bytes of LDS (16 chunks) are read at once without a conflict: the 16
+// rows of a 16-byte read at one c, and the 4 rows x 4 chunks of a transposed read.
+template <int D>
+struct Tile {
+  static constexpr int kChunks = D / 8;
+  static constexpr int kRowBytes = D * 2;
+  static constexpr int kBytes = kStep * kRowBytes;
+  static constexpr int kCopyRows = 64 / kChunks;              // rows that one copy brings
+  static constexpr int kCopies = kStep / kCopyRows / kWaves;  // of each wave
+  static __device__ __forceinline__ int swizzle(int r) {
+    if constexpr (D == 64) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);   // two rows in 256 bytes
+    else return (r & 3) << 2 | ((r >> 2) & 3);
+  }
+};
+
+// Copies rows [first, first + kStep) of one head, row `last` in place of those behind it, from HBM
+// into LDS, past the registers.  Copy n of wave w brings rows (4 n + w) kCopyRows ..
+template <int D>
+struct Copier {
+  using L = Tile<D>;
+  const char* base;            // row 0 of the sequence
+  uint32_t stride;             // bytes of a row
+  int row;                     // within the copies of this wave, of this lane
+  uint32_t chunk[2];           // byte in the row, for even and odd n
+  __device__ __forceinline__ void init(const void* p, int64_t element, int64_t token_stride, int lane,
+                                       int wave) {
+    base = static_cast<const char*>(p) + element * 2;
+    stride = (uint32_t)token_stride * 2u;
+    row = wave * L::kCopyRows + lane / L::kChunks;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      chunk[i] = (uint32_t)((lane % L::kChunks) ^ L::swizzle(row + i * kWaves * L::kCopyRows)) * 16u;
+  }
+  __device__ __forceinline__ void issue(char* lds, int wave, int first, int last) const {
+    const rsrc_t rs = make_rsrc(base + (int64_t)first * stride, 0x7fffffffu);
+    if (first + kStep - 1 <= last) {
+      const uint32_t off = (uint32_t)row * stride;
+#pragma unroll
+      for (int n = 0; n < L::kCopies; ++n)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, (lds_void_t*)(lds + (n * kWaves + wave) * 1024), 16, off + chunk[n & 1],
+            (uint32_t)(n * kWaves * L::kCopyRows) * stride, 0, 0);
+    } else {
+#pragma unroll
+      for (int n = 0; n < L::kCopies; ++n) {
+        const int r = row + n * kWaves * L::kCopyRows, most = last - first;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, (lds_void_t*)(lds + (n * kWaves + wave) * 1024), 16,
+            (uint32_t)(r < most ? r : most) * stride + chunk[n & 1], 0, 0, 0);
+      }
+    }
+  }
+};
+
+// Row operand: rows 32 t .. of a tile, places 16 i .. of the sum over D.
+template <int D>
+__device__ __forceinline__ u32x4 row_frag(const char* tile, int lane, int t, int i) {
+  const int c = lane & 31, h = lane >> 5;
+  const int at = c * Tile<D>::kRowBytes + (((2 * i) ^ (h ^ Tile<D>::swizzle(c))) << 4);
+  return *reinterpret_cast<const u32x4*>(tile + at + t * 32 * Tile<D>::kRowBytes);
+}
+
+// Column operand: columns 32 d .. of a tile, rows 16 t .. as the places of the sum.
+template <int D>
+__device__ __forceinline__ u32x4 col_frag(const char* tile, int lane, int d, int t) {
+  const int i = lane & 15, g = (lane >> 4) & 1, h = lane >> 5;
+  u32x4 r;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int row = 8 * u + 4 * h + (i >> 2);
+    const int chunk = (4 * d + 2 * g + ((i >> 1) & 1)) ^ Tile<D>::swizzle(row);
+    const char* p = tile + row * Tile<D>::kRowBytes + chunk * 16 + (i & 1) * 8 +
+                    t * 16 * Tile<D>::kRowBytes;
+    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    r[2 * u] = w[0], r[2 * u + 1] = w[1];
+  }
+  return r;
+}
+
+// Registers 8 t .. of a result as the B operand of the next product.
+template <int E>
+__device__ __forceinline__ u32x4 pack8(const f32x16& x, int t) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = pack16<E>(x[8 * t + 2 * i], x[8 * t + 2 * i + 1]);
+  return r;
+}
+
+// A row in global memory as row operands: places 16 i + 8 h ..
+template <int D>
+__device__ __forceinline__ void load_row(const uint16_t* row, int h, u32x4 (&f)[D / 16]) {
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+    f[i] = *reinterpret_cast<const u32x4*>(row + 16 * i + 8 * h);
+}
+
+// A lane's column of a transposed result [D x 32] times f, as a row in global memory.  The halves
+// exchange four rows each, so that every lane stores 16 bytes.
+template <int E, int D>
+__device__ __forceinline__ void store_row(uint16_t* row, int h, const f32x16 (&o)[D / 32], float f,
+                                          bool live) {
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {               // rows 16 p ..: 4 h .. and 8 + 4 h ..
+      uint32_t a[2], b[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        a[i] = pack16<E>(o[d][8 * p + 2 * i] * f, o[d][8 * p + 2 * i + 1] * f);
+        b[i] = pack16<E>(o[d][8 * p + 4 + 2 * i] * f, o[d][8 * p + 4 + 2 * i + 1] * f);
+      }
+      // Lane c keeps rows 0 .. 3 and receives 4 .. 7; lane c + 32 receives 8 .. 11, keeps 12 .. 15.
+      const auto x = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+      if (live)
+        *reinterpret_cast<u32x4*>(row + 32 * d + 16 * p + 8 * h) = u32x4{x[0], y[0], x[1], y[1]};
+    }
+}
+
+// ------------------------------------------------------------------------- sequences
+
+struct Sequences {
+  const int32_t* cu;           // of the rows that tiles are made of
+  const int32_t* other;        // of the other side's
+  int32_t B, T, Tother;
+};
+
+struct Place {
+  int32_t b;                   // -1: a tile behind the last one
+  int32_t tile;                // of the sequence; behind the last one: which
+  int32_t row, n;              // first row and length of the sequence
+  int32_t other, m;            // of the other side
+  int32_t end;                 // rows of all sequences
+};
+
+__device__ __forceinline__ int32_t clamped(int32_t v, int32_t most) {
+  return v < 0 ? 0 : v < most ? v : most;
+}
+__device__ __forceinline__ int32_t scalar(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Tile number `slot` of all sequences': from the last one backwards (REVERSED), where late tiles
+// see most, or from the first on.  Lane l counts the tiles of sequences l n .. (l + 1) n - 1.
+template <bool REVERSED>
+__device__ __forceinline__ Place place_of(const Sequences& s, int32_t slot) {
+  const int lane = threadIdx.x & 63;
+  const int each = (s.B + 63) / 64;
+  auto length = [&](int i, int32_t* row) {       // i: in the order of the tiles
+    const int b = REVERSED ? s.B - 1 - i : i;
+    const int32_t lo = clamped(s.cu[b], s.T), hi = clamped(s.cu[b + 1], s.T);
+    *row = lo;
+    return hi > lo ? hi - lo : 0;
+  };
+  const int first = lane * each, stop = first + each < s.B ? first + each : s.B;
+  int32_t mine = 0, row = 0;
+  for (int i = first; i < stop; ++i) mine += (length(i, &row) + kTile - 1) / kTile;
+  int32_t upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int32_t o = __shfl_up(upto, d);
+    upto += lane >= d ? o : 0;
+  }
+  Place p = {};
+  p.end = scalar(clamped(s.cu[s.B], s.T));
+  const int32_t total = __builtin_amdgcn_readlane(upto, 63);
+  if (slot >= total) {
+    p.b = -1;
+    p.tile = slot - total;
+    return p;
+  }
+  const uint64_t here = __ballot(slot >= upto - mine && slot < upto);
+  const int l = (int)__builtin_ctzll(here);
+  int32_t at = slot - __builtin_amdgcn_readlane(upto - mine, l);
+  int i = l * each;
+  int32_t n = scalar(length(i, &row)), tiles = (n + kTile - 1) / kTile;
+  while (at >= tiles) {                          // ends: the lane's tiles are more than `at`
+    at -= tiles;
+    n = scalar(length(++i, &row));
+    tiles = (n + kTile - 1) / kTile;
+  }
+  p.b = REVERSED ? s.B - 1 - i : i;
+  p.tile = REVERSED ? tiles - 1 - at : at;
+  p.row = scalar(row);
+  p.n = n;
+  const int32_t lo = scalar(clamped(s.other[p.b], s.Tother));
+  const int32_t hi = scalar(clamped(s.other[p.b + 1], s.Tother));
+  p.other = lo;
+  p.m = hi > lo ? hi - lo : 0;
+  return p;
+}
+
+// Tiles that a grid has room for: every sequence may end in a tile of its own.  Those behind the
+// last one are as many as the rows behind the last sequence fill, at least.
+inline int64_t tile_slots(int64_t T, int64_t B) { return (T + B * (kTile - 1) + kTile - 1) / kTile; }
+
+// ------------------------------------------------------------------------- host
+
+inline bool aligned(const void* p, uintptr_t a) {
+  return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
+}
+inline bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
+// T tokens of H rows of D elements of 16 bits, at token and head strides.
+struct Rows {
+  const void* p;
+  int64_t T, H, D, st, sh;
+  int64_t bytes() const { return T > 0 ? ((T - 1) * st + (H - 1) * sh + D) * 2 : 0; }
+};
+
+// Whether two sets of rows share an element (told exactly for heads that lie within a token's
+// stride, as views of one fused buffer do; otherwise by their ranges).
+inline bool overlap(const Rows& a, const Rows& b) {
+  if (!overlap(a.p, a.bytes(), b.p, b.bytes())) return false;
+  const int64_t wa = ((a.H - 1) * a.sh + a.D) * 2, wb = ((b.H - 1) * b.sh + b.D) * 2, s = a.st * 2;
+  if (a.st != b.st || a.T < 2 || b.T < 2 || wa > s || wb > s) return true;
+  const intptr_t pa = reinterpret_cast<intptr_t>(a.p), pb = reinterpret_cast<intptr_t>(b.p);
+  const int64_t off = ((pb - pa) % s + s) % s;   // b's heads start here in a's token
+  return off < wa || (off != 0 && s - off < wb);
+}
+
+// Rows that are written must not share an element among themselves.
+inline bool self_overlap(const Rows& r) {
+  const bool tokens_outside = (r.T < 2 || r.st >= (r.H - 1) * r.sh + r.D) && (r.H < 2 || r.sh >= r.D);
+  const bool heads_outside = (r.H < 2 || r.sh >= (r.T - 1) * r.st + r.D) && (r.T < 2 || r.st >= r.D);
+  return !tokens_outside && !heads_outside;
+}
+
+// {token, head} strides in elements.
+inline int check_strides(const int64_t* strides, int n) {
+  for (int i = 0; i < n; ++i) {
+    if (strides[i] < 0) return FAGQ_E_SHAPE;
+    if (strides[i] >= (i % 2 ? 1ll << 31 : 1ll << 24)) return FAGQ_E_TOO_LARGE;
+    if (strides[i] % 8 != 0) return FAGQ_E_ALIGN;
+  }
+  return FAGQ_OK;
+}
+
+inline int check_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
+  if (B < 0 || T < 0 || Tk < 0 || H < 1 || Hq < H || Hq % H != 0 || (D != 64 && D != 128 && D != 256))
+    return FAGQ_E_SHAPE;
+  if (B > (1ll << 24) || T > (1ll << 31) - 1 || Tk > (1ll << 31) - 1 || Hq > 4096 ||
+      tile_slots(T, B) * Hq >= kMostGroups)
+    return FAGQ_E_TOO_LARGE;
+  return FAGQ_OK;
+}
+
+}  // namespace prompt
+}  // namespace fagq

@@ -1,0 +1,442 @@
+// prompt_attn_bwd.hip - gradients of the causal attention of packed prompts (include/fagq_prompt.h).
+//
+// Two passes over the pairs of query and key, so that every sum has one owner and one order (no
+// atomics): seven products for the five of the formulas.
+//   prompt_dq     A workgroup takes 128 queries of one head, keys and values come through LDS.
+//                 S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.  It also leaves what the other
+//                 pass needs of each query: lse in units of log 2, and -delta.
+//   prompt_dkdv   A workgroup takes 128 keys of one head of k and v, the queries of all heads of
+//                 the group come through LDS.  S = Q K^T, dP = dO V^T, dV^T += dO^T P,
+//                 dK^T += Q^T dS.  Where there are few workgroups, each key tile's steps are cut
+//                 into parts of their own sums, which prompt_join adds up in order.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "fagq.h"
+#include "fagq_dispatch.hpp"
+#include "fagq_prompt.h"
+#include "prompt_attn.hpp"
+
+namespace fagq {
+namespace prompt {
+namespace {
+
+struct Args {
+  const uint16_t* dout;
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  const uint16_t* out;
+  const float* lse;
+  Sequences queries, keys;           // tiles of queries, of keys
+  uint16_t* dq;
+  uint16_t* dk;
+  uint16_t* dv;
+  float* lse2;                       // [Hq, T]; +inf for a query without keys
+  float* delta;                      // [Hq, T], negative
+  float* part;                       // [parts][Tk][H][D] of dk, then of dv
+  int64_t dos[2], qs[2], ks[2], vs[2], dqs[2], dks[2], dvs[2];   // {token, head} strides, elements
+  int32_t Hq, H, group, fill, parts;
+  float scale, scale2;               // sm_scale, and times log2(e)
+};
+
+template <int D>
+__device__ __forceinline__ void fill_tail(uint16_t* out, const int64_t (&s)[2], int head, int32_t rows,
+                                          const Place& p) {
+  const int64_t first = (int64_t)p.end + (int64_t)p.tile * kTile;
+  for (int i = threadIdx.x; i < kTile * (D / 8); i += 64 * kWaves) {
+    const int64_t row = first + i / (D / 8);
+    if (row >= rows) break;
+    *reinterpret_cast<u32x4*>(out + row * s[0] + (int64_t)head * s[1] + i % (D / 8) * 8) = u32x4{0, 0, 0, 0};
+  }
+}
+
+template <int E, int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void prompt_dq(Args a) {
+  using L = Tile<D>;
+  __shared__ __align__(16) char lds[2][2][L::kBytes];
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int wave = scalar((int)(threadIdx.x >> 6));
+  // Workgroup b runs on XCD b % 8: heads that share keys stay on one.
+  const int item = (int)blockIdx.x, kvh = item % a.H, rest = item / a.H;
+  const int hq = kvh * a.group + rest % a.group;
+  const Place p = place_of<true>(a.queries, rest / a.group);
+  if (p.b < 0) {
+    if (a.fill & FAGQ_FILL_DQ) fill_tail<D>(a.dq, a.dqs, hq, a.queries.T, p);
+    return;
+  }
+  const int32_t ahead = p.m - p.n;               // query i sees the keys up to i + ahead
+  const int32_t q0 = p.tile * kTile, mine = q0 + wave * kRows;
+  const int32_t i = mine + c, row = p.row + (i < p.n ? i : p.n - 1);
+  auto seen_by = [&](int32_t query) {
+    const int32_t n = query + ahead + 1;
+    return n < 0 ? 0 : n < p.m ? n : p.m;
+  };
+  const int32_t seen = i < p.n ? seen_by(i) : 0;
+  const int32_t all = seen_by(mine);             // keys that every query of the wave sees
+  const int32_t last = mine + kRows <= p.n ? mine + kRows - 1 : p.n - 1;
+  const int32_t end = mine < p.n ? seen_by(last) : 0;                    // that one of them sees
+  const int32_t stop = seen_by(q0 + kTile <= p.n ? q0 + kTile - 1 : p.n - 1);
+
+  Copier<D> ck, cv;
+  ck.init(a.k, (int64_t)p.other * a.ks[0] + (int64_t)kvh * a.ks[1], a.ks[0], lane, wave);
+  cv.init(a.v, (int64_t)p.other * a.vs[0] + (int64_t)kvh * a.vs[1], a.vs[0], lane, wave);
+  if (stop > 0) {
+    ck.issue(lds[0][0], wave, 0, p.m - 1);
+    cv.issue(lds[0][1], wave, 0, p.m - 1);
+  }
+  u32x4 q[D / 16], g[D / 16];
+  load_row<D>(a.q + (int64_t)row * a.qs[0] + (int64_t)hq * a.qs[1], h, q);
+  load_row<D>(a.dout + (int64_t)row * a.dos[0] + (int64_t)hq * a.dos[1], h, g);
+  float delta = 0.0f;
+  {
+    u32x4 out[D / 16];
+    load_row<D>(a.out + ((int64_t)row * a.Hq + hq) * D, h, out);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        delta = __builtin_fmaf(-lo16<E>(g[j][e]), lo16<E>(out[j][e]), delta);
+        delta = __builtin_fmaf(-hi16<E>(g[j][e]), hi16<E>(out[j][e]), delta);
+      }
+  }
+  delta = cross_sum(delta);
+  const float lse = a.lse[(int64_t)hq * a.queries.T + row];
+  const float lse2 = seen > 0 ? lse * kLog2e : INFINITY;
+  if (h == 0 && i < p.n) {
+    a.lse2[(int64_t)hq * a.queries.T + row] = lse2;
+    a.delta[(int64_t)hq * a.queries.T + row] = delta;
+  }
+  f32x16 dq[D / 32];
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) dq[d] = splat(0.0f);
+
+  int buf = 0;
+  for (int32_t tok = 0; tok < stop; tok += kStep, buf ^= 1) {
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);         // this step's tiles have landed, of this wave
+    lds_barrier();                               // of all; the last step's are done with
+    if (tok + kStep < stop) {
+      ck.issue(lds[buf ^ 1][0], wave, tok + kStep, p.m - 1);
+      cv.issue(lds[buf ^ 1][1], wave, tok + kStep, p.m - 1);
+    }
+    if (tok >= end) continue;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x16 x = splat(0.0f), y = splat(delta);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        x = mfma<E>(row_frag<D>(lds[buf][0], lane, t, j), q[j], x);
+        y = mfma<E>(row_frag<D>(lds[buf][1], lane, t, j), g[j], y);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -lse2));
+      if (tok + kStep > all) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = tok + 32 * t + row_of(r, h) < seen ? x[r] : 0.0f;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] *= y[r];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const u32x4 w = pack8<E>(x, u);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+          dq[d] = mfma<E>(col_frag<D>(lds[buf][0], lane, d, 2 * t + u), w, dq[d]);
+      }
+    }
+  }
+  store_row<E, D>(a.dq + (int64_t)row * a.dqs[0] + (int64_t)hq * a.dqs[1], h, dq, a.scale, i < p.n);
+}
+
+template <int E, int D>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_dkdv(Args a) {
+  using L = Tile<D>;
+  __shared__ __align__(16) char lds[2][2][L::kBytes];
+  __shared__ __align__(16) float stats[2][2][kStep];      // lse2, -delta
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int wave = scalar((int)(threadIdx.x >> 6));
+  const int item = (int)blockIdx.x, kvh = item % a.H, rest = item / a.H;
+  const int part = rest % a.parts;
+  const Place p = place_of<false>(a.keys, rest / a.parts);
+  if (p.b < 0) {
+    if (part == 0 && (a.fill & FAGQ_FILL_DK)) fill_tail<D>(a.dk, a.dks, kvh, a.keys.T, p);
+    if (part == 0 && (a.fill & FAGQ_FILL_DV)) fill_tail<D>(a.dv, a.dvs, kvh, a.keys.T, p);
+    return;
+  }
+  // n keys, m queries; query i sees the keys up to i + ahead.
+  const int32_t ahead = p.n - p.m, k0 = p.tile * kTile, mine = k0 + wave * kRows;
+  const int32_t j0 = mine + c, row = p.row + (j0 < p.n ? j0 : p.n - 1);
+  const int32_t first = k0 > ahead ? k0 - ahead : 0;       // query that sees one of the tile's keys
+  const int32_t steps = first < p.m ? (p.m - first + kStep - 1) / kStep : 0;
+  // Steps of all heads in a row, head by head: this part's share.
+  const int64_t total = (int64_t)steps * a.group;
+  const int32_t from = (int32_t)(total * part / a.parts), to = (int32_t)(total * (part + 1) / a.parts);
+
+  Copier<D> cq, cg;
+  cq.init(a.q, (int64_t)p.other * a.qs[0] + (int64_t)kvh * a.group * a.qs[1], a.qs[0], lane, wave);
+  cg.init(a.dout, (int64_t)p.other * a.dos[0] + (int64_t)kvh * a.group * a.dos[1], a.dos[0], lane, wave);
+  int32_t head = steps > 0 ? from / steps : 0, step = from - head * steps;
+  // The next step's rows.
+  auto issue = [&](int buf, int32_t head, int32_t step) {
+    const int32_t i0 = first + step * kStep;
+    Copier<D> x = cq, y = cg;
+    x.base += (int64_t)head * a.qs[1] * 2;
+    y.base += (int64_t)head * a.dos[1] * 2;
+    x.issue(lds[buf][0], wave, i0, p.m - 1);
+    y.issue(lds[buf][1], wave, i0, p.m - 1);
+    if (wave < 2) {
+      const int64_t at = (int64_t)(kvh * a.group + head) * a.keys.Tother + p.other + i0;
+      const int32_t most = p.m - 1 - i0;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          make_rsrc((wave == 0 ? a.lse2 : a.delta) + at, 0x7fffffffu),
+          (lds_void_t*)(wave == 0 ? stats[buf][0] : stats[buf][1]), 4,
+          (uint32_t)(lane < most ? lane : most) * 4u, 0, 0, 0);
+    }
+  };
+  if (from < to) issue(0, head, step);
+  u32x4 k[D / 16], v[D / 16];
+  load_row<D>(a.k + (int64_t)row * a.ks[0] + (int64_t)kvh * a.ks[1], h, k);
+  load_row<D>(a.v + (int64_t)row * a.vs[0] + (int64_t)kvh * a.vs[1], h, v);
+  f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) dk[d] = dv[d] = splat(0.0f);
+
+  int buf = 0;
+  for (int32_t it = from; it < to; ++it, buf ^= 1) {
+    const int32_t i0 = first + step * kStep;
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);         // this step's tiles have landed, of this wave
+    lds_barrier();                               // of all; the last step's are done with
+    if (++step == steps) step = 0, ++head;
+    if (it + 1 < to) issue(buf ^ 1, head, step);
+    if (mine >= p.n) continue;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int32_t first_query = i0 + 32 * t;
+      if (first_query >= p.m || first_query + 31 + ahead < mine) continue;
+      f32x16 x = splat(0.0f), y;
+      float lse2[16];
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const f32x4 s = *reinterpret_cast<const f32x4*>(&stats[buf][0][32 * t + row_of(r, h)]);
+        const f32x4 d = *reinterpret_cast<const f32x4*>(&stats[buf][1][32 * t + row_of(r, h)]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lse2[r + e] = s[e], y[r + e] = d[e];
+      }
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        x = mfma<E>(row_frag<D>(lds[buf][0], lane, t, j), k[j], x);
+        y = mfma<E>(row_frag<D>(lds[buf][1], lane, t, j), v[j], y);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -lse2[r]));
+      if (first_query + 32 > p.m || first_query + ahead < mine + kRows - 1) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int32_t i = first_query + row_of(r, h);
+          x[r] = i < p.m && j0 <= i + ahead ? x[r] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const u32x4 w = pack8<E>(x, u);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+          dv[d] = mfma<E>(col_frag<D>(lds[buf][1], lane, d, 2 * t + u), w, dv[d]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] *= y[r];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const u32x4 w = pack8<E>(x, u);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+          dk[d] = mfma<E>(col_frag<D>(lds[buf][0], lane, d, 2 * t + u), w, dk[d]);
+      }
+    }
+  }
+  if (a.parts == 1) {
+    store_row<E, D>(a.dk + (int64_t)row * a.dks[0] + (int64_t)kvh * a.dks[1], h, dk, a.scale, j0 < p.n);
+    store_row<E, D>(a.dv + (int64_t)row * a.dvs[0] + (int64_t)kvh * a.dvs[1], h, dv, 1.0f, j0 < p.n);
+  } else if (j0 < p.n) {
+    const int64_t plane = (int64_t)a.keys.T * a.H * D;
+    float* to_k = a.part + part * plane + ((int64_t)row * a.H + kvh) * D;
+    float* to_v = to_k + a.parts * plane;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        *reinterpret_cast<f32x4*>(to_k + 32 * d + row_of(r, h)) =
+            f32x4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+        *reinterpret_cast<f32x4*>(to_v + 32 * d + row_of(r, h)) =
+            f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+      }
+  }
+}
+
+// Sums of the parts.  A thread has 8 elements of dk or of dv.
+template <int E>
+__global__ __launch_bounds__(256) void prompt_join(Args a, int32_t D) {
+  const int64_t plane = (int64_t)a.keys.T * a.H * D;
+  const int64_t each = plane / 8, item = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (item >= 2 * each) return;
+  const bool values = item >= each;
+  const int64_t at = (values ? item - each : item) * 8;
+  const int64_t row = at / ((int64_t)a.H * D);
+  const int32_t rest = (int32_t)(at - row * a.H * D), head = rest / D, d = rest - head * D;
+  if (row >= clamped(a.keys.cu[a.keys.B], a.keys.T)) return;
+  const float* part = a.part + (values ? a.parts * plane : 0) + at;
+  f32x4 s[2] = {};
+  for (int i = 0; i < a.parts; ++i, part += plane) {
+    s[0] += *reinterpret_cast<const f32x4*>(part);
+    s[1] += *reinterpret_cast<const f32x4*>(part + 4);
+  }
+  const float f = values ? 1.0f : a.scale;
+  uint16_t* to = values ? a.dv + row * a.dvs[0] + (int64_t)head * a.dvs[1]
+                        : a.dk + row * a.dks[0] + (int64_t)head * a.dks[1];
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack16<E>(s[i / 2][2 * i % 4] * f, s[i / 2][2 * i % 4 + 1] * f);
+  *reinterpret_cast<u32x4*>(to + d) = w;
+}
+
+// ---------------------------------------------------------------------------------- host
+
+constexpr int64_t kSlots = 512;      // workgroups at a time
+constexpr int64_t kMostParts = 16;
+
+int check_bwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
+  const int st = check_sizes(B, T, Tk, Hq, H, D);
+  if (st != FAGQ_OK) return st;
+  // With all the parts there may be, and the joining kernel's workgroups.
+  const bool large = tile_slots(Tk, B) * H * kMostParts >= kMostGroups || Tk * H * D / 1024 >= kMostGroups - 1;
+  return large ? FAGQ_E_TOO_LARGE : FAGQ_OK;
+}
+
+// Parts of a key tile's steps, so that there are several workgroups for each place.
+int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H) {
+  const int64_t groups = std::max<int64_t>(1, (Tk + kTile - 1) / kTile * H);
+  const int64_t steps = Hq / H * ((T + kStep - 1) / kStep);
+  return std::max<int64_t>(1, std::min<int64_t>({(3 * kSlots + groups - 1) / groups, steps / 4, kMostParts}));
+}
+
+int64_t bytes_for(int64_t parts, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
+  const int64_t stats = (2 * Hq * T * 4 + 15) / 16 * 16;
+  return stats + (parts > 1 ? 2 * parts * Tk * H * D * 4 : 0);
+}
+
+template <int E>
+const void* dq_for(int64_t D) {
+  return D == 64    ? reinterpret_cast<const void*>(&prompt_dq<E, 64>)
+         : D == 128 ? reinterpret_cast<const void*>(&prompt_dq<E, 128>)
+                    : reinterpret_cast<const void*>(&prompt_dq<E, 256>);
+}
+template <int E>
+const void* dkdv_for(int64_t D) {
+  return D == 64    ? reinterpret_cast<const void*>(&prompt_dkdv<E, 64>)
+         : D == 128 ? reinterpret_cast<const void*>(&prompt_dkdv<E, 128>)
+                    : reinterpret_cast<const void*>(&prompt_dkdv<E, 256>);
+}
+
+}  // namespace
+}  // namespace prompt
+}  // namespace fagq
+
+extern "C" {
+
+FAGQ_API int64_t fagq_prompt_attention_bwd_workspace_bytes(int64_t B, int64_t T, int64_t Tk,
+                                                           int64_t Hq, int64_t H, int64_t D) {
+  using namespace fagq::prompt;
+  if (check_bwd_sizes(B, T, Tk, Hq, H, D) != FAGQ_OK) return -1;
+  return bytes_for(parts_for(B, T, Tk, Hq, H), T, Tk, Hq, H, D);
+}
+
+FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, const void* k,
+                                              const void* v, const void* out, const float* lse,
+                                              const int32_t* cu_seqlens,
+                                              const int32_t* cu_seqlens_k, void* dq, void* dk,
+                                              void* dv, void* workspace, int64_t workspace_bytes,
+                                              const int64_t* strides, int64_t B, int64_t T,
+                                              int64_t Tk, int64_t Hq, int64_t H, int64_t D,
+                                              float sm_scale, int dtype, int fill, void* stream) {
+  using namespace fagq;
+  using namespace fagq::prompt;
+  if ((T > 0 && (!dout || !q || !out || !lse || !dq)) || (Tk > 0 && (!k || !v || !dk || !dv)) ||
+      !cu_seqlens || !strides)
+    return FAGQ_E_NULL;
+  if (dtype != FAGQ_DT_BF16 && dtype != FAGQ_DT_F16) return FAGQ_E_FORMAT;
+  if (fill & ~(FAGQ_FILL_DQ | FAGQ_FILL_DK | FAGQ_FILL_DV)) return FAGQ_E_FORMAT;
+  if (!std::isfinite(sm_scale)) return FAGQ_E_SHAPE;
+  const int sizes = check_bwd_sizes(B, T, Tk, Hq, H, D);
+  if (sizes != FAGQ_OK) return sizes;
+  if (!cu_seqlens_k && T != Tk) return FAGQ_E_SHAPE;
+  const int strided = check_strides(strides, 14);
+  if (strided != FAGQ_OK) return strided;
+  for (const void* p : {dout, q, k, v, out, (const void*)dq, (const void*)dk, (const void*)dv,
+                        (const void*)workspace})
+    if (!aligned(p, 16)) return FAGQ_E_ALIGN;
+  if (!aligned(lse, 4) || !aligned(cu_seqlens, 4) || !aligned(cu_seqlens_k, 4)) return FAGQ_E_ALIGN;
+  const int64_t parts = parts_for(B, T, Tk, Hq, H), need = bytes_for(parts, T, Tk, Hq, H, D);
+  if (workspace_bytes < need) return FAGQ_E_SHAPE;
+  if (need > 0 && !workspace) return FAGQ_E_NULL;
+  if (T == 0 && Tk == 0) return FAGQ_OK;
+  Rows rows[7];
+  const void* const tensors[7] = {dout, q, k, v, dq, dk, dv};
+  for (int i = 0; i < 7; ++i) {
+    const bool kv = i == 2 || i == 3 || i > 4;
+    rows[i] = {tensors[i], kv ? Tk : T, kv ? H : Hq, D, strides[2 * i], strides[2 * i + 1]};
+  }
+  const void* flat[5] = {out, lse, cu_seqlens, cu_seqlens_k, workspace};
+  const int64_t nflat[5] = {T * Hq * D * 2, T * Hq * 4, (B + 1) * 4, cu_seqlens_k ? (B + 1) * 4 : 0, need};
+  for (int i = 4; i < 7; ++i) {
+    if (rows[i].T == 0) continue;
+    if (self_overlap(rows[i])) return FAGQ_E_ALIAS;
+    for (int j = 0; j < i; ++j)
+      if (rows[j].T > 0 && overlap(rows[i], rows[j])) return FAGQ_E_ALIAS;
+    for (int j = 0; j < 5; ++j)
+      if (overlap(rows[i].p, rows[i].bytes(), flat[j], nflat[j])) return FAGQ_E_ALIAS;
+  }
+  for (int j = 0; j < 4; ++j)
+    if (overlap(rows[j].p, rows[j].bytes(), workspace, need) || overlap(flat[j], nflat[j], workspace, need))
+      return FAGQ_E_ALIAS;
+  const int dcheck = device_check();
+  if (dcheck != FAGQ_OK) return dcheck;
+  Args a = {};
+  a.dout = static_cast<const uint16_t*>(dout), a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
+  a.out = static_cast<const uint16_t*>(out), a.lse = lse;
+  const int32_t* cu_k = cu_seqlens_k ? cu_seqlens_k : cu_seqlens;
+  a.queries = {cu_seqlens, cu_k, (int32_t)B, (int32_t)T, (int32_t)Tk};
+  a.keys = {cu_k, cu_seqlens, (int32_t)B, (int32_t)Tk, (int32_t)T};
+  a.dq = static_cast<uint16_t*>(dq), a.dk = static_cast<uint16_t*>(dk), a.dv = static_cast<uint16_t*>(dv);
+  a.lse2 = static_cast<float*>(workspace), a.delta = a.lse2 + Hq * T;
+  a.part = a.lse2 + (2 * Hq * T + 3) / 4 * 4;
+  int64_t(*to[7])[2] = {&a.dos, &a.qs, &a.ks, &a.vs, &a.dqs, &a.dks, &a.dvs};
+  for (int i = 0; i < 7; ++i) (*to[i])[0] = strides[2 * i], (*to[i])[1] = strides[2 * i + 1];
+  a.Hq = (int32_t)Hq, a.H = (int32_t)H, a.group = (int32_t)(Hq / H);
+  a.fill = fill, a.parts = (int32_t)parts;
+  a.scale = sm_scale, a.scale2 = sm_scale * kLog2e;
+  int32_t dim = (int32_t)D;
+  void* args[] = {&a, &dim};
+  const bool bf16 = dtype == FAGQ_DT_BF16;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (T > 0) {
+    const int ls = launch_kernel(bf16 ? dq_for<ET_BF16>(D) : dq_for<ET_F16>(D),
+                                 dim3((unsigned)(tile_slots(T, B) * Hq)), dim3(64 * kWaves), args, 0, st);
+    if (ls != FAGQ_OK) return ls;
+  }
+  if (Tk == 0) return FAGQ_OK;
+  const int ls = launch_kernel(bf16 ? dkdv_for<ET_BF16>(D) : dkdv_for<ET_F16>(D),
+                               dim3((unsigned)(tile_slots(Tk, B) * H * parts)), dim3(64 * kWaves), args, 0, st);
+  if (ls != FAGQ_OK || parts == 1) return ls;
+  const int64_t items = 2 * Tk * H * (D / 8);
+  return launch_kernel(bf16 ? reinterpret_cast<const void*>(&prompt_join<ET_BF16>)
+                            : reinterpret_cast<const void*>(&prompt_join<ET_F16>),
+                       dim3((unsigned)((items + 255) / 256)), dim3(256), args, 0, st);
+}
+
+}  // extern "C"

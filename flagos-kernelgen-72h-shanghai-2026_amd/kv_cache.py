@@ -8,7 +8,7 @@ Layout (contiguous tensors, ``empty_kv_cache`` allocates them):
 A value is ``code * scale``, one scale for each group of G values of a token's head row, in the
 formats of ``fused_add_rmsnorm_group_quant``.  ``kv_cache_write`` quantises keys and values into
 slots (page * page_size + offset), ``kv_cache_read`` gathers the pages of a ragged batch, and
-``paged_attention`` attends over them.  The kernels are libfagq.so's (include/fagq_cache.h);
+``paged_attention`` and, for drafted trees, ``paged_tree_attention`` attend over them.  The kernels are libfagq.so's (include/fagq_cache.h);
 there is no fallback.
 
 No counterpart in the reference repository; the page tables are those that
@@ -195,6 +195,16 @@ def attention_workspace_bytes(B: int, S: int, Hq: int, H: int, D: int, prefix_le
     return n
 
 
+def tree_attention_workspace_bytes(B: int, S: int, Hq: int, H: int, D: int, prefix_len: int,
+                                   max_kv_len: int) -> int:
+    """The same for a ``paged_tree_attention``."""
+    n = _lib.load().fagq_paged_tree_attention_workspace_bytes(B, S, Hq, H, D, prefix_len, max_kv_len)
+    if n < 0:
+        raise ValueError(f"no workspace size for B={B}, S={S}, Hq={Hq}, H={H}, D={D}, "
+                         f"prefix_len={prefix_len}, max_kv_len={max_kv_len}")
+    return n
+
+
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                     k_scale: torch.Tensor, v_scale: torch.Tensor, page_table: torch.Tensor,
                     kv_lens: torch.Tensor, sm_scale: float,
@@ -228,9 +238,38 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         if r != _lib.FAST_ARG_ERROR:
             _lib.check(r, "fagq_paged_attention_launch")
         # An argument the binding leaves to the checks below.
+    return _attention(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, None, sm_scale,
+                      prefix_pages, prefix_len, max_kv_len, out, workspace)
+
+
+def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         k_scale: torch.Tensor, v_scale: torch.Tensor, page_table: torch.Tensor,
+                         kv_lens: torch.Tensor, tree_mask: torch.Tensor, sm_scale: float,
+                         prefix_pages: torch.Tensor | None = None, prefix_len: int = 0,
+                         max_kv_len: int | None = None, out: torch.Tensor | None = None,
+                         workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the S drafted tokens of each of B sequences over the cache: ``paged_attention``
+    for a tree of drafts.  The newest S of a sequence's ``kv_lens[b]`` tokens are its drafts.  Query
+    s sees the shared prefix, all tokens before the drafts, and the drafts t with
+    ``tree_mask[b, s, t]`` (bool or uint8, [B, S, S], or [S, S] for all sequences; contiguous):
+    itself only if the mask says so.  Where a sequence has fewer than S tokens, its first drafts do
+    not exist.  Any mask will do; a query that sees nothing gets zeros.
+
+    S is at most 4096.  The other arguments, and what is returned, as in ``paged_attention``;
+    ``workspace`` has ``tree_attention_workspace_bytes(...)`` bytes.  Asynchronous on the current
+    stream."""
+    if not isinstance(tree_mask, torch.Tensor):
+        raise TypeError(f"tree_mask must be a tensor, got {type(tree_mask).__name__}")
+    return _attention(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, tree_mask, sm_scale,
+                      prefix_pages, prefix_len, max_kv_len, out, workspace)
+
+
+def _attention(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, tree_mask, sm_scale,
+               prefix_pages, prefix_len, max_kv_len, out, workspace):
+    """Either attention from its checks on; tree_mask: None without a tree."""
     P, H, page, D, G, qf, sf = _check_cache(k_cache, v_cache, k_scale, v_scale)
     if v_cache is None:
-        raise ValueError("paged_attention needs a cache of keys and values")
+        raise ValueError("attention needs a cache of keys and values")
     dev = k_cache.device
     if q.dim() != 4 or q.shape[3] != D:
         raise ValueError(f"q must be [B, S, Hq, {D}], got {tuple(q.shape)}")
@@ -250,6 +289,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"page_table must have {B} rows, got {tb}")
     if kv_lens.device != dev or tuple(kv_lens.shape) != (B,) or not kv_lens.is_contiguous():
         raise ValueError(f"kv_lens must be a contiguous tensor of shape ({B},) on {dev}")
+    if tree_mask is not None and (
+            tree_mask.device != dev or tree_mask.dtype not in (torch.bool, torch.uint8)
+            or tuple(tree_mask.shape) not in ((B, S, S), (S, S)) or not tree_mask.is_contiguous()):
+        raise ValueError(f"tree_mask must be a contiguous bool or uint8 tensor of shape ({B}, {S}, {S}) "
+                         f"or ({S}, {S}) on {dev}")
     prefix_len = int(prefix_len)
     if prefix_len < 0:
         raise ValueError(f"prefix_len must not be negative, got {prefix_len}")
@@ -273,7 +317,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         return out
     if P == 0:
         return out.zero_()
-    need = attention_workspace_bytes(B, S, Hq, H, D, prefix_len, most)
+    size = attention_workspace_bytes if tree_mask is None else tree_attention_workspace_bytes
+    need = size(B, S, Hq, H, D, prefix_len, most)
     if workspace is not None:
         check_workspace(workspace, need, dev)
     elif need:
@@ -282,13 +327,18 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     lib = _lib.load()
     with torch.cuda.device(dev):
         stream = torch.cuda.current_stream(dev).cuda_stream
-        st = lib.fagq_paged_attention_launch(
-            _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
-            _ptr(page_table) if width else None, _ptr(kv_lens),
-            _ptr(prefix_pages) if prefix_len else None, _ptr(out),
-            _ptr(workspace) if need else None,
-            workspace.numel() * workspace.element_size() if need else 0,
-            (ctypes.c_int64 * 3)(*strides), B, S, Hq, H, D, P, page, width, prefix_len, most,
-            float(sm_scale), _DTYPES[q.dtype], qf, sf, idx, ctypes.c_void_p(stream))
-    _lib.check(st, "fagq_paged_attention_launch")
+        head = (_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
+                _ptr(page_table) if width else None, _ptr(kv_lens),
+                _ptr(prefix_pages) if prefix_len else None)
+        rest = (_ptr(out), _ptr(workspace) if need else None,
+                workspace.numel() * workspace.element_size() if need else 0,
+                (ctypes.c_int64 * 3)(*strides), B, S, Hq, H, D, P, page, width, prefix_len, most,
+                float(sm_scale), _DTYPES[q.dtype], qf, sf, idx, ctypes.c_void_p(stream))
+        if tree_mask is None:
+            name, st = "fagq_paged_attention_launch", lib.fagq_paged_attention_launch(*head, *rest)
+        else:
+            name = "fagq_paged_tree_attention_launch"
+            st = lib.fagq_paged_tree_attention_launch(*head, _ptr(tree_mask),
+                                                      int(tree_mask.dim() == 2), *rest)
+    _lib.check(st, name)
     return out

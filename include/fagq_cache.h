@@ -107,6 +107,55 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
                                          int dtype, int q_format, int scale_format,
                                          int index_dtype, void* stream);
 
+/* Attention of drafted tokens: as above, but the newest S tokens of a sequence are
+ * the drafts of a tree.  With len = min(kv_lens[b], max_kv_len, the table's room),
+ * query s sees the prefix, the tokens j < len - S, and of the drafts t (token
+ * len - S + t, if that is not negative) those whose byte [s][t] of the mask is not 0;
+ * itself only if its own byte says so.  Any mask will do.
+ * tree_mask: uint8 [B][S][S], or [S][S] for all sequences (shared_mask not 0).
+ * S <= FAGQ_TREE_MAX_S.  The workspace has a size of its own. */
+#define FAGQ_TREE_MAX_S 4096
+FAGQ_API int64_t fagq_paged_tree_attention_workspace_bytes(int64_t B, int64_t S, int64_t Hq,
+                                                           int64_t H, int64_t D,
+                                                           int64_t prefix_len,
+                                                           int64_t max_kv_len);
+FAGQ_API int fagq_paged_tree_attention_launch(
+    const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
+    const void* v_scale, const int32_t* page_table, const void* kv_lens,
+    const int32_t* prefix_pages, const uint8_t* tree_mask, int shared_mask, void* out,
+    void* workspace, int64_t workspace_bytes, const int64_t* strides, int64_t B, int64_t S,
+    int64_t Hq, int64_t H, int64_t D, int64_t num_pages, int64_t page_size, int64_t table_width,
+    int64_t prefix_len, int64_t max_kv_len, float sm_scale, int dtype, int q_format,
+    int scale_format, int index_dtype, void* stream);
+
+/* The index tensors of a step, from the lengths of its B requests: request b has
+ * context_lens[b] tokens in the cache, on the first ceil(context / page_size) pages
+ * of its row of page_table, and new_lens[b] new ones (index_dtype; negative: 0).
+ * The new tokens lie packed, request by request, in `rows` rows; those that do not
+ * fit are not part of the step.  Writes
+ *   cu_seqlens [B + 1]     where each request's rows begin
+ *   kv_lens [B]            context and new tokens
+ *   cu_seqlens_k [B + 1]   their running sums
+ *   page_table             the entries that the new tokens need, from
+ *                          free_pages[free_start] on, request by request; the others
+ *                          are left as they were
+ *   positions, slots [rows]  of each new token in its request and in the cache; -1 in
+ *                          rows behind the last one
+ *   free_end [1]           free_start and the pages taken
+ * Where free_pages (num_free of them) are too few, free_end is larger than num_free,
+ * and the entries and slots that are missing are -1, as are the slots of tokens behind
+ * the table's last page.  free_start: one int32, or null for 0; below 0 it counts as 0.
+ * Numbers past 2^31 - 1 are cut to it.  Pages are what the tensors say: what they lead
+ * to is for the calls that use them to check.
+ * B <= 2^24, num_free, table_width, rows < 2^31. */
+FAGQ_API int fagq_batch_tables_launch(const void* context_lens, const void* new_lens,
+                                      const int32_t* free_pages, const int32_t* free_start,
+                                      int32_t* page_table, int32_t* cu_seqlens,
+                                      int32_t* cu_seqlens_k, int32_t* kv_lens, int32_t* positions,
+                                      int64_t* slots, int32_t* free_end, int64_t B, int64_t rows,
+                                      int64_t num_free, int64_t page_size, int64_t table_width,
+                                      int index_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
