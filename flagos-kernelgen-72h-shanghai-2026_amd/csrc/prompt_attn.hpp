@@ -56,6 +56,8 @@ __device__ __forceinline__ f32x16 splat(float v) {
   return r;
 }
 
+__device__ __forceinline__ int32_t scalar(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // Row of a 32 x 32 result at register r.
 __device__ __forceinline__ int row_of(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
 
@@ -73,27 +75,27 @@ __device__ __forceinline__ float cross_sum(float v) {
 
 // ------------------------------------------------------------------------- tiles in LDS
 
-// A tile of kStep rows of D elements, row by row, in 16-byte chunks; chunk c of row r lies at chunk
+// A tile of ROWS rows of D elements, row by row, in 16-byte chunks; chunk c of row r lies at chunk
 // c ^ swizzle(r) of it.  256 bytes of LDS (16 chunks) are read at once without a conflict: the 16
 // rows of a 16-byte read at one c, and the 4 rows x 4 chunks of a transposed read.
-template <int D>
+template <int D, int ROWS = kStep>
 struct Tile {
   static constexpr int kChunks = D / 8;
   static constexpr int kRowBytes = D * 2;
-  static constexpr int kBytes = kStep * kRowBytes;
+  static constexpr int kBytes = ROWS * kRowBytes;
   static constexpr int kCopyRows = 64 / kChunks;              // rows that one copy brings
-  static constexpr int kCopies = kStep / kCopyRows / kWaves;  // of each wave
+  static constexpr int kCopies = ROWS / kCopyRows / kWaves;  // of each wave
   static __device__ __forceinline__ int swizzle(int r) {
     if constexpr (D == 64) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);   // two rows in 256 bytes
     else return (r & 3) << 2 | ((r >> 2) & 3);
   }
 };
 
-// Copies rows [first, first + kStep) of one head, row `last` in place of those behind it, from HBM
+// Copies rows [first, first + ROWS) of one head, row `last` in place of those behind it, from HBM
 // into LDS, past the registers.  Copy n of wave w brings rows (4 n + w) kCopyRows ..
-template <int D>
+template <int D, int ROWS = kStep>
 struct Copier {
-  using L = Tile<D>;
+  using L = Tile<D, ROWS>;
   const char* base;            // row 0 of the sequence
   uint32_t stride;             // bytes of a row
   int row;                     // within the copies of this wave, of this lane
@@ -109,7 +111,7 @@ struct Copier {
   }
   __device__ __forceinline__ void issue(char* lds, int wave, int first, int last) const {
     const rsrc_t rs = make_rsrc(base + (int64_t)first * stride, 0x7fffffffu);
-    if (first + kStep - 1 <= last) {
+    if (first + ROWS - 1 <= last) {
       const uint32_t off = (uint32_t)row * stride;
 #pragma unroll
       for (int n = 0; n < L::kCopies; ++n)
@@ -163,6 +165,16 @@ __device__ __forceinline__ u32x4 pack8(const f32x16& x, int t) {
   return r;
 }
 
+// What packing lost of them, packed: a product with both terms has twice the bits.
+template <int E>
+__device__ __forceinline__ u32x4 pack_rest8(const f32x16& x, int t, const u32x4& w) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = pack16<E>(x[8 * t + 2 * i] - lo16<E>(w[i]), x[8 * t + 2 * i + 1] - hi16<E>(w[i]));
+  return r;
+}
+
 // A row in global memory as row operands: places 16 i + 8 h ..
 template <int D>
 __device__ __forceinline__ void load_row(const uint16_t* row, int h, u32x4 (&f)[D / 16]) {
@@ -213,7 +225,6 @@ struct Place {
 __device__ __forceinline__ int32_t clamped(int32_t v, int32_t most) {
   return v < 0 ? 0 : v < most ? v : most;
 }
-__device__ __forceinline__ int32_t scalar(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Tile number `slot` of all sequences': from the last one backwards (REVERSED), where late tiles
 // see most, or from the first on.  Lane l counts the tiles of sequences l n .. (l + 1) n - 1.

@@ -142,21 +142,28 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_dq(Args a) {
       for (int r = 0; r < 16; ++r) x[r] *= y[r];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const u32x4 w = pack8<E>(x, u);
+        const u32x4 w = pack8<E>(x, u), rest = pack_rest8<E>(x, u, w);
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-          dq[d] = mfma<E>(col_frag<D>(lds[buf][0], lane, d, 2 * t + u), w, dq[d]);
+        for (int d = 0; d < D / 32; ++d) {
+          const u32x4 k = col_frag<D>(lds[buf][0], lane, d, 2 * t + u);
+          dq[d] = mfma<E>(k, w, dq[d]);
+          dq[d] = mfma<E>(k, rest, dq[d]);
+        }
       }
     }
   }
   store_row<E, D>(a.dq + (int64_t)row * a.dqs[0] + (int64_t)hq * a.dqs[1], h, dq, a.scale, i < p.n);
 }
 
-template <int E, int D>
+template <int E, int D, bool TWO>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_dkdv(Args a) {
-  using L = Tile<D>;
+  constexpr int kQueries = D == 128 ? 32 : 64;            // in LDS at a time
+  using L = Tile<D, kQueries>;
+  using V = Tile<D, kTile>;
+  constexpr bool kVInLds = D <= 128;
   __shared__ __align__(16) char lds[2][2][L::kBytes];
-  __shared__ __align__(16) float stats[2][2][kStep];      // lse2, -delta
+  __shared__ __align__(16) char lds_v[kVInLds ? V::kBytes : 16];
+  __shared__ __align__(16) float stats[2][2][kQueries];   // lse2, -delta
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int wave = scalar((int)(threadIdx.x >> 6));
   const int item = (int)blockIdx.x, kvh = item % a.H, rest = item / a.H;
@@ -169,26 +176,25 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_dkdv(Arg
   }
   // n keys, m queries; query i sees the keys up to i + ahead.
   const int32_t ahead = p.n - p.m, k0 = p.tile * kTile, mine = k0 + wave * kRows;
-  const int32_t j0 = mine + c, row = p.row + (j0 < p.n ? j0 : p.n - 1);
+  const int32_t j0 = mine + c;
   const int32_t first = k0 > ahead ? k0 - ahead : 0;       // query that sees one of the tile's keys
-  const int32_t steps = first < p.m ? (p.m - first + kStep - 1) / kStep : 0;
+  const int32_t steps = first < p.m ? (p.m - first + kQueries - 1) / kQueries : 0;
   // Steps of all heads in a row, head by head: this part's share.
   const int64_t total = (int64_t)steps * a.group;
   const int32_t from = (int32_t)(total * part / a.parts), to = (int32_t)(total * (part + 1) / a.parts);
 
-  Copier<D> cq, cg;
+  Copier<D, kQueries> cq, cg;
   cq.init(a.q, (int64_t)p.other * a.qs[0] + (int64_t)kvh * a.group * a.qs[1], a.qs[0], lane, wave);
   cg.init(a.dout, (int64_t)p.other * a.dos[0] + (int64_t)kvh * a.group * a.dos[1], a.dos[0], lane, wave);
   int32_t head = steps > 0 ? from / steps : 0, step = from - head * steps;
-  // The next step's rows.
   auto issue = [&](int buf, int32_t head, int32_t step) {
-    const int32_t i0 = first + step * kStep;
-    Copier<D> x = cq, y = cg;
+    const int32_t i0 = first + step * kQueries;
+    Copier<D, kQueries> x = cq, y = cg;
     x.base += (int64_t)head * a.qs[1] * 2;
     y.base += (int64_t)head * a.dos[1] * 2;
     x.issue(lds[buf][0], wave, i0, p.m - 1);
     y.issue(lds[buf][1], wave, i0, p.m - 1);
-    if (wave < 2) {
+    if (wave < 2 && lane < kQueries) {
       const int64_t at = (int64_t)(kvh * a.group + head) * a.keys.Tother + p.other + i0;
       const int32_t most = p.m - 1 - i0;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -198,73 +204,99 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_dkdv(Arg
     }
   };
   if (from < to) issue(0, head, step);
-  u32x4 k[D / 16], v[D / 16];
-  load_row<D>(a.k + (int64_t)row * a.ks[0] + (int64_t)kvh * a.ks[1], h, k);
-  load_row<D>(a.v + (int64_t)row * a.vs[0] + (int64_t)kvh * a.vs[1], h, v);
+  u32x4 k[D / 16], v[kVInLds ? 1 : D / 16];
+  {
+    const int64_t row = p.row + (j0 < p.n ? j0 : p.n - 1);
+    load_row<D>(a.k + row * a.ks[0] + (int64_t)kvh * a.ks[1], h, k);
+    if constexpr (!kVInLds) load_row<D>(a.v + row * a.vs[0] + (int64_t)kvh * a.vs[1], h, v);
+  }
+  if constexpr (kVInLds) {
+    Copier<D, kTile> cv;
+    cv.init(a.v, (int64_t)p.row * a.vs[0] + (int64_t)kvh * a.vs[1], a.vs[0], lane, wave);
+    cv.issue(lds_v, wave, k0, p.n - 1);
+  }
+  const char* tv = lds_v + wave * kRows * V::kRowBytes;
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) dk[d] = dv[d] = splat(0.0f);
 
   int buf = 0;
   for (int32_t it = from; it < to; ++it, buf ^= 1) {
-    const int32_t i0 = first + step * kStep;
+    const int32_t i0 = first + step * kQueries;
     __builtin_amdgcn_s_waitcnt(kVmcnt0);         // this step's tiles have landed, of this wave
     lds_barrier();                               // of all; the last step's are done with
     if (++step == steps) step = 0, ++head;
     if (it + 1 < to) issue(buf ^ 1, head, step);
     if (mine >= p.n) continue;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int32_t first_query = i0 + 32 * t;
-      if (first_query >= p.m || first_query + 31 + ahead < mine) continue;
+#pragma unroll 1
+    for (int t = 0; t < kQueries / 32; ++t) {
+      const int32_t query = i0 + 32 * t;
+      if (query >= p.m || query + 31 + ahead < mine) continue;
+      const char* tq = lds[buf][0] + t * 32 * L::kRowBytes;
+      const char* tg = lds[buf][1] + t * 32 * L::kRowBytes;
       f32x16 x = splat(0.0f), y;
-      float lse2[16];
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) x = mfma<E>(row_frag<D>(tq, lane, 0, j), k[j], x);
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
-        const f32x4 s = *reinterpret_cast<const f32x4*>(&stats[buf][0][32 * t + row_of(r, h)]);
-        const f32x4 d = *reinterpret_cast<const f32x4*>(&stats[buf][1][32 * t + row_of(r, h)]);
+        const f32x4 s = *reinterpret_cast<const f32x4*>(&stats[buf][1][32 * t + row_of(r, h)]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) lse2[r + e] = s[e], y[r + e] = d[e];
+        for (int e = 0; e < 4; ++e) y[r + e] = s[e];
       }
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) {
-        x = mfma<E>(row_frag<D>(lds[buf][0], lane, t, j), k[j], x);
-        y = mfma<E>(row_frag<D>(lds[buf][1], lane, t, j), v[j], y);
+        if constexpr (kVInLds) y = mfma<E>(row_frag<D>(tg, lane, 0, j), row_frag<D>(tv, lane, 0, j), y);
+        else y = mfma<E>(row_frag<D>(tg, lane, 0, j), v[j], y);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -lse2[r]));
-      if (first_query + 32 > p.m || first_query + ahead < mine + kRows - 1) {
+      for (int r = 0; r < 16; r += 4) {
+        const f32x4 s = *reinterpret_cast<const f32x4*>(&stats[buf][0][32 * t + row_of(r, h)]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r + e], a.scale2, -s[e]));
+      }
+      if (query + 32 > p.m || query + ahead < mine + kRows - 1) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int32_t i = first_query + row_of(r, h);
+          const int32_t i = query + row_of(r, h);
           x[r] = i < p.m && j0 <= i + ahead ? x[r] : 0.0f;
         }
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const u32x4 w = pack8<E>(x, u);
+        u32x4 rest;
+        if constexpr (TWO) rest = pack_rest8<E>(x, u, w);
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-          dv[d] = mfma<E>(col_frag<D>(lds[buf][1], lane, d, 2 * t + u), w, dv[d]);
+        for (int d = 0; d < D / 32; ++d) {
+          const u32x4 g = col_frag<D>(tg, lane, d, u);
+          dv[d] = mfma<E>(g, w, dv[d]);
+          if constexpr (TWO) dv[d] = mfma<E>(g, rest, dv[d]);
+        }
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] *= y[r];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const u32x4 w = pack8<E>(x, u);
+        u32x4 rest;
+        if constexpr (TWO) rest = pack_rest8<E>(x, u, w);
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-          dk[d] = mfma<E>(col_frag<D>(lds[buf][0], lane, d, 2 * t + u), w, dk[d]);
+        for (int d = 0; d < D / 32; ++d) {
+          const u32x4 q = col_frag<D>(tq, lane, d, u);
+          dk[d] = mfma<E>(q, w, dk[d]);
+          if constexpr (TWO) dk[d] = mfma<E>(q, rest, dk[d]);
+        }
       }
     }
   }
+  const int64_t row = p.row + j0;
   if (a.parts == 1) {
-    store_row<E, D>(a.dk + (int64_t)row * a.dks[0] + (int64_t)kvh * a.dks[1], h, dk, a.scale, j0 < p.n);
-    store_row<E, D>(a.dv + (int64_t)row * a.dvs[0] + (int64_t)kvh * a.dvs[1], h, dv, 1.0f, j0 < p.n);
+    store_row<E, D>(a.dk + row * a.dks[0] + (int64_t)kvh * a.dks[1], h, dk, a.scale, j0 < p.n);
+    store_row<E, D>(a.dv + row * a.dvs[0] + (int64_t)kvh * a.dvs[1], h, dv, 1.0f, j0 < p.n);
   } else if (j0 < p.n) {
     const int64_t plane = (int64_t)a.keys.T * a.H * D;
-    float* to_k = a.part + part * plane + ((int64_t)row * a.H + kvh) * D;
+    float* to_k = a.part + part * plane + (row * a.H + kvh) * D;
     float* to_v = to_k + a.parts * plane;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
@@ -317,12 +349,19 @@ int check_bwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int
   return large ? FAGQ_E_TOO_LARGE : FAGQ_OK;
 }
 
-// Parts of a key tile's steps, so that there are several workgroups for each place.
-int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H) {
+// Parts of a key tile's steps: two workgroups for each place that the GPU has (tiles with few queries
+// then fill what the first ones leave), but four steps for each.
+int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
   const int64_t groups = std::max<int64_t>(1, (Tk + kTile - 1) / kTile * H);
-  const int64_t steps = Hq / H * ((T + kStep - 1) / kStep);
-  return std::max<int64_t>(1, std::min<int64_t>({(3 * kSlots + groups - 1) / groups, steps / 4, kMostParts}));
+  const int64_t slots = D == 256 ? kSlots / 2 : kSlots;
+  const int64_t steps = Hq / H * ((T + kStep - 1) / kStep) / std::max<int64_t>(1, B);
+  return std::max<int64_t>(1, std::min<int64_t>({(2 * slots + groups - 1) / groups, steps / 4, kMostParts}));
 }
+
+// Whether dk and dv take two terms (of 16 bits each) of P and dS, as dq always does.  One leaves them
+// 1.4 times the error that their own rounding makes, as long as there are many roundings to average
+// over; a call of few rows has few, and costs the same either way.
+bool two_terms(int64_t T, int64_t Hq) { return T * Hq <= 4096; }
 
 int64_t bytes_for(int64_t parts, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
   const int64_t stats = (2 * Hq * T * 4 + 15) / 16 * 16;
@@ -335,11 +374,11 @@ const void* dq_for(int64_t D) {
          : D == 128 ? reinterpret_cast<const void*>(&prompt_dq<E, 128>)
                     : reinterpret_cast<const void*>(&prompt_dq<E, 256>);
 }
-template <int E>
+template <int E, bool TWO>
 const void* dkdv_for(int64_t D) {
-  return D == 64    ? reinterpret_cast<const void*>(&prompt_dkdv<E, 64>)
-         : D == 128 ? reinterpret_cast<const void*>(&prompt_dkdv<E, 128>)
-                    : reinterpret_cast<const void*>(&prompt_dkdv<E, 256>);
+  return D == 64    ? reinterpret_cast<const void*>(&prompt_dkdv<E, 64, TWO>)
+         : D == 128 ? reinterpret_cast<const void*>(&prompt_dkdv<E, 128, TWO>)
+                    : reinterpret_cast<const void*>(&prompt_dkdv<E, 256, TWO>);
 }
 
 }  // namespace
@@ -352,7 +391,7 @@ FAGQ_API int64_t fagq_prompt_attention_bwd_workspace_bytes(int64_t B, int64_t T,
                                                            int64_t Hq, int64_t H, int64_t D) {
   using namespace fagq::prompt;
   if (check_bwd_sizes(B, T, Tk, Hq, H, D) != FAGQ_OK) return -1;
-  return bytes_for(parts_for(B, T, Tk, Hq, H), T, Tk, Hq, H, D);
+  return bytes_for(parts_for(B, T, Tk, Hq, H, D), T, Tk, Hq, H, D);
 }
 
 FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, const void* k,
@@ -380,7 +419,7 @@ FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, c
                         (const void*)workspace})
     if (!aligned(p, 16)) return FAGQ_E_ALIGN;
   if (!aligned(lse, 4) || !aligned(cu_seqlens, 4) || !aligned(cu_seqlens_k, 4)) return FAGQ_E_ALIGN;
-  const int64_t parts = parts_for(B, T, Tk, Hq, H), need = bytes_for(parts, T, Tk, Hq, H, D);
+  const int64_t parts = parts_for(B, T, Tk, Hq, H, D), need = bytes_for(parts, T, Tk, Hq, H, D);
   if (workspace_bytes < need) return FAGQ_E_SHAPE;
   if (need > 0 && !workspace) return FAGQ_E_NULL;
   if (T == 0 && Tk == 0) return FAGQ_OK;
@@ -430,7 +469,8 @@ FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, c
     if (ls != FAGQ_OK) return ls;
   }
   if (Tk == 0) return FAGQ_OK;
-  const int ls = launch_kernel(bf16 ? dkdv_for<ET_BF16>(D) : dkdv_for<ET_F16>(D),
+  const int ls = launch_kernel(two_terms(T, Hq) ? (bf16 ? dkdv_for<ET_BF16, true>(D) : dkdv_for<ET_F16, true>(D))
+                                                : (bf16 ? dkdv_for<ET_BF16, false>(D) : dkdv_for<ET_F16, false>(D)),
                                dim3((unsigned)(tile_slots(Tk, B) * H * parts)), dim3(64 * kWaves), args, 0, st);
   if (ls != FAGQ_OK || parts == 1) return ls;
   const int64_t items = 2 * Tk * H * (D / 8);
