@@ -198,6 +198,14 @@ def fast_launch():
                                            lib.fagq_kv_cache_read_launch,
                                            lib.fagq_paged_attention_workspace_bytes,
                                            lib.fagq_paged_attention_launch)])
+                _fagq_py.bind_prompts(*[ctypes.cast(fn, ctypes.c_void_p).value for fn in
+                                        (lib.fagq_paged_tree_attention_workspace_bytes,
+                                         lib.fagq_paged_tree_attention_launch,
+                                         lib.fagq_batch_tables_launch,
+                                         lib.fagq_prompt_attention_workspace_bytes,
+                                         lib.fagq_prompt_attention_launch,
+                                         lib.fagq_prompt_attention_bwd_workspace_bytes,
+                                         lib.fagq_prompt_attention_bwd_launch)])
                 _fast = _fagq_py.launch
                 _fast_mod = _fagq_py
             except (ImportError, AttributeError):

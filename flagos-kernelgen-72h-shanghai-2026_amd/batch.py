@@ -43,6 +43,15 @@ def batch_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, free_pages:
     free_pages runs out, ``free_end`` is larger than F, and the missing entries and slots are -1,
     as are slots past the table's width.  page_table's other entries are left as they were: a call
     with the same lengths gives the same results again.  Asynchronous on the current stream."""
+    mod, fast_stream = _lib.fast_module(page_table)
+    if mod is not None:
+        r = mod.tables(context_lens, new_lens, free_pages, page_table, page_size, num_tokens, free_start,
+                       fast_stream)
+        if type(r) is not int:
+            return r
+        if r != _lib.FAST_ARG_ERROR:
+            _lib.check(r, "fagq_batch_tables_launch")
+        # An argument the binding leaves to the checks below.
     dev = page_table.device
     if dev.type != "cuda":
         raise ValueError("page_table must be a GPU (HIP) tensor; this operator has no CPU path")

@@ -21,8 +21,9 @@
 //     (dsa and mla: 0), the library's status as an int where it is an error, or
 //     kArgError for any argument that the Python layer should look at: it then takes
 //     the call from the start, with the same results and its own wording of the errors.
-//   rope(...), rope_bwd(...), cache_write(...), cache_read(...), attention(...): the
-//     attention side, by the same rules.
+//   rope(...), rope_bwd(...), cache_write(...), cache_read(...), attention(...),
+//     tree_attention(...), tables(...), prompt(...), prompt_bwd(...): the attention side, by the
+//     same rules.
 //     Nothing is allocated or launched before all arguments are accepted.  The
 //     allocations (which may reach hipMalloc, or wait for the device to free cached
 //     blocks) and the launch run without the GIL, as torch's and ctypes' own calls do.
@@ -44,6 +45,7 @@
 #include "fagq_dsa.h"
 #include "fagq_gemm.h"
 #include "fagq_mla.h"
+#include "fagq_prompt.h"
 #include "fagq_rope.h"
 
 namespace {
@@ -69,6 +71,13 @@ decltype(&fagq_kv_cache_write_launch) g_cache_write = nullptr;
 decltype(&fagq_kv_cache_read_launch) g_cache_read = nullptr;
 decltype(&fagq_paged_attention_workspace_bytes) g_attention_bytes = nullptr;
 decltype(&fagq_paged_attention_launch) g_attention = nullptr;
+decltype(&fagq_paged_tree_attention_workspace_bytes) g_tree_bytes = nullptr;
+decltype(&fagq_paged_tree_attention_launch) g_tree = nullptr;
+decltype(&fagq_batch_tables_launch) g_tables = nullptr;
+decltype(&fagq_prompt_attention_workspace_bytes) g_prompt_bytes = nullptr;
+decltype(&fagq_prompt_attention_launch) g_prompt = nullptr;
+decltype(&fagq_prompt_attention_bwd_workspace_bytes) g_prompt_bwd_bytes = nullptr;
+decltype(&fagq_prompt_attention_bwd_launch) g_prompt_bwd = nullptr;
 
 bool is_tensor(PyObject* o) { return THPVariable_Check(o); }
 
@@ -783,18 +792,14 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 // attention(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, sm_scale,
 //           prefix_pages or None, prefix_len, max_kv_len or None, out or None, stream) -> out;
-// the workspace is allocated here.
-PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  HANDLE_TH_ERRORS
-  if (nargs != 13) {
-    PyErr_SetString(PyExc_TypeError, "attention() takes 13 arguments");
-    return nullptr;
-  }
+// the workspace is allocated here.  `mask`: tree_attention's, null for attention.
+PyObject* attend(PyObject* const* args, PyObject* mask) {
   Cache c;
   void* stream;
   double scale;
   long long prefix_len, most = 0;
-  if (!g_attention || !g_attention_bytes || !stream_arg(args[12], &stream) || !is_plain(args[0]) ||
+  const bool tree = mask != nullptr;
+  if (!(tree ? g_tree && g_tree_bytes : g_attention && g_attention_bytes) || !stream_arg(args[12], &stream) || !is_plain(args[0]) ||
       !is_plain(args[5]) || !is_plain(args[6]) || !float_arg(args[7], &scale) ||
       !int_arg(args[9], 0, 1 << 30, &prefix_len) ||
       (args[10] != Py_None && !int_arg(args[10], 0, INT64_MAX, &most)) ||
@@ -812,6 +817,18 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       !q.is_cuda() || q.get_device() != c.dev || !rows_ok(table, ts, c.dev, at::kInt) ||
       !rows_ok(lens, ls, c.dev, lens.scalar_type()))
     return arg_error();
+  const uint8_t* seen = nullptr;
+  bool shared = false;
+  if (tree) {
+    if (!is_plain(mask)) return arg_error();
+    const at::Tensor& t = THPVariable_Unpack(mask);
+    const int64_t each[3] = {B, S, S};
+    shared = t.dim() == 2;
+    if ((t.scalar_type() != at::kBool && t.scalar_type() != at::kByte) ||
+        !rows_ok(t, at::IntArrayRef(each + shared, 3 - shared), c.dev, t.scalar_type()))
+      return arg_error();
+    seen = static_cast<const uint8_t*>(t.data_ptr());
+  }
   const int32_t* prefix = nullptr;
   if (prefix_len > 0) {
     if (!is_plain(args[8])) return arg_error();
@@ -829,7 +846,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     out = THPVariable_Unpack(args[11]);
     if (!rows_ok(out, q.sizes(), c.dev, type)) return arg_error();
   }
-  const int64_t need = g_attention_bytes(B, S, Hq, c.H, c.D, prefix_len, most);
+  const int64_t need = (tree ? g_tree_bytes : g_attention_bytes)(B, S, Hq, c.H, c.D, prefix_len, most);
   if (need < 0) return arg_error();
   int64_t strides[3];
   for (int i = 0; i < 3; ++i) strides[i] = q.size(i) > 1 ? q.stride(i) : 0;
@@ -843,13 +860,235 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!out.defined()) out = at::empty(os, options);
     at::Tensor ws;
     if (need > 0) ws = at::empty({need}, options.dtype(at::kByte));
-    st = g_attention(p[0], p[1], p[2], p[3], p[4], static_cast<const int32_t*>(p[5]), p[6], prefix,
-                     out.data_ptr(), need > 0 ? ws.data_ptr() : nullptr, need, strides, B, S, Hq,
-                     c.H, c.D, c.P, c.page, width, prefix_len, most, (float)scale, dtype, c.codes,
-                     c.scales, index, stream);
+    void* const w = need > 0 ? ws.data_ptr() : nullptr;
+    const auto* pages = static_cast<const int32_t*>(p[5]);
+    st = tree ? g_tree(p[0], p[1], p[2], p[3], p[4], pages, p[6], prefix, seen, shared, out.data_ptr(), w,
+                       need, strides, B, S, Hq, c.H, c.D, c.P, c.page, width, prefix_len, most,
+                       (float)scale, dtype, c.codes, c.scales, index, stream)
+              : g_attention(p[0], p[1], p[2], p[3], p[4], pages, p[6], prefix, out.data_ptr(), w, need,
+                            strides, B, S, Hq, c.H, c.D, c.P, c.page, width, prefix_len, most,
+                            (float)scale, dtype, c.codes, c.scales, index, stream);
   }
   if (st != FAGQ_OK) return PyLong_FromLong(st);
   return THPVariable_Wrap(out);
+}
+
+PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 13) {
+    PyErr_SetString(PyExc_TypeError, "attention() takes 13 arguments");
+    return nullptr;
+  }
+  return attend(args, nullptr);
+  END_HANDLE_TH_ERRORS
+}
+
+// tree_attention(attention's arguments, tree_mask) -> out
+PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 14) {
+    PyErr_SetString(PyExc_TypeError, "tree_attention() takes 14 arguments");
+    return nullptr;
+  }
+  return attend(args, args[13]);
+  END_HANDLE_TH_ERRORS
+}
+
+// tables(context_lens, new_lens, free_pages, page_table, page_size, num_tokens, free_start or None,
+//        stream) -> (cu_seqlens, cu_seqlens_k, kv_lens, positions, slots, free_end)
+PyObject* tables(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 8) {
+    PyErr_SetString(PyExc_TypeError, "tables() takes 8 arguments");
+    return nullptr;
+  }
+  long long page, rows;
+  void* stream;
+  if (!g_tables || !stream_arg(args[7], &stream) || !int_arg(args[4], 1, INT64_MAX, &page) ||
+      !int_arg(args[5], 0, INT64_MAX, &rows))
+    return arg_error();
+  for (int i = 0; i < 4; ++i)
+    if (!is_plain(args[i])) return arg_error();
+  const at::Tensor &context = THPVariable_Unpack(args[0]), &fresh = THPVariable_Unpack(args[1]);
+  const at::Tensor &free = THPVariable_Unpack(args[2]), &table = THPVariable_Unpack(args[3]);
+  if (table.dim() != 2 || free.dim() != 1 || !table.is_cuda() || page < FAGQ_CACHE_MIN_PAGE ||
+      page > FAGQ_CACHE_MAX_PAGE || (page & (page - 1)) || rows > (1ll << 31) - 1)
+    return arg_error();
+  const c10::DeviceIndex dev = table.get_device();
+  const int64_t B = table.size(0), width = table.size(1), bs[1] = {B};
+  const at::ScalarType type = context.scalar_type();
+  const int index = index_code(type);
+  if (index < 0 || !rows_ok(context, bs, dev, type) || !rows_ok(fresh, bs, dev, type) ||
+      !rows_ok(free, free.sizes(), dev, at::kInt) || !rows_ok(table, table.sizes(), dev, at::kInt))
+    return arg_error();
+  const int32_t* start = nullptr;
+  if (args[6] != Py_None) {
+    if (!is_plain(args[6])) return arg_error();
+    const at::Tensor& t = THPVariable_Unpack(args[6]);
+    const int64_t one[1] = {1};
+    if (!rows_ok(t, one, dev, at::kInt)) return arg_error();
+    start = t.data_ptr<int32_t>();
+  }
+  const void* p[4] = {context.data_ptr(), fresh.data_ptr(), free.data_ptr(), table.data_ptr()};
+  const auto i32 = table.options();
+  at::Tensor out[6];
+  int st;
+  {
+    NoGil no_gil;
+    const int64_t sizes[6] = {B + 1, B + 1, B, rows, rows, 1};
+    for (int i = 0; i < 6; ++i) out[i] = at::empty({sizes[i]}, i == 4 ? i32.dtype(at::kLong) : i32);
+    int32_t* o[6];
+    for (int i = 0; i < 6; ++i) o[i] = static_cast<int32_t*>(out[i].data_ptr());
+    st = g_tables(p[0], p[1], static_cast<const int32_t*>(p[2]), start,
+                  static_cast<int32_t*>(const_cast<void*>(p[3])), o[0], o[1], o[2], o[3],
+                  static_cast<int64_t*>(out[4].data_ptr()), o[5], B, rows, free.size(0), page, width,
+                  index, stream);
+  }
+  if (st != FAGQ_OK) return PyLong_FromLong(st);
+  return tuple_of(out, 6);
+  END_HANDLE_TH_ERRORS
+}
+
+// What both directions of the prompts' attention take: q, k, v, cu_seqlens, cu_seqlens_k or None,
+// sm_scale.
+struct PromptIn {
+  const at::Tensor* t[4];     // q, k, v, cu_seqlens
+  const int32_t* cu_k;
+  int64_t B, T, Tk, Hq, H, D;
+  int64_t strides[6];         // q, k, v
+  double scale;
+  int dtype;
+  c10::DeviceIndex dev;
+};
+bool prompt_in(PyObject* const* args, PromptIn* r) {
+  for (int i = 0; i < 4; ++i) {
+    if (!is_plain(args[i])) return false;
+    r->t[i] = &THPVariable_Unpack(args[i]);
+  }
+  const at::Tensor &q = *r->t[0], &k = *r->t[1], &cu = *r->t[3];
+  if (!float_arg(args[5], &r->scale) || q.dim() != 3 || k.dim() != 3 || cu.dim() != 1 || !q.is_cuda())
+    return false;
+  const at::ScalarType st = q.scalar_type();
+  r->dtype = st == at::kBFloat16 ? FAGQ_DT_BF16 : st == at::kHalf ? FAGQ_DT_F16 : -1;
+  r->dev = q.get_device();
+  r->T = q.size(0), r->Hq = q.size(1), r->D = q.size(2), r->Tk = k.size(0), r->H = k.size(1);
+  r->B = cu.size(0) - 1;
+  const int64_t qs[3] = {r->T, r->Hq, r->D}, ks[3] = {r->Tk, r->H, r->D}, cs[1] = {r->B + 1};
+  if (r->dtype < 0 || r->B < 0 || r->T < 1 || r->Tk < 1 || r->H < 1 || r->Hq < 1 || r->Hq % r->H != 0 ||
+      (r->D != 64 && r->D != 128 && r->D != 256) || !heads_ok(q, qs, r->dev, st, r->strides) ||
+      !heads_ok(k, ks, r->dev, st, r->strides + 2) ||
+      !heads_ok(*r->t[2], ks, r->dev, st, r->strides + 4) || !rows_ok(cu, cs, r->dev, at::kInt))
+    return false;
+  r->cu_k = nullptr;
+  if (args[4] == Py_None) return r->T == r->Tk;
+  if (!is_plain(args[4])) return false;
+  const at::Tensor& cu_k = THPVariable_Unpack(args[4]);
+  if (!rows_ok(cu_k, cs, r->dev, at::kInt)) return false;
+  r->cu_k = cu_k.data_ptr<int32_t>();
+  return true;
+}
+
+// prompt(q, k, v, cu_seqlens, cu_seqlens_k or None, sm_scale, return_lse, out or None, stream)
+// -> out or (out, lse); the workspace is allocated here.
+PyObject* prompt(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 9) {
+    PyErr_SetString(PyExc_TypeError, "prompt() takes 9 arguments");
+    return nullptr;
+  }
+  PromptIn r;
+  void* stream;
+  int with_lse;
+  if (!g_prompt || !g_prompt_bytes || !stream_arg(args[8], &stream) || !bool_arg(args[6], &with_lse) ||
+      !prompt_in(args, &r))
+    return arg_error();
+  const at::Tensor& q = *r.t[0];
+  const int64_t os[3] = {r.T, r.Hq, r.D};
+  at::Tensor out[2];
+  int fill = FAGQ_FILL_LSE;
+  if (args[7] == Py_None) {
+    fill |= FAGQ_FILL_OUT;
+  } else {
+    if (!is_plain(args[7])) return arg_error();
+    out[0] = THPVariable_Unpack(args[7]);
+    if (!rows_ok(out[0], os, r.dev, q.scalar_type())) return arg_error();
+  }
+  const int64_t need = g_prompt_bytes(r.B, r.T, r.Tk, r.Hq, r.H, r.D);
+  if (need < 0) return arg_error();
+  const void* p[4];
+  for (int i = 0; i < 4; ++i) p[i] = r.t[i]->data_ptr();
+  const auto options = q.options();
+  int st;
+  {
+    NoGil no_gil;
+    if (!out[0].defined()) out[0] = at::empty(os, options);
+    if (with_lse) out[1] = at::empty({r.Hq, r.T}, options.dtype(at::kFloat));
+    at::Tensor ws;
+    if (need > 0) ws = at::empty({need}, options.dtype(at::kByte));
+    st = g_prompt(p[0], p[1], p[2], static_cast<const int32_t*>(p[3]), r.cu_k, out[0].data_ptr(),
+                  with_lse ? out[1].data_ptr<float>() : nullptr, need > 0 ? ws.data_ptr() : nullptr,
+                  need, r.strides, r.B, r.T, r.Tk, r.Hq, r.H, r.D, (float)r.scale, r.dtype, fill, stream);
+  }
+  if (st != FAGQ_OK) return PyLong_FromLong(st);
+  return with_lse ? tuple_of(out, 2) : THPVariable_Wrap(out[0]);
+  END_HANDLE_TH_ERRORS
+}
+
+// prompt_bwd(q, k, v, cu_seqlens, cu_seqlens_k or None, sm_scale, dout, out, lse, dq or None,
+//            dk or None, dv or None, stream) -> (dq, dk, dv); the workspace is allocated here.
+PyObject* prompt_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 13) {
+    PyErr_SetString(PyExc_TypeError, "prompt_bwd() takes 13 arguments");
+    return nullptr;
+  }
+  PromptIn r;
+  void* stream;
+  if (!g_prompt_bwd || !g_prompt_bwd_bytes || !stream_arg(args[12], &stream) || !is_plain(args[6]) ||
+      !is_plain(args[7]) || !is_plain(args[8]) || !prompt_in(args, &r))
+    return arg_error();
+  const at::ScalarType type = r.t[0]->scalar_type();
+  const at::Tensor &dout = THPVariable_Unpack(args[6]), &out = THPVariable_Unpack(args[7]);
+  const at::Tensor& lse = THPVariable_Unpack(args[8]);
+  const int64_t qs[3] = {r.T, r.Hq, r.D}, ks[3] = {r.Tk, r.H, r.D}, ls[2] = {r.Hq, r.T};
+  int64_t strides[14];
+  std::copy(r.strides, r.strides + 6, strides + 2);
+  if (!heads_ok(dout, qs, r.dev, type, strides) || !rows_ok(out, qs, r.dev, type) ||
+      !rows_ok(lse, ls, r.dev, at::kFloat))
+    return arg_error();
+  at::Tensor grad[3];
+  int fill = 0;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t H = i ? r.H : r.Hq;
+    strides[8 + 2 * i] = H * r.D, strides[9 + 2 * i] = r.D;
+    if (args[9 + i] == Py_None) {
+      fill |= i == 0 ? FAGQ_FILL_DQ : i == 1 ? FAGQ_FILL_DK : FAGQ_FILL_DV;
+      continue;
+    }
+    if (!is_plain(args[9 + i])) return arg_error();
+    grad[i] = THPVariable_Unpack(args[9 + i]);
+    if (!heads_ok(grad[i], i ? ks : qs, r.dev, type, strides + 8 + 2 * i)) return arg_error();
+  }
+  const int64_t need = g_prompt_bwd_bytes(r.B, r.T, r.Tk, r.Hq, r.H, r.D);
+  if (need < 0) return arg_error();
+  const void* p[6];
+  for (int i = 0; i < 4; ++i) p[i] = r.t[i]->data_ptr();
+  p[4] = dout.data_ptr(), p[5] = out.data_ptr();
+  const float* l = lse.data_ptr<float>();
+  const auto options = r.t[0]->options();
+  int st;
+  {
+    NoGil no_gil;
+    for (int i = 0; i < 3; ++i)
+      if (!grad[i].defined()) grad[i] = at::empty(i ? ks : qs, options);
+    const at::Tensor ws = at::empty({std::max<int64_t>(need, 16)}, options.dtype(at::kByte));
+    st = g_prompt_bwd(p[4], p[0], p[1], p[2], p[5], l, static_cast<const int32_t*>(p[3]), r.cu_k,
+                      grad[0].data_ptr(), grad[1].data_ptr(), grad[2].data_ptr(), ws.data_ptr(),
+                      ws.numel(), strides, r.B, r.T, r.Tk, r.Hq, r.H, r.D, (float)r.scale, r.dtype, fill,
+                      stream);
+  }
+  if (st != FAGQ_OK) return PyLong_FromLong(st);
+  return tuple_of(grad, 3);
   END_HANDLE_TH_ERRORS
 }
 
@@ -883,6 +1122,22 @@ PyObject* bind_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   g_cache_read = reinterpret_cast<decltype(g_cache_read)>(p[4]);
   g_attention_bytes = reinterpret_cast<decltype(g_attention_bytes)>(p[5]);
   g_attention = reinterpret_cast<decltype(g_attention)>(p[6]);
+  Py_RETURN_NONE;
+}
+
+// bind_prompts(addresses of fagq_paged_tree_attention_workspace_bytes, fagq_paged_tree_attention_launch,
+// fagq_batch_tables_launch, fagq_prompt_attention_workspace_bytes, fagq_prompt_attention_launch,
+// fagq_prompt_attention_bwd_workspace_bytes, fagq_prompt_attention_bwd_launch).
+PyObject* bind_prompts(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  void* p[7];
+  if (!addresses(args, nargs, 7, "bind_prompts", p)) return nullptr;
+  g_tree_bytes = reinterpret_cast<decltype(g_tree_bytes)>(p[0]);
+  g_tree = reinterpret_cast<decltype(g_tree)>(p[1]);
+  g_tables = reinterpret_cast<decltype(g_tables)>(p[2]);
+  g_prompt_bytes = reinterpret_cast<decltype(g_prompt_bytes)>(p[3]);
+  g_prompt = reinterpret_cast<decltype(g_prompt)>(p[4]);
+  g_prompt_bwd_bytes = reinterpret_cast<decltype(g_prompt_bwd_bytes)>(p[5]);
+  g_prompt_bwd = reinterpret_cast<decltype(g_prompt_bwd)>(p[6]);
   Py_RETURN_NONE;
 }
 
@@ -954,6 +1209,16 @@ PyMethodDef kMethods[] = {
      METH_FASTCALL, "Gathers cache pages; returns the status."},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&attention)),
      METH_FASTCALL, "Attention over the cache, with a workspace of its own."},
+    {"tree_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&tree_attention)),
+     METH_FASTCALL, "Attention of drafted trees over the cache, with a workspace of its own."},
+    {"tables", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&tables)),
+     METH_FASTCALL, "A step's index tensors: allocates and launches."},
+    {"prompt", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&prompt)),
+     METH_FASTCALL, "Attention of packed prompts, with a workspace of its own."},
+    {"prompt_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&prompt_bwd)),
+     METH_FASTCALL, "Its gradients, with outputs and a workspace of its own."},
+    {"bind_prompts", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&bind_prompts)),
+     METH_FASTCALL, "Sets the addresses of the prompts', trees' and tables' entry points."},
     {"bind_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&bind_attention)),
      METH_FASTCALL, "Sets the addresses of the attention side's entry points."},
     {nullptr, nullptr, 0, nullptr}};

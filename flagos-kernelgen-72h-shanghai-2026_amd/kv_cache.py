@@ -260,6 +260,15 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     stream."""
     if not isinstance(tree_mask, torch.Tensor):
         raise TypeError(f"tree_mask must be a tensor, got {type(tree_mask).__name__}")
+    mod, fast_stream = _lib.fast_module(k_cache) if workspace is None else (None, None)
+    if mod is not None:
+        r = mod.tree_attention(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, sm_scale,
+                               prefix_pages, prefix_len, max_kv_len, out, fast_stream, tree_mask)
+        if type(r) is not int:
+            return r
+        if r != _lib.FAST_ARG_ERROR:
+            _lib.check(r, "fagq_paged_tree_attention_launch")
+        # An argument the binding leaves to the checks below.
     return _attention(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, tree_mask, sm_scale,
                       prefix_pages, prefix_len, max_kv_len, out, workspace)
 

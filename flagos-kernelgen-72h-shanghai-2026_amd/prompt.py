@@ -90,6 +90,14 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ``workspace`` (optional): a uint8 GPU tensor of at least ``workspace_bytes(...)`` bytes, which
     calls that may overlap do not share.  The rows that sequences name are finite; others are not
     read.  Autograd does not see the call.  Asynchronous on the current stream."""
+    mod, fast_stream = _lib.fast_module(q) if workspace is None else (None, None)
+    if mod is not None:
+        r = mod.prompt(q, k, v, cu_seqlens, cu_seqlens_k, sm_scale, return_lse, out, fast_stream)
+        if type(r) is not int:
+            return r
+        if r != _lib.FAST_ARG_ERROR:
+            _lib.check(r, "fagq_prompt_attention_launch")
+        # An argument the binding leaves to the checks below.
     B, T, Tk, Hq, H, D = _check(q, k, v, cu_seqlens, cu_seqlens_k)
     dev = q.device
     strides = (_heads(q, "q", (T, Hq, D), q.dtype, dev) + _heads(k, "k", (Tk, H, D), q.dtype, dev)
@@ -143,6 +151,15 @@ def prompt_attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     given ones, zeros otherwise.  Equal calls give equal bits.  ``workspace`` (optional): a uint8
     GPU tensor of at least ``bwd_workspace_bytes(...)`` bytes, which calls that may overlap do not
     share.  Asynchronous on the current stream."""
+    mod, fast_stream = _lib.fast_module(q) if workspace is None else (None, None)
+    if mod is not None:
+        r = mod.prompt_bwd(q, k, v, cu_seqlens, cu_seqlens_k, sm_scale, dout, out, lse, dq, dk, dv,
+                           fast_stream)
+        if type(r) is not int:
+            return r
+        if r != _lib.FAST_ARG_ERROR:
+            _lib.check(r, "fagq_prompt_attention_bwd_launch")
+        # An argument the binding leaves to the checks below.
     B, T, Tk, Hq, H, D = _check(q, k, v, cu_seqlens, cu_seqlens_k)
     dev = q.device
     if out.dtype != q.dtype or tuple(out.shape) != (T, Hq, D) or not out.is_contiguous() \
