@@ -2,12 +2,15 @@
 //
 // One pass with a running maximum m and sum l of the softmax: for key j with score x (in units of
 // log 2), p = 2^(x - m), l = sum p, o = sum p v.  A workgroup takes 128 queries of one head, each
-// wave 32; keys and values come through LDS in tiles of 64, the next ones under way while these
-// are worked on.
+// wave 32; keys and values come through LDS in tiles of 64 (heads of 256: 32), the next ones under
+// way while these are worked on.
 //   scores   S^T = K Q^T: lane (c, h) has query c's scores of half of the keys.
 //   output   O^T = V^T P^T: the packed probabilities are its B operand as they are.
+// Where there are few workgroups, each one's keys are cut into parts with m, l and o of their own,
+// which prompt_attention_join puts together: o = sum 2^(m_i - m) o_i.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -32,8 +35,9 @@ struct Args {
   Sequences seq;
   uint16_t* out;
   float* lse;
+  float* part;                       // [parts][T][Hq][D], then {m, l} [parts][T][Hq][2]
   int64_t qs[2], ks[2], vs[2];       // {token, head} strides, elements
-  int32_t Hq, H, group, fill;
+  int32_t Hq, H, group, fill, parts;
   float scale2;                      // |sm_scale| log2(e), not 0
   uint32_t flip;                     // signs of a pair of queries' values, where sm_scale < 0
 };
@@ -53,16 +57,17 @@ __device__ __forceinline__ void fill_tail(const Args& a, const Place& p, int hq)
 
 template <int E, int D>
 __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention(Args a) {
-  using L = Tile<D>;
+  constexpr int kKeys = D == 256 ? 32 : 64;      // in LDS at a time
+  using L = Tile<D, kKeys>;
   __shared__ __align__(16) char lds[2][2][L::kBytes];
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int wave = scalar((int)(threadIdx.x >> 6));
   // Workgroup b runs on XCD b % 8: heads that share keys stay on one.
-  const int item = (int)blockIdx.x, kvh = item % a.H, rest = item / a.H;
-  const int hq = kvh * a.group + rest % a.group;
-  const Place p = place_of<true>(a.seq, rest / a.group);
+  const int item = (int)blockIdx.x, kvh = item % a.H, heads = item / a.H;
+  const int hq = kvh * a.group + heads % a.group, rest = heads / a.group, part = rest % a.parts;
+  const Place p = place_of<true>(a.seq, rest / a.parts);
   if (p.b < 0) {
-    if (a.fill) fill_tail<D>(a, p, hq);
+    if (a.fill && part == 0) fill_tail<D>(a, p, hq);
     return;
   }
   const int32_t ahead = p.m - p.n;               // query i sees the keys up to i + ahead
@@ -76,14 +81,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention(Args a) {
   const int32_t all = seen_by(mine);             // keys that every query of the wave sees
   const int32_t last = mine + kRows <= p.n ? mine + kRows - 1 : p.n - 1;
   const int32_t end = mine < p.n ? seen_by(last) : 0;                    // that one of them sees
-  const int32_t stop = seen_by(q0 + kTile <= p.n ? q0 + kTile - 1 : p.n - 1);
+  // Steps of the workgroup, this part's share of them.
+  const int32_t steps = (seen_by(q0 + kTile <= p.n ? q0 + kTile - 1 : p.n - 1) + kKeys - 1) / kKeys;
+  const int32_t from = (int32_t)((int64_t)steps * part / a.parts) * kKeys;
+  const int32_t stop = (int32_t)((int64_t)steps * (part + 1) / a.parts) * kKeys;
 
-  Copier<D> ck, cv;
+  Copier<D, kKeys> ck, cv;
   ck.init(a.k, (int64_t)p.other * a.ks[0] + (int64_t)kvh * a.ks[1], a.ks[0], lane, wave);
   cv.init(a.v, (int64_t)p.other * a.vs[0] + (int64_t)kvh * a.vs[1], a.vs[0], lane, wave);
-  if (stop > 0) {
-    ck.issue(lds[0][0], wave, 0, p.m - 1);
-    cv.issue(lds[0][1], wave, 0, p.m - 1);
+  if (from < stop) {
+    ck.issue(lds[0][0], wave, from, p.m - 1);
+    cv.issue(lds[0][1], wave, from, p.m - 1);
   }
   u32x4 q[D / 16];
   load_row<D>(a.q + (int64_t)(p.row + (i < p.n ? i : p.n - 1)) * a.qs[0] + (int64_t)hq * a.qs[1], h, q);
@@ -95,31 +103,31 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention(Args a) {
   float m = kLow, l = 0.0f;
 
   int buf = 0;
-  for (int32_t tok = 0; tok < stop; tok += kStep, buf ^= 1) {
+  for (int32_t tok = from; tok < stop; tok += kKeys, buf ^= 1) {
     __builtin_amdgcn_s_waitcnt(kVmcnt0);         // this step's tiles have landed, of this wave
     lds_barrier();                               // of all; the last step's are done with
-    if (tok + kStep < stop) {
-      ck.issue(lds[buf ^ 1][0], wave, tok + kStep, p.m - 1);
-      cv.issue(lds[buf ^ 1][1], wave, tok + kStep, p.m - 1);
+    if (tok + kKeys < stop) {
+      ck.issue(lds[buf ^ 1][0], wave, tok + kKeys, p.m - 1);
+      cv.issue(lds[buf ^ 1][1], wave, tok + kKeys, p.m - 1);
     }
     if (tok >= end) continue;
-    f32x16 x[2];
+    f32x16 x[kKeys / 32];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < kKeys / 32; ++t) {
       x[t] = splat(0.0f);
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) x[t] = mfma<E>(row_frag<D>(lds[buf][0], lane, t, j), q[j], x[t]);
     }
-    if (tok + kStep > all) {
+    if (tok + kKeys > all) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < kKeys / 32; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           x[t][r] = tok + 32 * t + row_of(r, h) < seen ? x[t][r] : -INFINITY;
     }
     float top = x[0][0];
 #pragma unroll
-    for (int r = 1; r < 32; ++r) top = fmaxf(top, x[r / 16][r % 16]);
+    for (int r = 1; r < kKeys / 2; ++r) top = fmaxf(top, x[r / 16][r % 16]);
     if (__any(__builtin_fmaf(top, a.scale2, -m) > kSlack)) {
       const float next = fmaxf(m, cross_max(top) * a.scale2);
       const float f = __builtin_amdgcn_exp2f(m - next);
@@ -130,9 +138,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention(Args a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= f;
     }
-    u32x4 w[4];
+    u32x4 w[kKeys / 16];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < kKeys / 32; ++t) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         x[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][r], a.scale2, -m));
@@ -144,14 +152,82 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention(Args a) {
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) o[d] = mfma<E>(col_frag<D>(lds[buf][1], lane, d, t), w[t], o[d]);
+      for (int t = 0; t < kKeys / 16; ++t)
+        o[d] = mfma<E>(col_frag<D>(lds[buf][1], lane, d, t), w[t], o[d]);
   }
   l = cross_sum(l);
   const int64_t row = p.row + i;
-  store_row<E, D>(a.out + (row * a.Hq + hq) * D, h, o, l > 0.0f ? 1.0f / l : 0.0f, i < p.n);
-  if (a.lse && h == 0 && i < p.n)
-    a.lse[(int64_t)hq * a.seq.T + row] =
+  if (a.parts == 1) {
+    store_row<E, D>(a.out + (row * a.Hq + hq) * D, h, o, l > 0.0f ? 1.0f / l : 0.0f, i < p.n);
+    if (a.lse && h == 0 && i < p.n)
+      a.lse[(int64_t)hq * a.seq.T + row] =
+          l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * (1.0f / kLog2e) : -INFINITY;
+  } else if (i < p.n) {
+    const int64_t at = ((int64_t)part * a.seq.T + row) * a.Hq + hq;
+    float* to = a.part + at * D;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<f32x4*>(to + 32 * d + row_of(r, h)) =
+            f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+    if (h == 0) {
+      float* ml = a.part + (int64_t)a.parts * a.seq.T * a.Hq * D + 2 * at;
+      ml[0] = m;
+      ml[1] = l;
+    }
+  }
+}
+
+// Joins the parts of a query's keys.  D / 8 threads have a query and head, each 8 of its values.
+template <int E, int D>
+__global__ __launch_bounds__(256) void prompt_attention_join(Args a) {
+  constexpr int kThreads = D / 8;
+  const int64_t item = (int64_t)blockIdx.x * (256 / kThreads) + threadIdx.x / kThreads;
+  const int d = threadIdx.x % kThreads * 8;
+  const int64_t rows = (int64_t)a.seq.T * a.Hq, row = item / a.Hq;
+  if (row >= clamped(a.seq.cu[a.seq.B], a.seq.T)) return;
+  const float* ml = a.part + a.parts * rows * D + 2 * item;
+  float m = kLow;
+  for (int i = 0; i < a.parts; ++i) m = fmaxf(m, ml[2 * i * rows]);
+  float l = 0.0f;
+  f32x4 o[2] = {};
+  for (int i = 0; i < a.parts; ++i) {
+    const float f = __builtin_amdgcn_exp2f(ml[2 * i * rows] - m);
+    const float* part = a.part + (i * rows + item) * D + d;
+    l = __builtin_fmaf(ml[2 * i * rows + 1], f, l);
+    o[0] += *reinterpret_cast<const f32x4*>(part) * f;
+    o[1] += *reinterpret_cast<const f32x4*>(part + 4) * f;
+  }
+  const float f = l > 0.0f ? 1.0f / l : 0.0f;
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack16<E>(o[i / 2][2 * i % 4] * f, o[i / 2][2 * i % 4 + 1] * f);
+  *reinterpret_cast<u32x4*>(a.out + item * D + d) = w;
+  if (a.lse && d == 0)
+    a.lse[item % a.Hq * a.seq.T + row] =
         l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * (1.0f / kLog2e) : -INFINITY;
+}
+
+// Parts of a workgroup's keys: as many as fill the GPU's places for two workgroups on each CU, but at
+// least four steps for each.
+constexpr int64_t kSlots = 512;
+constexpr int64_t kMostParts = 16;
+int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t D) {
+  const int64_t groups = std::max<int64_t>(1, (T + kTile - 1) / kTile * Hq);
+  const int64_t steps = Tk / std::max<int64_t>(1, B) / (D == 256 ? 32 : 64);
+  return std::max<int64_t>(1, std::min<int64_t>({kSlots / groups, steps / 4, kMostParts}));
+}
+
+int check_fwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
+  const int st = check_sizes(B, T, Tk, Hq, H, D);
+  return st != FAGQ_OK ? st : tile_slots(T, B) * Hq * parts_for(B, T, Tk, Hq, D) >= kMostGroups ? FAGQ_E_TOO_LARGE
+                                                                                               : FAGQ_OK;
+}
+
+int64_t bytes_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t D) {
+  const int64_t parts = parts_for(B, T, Tk, Hq, D);
+  return parts > 1 ? parts * T * Hq * (D + 2) * 4 : 0;
 }
 
 template <int E>
@@ -159,6 +235,12 @@ const void* kernel_for(int64_t D) {
   return D == 64    ? reinterpret_cast<const void*>(&prompt_attention<E, 64>)
          : D == 128 ? reinterpret_cast<const void*>(&prompt_attention<E, 128>)
                     : reinterpret_cast<const void*>(&prompt_attention<E, 256>);
+}
+template <int E>
+const void* join_for(int64_t D) {
+  return D == 64    ? reinterpret_cast<const void*>(&prompt_attention_join<E, 64>)
+         : D == 128 ? reinterpret_cast<const void*>(&prompt_attention_join<E, 128>)
+                    : reinterpret_cast<const void*>(&prompt_attention_join<E, 256>);
 }
 
 }  // namespace
@@ -169,7 +251,8 @@ extern "C" {
 
 FAGQ_API int64_t fagq_prompt_attention_workspace_bytes(int64_t B, int64_t T, int64_t Tk,
                                                        int64_t Hq, int64_t H, int64_t D) {
-  return fagq::prompt::check_sizes(B, T, Tk, Hq, H, D) == FAGQ_OK ? 0 : -1;
+  using namespace fagq::prompt;
+  return check_fwd_sizes(B, T, Tk, Hq, H, D) == FAGQ_OK ? bytes_for(B, T, Tk, Hq, D) : -1;
 }
 
 FAGQ_API int fagq_prompt_attention_launch(const void* q, const void* k, const void* v,
@@ -181,19 +264,21 @@ FAGQ_API int fagq_prompt_attention_launch(const void* q, const void* k, const vo
                                           void* stream) {
   using namespace fagq;
   using namespace fagq::prompt;
-  (void)workspace, (void)workspace_bytes;
   if (!q || (Tk > 0 && (!k || !v)) || !cu_seqlens || !out || !strides) return FAGQ_E_NULL;
   if (dtype != FAGQ_DT_BF16 && dtype != FAGQ_DT_F16) return FAGQ_E_FORMAT;
   if (fill & ~(FAGQ_FILL_OUT | FAGQ_FILL_LSE)) return FAGQ_E_FORMAT;
   if (!std::isfinite(sm_scale)) return FAGQ_E_SHAPE;
-  const int sizes = check_sizes(B, T, Tk, Hq, H, D);
+  const int sizes = check_fwd_sizes(B, T, Tk, Hq, H, D);
   if (sizes != FAGQ_OK) return sizes;
   if (!cu_seqlens_k && T != Tk) return FAGQ_E_SHAPE;
   const int st = check_strides(strides, 6);
   if (st != FAGQ_OK) return st;
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(lse, 4) ||
-      !aligned(cu_seqlens, 4) || !aligned(cu_seqlens_k, 4))
+      !aligned(cu_seqlens, 4) || !aligned(cu_seqlens_k, 4) || !aligned(workspace, 16))
     return FAGQ_E_ALIGN;
+  const int64_t need = bytes_for(B, T, Tk, Hq, D);
+  if (workspace_bytes < need) return FAGQ_E_SHAPE;
+  if (need > 0 && !workspace) return FAGQ_E_NULL;
   if (T == 0) return FAGQ_OK;
   const Rows rows[3] = {{q, T, Hq, D, strides[0], strides[1]},
                         {k, Tk, H, D, strides[2], strides[3]},
@@ -203,8 +288,11 @@ FAGQ_API int fagq_prompt_attention_launch(const void* q, const void* k, const vo
                           cu_seqlens_k ? (B + 1) * 4 : 0};
   const int64_t nout = T * Hq * D * 2, nlse = lse ? T * Hq * 4 : 0;
   for (int i = 0; i < 5; ++i)
-    if (overlap(out, nout, ins[i], nin[i]) || overlap(lse, nlse, ins[i], nin[i])) return FAGQ_E_ALIAS;
-  if (overlap(out, nout, lse, nlse)) return FAGQ_E_ALIAS;
+    if (overlap(out, nout, ins[i], nin[i]) || overlap(lse, nlse, ins[i], nin[i]) ||
+        overlap(workspace, need, ins[i], nin[i]))
+      return FAGQ_E_ALIAS;
+  if (overlap(out, nout, lse, nlse) || overlap(workspace, need, out, nout) || overlap(workspace, need, lse, nlse))
+    return FAGQ_E_ALIAS;
   const int dcheck = device_check();
   if (dcheck != FAGQ_OK) return dcheck;
   Args a = {};
@@ -218,10 +306,15 @@ FAGQ_API int fagq_prompt_attention_launch(const void* q, const void* k, const vo
   // What a query does not see has the score -inf, which times 0 would be no number.
   a.scale2 = std::fmax(std::fabs(sm_scale) * kLog2e, 0x1p-126f);
   a.flip = sm_scale < 0.0f ? 0x80008000u : 0u;
+  a.parts = (int32_t)parts_for(B, T, Tk, Hq, D), a.part = static_cast<float*>(workspace);
   void* args[] = {&a};
-  return launch_kernel(dtype == FAGQ_DT_BF16 ? kernel_for<ET_BF16>(D) : kernel_for<ET_F16>(D),
-                       dim3((unsigned)(tile_slots(T, B) * Hq)), dim3(64 * kWaves), args, 0,
-                       static_cast<hipStream_t>(stream));
+  const bool bf16 = dtype == FAGQ_DT_BF16;
+  hipStream_t to = static_cast<hipStream_t>(stream);
+  const int ls = launch_kernel(bf16 ? kernel_for<ET_BF16>(D) : kernel_for<ET_F16>(D),
+                               dim3((unsigned)(tile_slots(T, B) * Hq * a.parts)), dim3(64 * kWaves), args, 0, to);
+  if (ls != FAGQ_OK || a.parts == 1) return ls;
+  return launch_kernel(bf16 ? join_for<ET_BF16>(D) : join_for<ET_F16>(D),
+                       dim3((unsigned)((T * Hq * (D / 8) + 255) / 256)), dim3(256), args, 0, to);
 }
 
 }  // extern "C"

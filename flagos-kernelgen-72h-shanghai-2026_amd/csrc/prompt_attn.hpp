@@ -227,52 +227,60 @@ __device__ __forceinline__ int32_t clamped(int32_t v, int32_t most) {
 }
 
 // Tile number `slot` of all sequences': from the last one backwards (REVERSED), where late tiles
-// see most, or from the first on.  Lane l counts the tiles of sequences l n .. (l + 1) n - 1.
+// see most, or from the first on.  Lane l counts the tiles of sequences l n .. (l + 1) n - 1; up to 64
+// sequences it has everything about its own in registers, and one trip to memory is enough.
 template <bool REVERSED>
 __device__ __forceinline__ Place place_of(const Sequences& s, int32_t slot) {
   const int lane = threadIdx.x & 63;
   const int each = (s.B + 63) / 64;
-  auto length = [&](int i, int32_t* row) {       // i: in the order of the tiles
+  struct Sequence {
+    int32_t row, n, other, m;
+  };
+  auto sequence = [&](int i) {                   // i: in the order of the tiles
     const int b = REVERSED ? s.B - 1 - i : i;
     const int32_t lo = clamped(s.cu[b], s.T), hi = clamped(s.cu[b + 1], s.T);
-    *row = lo;
-    return hi > lo ? hi - lo : 0;
+    const int32_t lo2 = clamped(s.other[b], s.Tother), hi2 = clamped(s.other[b + 1], s.Tother);
+    return Sequence{lo, hi > lo ? hi - lo : 0, lo2, hi2 > lo2 ? hi2 - lo2 : 0};
   };
+  auto tiles_of = [](int32_t n) { return (n + kTile - 1) / kTile; };
+  Place p = {};
+  p.end = scalar(clamped(s.cu[s.B], s.T));
   const int first = lane * each, stop = first + each < s.B ? first + each : s.B;
-  int32_t mine = 0, row = 0;
-  for (int i = first; i < stop; ++i) mine += (length(i, &row) + kTile - 1) / kTile;
-  int32_t upto = mine;
+  Sequence mine = {};
+  int32_t count = 0;
+  for (int i = first; i < stop; ++i) {
+    mine = sequence(i);
+    count += tiles_of(mine.n);
+  }
+  int32_t upto = count;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const int32_t o = __shfl_up(upto, d);
     upto += lane >= d ? o : 0;
   }
-  Place p = {};
-  p.end = scalar(clamped(s.cu[s.B], s.T));
   const int32_t total = __builtin_amdgcn_readlane(upto, 63);
   if (slot >= total) {
     p.b = -1;
     p.tile = slot - total;
     return p;
   }
-  const uint64_t here = __ballot(slot >= upto - mine && slot < upto);
+  const uint64_t here = __ballot(slot >= upto - count && slot < upto);
   const int l = (int)__builtin_ctzll(here);
-  int32_t at = slot - __builtin_amdgcn_readlane(upto - mine, l);
+  int32_t at = slot - __builtin_amdgcn_readlane(upto - count, l);
   int i = l * each;
-  int32_t n = scalar(length(i, &row)), tiles = (n + kTile - 1) / kTile;
-  while (at >= tiles) {                          // ends: the lane's tiles are more than `at`
-    at -= tiles;
-    n = scalar(length(++i, &row));
-    tiles = (n + kTile - 1) / kTile;
+  if (each == 1) {
+    p.row = __builtin_amdgcn_readlane(mine.row, l), p.n = __builtin_amdgcn_readlane(mine.n, l);
+    p.other = __builtin_amdgcn_readlane(mine.other, l), p.m = __builtin_amdgcn_readlane(mine.m, l);
+  } else {
+    Sequence q = sequence(i);
+    while (at >= tiles_of(scalar(q.n))) {        // ends: the lane's tiles are more than `at`
+      at -= tiles_of(scalar(q.n));
+      q = sequence(++i);
+    }
+    p.row = scalar(q.row), p.n = scalar(q.n), p.other = scalar(q.other), p.m = scalar(q.m);
   }
   p.b = REVERSED ? s.B - 1 - i : i;
-  p.tile = REVERSED ? tiles - 1 - at : at;
-  p.row = scalar(row);
-  p.n = n;
-  const int32_t lo = scalar(clamped(s.other[p.b], s.Tother));
-  const int32_t hi = scalar(clamped(s.other[p.b + 1], s.Tother));
-  p.other = lo;
-  p.m = hi > lo ? hi - lo : 0;
+  p.tile = REVERSED ? tiles_of(p.n) - 1 - at : at;
   return p;
 }
 
