@@ -1,8 +1,12 @@
 // batch_tables.hip - the index tensors of a step from its requests' lengths (include/fagq_cache.h).
 //
-// Everything follows from two running sums over the requests, of new tokens and of new pages.  One
+// Everything follows from running sums over the requests, of new tokens, new pages and keys.  One
 // launch: every workgroup works the sums out for itself (8 bytes a request, from L2) and then writes
 // its share of the tokens and of the new pages, so none waits for another.
+//
+// Bound by latency: the lengths, then a page of the table, each a trip to memory, and between them one
+// exchange of sums (the page that a request's first new token goes to is read ahead of it, by the
+// thread that has the request, so that a decode step needs no search).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -16,10 +20,13 @@ namespace fagq {
 namespace tables {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int64_t kMostGroups = 256;            // workgroups: one on each CU
-constexpr int64_t kTokensEach = 2048;           // of a workgroup, at least
+constexpr int kEach = 4;                        // requests of a thread, at most
+constexpr int kRequests = kThreads * kEach;     // of a pass
+constexpr int kRun = 4;                         // tokens that a thread writes at a time
+constexpr int64_t kMostGroups = 1024;           // workgroups: four on each CU
+constexpr int64_t kTokensEach = kThreads * kRun;   // of a workgroup, at least
 constexpr int32_t kMost = 0x7fffffff;
 
 struct Args {
@@ -36,6 +43,7 @@ struct Args {
   int32_t* free_end;
   int64_t num_free, width;
   int32_t B, rows, shift, idx64;
+  int32_t wide;              // positions and slots are 16-byte aligned
 };
 
 __device__ __forceinline__ int64_t length(const void* p, int idx64, int b, int64_t most) {
@@ -44,19 +52,31 @@ __device__ __forceinline__ int64_t length(const void* p, int idx64, int b, int64
   return n < 0 ? 0 : n < most ? n : most;
 }
 
-// Inclusive sum over the workgroup's threads.
-__device__ __forceinline__ int64_t scan(int64_t v, int64_t (&sums)[kWaves]) {
+// Three sums at once: of the threads before this one, and of all.
+struct Sums {
+  int64_t tokens, pages, keys;
+};
+__device__ __forceinline__ Sums operator+(const Sums& a, const Sums& b) {
+  return {a.tokens + b.tokens, a.pages + b.pages, a.keys + b.keys};
+}
+__device__ __forceinline__ Sums before(const Sums& mine, Sums (&waves)[kWaves], Sums* all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Sums v = mine;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const int64_t o = __shfl_up(v, d);
-    v += lane >= d ? o : 0;
+    const Sums o = {__shfl_up(v.tokens, d), __shfl_up(v.pages, d), __shfl_up(v.keys, d)};
+    if (lane >= d) v = v + o;
   }
   __syncthreads();                              // the last sums have been read
-  if (lane == 63) sums[wave] = v;
+  if (lane == 63) waves[wave] = v;
   __syncthreads();
+  v = {v.tokens - mine.tokens, v.pages - mine.pages, v.keys - mine.keys};
+  *all = {};
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) v += w < wave ? sums[w] : 0;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) v = v + waves[w];
+    *all = *all + waves[w];
+  }
   return v;
 }
 
@@ -73,75 +93,138 @@ __device__ __forceinline__ int owner(const T* first, int n, T i) {
 }
 
 __global__ __launch_bounds__(kThreads) void batch_tables(Args a) {
-  __shared__ int64_t sums[kWaves];
-  __shared__ int32_t row[kThreads + 1], context[kThreads], have[kThreads];
-  __shared__ int64_t page[kThreads + 1];        // new pages of the requests before
+  __shared__ Sums waves[kWaves];
+  __shared__ int32_t row[kRequests + 1], context[kRequests], have[kRequests];
+  __shared__ int64_t page[kRequests + 1];       // new pages of the requests before
   const int tid = threadIdx.x, groups = gridDim.x, me = blockIdx.x;
-  const int32_t each = (a.rows + groups - 1) / groups;
-  const int64_t lo = (int64_t)me * each, hi = lo + each < a.rows ? lo + each : a.rows;
+  const int64_t each = ((a.rows + groups - 1) / groups + kRun - 1) / kRun * kRun;
+  const int64_t lo = me * each < a.rows ? me * each : a.rows, hi = lo + each < a.rows ? lo + each : a.rows;
   const int64_t start = a.free_start ? (a.free_start[0] > 0 ? a.free_start[0] : 0) : 0;
-  int64_t rows = 0, pages = 0, keys = 0;        // of the requests so far
+  const int64_t unit = 1ll << a.shift;
+  Sums so_far = {};
+  auto pages_of = [&](int64_t tokens) { return std::min(a.width, (tokens + unit - 1) >> a.shift); };
   auto free_page = [&](int64_t i) {
     i += start;
     return i < a.num_free ? a.free_pages[i] : -1;
   };
+  auto put = [&](int64_t r, int64_t at, int64_t p) {
+    a.positions[r] = (int32_t)(at < kMost ? at : kMost);
+    a.slots[r] = p < 0 ? -1 : (p << a.shift) + (at & (unit - 1));
+  };
   if (me == 0 && tid == 0) a.cu[0] = a.cu_k[0] = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-    const int b = b0 + tid, n = a.B - b0 < kThreads ? a.B - b0 : kThreads;
-    const int64_t ctx = b < a.B ? length(a.context, a.idx64, b, kMost) : 0;
-    const int64_t want = b < a.B ? length(a.fresh, a.idx64, b, a.rows) : 0;
-    // Rows behind the last one there is room for are no part of this step.
-    const int64_t upto = rows + scan(want, sums), from = upto - want;
-    const int64_t end = upto < a.rows ? upto : a.rows, mine = end - (from < a.rows ? from : a.rows);
-    const int64_t len = ctx + mine < kMost ? ctx + mine : kMost;
-    const int64_t unit = 1ll << a.shift;
-    const int64_t old = std::min(a.width, (ctx + unit - 1) >> a.shift);
-    const int64_t all = std::min(a.width, (len + unit - 1) >> a.shift);
-    const int64_t need = all > old ? all - old : 0;
-    const int64_t pages_upto = pages + scan(need, sums);
-    const int64_t keys_upto = keys + scan(b < a.B ? len : 0, sums);
-    __syncthreads();                            // the last requests' have been read
+  for (int b0 = 0; b0 < a.B; b0 += kRequests) {
+    const int n = a.B - b0 < kRequests ? a.B - b0 : kRequests, k = (n + kThreads - 1) / kThreads;
+    const int s0 = tid * k;                     // this thread's requests: s0 .. s0 + k - 1
+    int64_t ctx[kEach], mine[kEach];
+    int32_t next[kEach];                        // the page that the first new token goes to, if it is there
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const bool live = i < k && s0 + i < n;
+      ctx[i] = live ? length(a.context, a.idx64, b0 + s0 + i, kMost) : 0;
+      mine[i] = live ? length(a.fresh, a.idx64, b0 + s0 + i, a.rows) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      next[i] = mine[i] > 0 && (ctx[i] >> a.shift) < pages_of(ctx[i])
+                    ? a.table[(int64_t)(b0 + s0 + i) * a.width + (ctx[i] >> a.shift)] : -1;
+    auto sums = [&] {
+      Sums t = {};
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int64_t len = ctx[i] + mine[i] < kMost ? ctx[i] + mine[i] : kMost;
+        t = t + Sums{mine[i], pages_of(len) - pages_of(ctx[i]), i < k && s0 + i < n ? len : 0};
+      }
+      return t;
+    };
+    Sums all, from = before(sums(), waves, &all);
+    if (so_far.tokens + all.tokens > a.rows) {
+      // Rows behind the last one there is room for are no part of this step.
+      int64_t at = so_far.tokens + from.tokens;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int64_t room = a.rows > at ? a.rows - at : 0;
+        at += mine[i];
+        mine[i] = mine[i] < room ? mine[i] : room;
+      }
+      from = before(sums(), waves, &all);
+    }
+    __syncthreads();                            // the last requests' tables have been read
+    Sums at = so_far + from;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int s = s0 + i;
+      if (i < k && s < n) {
+        const int64_t len = ctx[i] + mine[i] < kMost ? ctx[i] + mine[i] : kMost;
+        const int64_t old = pages_of(ctx[i]);
+        row[s] = (int32_t)at.tokens;
+        page[s] = at.pages;
+        context[s] = (int32_t)ctx[i];
+        have[s] = (int32_t)old;
+        if (mine[i] > 0 && at.tokens >= lo && at.tokens < hi) {
+          const int64_t first = ctx[i] >> a.shift;
+          put(at.tokens, ctx[i], first < old ? next[i] : first < a.width ? free_page(at.pages + (first - old)) : -1);
+        }
+        at = at + Sums{mine[i], pages_of(len) - old, len};
+        if (me == 0) {
+          a.cu[b0 + s + 1] = (int32_t)at.tokens;
+          a.cu_k[b0 + s + 1] = (int32_t)(at.keys < kMost ? at.keys : kMost);
+          a.lens[b0 + s] = (int32_t)len;
+        }
+      }
+    }
+    const Sums end = so_far + all;
     if (tid == 0) {
-      row[0] = (int32_t)rows;
-      page[0] = pages;
+      row[n] = (int32_t)end.tokens;
+      page[n] = end.pages;
     }
-    row[tid + 1] = (int32_t)end;
-    page[tid + 1] = pages_upto;
-    context[tid] = (int32_t)ctx;
-    have[tid] = (int32_t)old;
-    if (me == 0 && b < a.B) {
-      a.cu[b + 1] = (int32_t)end;
-      a.cu_k[b + 1] = (int32_t)(keys_upto < kMost ? keys_upto : kMost);
-      a.lens[b] = (int32_t)len;
+    bool two = false;                           // whether some request has two new tokens
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) two |= mine[i] > 1;
+    const bool more = __syncthreads_or(two);
+    // Tokens behind their request's first.
+    const int64_t stop = end.tokens < hi ? end.tokens : hi;
+    for (int64_t r0 = lo + tid * kRun; more && r0 < stop; r0 += kThreads * kRun) {
+      const int64_t r1 = r0 + kRun < stop ? r0 + kRun : stop;
+      int64_t r = r0 > so_far.tokens ? r0 : so_far.tokens;
+      if (r >= r1) continue;
+      int s = owner(row, n, (int32_t)r);
+      const bool whole = r == r0 && r1 == r0 + kRun && a.wide;
+      int32_t positions[kRun];
+      int64_t slots[kRun];
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+        if (r0 + i < r || r0 + i >= r1) continue;
+        while (r0 + i >= row[s + 1]) ++s;       // ends: row[n] is larger
+        const int64_t at = (int64_t)context[s] + (r0 + i - row[s]), g = at >> a.shift;
+        int64_t p = -1;
+        if (g < have[s]) p = a.table[(int64_t)(b0 + s) * a.width + g];
+        else if (g < a.width) p = free_page(page[s] + (g - have[s]));
+        if (!whole) put(r0 + i, at, p);
+        positions[i] = (int32_t)(at < kMost ? at : kMost);
+        slots[i] = p < 0 ? -1 : (p << a.shift) + (at & (unit - 1));
+      }
+      if (whole) {
+        typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+        typedef int64_t i64x2 __attribute__((ext_vector_type(2)));
+        *reinterpret_cast<i32x4*>(a.positions + r0) = i32x4{positions[0], positions[1], positions[2], positions[3]};
+        *reinterpret_cast<i64x2*>(a.slots + r0) = i64x2{slots[0], slots[1]};
+        *reinterpret_cast<i64x2*>(a.slots + r0 + 2) = i64x2{slots[2], slots[3]};
+      }
     }
-    __syncthreads();
-    const int64_t stop = row[n] < hi ? row[n] : hi;
-    for (int64_t r = (rows > lo ? rows : lo) + tid; r < stop; r += kThreads) {
-      const int s = owner(row, n, (int32_t)r);
-      const int64_t at = (int64_t)context[s] + (r - row[s]), i = at >> a.shift;
-      int64_t p = -1;
-      if (i < have[s]) p = a.table[(int64_t)(b0 + s) * a.width + i];
-      else if (i < a.width) p = free_page(page[s] + (i - have[s]));
-      a.positions[r] = (int32_t)(at < kMost ? at : kMost);
-      a.slots[r] = p < 0 ? -1 : (p << a.shift) + (at & (unit - 1));
-    }
-    const int64_t fresh = page[n] - page[0];
-    const int64_t first = page[0] + fresh * me / groups, last = page[0] + fresh * (me + 1) / groups;
+    const int64_t first = so_far.pages + all.pages * me / groups;
+    const int64_t last = so_far.pages + all.pages * (me + 1) / groups;
     for (int64_t f = first + tid; f < last; f += kThreads) {
       const int s = owner(page, n, f);
       a.table[(int64_t)(b0 + s) * a.width + have[s] + (f - page[s])] = free_page(f);
     }
-    rows = row[n];
-    pages = page[n];
-    // The last scan's sums are still there.
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) keys += sums[w];
+    so_far = end;
   }
-  for (int64_t r = (rows > lo ? rows : lo) + tid; r < hi; r += kThreads) {
+  for (int64_t r = (so_far.tokens > lo ? so_far.tokens : lo) + tid; r < hi; r += kThreads) {
     a.positions[r] = -1;
     a.slots[r] = -1;
   }
-  if (me == 0 && tid == 0) a.free_end[0] = (int32_t)(start + pages < kMost ? start + pages : kMost);
+  if (me == 0 && tid == 0)
+    a.free_end[0] = (int32_t)(start + so_far.pages < kMost ? start + so_far.pages : kMost);
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -194,8 +277,9 @@ FAGQ_API int fagq_batch_tables_launch(
   if (dcheck != FAGQ_OK) return dcheck;
   Args a = {context_lens, new_lens,  free_pages, free_start, page_table, cu_seqlens,
             cu_seqlens_k, kv_lens,   positions,  slots,      free_end,   num_free,
-            table_width,  (int32_t)B, (int32_t)rows, 0, index_dtype == FAGQ_IDX_I64};
+            table_width,  (int32_t)B, (int32_t)rows, 0, index_dtype == FAGQ_IDX_I64, 0};
   while ((1ll << a.shift) < page_size) ++a.shift;
+  a.wide = aligned(positions, 16) && aligned(slots, 16);
   void* args[] = {&a};
   const int64_t groups = std::max<int64_t>(1, std::min(kMostGroups, (rows + kTokensEach - 1) / kTokensEach));
   return launch_kernel(reinterpret_cast<const void*>(&batch_tables), dim3((unsigned)groups),

