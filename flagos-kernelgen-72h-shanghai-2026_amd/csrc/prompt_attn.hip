@@ -210,13 +210,13 @@ __global__ __launch_bounds__(256) void prompt_attention_join(Args a) {
 }
 
 // Parts of a workgroup's keys: as many as fill the GPU's places for two workgroups on each CU, but at
-// least four steps for each.
+// least 16 steps for each, which take about as long as the join.
 constexpr int64_t kSlots = 512;
 constexpr int64_t kMostParts = 16;
 int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t D) {
   const int64_t groups = std::max<int64_t>(1, (T + kTile - 1) / kTile * Hq);
   const int64_t steps = Tk / std::max<int64_t>(1, B) / (D == 256 ? 32 : 64);
-  return std::max<int64_t>(1, std::min<int64_t>({kSlots / groups, steps / 4, kMostParts}));
+  return std::max<int64_t>(1, std::min<int64_t>({kSlots / groups, steps / 16, kMostParts}));
 }
 
 int check_fwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {

@@ -7,8 +7,9 @@
 //                 pass needs of each query: lse in units of log 2, and -delta.
 //   prompt_dkdv   A workgroup takes 128 keys of one head of k and v, the queries of all heads of
 //                 the group come through LDS.  S = Q K^T, dP = dO V^T, dV^T += dO^T P,
-//                 dK^T += Q^T dS.  Where there are few workgroups, each key tile's steps are cut
-//                 into parts of their own sums, which prompt_join adds up in order.
+//                 dK^T += Q^T dS.  Two teams of four waves share the steps of a tile and join
+//                 their sums through LDS; where there are few workgroups, the steps are cut into
+//                 parts of their own sums besides, which prompt_join adds up in order.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -155,17 +156,23 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_dq(Args a) {
   store_row<E, D>(a.dq + (int64_t)row * a.dqs[0] + (int64_t)hq * a.dqs[1], h, dq, a.scale, i < p.n);
 }
 
+// Teams of four waves in a workgroup, which share its steps and join their sums through LDS.
+constexpr int teams(int64_t D) { return D == 256 ? 1 : 2; }
+constexpr int queries(int64_t D) { return D == 128 ? 32 : 64; }   // of a team in LDS at a time
+
 template <int E, int D, bool TWO>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_dkdv(Args a) {
-  constexpr int kQueries = D == 128 ? 32 : 64;            // in LDS at a time
+__global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(Args a) {
+  constexpr int kQueries = queries(D);
   using L = Tile<D, kQueries>;
   using V = Tile<D, kTile>;
   constexpr bool kVInLds = D <= 128;
-  __shared__ __align__(16) char lds[2][2][L::kBytes];
+  __shared__ __align__(16) char lds_all[teams(D)][2][2][L::kBytes];
   __shared__ __align__(16) char lds_v[kVInLds ? V::kBytes : 16];
-  __shared__ __align__(16) float stats[2][2][kQueries];   // lse2, -delta
+  __shared__ __align__(16) float stats_all[teams(D)][2][2][kQueries];   // lse2, -delta
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
-  const int wave = scalar((int)(threadIdx.x >> 6));
+  const int waves = scalar((int)(threadIdx.x >> 6)), wave = waves % kWaves, team = waves / kWaves;
+  auto& lds = lds_all[team];
+  auto& stats = stats_all[team];
   const int item = (int)blockIdx.x, kvh = item % a.H, rest = item / a.H;
   const int part = rest % a.parts;
   const Place p = place_of<false>(a.keys, rest / a.parts);
@@ -179,9 +186,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_dkdv(Arg
   const int32_t j0 = mine + c;
   const int32_t first = k0 > ahead ? k0 - ahead : 0;       // query that sees one of the tile's keys
   const int32_t steps = first < p.m ? (p.m - first + kQueries - 1) / kQueries : 0;
-  // Steps of all heads in a row, head by head: this part's share.
+  // Steps of all heads in a row, head by head: this part's share, and its longest team's number.
   const int64_t total = (int64_t)steps * a.group;
-  const int32_t from = (int32_t)(total * part / a.parts), to = (int32_t)(total * (part + 1) / a.parts);
+  const int32_t shares = a.parts * teams(D), share = part * teams(D) + team;
+  const int32_t from = (int32_t)(total * share / shares), to = (int32_t)(total * (share + 1) / shares);
+  const int32_t rounds = (int32_t)((total + shares - 1) / shares);
 
   Copier<D, kQueries> cq, cg;
   cq.init(a.q, (int64_t)p.other * a.qs[0] + (int64_t)kvh * a.group * a.qs[1], a.qs[0], lane, wave);
@@ -210,7 +219,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_dkdv(Arg
     load_row<D>(a.k + row * a.ks[0] + (int64_t)kvh * a.ks[1], h, k);
     if constexpr (!kVInLds) load_row<D>(a.v + row * a.vs[0] + (int64_t)kvh * a.vs[1], h, v);
   }
-  if constexpr (kVInLds) {
+  if (kVInLds && team == 0) {
     Copier<D, kTile> cv;
     cv.init(a.v, (int64_t)p.row * a.vs[0] + (int64_t)kvh * a.vs[1], a.vs[0], lane, wave);
     cv.issue(lds_v, wave, k0, p.n - 1);
@@ -221,13 +230,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_dkdv(Arg
   for (int d = 0; d < D / 32; ++d) dk[d] = dv[d] = splat(0.0f);
 
   int buf = 0;
-  for (int32_t it = from; it < to; ++it, buf ^= 1) {
+  for (int32_t round = 0; round < rounds; ++round, buf ^= 1) {
+    const int32_t it = from + round;
     const int32_t i0 = first + step * kQueries;
     __builtin_amdgcn_s_waitcnt(kVmcnt0);         // this step's tiles have landed, of this wave
     lds_barrier();                               // of all; the last step's are done with
     if (++step == steps) step = 0, ++head;
     if (it + 1 < to) issue(buf ^ 1, head, step);
-    if (mine >= p.n) continue;
+    if (mine >= p.n || it >= to) continue;
 #pragma unroll 1
     for (int t = 0; t < kQueries / 32; ++t) {
       const int32_t query = i0 + 32 * t;
@@ -290,6 +300,34 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_dkdv(Arg
       }
     }
   }
+  if constexpr (teams(D) > 1) {
+    // The second team hands its sums over, dk's, then dv's.
+    f32x4* sums = reinterpret_cast<f32x4*>(lds_all);
+    static_assert(sizeof(lds_all) >= kWaves * D / 32 * 4 * 64 * sizeof(f32x4), "room for one of them");
+    auto hand = [&](f32x16 (&x)[D / 32]) {
+      __syncthreads();
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          f32x4& at = sums[((wave * (D / 32) + d) * 4 + r) * 64 + lane];
+          if (team) at = f32x4{x[d][4 * r], x[d][4 * r + 1], x[d][4 * r + 2], x[d][4 * r + 3]};
+        }
+      __syncthreads();
+      if (team) return;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const f32x4 v = sums[((wave * (D / 32) + d) * 4 + r) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[d][4 * r + e] += v[e];
+        }
+    };
+    hand(dk);
+    hand(dv);
+    if (team) return;
+  }
   const int64_t row = p.row + j0;
   if (a.parts == 1) {
     store_row<E, D>(a.dk + row * a.dks[0] + (int64_t)kvh * a.dks[1], h, dk, a.scale, j0 < p.n);
@@ -338,7 +376,7 @@ __global__ __launch_bounds__(256) void prompt_join(Args a, int32_t D) {
 
 // ---------------------------------------------------------------------------------- host
 
-constexpr int64_t kSlots = 512;      // workgroups at a time
+constexpr int64_t kCUs = 256;        // a workgroup on each
 constexpr int64_t kMostParts = 16;
 
 int check_bwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
@@ -349,13 +387,12 @@ int check_bwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int
   return large ? FAGQ_E_TOO_LARGE : FAGQ_OK;
 }
 
-// Parts of a key tile's steps: two workgroups for each place that the GPU has (tiles with few queries
-// then fill what the first ones leave), but four steps for each.
+// Parts of a key tile's steps: as many as let the tile with most of them, twice the average, not take
+// longer than all together, but four steps for each team.
 int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
   const int64_t groups = std::max<int64_t>(1, (Tk + kTile - 1) / kTile * H);
-  const int64_t slots = D == 256 ? kSlots / 2 : kSlots;
-  const int64_t steps = Hq / H * ((T + kStep - 1) / kStep) / std::max<int64_t>(1, B);
-  return std::max<int64_t>(1, std::min<int64_t>({(2 * slots + groups - 1) / groups, steps / 4, kMostParts}));
+  const int64_t steps = Hq / H * ((T + queries(D) - 1) / queries(D)) / std::max<int64_t>(1, B);
+  return std::max<int64_t>(1, std::min<int64_t>({2 * kCUs / groups, steps / (4 * teams(D)), kMostParts}));
 }
 
 // Whether dk and dv take two terms (of 16 bits each) of P and dS, as dq always does.  One leaves them
@@ -471,7 +508,8 @@ FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, c
   if (Tk == 0) return FAGQ_OK;
   const int ls = launch_kernel(two_terms(T, Hq) ? (bf16 ? dkdv_for<ET_BF16, true>(D) : dkdv_for<ET_F16, true>(D))
                                                 : (bf16 ? dkdv_for<ET_BF16, false>(D) : dkdv_for<ET_F16, false>(D)),
-                               dim3((unsigned)(tile_slots(Tk, B) * H * parts)), dim3(64 * kWaves), args, 0, st);
+                               dim3((unsigned)(tile_slots(Tk, B) * H * parts)),
+                               dim3((unsigned)(64 * kWaves * teams(D))), args, 0, st);
   if (ls != FAGQ_OK || parts == 1) return ls;
   const int64_t items = 2 * Tk * H * (D / 8);
   return launch_kernel(bf16 ? reinterpret_cast<const void*>(&prompt_join<ET_BF16>)
