@@ -28,7 +28,7 @@ constexpr int kTile = kRows * kWaves;           // of a workgroup
 constexpr int kStep = 64;                       // rows of the other side that are in LDS at a time
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int64_t kMostGroups = 1ll << 24;      // a grid of 2^32 threads is too large
-constexpr int kVmcnt0 = 0x0F70;                 // s_waitcnt vmcnt(0), other counters not waited
+constexpr int kVmcnt0 = 0x0F70;                 // s_waitcnt vmcnt(0), other counters not waited; + n < 16
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -55,6 +55,7 @@ __device__ __forceinline__ f32x16 splat(float v) {
   for (int i = 0; i < 16; ++i) r[i] = v;
   return r;
 }
+
 
 __device__ __forceinline__ int32_t scalar(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -91,6 +92,33 @@ struct Tile {
   }
 };
 
+// 16 (4) bytes a lane from `rs` at voff + soff past the registers to LDS, lane by lane from `lds` on
+// (which m0 tells the instruction; it is put back, the compiler keeps it).  In assembly, so that only
+// the kernel's own waits are for it: of the builtin the compiler has every transposed read of LDS
+// wait for all copies under way, the ones for later steps among them.
+__device__ __forceinline__ void copy16(const u32x4& rs, char* lds, uint32_t voff, uint32_t soff) {
+  uint32_t old;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+               "buffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(old)
+               : "s"((uint32_t)(uintptr_t)(lds_void_t*)lds), "v"(voff), "s"(rs), "s"(soff)
+               : "memory");
+}
+__device__ __forceinline__ void copy4(const u32x4& rs, char* lds, uint32_t voff) {
+  uint32_t old;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+               "buffer_load_dword %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(old)
+               : "s"((uint32_t)(uintptr_t)(lds_void_t*)lds), "v"(voff), "s"(rs)
+               : "memory");
+}
+// A buffer from p on, of any size: callers keep their offsets inside the tensor.
+__device__ __forceinline__ u32x4 buffer_at(const void* p) {
+  const uintptr_t v = reinterpret_cast<uintptr_t>(p);
+  return {(uint32_t)scalar((int32_t)(uint32_t)v), (uint32_t)scalar((int32_t)(uint32_t)(v >> 32)) & 0xffffu,
+          0x7fffffffu, kRsrcWord3};
+}
+
 // Copies rows [first, first + ROWS) of one head, row `last` in place of those behind it, from HBM
 // into LDS, past the registers.  Copy n of wave w brings rows (4 n + w) kCopyRows ..
 template <int D, int ROWS = kStep>
@@ -110,21 +138,19 @@ struct Copier {
       chunk[i] = (uint32_t)((lane % L::kChunks) ^ L::swizzle(row + i * kWaves * L::kCopyRows)) * 16u;
   }
   __device__ __forceinline__ void issue(char* lds, int wave, int first, int last) const {
-    const rsrc_t rs = make_rsrc(base + (int64_t)first * stride, 0x7fffffffu);
+    const u32x4 rs = buffer_at(base + (int64_t)first * stride);
     if (first + ROWS - 1 <= last) {
       const uint32_t off = (uint32_t)row * stride;
 #pragma unroll
       for (int n = 0; n < L::kCopies; ++n)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rs, (lds_void_t*)(lds + (n * kWaves + wave) * 1024), 16, off + chunk[n & 1],
-            (uint32_t)(n * kWaves * L::kCopyRows) * stride, 0, 0);
+        copy16(rs, lds + (n * kWaves + wave) * 1024, off + chunk[n & 1],
+               (uint32_t)(n * kWaves * L::kCopyRows) * stride);
     } else {
 #pragma unroll
       for (int n = 0; n < L::kCopies; ++n) {
         const int r = row + n * kWaves * L::kCopyRows, most = last - first;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rs, (lds_void_t*)(lds + (n * kWaves + wave) * 1024), 16,
-            (uint32_t)(r < most ? r : most) * stride + chunk[n & 1], 0, 0, 0);
+        copy16(rs, lds + (n * kWaves + wave) * 1024, (uint32_t)(r < most ? r : most) * stride + chunk[n & 1],
+               0);
       }
     }
   }

@@ -166,9 +166,10 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
   using L = Tile<D, kQueries>;
   using V = Tile<D, kTile>;
   constexpr bool kVInLds = D <= 128;
-  __shared__ __align__(16) char lds_all[teams(D)][2][2][L::kBytes];
+  constexpr int kAhead = D == 256 ? 1 : 2;                // steps whose tiles are under way
+  __shared__ __align__(16) char lds_all[teams(D)][kAhead + 1][2][L::kBytes];
   __shared__ __align__(16) char lds_v[kVInLds ? V::kBytes : 16];
-  __shared__ __align__(16) float stats_all[teams(D)][2][2][kQueries];   // lse2, -delta
+  __shared__ __align__(16) float stats_all[teams(D)][kAhead + 1][2][kQueries];   // lse2, -delta
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int waves = scalar((int)(threadIdx.x >> 6)), wave = waves % kWaves, team = waves / kWaves;
   auto& lds = lds_all[team];
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
   Copier<D, kQueries> cq, cg;
   cq.init(a.q, (int64_t)p.other * a.qs[0] + (int64_t)kvh * a.group * a.qs[1], a.qs[0], lane, wave);
   cg.init(a.dout, (int64_t)p.other * a.dos[0] + (int64_t)kvh * a.group * a.dos[1], a.dos[0], lane, wave);
-  int32_t head = steps > 0 ? from / steps : 0, step = from - head * steps;
+  int32_t head = steps > 0 ? from / steps : 0, step = from - head * steps;   // of the next copies
   auto issue = [&](int buf, int32_t head, int32_t step) {
     const int32_t i0 = first + step * kQueries;
     Copier<D, kQueries> x = cq, y = cg;
@@ -206,23 +207,30 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
     if (wave < 2 && lane < kQueries) {
       const int64_t at = (int64_t)(kvh * a.group + head) * a.keys.Tother + p.other + i0;
       const int32_t most = p.m - 1 - i0;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          make_rsrc((wave == 0 ? a.lse2 : a.delta) + at, 0x7fffffffu),
-          (lds_void_t*)(wave == 0 ? stats[buf][0] : stats[buf][1]), 4,
-          (uint32_t)(lane < most ? lane : most) * 4u, 0, 0, 0);
+      copy4(buffer_at((wave == 0 ? a.lse2 : a.delta) + at),
+            reinterpret_cast<char*>(wave == 0 ? stats[buf][0] : stats[buf][1]),
+            (uint32_t)(lane < most ? lane : most) * 4u);
     }
   };
-  if (from < to) issue(0, head, step);
   u32x4 k[D / 16], v[kVInLds ? 1 : D / 16];
   {
     const int64_t row = p.row + (j0 < p.n ? j0 : p.n - 1);
     load_row<D>(a.k + row * a.ks[0] + (int64_t)kvh * a.ks[1], h, k);
     if constexpr (!kVInLds) load_row<D>(a.v + row * a.vs[0] + (int64_t)kvh * a.vs[1], h, v);
   }
-  if (kVInLds && team == 0) {
+  if (kVInLds && team == 0) {                    // ahead of the others: the first wait is for them too
     Copier<D, kTile> cv;
     cv.init(a.v, (int64_t)p.row * a.vs[0] + (int64_t)kvh * a.vs[1], a.vs[0], lane, wave);
     cv.issue(lds_v, wave, k0, p.n - 1);
+  }
+  auto next = [&] {
+    if (++step == steps) step = 0, ++head;
+  };
+  int32_t i0 = first + step * kQueries;          // of the step that is worked on
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    if (from + u < to) issue(u, head, step);
+    next();
   }
   const char* tv = lds_v + wave * kRows * V::kRowBytes;
   f32x16 dk[D / 32], dv[D / 32];
@@ -230,13 +238,17 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
   for (int d = 0; d < D / 32; ++d) dk[d] = dv[d] = splat(0.0f);
 
   int buf = 0;
-  for (int32_t round = 0; round < rounds; ++round, buf ^= 1) {
+  for (int32_t round = 0; round < rounds; ++round, buf = buf == kAhead ? 0 : buf + 1, i0 += kQueries) {
     const int32_t it = from + round;
-    const int32_t i0 = first + step * kQueries;
-    __builtin_amdgcn_s_waitcnt(kVmcnt0);         // this step's tiles have landed, of this wave
+    if (i0 >= p.m) i0 = first;
+    // This step's tiles have landed, of this wave: later steps' copies may be under way.
+    constexpr int kCopies = 2 * L::kCopies;
+    if (kAhead == 1 || it + 1 >= to) __builtin_amdgcn_s_waitcnt(kVmcnt0);
+    else if (wave < 2) __builtin_amdgcn_s_waitcnt(kVmcnt0 + kCopies + 1);
+    else __builtin_amdgcn_s_waitcnt(kVmcnt0 + kCopies);
     lds_barrier();                               // of all; the last step's are done with
-    if (++step == steps) step = 0, ++head;
-    if (it + 1 < to) issue(buf ^ 1, head, step);
+    if (it + kAhead < to) issue(buf == 0 ? kAhead : buf - 1, head, step);
+    next();
     if (mine >= p.n || it >= to) continue;
 #pragma unroll 1
     for (int t = 0; t < kQueries / 32; ++t) {
