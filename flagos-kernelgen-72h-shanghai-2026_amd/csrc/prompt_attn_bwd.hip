@@ -160,16 +160,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_dq(Args a) {
 constexpr int teams(int64_t D) { return D == 256 ? 1 : 2; }
 constexpr int queries(int64_t D) { return D == 128 ? 32 : 64; }   // of a team in LDS at a time
 
+// The order of a stretch of N products: eight reads of LDS ahead of the first, two between any two.
+template <int N>
+__device__ __forceinline__ void read_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+  }
+}
+
 template <int E, int D, bool TWO>
 __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(Args a) {
   constexpr int kQueries = queries(D);
   using L = Tile<D, kQueries>;
-  using V = Tile<D, kTile>;
-  constexpr bool kVInLds = D <= 128;
-  constexpr int kAhead = D == 256 ? 1 : 2;                // steps whose tiles are under way
-  __shared__ __align__(16) char lds_all[teams(D)][kAhead + 1][2][L::kBytes];
-  __shared__ __align__(16) char lds_v[kVInLds ? V::kBytes : 16];
-  __shared__ __align__(16) float stats_all[teams(D)][kAhead + 1][2][kQueries];   // lse2, -delta
+  using KV = Tile<D, kTile>;
+  constexpr bool kInLds = D <= 128;                       // k and v; else in registers
+  __shared__ __align__(16) char lds_all[teams(D)][2][2][L::kBytes];
+  __shared__ __align__(16) char lds_kv[2][kInLds ? KV::kBytes : 16];
+  __shared__ __align__(16) float stats_all[teams(D)][2][2][kQueries];   // lse2, -delta
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int waves = scalar((int)(threadIdx.x >> 6)), wave = waves % kWaves, team = waves / kWaves;
   auto& lds = lds_all[team];
@@ -212,43 +222,35 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
             (uint32_t)(lane < most ? lane : most) * 4u);
     }
   };
-  u32x4 k[D / 16], v[kVInLds ? 1 : D / 16];
-  {
+  u32x4 k[kInLds ? 1 : D / 16], v[kInLds ? 1 : D / 16];
+  if constexpr (!kInLds) {
     const int64_t row = p.row + (j0 < p.n ? j0 : p.n - 1);
     load_row<D>(a.k + row * a.ks[0] + (int64_t)kvh * a.ks[1], h, k);
-    if constexpr (!kVInLds) load_row<D>(a.v + row * a.vs[0] + (int64_t)kvh * a.vs[1], h, v);
+    load_row<D>(a.v + row * a.vs[0] + (int64_t)kvh * a.vs[1], h, v);
   }
-  if (kVInLds && team == 0) {                    // ahead of the others: the first wait is for them too
+  if (kInLds && team == 0) {
     Copier<D, kTile> cv;
     cv.init(a.v, (int64_t)p.row * a.vs[0] + (int64_t)kvh * a.vs[1], a.vs[0], lane, wave);
-    cv.issue(lds_v, wave, k0, p.n - 1);
+    cv.issue(lds_kv[1], wave, k0, p.n - 1);
+    cv.init(a.k, (int64_t)p.row * a.ks[0] + (int64_t)kvh * a.ks[1], a.ks[0], lane, wave);
+    cv.issue(lds_kv[0], wave, k0, p.n - 1);
   }
-  auto next = [&] {
-    if (++step == steps) step = 0, ++head;
-  };
   int32_t i0 = first + step * kQueries;          // of the step that is worked on
-#pragma unroll
-  for (int u = 0; u < kAhead; ++u) {
-    if (from + u < to) issue(u, head, step);
-    next();
-  }
-  const char* tv = lds_v + wave * kRows * V::kRowBytes;
+  if (from < to) issue(0, head, step);
+  const char* tk = lds_kv[0] + wave * kRows * KV::kRowBytes;
+  const char* tv = lds_kv[1] + wave * kRows * KV::kRowBytes;
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) dk[d] = dv[d] = splat(0.0f);
 
   int buf = 0;
-  for (int32_t round = 0; round < rounds; ++round, buf = buf == kAhead ? 0 : buf + 1, i0 += kQueries) {
+  for (int32_t round = 0; round < rounds; ++round, buf ^= 1, i0 += kQueries) {
     const int32_t it = from + round;
     if (i0 >= p.m) i0 = first;
-    // This step's tiles have landed, of this wave: later steps' copies may be under way.
-    constexpr int kCopies = 2 * L::kCopies;
-    if (kAhead == 1 || it + 1 >= to) __builtin_amdgcn_s_waitcnt(kVmcnt0);
-    else if (wave < 2) __builtin_amdgcn_s_waitcnt(kVmcnt0 + kCopies + 1);
-    else __builtin_amdgcn_s_waitcnt(kVmcnt0 + kCopies);
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);         // this step's tiles have landed, of this wave
     lds_barrier();                               // of all; the last step's are done with
-    if (it + kAhead < to) issue(buf == 0 ? kAhead : buf - 1, head, step);
-    next();
+    if (++step == steps) step = 0, ++head;
+    if (it + 1 < to) issue(buf ^ 1, head, step);
     if (mine >= p.n || it >= to) continue;
 #pragma unroll 1
     for (int t = 0; t < kQueries / 32; ++t) {
@@ -258,7 +260,10 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
       const char* tg = lds[buf][1] + t * 32 * L::kRowBytes;
       f32x16 x = splat(0.0f), y;
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j) x = mfma<E>(row_frag<D>(tq, lane, 0, j), k[j], x);
+      for (int j = 0; j < D / 16; ++j) {
+        if constexpr (kInLds) x = mfma<E>(row_frag<D>(tq, lane, 0, j), row_frag<D>(tk, lane, 0, j), x);
+        else x = mfma<E>(row_frag<D>(tq, lane, 0, j), k[j], x);
+      }
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const f32x4 s = *reinterpret_cast<const f32x4*>(&stats[buf][1][32 * t + row_of(r, h)]);
@@ -267,7 +272,7 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
       }
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) {
-        if constexpr (kVInLds) y = mfma<E>(row_frag<D>(tg, lane, 0, j), row_frag<D>(tv, lane, 0, j), y);
+        if constexpr (kInLds) y = mfma<E>(row_frag<D>(tg, lane, 0, j), row_frag<D>(tv, lane, 0, j), y);
         else y = mfma<E>(row_frag<D>(tg, lane, 0, j), v[j], y);
       }
 #pragma unroll
@@ -277,6 +282,7 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
         for (int e = 0; e < 4; ++e)
           x[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r + e], a.scale2, -s[e]));
       }
+      if constexpr (kInLds) read_ahead<D / 8>();
       if (query + 32 > p.m || query + ahead < mine + kRows - 1) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -310,6 +316,7 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
           if constexpr (TWO) dk[d] = mfma<E>(q, rest, dk[d]);
         }
       }
+      if constexpr (kInLds) read_ahead<D / 8>();
     }
   }
   if constexpr (teams(D) > 1) {
