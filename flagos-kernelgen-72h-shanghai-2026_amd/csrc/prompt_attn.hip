@@ -118,6 +118,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention(Args a) {
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) x[t] = mfma<E>(row_frag<D>(lds[buf][0], lane, t, j), q[j], x[t]);
     }
+    read_ahead<4, 1, kKeys / 32 * (D / 16)>();
     if (tok + kKeys > all) {
 #pragma unroll
       for (int t = 0; t < kKeys / 32; ++t)
@@ -154,6 +155,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention(Args a) {
 #pragma unroll
       for (int t = 0; t < kKeys / 16; ++t)
         o[d] = mfma<E>(col_frag<D>(lds[buf][1], lane, d, t), w[t], o[d]);
+    read_ahead<8, 2, kKeys / 16 * (D / 32)>();
   }
   l = cross_sum(l);
   const int64_t row = p.row + i;

@@ -95,7 +95,8 @@ struct Tile {
 // 16 (4) bytes a lane from `rs` at voff + soff past the registers to LDS, lane by lane from `lds` on
 // (which m0 tells the instruction; it is put back, the compiler keeps it).  In assembly, so that only
 // the kernel's own waits are for it: of the builtin the compiler has every transposed read of LDS
-// wait for all copies under way, the ones for later steps among them.
+// wait for all copies under way, the ones for the next step among them (dk and dv of 8192 tokens,
+// 32 + 8 heads of 128: 1075 us, with the builtin 1145; the other kernels take as long with either).
 __device__ __forceinline__ void copy16(const u32x4& rs, char* lds, uint32_t voff, uint32_t soff) {
   uint32_t old;
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
@@ -180,6 +181,17 @@ __device__ __forceinline__ u32x4 col_frag(const char* tile, int lane, int d, int
     r[2 * u] = w[0], r[2 * u + 1] = w[1];
   }
   return r;
+}
+
+// The order of a stretch of N products: FIRST reads of LDS ahead of the first, EACH between any two.
+template <int FIRST, int EACH, int N>
+__device__ __forceinline__ void read_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+  }
 }
 
 // Registers 8 t .. of a result as the B operand of the next product.

@@ -160,17 +160,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_dq(Args a) {
 constexpr int teams(int64_t D) { return D == 256 ? 1 : 2; }
 constexpr int queries(int64_t D) { return D == 128 ? 32 : 64; }   // of a team in LDS at a time
 
-// The order of a stretch of N products: eight reads of LDS ahead of the first, two between any two.
-template <int N>
-__device__ __forceinline__ void read_ahead() {
-  __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-  }
-}
-
 template <int E, int D, bool TWO>
 __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(Args a) {
   constexpr int kQueries = queries(D);
@@ -282,7 +271,7 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
         for (int e = 0; e < 4; ++e)
           x[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r + e], a.scale2, -s[e]));
       }
-      if constexpr (kInLds) read_ahead<D / 8>();
+      if constexpr (kInLds) read_ahead<8, 2, D / 8>();
       if (query + 32 > p.m || query + ahead < mine + kRows - 1) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -316,7 +305,7 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
           if constexpr (TWO) dk[d] = mfma<E>(q, rest, dk[d]);
         }
       }
-      if constexpr (kInLds) read_ahead<D / 8>();
+      if constexpr (kInLds) read_ahead<8, 2, D / 8>();
     }
   }
   if constexpr (teams(D) > 1) {
