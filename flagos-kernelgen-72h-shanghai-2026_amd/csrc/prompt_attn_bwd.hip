@@ -10,6 +10,8 @@
 //                 dK^T += Q^T dS.  Two teams of four waves share the steps of a tile and join
 //                 their sums through LDS; where there are few workgroups, the steps are cut into
 //                 parts of their own sums besides, which prompt_join adds up in order.
+// Calls of few rows, where a launch is what counts, take both passes in one (prompt_bwd_small): the
+// second then works out lse and delta of its queries by itself.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -36,11 +38,12 @@ struct Args {
   uint16_t* dq;
   uint16_t* dk;
   uint16_t* dv;
-  float* lse2;                       // [Hq, T]; +inf for a query without keys
+  float* lse2;                       // [Hq, T]; +inf for a query without keys.  Null: small calls
   float* delta;                      // [Hq, T], negative
   float* part;                       // [parts][Tk][H][D] of dk, then of dv
   int64_t dos[2], qs[2], ks[2], vs[2], dqs[2], dks[2], dvs[2];   // {token, head} strides, elements
   int32_t Hq, H, group, fill, parts;
+  int32_t dq_items;                  // small calls: workgroups of the first pass
   float scale, scale2;               // sm_scale, and times log2(e)
 };
 
@@ -55,14 +58,21 @@ __device__ __forceinline__ void fill_tail(uint16_t* out, const int64_t (&s)[2], 
   }
 }
 
+// An lse in units of log 2, as the exponentials take it.
+__device__ __forceinline__ float lse_in_2(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
+
+template <int D>
+struct DqLds {
+  char tile[2][2][Tile<D>::kBytes];
+};
+
 template <int E, int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void prompt_dq(Args a) {
-  using L = Tile<D>;
-  __shared__ __align__(16) char lds[2][2][L::kBytes];
+__device__ __forceinline__ void run_dq(const Args& a, int item, DqLds<D>& shared) {
+  auto& lds = shared.tile;
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int wave = scalar((int)(threadIdx.x >> 6));
   // Workgroup b runs on XCD b % 8: heads that share keys stay on one.
-  const int item = (int)blockIdx.x, kvh = item % a.H, rest = item / a.H;
+  const int kvh = item % a.H, rest = item / a.H;
   const int hq = kvh * a.group + rest % a.group;
   const Place p = place_of<true>(a.queries, rest / a.group);
   if (p.b < 0) {
@@ -106,8 +116,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_dq(Args a) {
   }
   delta = cross_sum(delta);
   const float lse = a.lse[(int64_t)hq * a.queries.T + row];
-  const float lse2 = seen > 0 ? lse * kLog2e : INFINITY;
-  if (h == 0 && i < p.n) {
+  const float lse2 = lse_in_2(lse);
+  if (a.lse2 && h == 0 && i < p.n) {
     a.lse2[(int64_t)hq * a.queries.T + row] = lse2;
     a.delta[(int64_t)hq * a.queries.T + row] = delta;
   }
@@ -156,24 +166,39 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_dq(Args a) {
   store_row<E, D>(a.dq + (int64_t)row * a.dqs[0] + (int64_t)hq * a.dqs[1], h, dq, a.scale, i < p.n);
 }
 
+template <int E, int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void prompt_dq(Args a) {
+  __shared__ __align__(16) DqLds<D> lds;
+  run_dq<E, D>(a, (int)blockIdx.x, lds);
+}
+
 // Teams of four waves in a workgroup, which share its steps and join their sums through LDS.
-constexpr int teams(int64_t D) { return D == 256 ? 1 : 2; }
+constexpr int teams(int64_t D, bool small) { return D == 256 || small ? 1 : 2; }
 constexpr int queries(int64_t D) { return D == 128 ? 32 : 64; }   // of a team in LDS at a time
 
-template <int E, int D, bool TWO>
-__global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(Args a) {
-  constexpr int kQueries = queries(D);
+template <int D, bool SMALL>
+struct DkdvLds {
+  static constexpr bool kInLds = D <= 128;                // k and v; else in registers
+  char tile[teams(D, SMALL)][2][2][Tile<D, queries(D)>::kBytes];
+  char kv[2][kInLds ? Tile<D, kTile>::kBytes : 16];
+  float stats[teams(D, SMALL)][2][2][queries(D)];         // lse2, -delta
+};
+
+// SMALL: one team, lse2 and delta worked out here, and two terms (of 16 bits each) of P and dS, as dq
+// always has.  One leaves dk and dv 1.4 times the error that their own rounding makes, as long as
+// there are many roundings to average over, and takes a quarter of the products less.
+template <int E, int D, bool SMALL>
+__device__ __forceinline__ void run_dkdv(const Args& a, int item, DkdvLds<D, SMALL>& shared) {
+  constexpr int kQueries = queries(D), kTeams = teams(D, SMALL);
   using L = Tile<D, kQueries>;
   using KV = Tile<D, kTile>;
-  constexpr bool kInLds = D <= 128;                       // k and v; else in registers
-  __shared__ __align__(16) char lds_all[teams(D)][2][2][L::kBytes];
-  __shared__ __align__(16) char lds_kv[2][kInLds ? KV::kBytes : 16];
-  __shared__ __align__(16) float stats_all[teams(D)][2][2][kQueries];   // lse2, -delta
+  constexpr bool kInLds = DkdvLds<D, SMALL>::kInLds;
+  auto& lds_kv = shared.kv;
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int waves = scalar((int)(threadIdx.x >> 6)), wave = waves % kWaves, team = waves / kWaves;
-  auto& lds = lds_all[team];
-  auto& stats = stats_all[team];
-  const int item = (int)blockIdx.x, kvh = item % a.H, rest = item / a.H;
+  auto& lds = shared.tile[team];
+  auto& stats = shared.stats[team];
+  const int kvh = item % a.H, rest = item / a.H;
   const int part = rest % a.parts;
   const Place p = place_of<false>(a.keys, rest / a.parts);
   if (p.b < 0) {
@@ -188,7 +213,7 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
   const int32_t steps = first < p.m ? (p.m - first + kQueries - 1) / kQueries : 0;
   // Steps of all heads in a row, head by head: this part's share, and its longest team's number.
   const int64_t total = (int64_t)steps * a.group;
-  const int32_t shares = a.parts * teams(D), share = part * teams(D) + team;
+  const int32_t shares = a.parts * kTeams, share = part * kTeams + team;
   const int32_t from = (int32_t)(total * share / shares), to = (int32_t)(total * (share + 1) / shares);
   const int32_t rounds = (int32_t)((total + shares - 1) / shares);
 
@@ -203,12 +228,46 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
     y.base += (int64_t)head * a.dos[1] * 2;
     x.issue(lds[buf][0], wave, i0, p.m - 1);
     y.issue(lds[buf][1], wave, i0, p.m - 1);
-    if (wave < 2 && lane < kQueries) {
+    if (!SMALL && wave < 2 && lane < kQueries) {
       const int64_t at = (int64_t)(kvh * a.group + head) * a.keys.Tother + p.other + i0;
       const int32_t most = p.m - 1 - i0;
       copy4(buffer_at((wave == 0 ? a.lse2 : a.delta) + at),
             reinterpret_cast<char*>(wave == 0 ? stats[buf][0] : stats[buf][1]),
             (uint32_t)(lane < most ? lane : most) * 4u);
+    }
+  };
+  // SMALL: dout, out and lse of the step under way; kThreads have a row.
+  constexpr int kThreads = 64 * kWaves / kQueries, kOwn = SMALL ? D / kThreads / 8 : 1;
+  const int own_row = (int)threadIdx.x / kThreads, own_at = (int)threadIdx.x % kThreads * (D / kThreads);
+  u32x4 own_g[kOwn], own_o[kOwn];
+  float own_lse = 0.0f;
+  auto load_stats = [&](int32_t head, int32_t step) {
+    const int32_t i = first + step * kQueries + own_row;
+    const int64_t row = p.other + (i < p.m ? i : p.m - 1);
+    const int hq = kvh * a.group + head;
+    const uint16_t* g = a.dout + row * a.dos[0] + (int64_t)hq * a.dos[1] + own_at;
+    const uint16_t* o = a.out + (row * a.Hq + hq) * D + own_at;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      own_g[i] = *reinterpret_cast<const u32x4*>(g + 8 * i);
+      own_o[i] = *reinterpret_cast<const u32x4*>(o + 8 * i);
+    }
+    own_lse = a.lse[(int64_t)hq * a.keys.Tother + row];
+  };
+  auto store_stats = [&](int buf) {
+    float delta = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        delta = __builtin_fmaf(-lo16<E>(own_g[i][e]), lo16<E>(own_o[i][e]), delta);
+        delta = __builtin_fmaf(-hi16<E>(own_g[i][e]), hi16<E>(own_o[i][e]), delta);
+      }
+#pragma unroll
+    for (int d = 1; d < kThreads; d *= 2) delta += __shfl_xor(delta, d);
+    if (own_at == 0) {
+      stats[buf][0][own_row] = lse_in_2(own_lse);
+      stats[buf][1][own_row] = delta;
     }
   };
   u32x4 k[kInLds ? 1 : D / 16], v[kInLds ? 1 : D / 16];
@@ -225,7 +284,13 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
     cv.issue(lds_kv[0], wave, k0, p.n - 1);
   }
   int32_t i0 = first + step * kQueries;          // of the step that is worked on
-  if (from < to) issue(0, head, step);
+  if (from < to) {
+    issue(0, head, step);
+    if constexpr (SMALL) {
+      load_stats(head, step);
+      store_stats(0);
+    }
+  }
   const char* tk = lds_kv[0] + wave * kRows * KV::kRowBytes;
   const char* tv = lds_kv[1] + wave * kRows * KV::kRowBytes;
   f32x16 dk[D / 32], dv[D / 32];
@@ -239,12 +304,14 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
     __builtin_amdgcn_s_waitcnt(kVmcnt0);         // this step's tiles have landed, of this wave
     lds_barrier();                               // of all; the last step's are done with
     if (++step == steps) step = 0, ++head;
-    if (it + 1 < to) issue(buf ^ 1, head, step);
-    if (mine >= p.n || it >= to) continue;
+    if (it + 1 < to) {
+      issue(buf ^ 1, head, step);
+      if constexpr (SMALL && kInLds) load_stats(head, step);
+    }
 #pragma unroll 1
     for (int t = 0; t < kQueries / 32; ++t) {
       const int32_t query = i0 + 32 * t;
-      if (query >= p.m || query + 31 + ahead < mine) continue;
+      if (mine >= p.n || it >= to || query >= p.m || query + 31 + ahead < mine) continue;
       const char* tq = lds[buf][0] + t * 32 * L::kRowBytes;
       const char* tg = lds[buf][1] + t * 32 * L::kRowBytes;
       f32x16 x = splat(0.0f), y;
@@ -283,12 +350,12 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
       for (int u = 0; u < 2; ++u) {
         const u32x4 w = pack8<E>(x, u);
         u32x4 rest;
-        if constexpr (TWO) rest = pack_rest8<E>(x, u, w);
+        if constexpr (SMALL) rest = pack_rest8<E>(x, u, w);
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
           const u32x4 g = col_frag<D>(tg, lane, d, u);
           dv[d] = mfma<E>(g, w, dv[d]);
-          if constexpr (TWO) dv[d] = mfma<E>(g, rest, dv[d]);
+          if constexpr (SMALL) dv[d] = mfma<E>(g, rest, dv[d]);
         }
       }
 #pragma unroll
@@ -297,21 +364,25 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
       for (int u = 0; u < 2; ++u) {
         const u32x4 w = pack8<E>(x, u);
         u32x4 rest;
-        if constexpr (TWO) rest = pack_rest8<E>(x, u, w);
+        if constexpr (SMALL) rest = pack_rest8<E>(x, u, w);
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
           const u32x4 q = col_frag<D>(tq, lane, d, u);
           dk[d] = mfma<E>(q, w, dk[d]);
-          if constexpr (TWO) dk[d] = mfma<E>(q, rest, dk[d]);
+          if constexpr (SMALL) dk[d] = mfma<E>(q, rest, dk[d]);
         }
       }
       if constexpr (kInLds) read_ahead<8, 2, D / 8>();
     }
+    if (SMALL && it + 1 < to) {
+      if constexpr (SMALL && !kInLds) load_stats(head, step);   // no registers to hold them that long
+      store_stats(buf ^ 1);
+    }
   }
-  if constexpr (teams(D) > 1) {
+  if constexpr (kTeams > 1) {
     // The second team hands its sums over, dk's, then dv's.
-    f32x4* sums = reinterpret_cast<f32x4*>(lds_all);
-    static_assert(sizeof(lds_all) >= kWaves * D / 32 * 4 * 64 * sizeof(f32x4), "room for one of them");
+    f32x4* sums = reinterpret_cast<f32x4*>(shared.tile);
+    static_assert(sizeof(shared.tile) >= kWaves * D / 32 * 4 * 64 * sizeof(f32x4), "room for one of them");
     auto hand = [&](f32x16 (&x)[D / 32]) {
       __syncthreads();
 #pragma unroll
@@ -356,6 +427,22 @@ __global__ __launch_bounds__(64 * kWaves * teams(D), teams(D)) void prompt_dkdv(
   }
 }
 
+template <int E, int D>
+__global__ __launch_bounds__(64 * kWaves * teams(D, false), teams(D, false)) void prompt_dkdv(Args a) {
+  __shared__ __align__(16) DkdvLds<D, false> lds;
+  run_dkdv<E, D, false>(a, (int)blockIdx.x, lds);
+}
+
+template <int E, int D>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_bwd_small(Args a) {
+  __shared__ __align__(16) union {
+    DqLds<D> dq;
+    DkdvLds<D, true> dkdv;
+  } lds;
+  if ((int)blockIdx.x < a.dq_items) run_dq<E, D>(a, (int)blockIdx.x, lds.dq);
+  else run_dkdv<E, D, true>(a, (int)blockIdx.x - a.dq_items, lds.dkdv);
+}
+
 // Sums of the parts.  A thread has 8 elements of dk or of dv.
 template <int E>
 __global__ __launch_bounds__(256) void prompt_join(Args a, int32_t D) {
@@ -391,25 +478,25 @@ int check_bwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int
   const int st = check_sizes(B, T, Tk, Hq, H, D);
   if (st != FAGQ_OK) return st;
   // With all the parts there may be, and the joining kernel's workgroups.
-  const bool large = tile_slots(Tk, B) * H * kMostParts >= kMostGroups || Tk * H * D / 1024 >= kMostGroups - 1;
+  const bool large = tile_slots(Tk, B) * H * kMostParts + 4096 + B >= kMostGroups || Tk * H * D / 1024 >= kMostGroups - 1;
   return large ? FAGQ_E_TOO_LARGE : FAGQ_OK;
 }
+
+// Calls of few rows: both passes in one launch (5 sequences of up to 77 tokens, 12 heads of 64: SMALL_US us,
+// two launches 14.0), and two terms cost nothing there.
+bool small(int64_t T, int64_t Hq) { return T * Hq <= 4096; }
 
 // Parts of a key tile's steps: as many as let the tile with most of them, twice the average, not take
 // longer than all together, but four steps for each team.
 int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
   const int64_t groups = std::max<int64_t>(1, (Tk + kTile - 1) / kTile * H);
   const int64_t steps = Hq / H * ((T + queries(D) - 1) / queries(D)) / std::max<int64_t>(1, B);
-  return std::max<int64_t>(1, std::min<int64_t>({2 * kCUs / groups, steps / (4 * teams(D)), kMostParts}));
+  return std::max<int64_t>(
+      1, std::min<int64_t>({2 * kCUs / groups, steps / (4 * teams(D, small(T, Hq))), kMostParts}));
 }
 
-// Whether dk and dv take two terms (of 16 bits each) of P and dS, as dq always does.  One leaves them
-// 1.4 times the error that their own rounding makes, as long as there are many roundings to average
-// over; a call of few rows has few, and costs the same either way.
-bool two_terms(int64_t T, int64_t Hq) { return T * Hq <= 4096; }
-
 int64_t bytes_for(int64_t parts, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
-  const int64_t stats = (2 * Hq * T * 4 + 15) / 16 * 16;
+  const int64_t stats = small(T, Hq) ? 0 : (2 * Hq * T * 4 + 15) / 16 * 16;
   return stats + (parts > 1 ? 2 * parts * Tk * H * D * 4 : 0);
 }
 
@@ -419,11 +506,17 @@ const void* dq_for(int64_t D) {
          : D == 128 ? reinterpret_cast<const void*>(&prompt_dq<E, 128>)
                     : reinterpret_cast<const void*>(&prompt_dq<E, 256>);
 }
-template <int E, bool TWO>
+template <int E>
 const void* dkdv_for(int64_t D) {
-  return D == 64    ? reinterpret_cast<const void*>(&prompt_dkdv<E, 64, TWO>)
-         : D == 128 ? reinterpret_cast<const void*>(&prompt_dkdv<E, 128, TWO>)
-                    : reinterpret_cast<const void*>(&prompt_dkdv<E, 256, TWO>);
+  return D == 64    ? reinterpret_cast<const void*>(&prompt_dkdv<E, 64>)
+         : D == 128 ? reinterpret_cast<const void*>(&prompt_dkdv<E, 128>)
+                    : reinterpret_cast<const void*>(&prompt_dkdv<E, 256>);
+}
+template <int E>
+const void* small_for(int64_t D) {
+  return D == 64    ? reinterpret_cast<const void*>(&prompt_bwd_small<E, 64>)
+         : D == 128 ? reinterpret_cast<const void*>(&prompt_bwd_small<E, 128>)
+                    : reinterpret_cast<const void*>(&prompt_bwd_small<E, 256>);
 }
 
 }  // namespace
@@ -497,8 +590,12 @@ FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, c
   a.queries = {cu_seqlens, cu_k, (int32_t)B, (int32_t)T, (int32_t)Tk};
   a.keys = {cu_k, cu_seqlens, (int32_t)B, (int32_t)Tk, (int32_t)T};
   a.dq = static_cast<uint16_t*>(dq), a.dk = static_cast<uint16_t*>(dk), a.dv = static_cast<uint16_t*>(dv);
-  a.lse2 = static_cast<float*>(workspace), a.delta = a.lse2 + Hq * T;
-  a.part = a.lse2 + (2 * Hq * T + 3) / 4 * 4;
+  const bool one_launch = small(T, Hq);
+  a.part = static_cast<float*>(workspace);
+  if (!one_launch) {
+    a.lse2 = a.part, a.delta = a.lse2 + Hq * T;
+    a.part += (2 * Hq * T + 3) / 4 * 4;
+  }
   int64_t(*to[7])[2] = {&a.dos, &a.qs, &a.ks, &a.vs, &a.dqs, &a.dks, &a.dvs};
   for (int i = 0; i < 7; ++i) (*to[i])[0] = strides[2 * i], (*to[i])[1] = strides[2 * i + 1];
   a.Hq = (int32_t)Hq, a.H = (int32_t)H, a.group = (int32_t)(Hq / H);
@@ -508,17 +605,20 @@ FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, c
   void* args[] = {&a, &dim};
   const bool bf16 = dtype == FAGQ_DT_BF16;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (T > 0) {
-    const int ls = launch_kernel(bf16 ? dq_for<ET_BF16>(D) : dq_for<ET_F16>(D),
-                                 dim3((unsigned)(tile_slots(T, B) * Hq)), dim3(64 * kWaves), args, 0, st);
-    if (ls != FAGQ_OK) return ls;
+  const int64_t dq_items = tile_slots(T, B) * Hq, dkdv_items = Tk > 0 ? tile_slots(Tk, B) * H * parts : 0;
+  if (one_launch) {
+    a.dq_items = T > 0 ? (int32_t)dq_items : 0;
+    const int ls = launch_kernel(bf16 ? small_for<ET_BF16>(D) : small_for<ET_F16>(D),
+                                 dim3((unsigned)(a.dq_items + dkdv_items)), dim3(64 * kWaves), args, 0, st);
+    if (ls != FAGQ_OK || parts == 1) return ls;
+  } else {
+    int ls = launch_kernel(bf16 ? dq_for<ET_BF16>(D) : dq_for<ET_F16>(D), dim3((unsigned)dq_items),
+                           dim3(64 * kWaves), args, 0, st);
+    if (ls != FAGQ_OK || dkdv_items == 0) return ls;
+    ls = launch_kernel(bf16 ? dkdv_for<ET_BF16>(D) : dkdv_for<ET_F16>(D), dim3((unsigned)dkdv_items),
+                       dim3((unsigned)(64 * kWaves * teams(D, false))), args, 0, st);
+    if (ls != FAGQ_OK || parts == 1) return ls;
   }
-  if (Tk == 0) return FAGQ_OK;
-  const int ls = launch_kernel(two_terms(T, Hq) ? (bf16 ? dkdv_for<ET_BF16, true>(D) : dkdv_for<ET_F16, true>(D))
-                                                : (bf16 ? dkdv_for<ET_BF16, false>(D) : dkdv_for<ET_F16, false>(D)),
-                               dim3((unsigned)(tile_slots(Tk, B) * H * parts)),
-                               dim3((unsigned)(64 * kWaves * teams(D))), args, 0, st);
-  if (ls != FAGQ_OK || parts == 1) return ls;
   const int64_t items = 2 * Tk * H * (D / 8);
   return launch_kernel(bf16 ? reinterpret_cast<const void*>(&prompt_join<ET_BF16>)
                             : reinterpret_cast<const void*>(&prompt_join<ET_F16>),
