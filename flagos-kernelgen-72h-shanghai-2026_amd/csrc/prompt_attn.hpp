@@ -117,7 +117,7 @@ __device__ __forceinline__ void copy4(const u32x4& rs, char* lds, uint32_t voff)
 __device__ __forceinline__ u32x4 buffer_at(const void* p) {
   const uintptr_t v = reinterpret_cast<uintptr_t>(p);
   return {(uint32_t)scalar((int32_t)(uint32_t)v), (uint32_t)scalar((int32_t)(uint32_t)(v >> 32)) & 0xffffu,
-          0x7fffffffu, kRsrcWord3};
+          0xffffffffu, kRsrcWord3};
 }
 
 // Copies rows [first, first + ROWS) of one head, row `last` in place of those behind it, from HBM
