@@ -264,10 +264,15 @@ __device__ __forceinline__ int32_t clamped(int32_t v, int32_t most) {
   return v < 0 ? 0 : v < most ? v : most;
 }
 
-// Tile number `slot` of all sequences': from the last one backwards (REVERSED), where late tiles
-// see most, or from the first on.  Lane l counts the tiles of sequences l n .. (l + 1) n - 1; up to 64
-// sequences it has everything about its own in registers, and one trip to memory is enough.
-template <bool REVERSED>
+// Tile number `slot` of all sequences'.  Late tiles have most work (LATE: tiles of queries), or early
+// ones: of up to 64 sequences of up to kLevels tiles those with most come first, whichever sequence
+// they are of, so that the last workgroups to start are the shortest (32 + 8 heads of 128, us, so /
+// sequence by sequence: dk and dv of 16 sequences of 166 to 1000 tokens 141 / 180, four prompts of 800
+// 36 / 42).  Of more, or longer ones, the tiles come sequence by sequence, each one's in that order.  Lane l
+// counts the tiles of sequences l n .. (l + 1) n - 1; up to 64 sequences it has everything about its
+// own in registers, and one trip to memory is enough.
+constexpr int kLevels = 64;
+template <bool LATE>
 __device__ __forceinline__ Place place_of(const Sequences& s, int32_t slot) {
   const int lane = threadIdx.x & 63;
   const int each = (s.B + 63) / 64;
@@ -275,7 +280,7 @@ __device__ __forceinline__ Place place_of(const Sequences& s, int32_t slot) {
     int32_t row, n, other, m;
   };
   auto sequence = [&](int i) {                   // i: in the order of the tiles
-    const int b = REVERSED ? s.B - 1 - i : i;
+    const int b = LATE ? s.B - 1 - i : i;
     const int32_t lo = clamped(s.cu[b], s.T), hi = clamped(s.cu[b + 1], s.T);
     const int32_t lo2 = clamped(s.other[b], s.Tother), hi2 = clamped(s.other[b + 1], s.Tother);
     return Sequence{lo, hi > lo ? hi - lo : 0, lo2, hi2 > lo2 ? hi2 - lo2 : 0};
@@ -302,10 +307,32 @@ __device__ __forceinline__ Place place_of(const Sequences& s, int32_t slot) {
     p.tile = slot - total;
     return p;
   }
-  const uint64_t here = __ballot(slot >= upto - count && slot < upto);
-  const int l = (int)__builtin_ctzll(here);
-  int32_t at = slot - __builtin_amdgcn_readlane(upto - count, l);
-  int i = l * each;
+  int l, i;
+  int32_t at;
+  const bool level = each == 1 && __ballot(count > kLevels) == 0 && __popcll(__ballot(count > 0)) > 1;
+  if (level) {
+    // Tile `at` counted from the one with most work: tiles with as many behind them in their sequence
+    // as a level says, from the highest level on.
+    int32_t left = slot, most = 0;
+#pragma unroll
+    for (int bit = kLevels; bit > 0; bit /= 2)
+      if (__ballot(count >= most + bit)) most += bit;
+    uint64_t mask = 0;
+    for (at = most - 1; at >= 0; --at) {         // ends before: slot < total
+      mask = __ballot(count > at);
+      const int n = __popcll(mask);
+      if (left < n) break;
+      left -= n;
+    }
+    const bool mine = (mask >> lane & 1) && __popcll(mask & ((1ull << lane) - 1)) == left;
+    l = i = (int)__builtin_ctzll(__ballot(mine));
+    at = __builtin_amdgcn_readlane(count, l) - 1 - at;
+  } else {
+    const uint64_t here = __ballot(slot >= upto - count && slot < upto);
+    l = (int)__builtin_ctzll(here);
+    at = slot - __builtin_amdgcn_readlane(upto - count, l);
+    i = l * each;
+  }
   if (each == 1) {
     p.row = __builtin_amdgcn_readlane(mine.row, l), p.n = __builtin_amdgcn_readlane(mine.n, l);
     p.other = __builtin_amdgcn_readlane(mine.other, l), p.m = __builtin_amdgcn_readlane(mine.m, l);
@@ -317,8 +344,8 @@ __device__ __forceinline__ Place place_of(const Sequences& s, int32_t slot) {
     }
     p.row = scalar(q.row), p.n = scalar(q.n), p.other = scalar(q.other), p.m = scalar(q.m);
   }
-  p.b = REVERSED ? s.B - 1 - i : i;
-  p.tile = REVERSED ? tiles_of(p.n) - 1 - at : at;
+  p.b = LATE ? s.B - 1 - i : i;
+  p.tile = LATE ? tiles_of(p.n) - 1 - at : at;
   return p;
 }
 
