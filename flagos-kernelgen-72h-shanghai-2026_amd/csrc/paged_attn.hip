@@ -291,6 +291,20 @@ Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t pr
     cut(most, B * H * p.tiles, key_cost(p.R), part_cost(p.rows, D), &p.chunk, &p.chunks);
     if (p.chunks < 1) p.chunks = 1;     // rows without keys are written all the same
     p.items = B * H * p.tiles * p.chunks;
+    // Drafts' own keys are few, but their workgroups may make a second round.  The prefix is cut into
+    // fewer chunks where that leaves one round and adds little to a chunk: of 25 sizes with such a cut
+    // 18 are within this bound, at 0.90 of the time (8 x 63 drafts behind 2047 shared tokens, 16 + 4
+    // heads of 64, chunks of 1024 / 512 keys: 24.5 / 31 us), and 7 beyond it, at 1.12 (6 x 48 behind
+    // 5553, 10 + 2 heads of 128, 1920 / 1152: 41.2 / 34.9).
+    const int64_t fit = tree && p.prefix_items > 0 ? (kSlots - p.items) / (H * p.prefix_tiles) : 0;
+    if (p.prefix_items <= kSlots && fit < p.prefix_chunks && 2 * fit >= p.prefix_chunks) {
+      const int64_t chunk = ((prefix_len + fit - 1) / fit + kRound - 1) / kRound * kRound;
+      if ((chunk - p.prefix_chunk) * key_cost(p.RP) <= 4 * kFixed) {
+        p.prefix_chunk = chunk;
+        p.prefix_chunks = (prefix_len + chunk - 1) / chunk;
+        p.prefix_items = H * p.prefix_tiles * p.prefix_chunks;
+      }
+    }
     p.row_parts = p.prefix_chunks + p.chunks;
     p.parts = p.row_parts > 1 ? p.rows * p.row_parts : 0;
   } else {
