@@ -223,8 +223,8 @@ int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t D) {
 
 int check_fwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
   const int st = check_sizes(B, T, Tk, Hq, H, D);
-  return st != FAGQ_OK ? st : tile_slots(T, B) * Hq * parts_for(B, T, Tk, Hq, D) >= kMostGroups ? FAGQ_E_TOO_LARGE
-                                                                                               : FAGQ_OK;
+  if (st != FAGQ_OK) return st;
+  return tile_slots(T, B) * Hq * parts_for(B, T, Tk, Hq, D) >= kMostGroups ? FAGQ_E_TOO_LARGE : FAGQ_OK;
 }
 
 int64_t bytes_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t D) {
@@ -293,7 +293,8 @@ FAGQ_API int fagq_prompt_attention_launch(const void* q, const void* k, const vo
     if (overlap(out, nout, ins[i], nin[i]) || overlap(lse, nlse, ins[i], nin[i]) ||
         overlap(workspace, need, ins[i], nin[i]))
       return FAGQ_E_ALIAS;
-  if (overlap(out, nout, lse, nlse) || overlap(workspace, need, out, nout) || overlap(workspace, need, lse, nlse))
+  if (overlap(out, nout, lse, nlse) || overlap(workspace, need, out, nout) ||
+      overlap(workspace, need, lse, nlse))
     return FAGQ_E_ALIAS;
   const int dcheck = device_check();
   if (dcheck != FAGQ_OK) return dcheck;

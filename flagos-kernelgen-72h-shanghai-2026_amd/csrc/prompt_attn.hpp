@@ -28,6 +28,7 @@ constexpr int kTile = kRows * kWaves;           // of a workgroup
 constexpr int kStep = 64;                       // rows of the other side that are in LDS at a time
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int64_t kMostGroups = 1ll << 24;      // a grid of 2^32 threads is too large
+constexpr int64_t kMostTokens = (1ll << 31) - 1024;   // a tile past the last token has 32-bit numbers
 constexpr int kVmcnt0 = 0x0F70;                 // s_waitcnt vmcnt(0), other counters not waited; + n < 16
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -55,7 +56,6 @@ __device__ __forceinline__ f32x16 splat(float v) {
   for (int i = 0; i < 16; ++i) r[i] = v;
   return r;
 }
-
 
 __device__ __forceinline__ int32_t scalar(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -268,9 +268,9 @@ __device__ __forceinline__ int32_t clamped(int32_t v, int32_t most) {
 // ones: of up to 64 sequences of up to kLevels tiles those with most come first, whichever sequence
 // they are of, so that the last workgroups to start are the shortest (32 + 8 heads of 128, us, so /
 // sequence by sequence: dk and dv of 16 sequences of 166 to 1000 tokens 141 / 180, four prompts of 800
-// 36 / 42).  Of more, or longer ones, the tiles come sequence by sequence, each one's in that order.  Lane l
-// counts the tiles of sequences l n .. (l + 1) n - 1; up to 64 sequences it has everything about its
-// own in registers, and one trip to memory is enough.
+// 36 / 42).  Of more, or longer ones, the tiles come sequence by sequence, each one's in that order.
+// Lane l counts the tiles of sequences l n .. (l + 1) n - 1; up to 64 sequences it has everything about
+// its own in registers, and one trip to memory is enough.
 constexpr int kLevels = 64;
 template <bool LATE>
 __device__ __forceinline__ Place place_of(const Sequences& s, int32_t slot) {
@@ -293,7 +293,9 @@ __device__ __forceinline__ Place place_of(const Sequences& s, int32_t slot) {
   int32_t count = 0;
   for (int i = first; i < stop; ++i) {
     mine = sequence(i);
-    count += tiles_of(mine.n);
+    // Lengths that overlap may add up to any number: cut, so that 64 lanes' do not pass 31 bits.  No
+    // grid has as many workgroups.
+    count = clamped(count + tiles_of(mine.n), (int32_t)kMostGroups);
   }
   int32_t upto = count;
 #pragma unroll
@@ -401,7 +403,7 @@ inline int check_strides(const int64_t* strides, int n) {
 inline int check_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
   if (B < 0 || T < 0 || Tk < 0 || H < 1 || Hq < H || Hq % H != 0 || (D != 64 && D != 128 && D != 256))
     return FAGQ_E_SHAPE;
-  if (B > (1ll << 24) || T > (1ll << 31) - 1 || Tk > (1ll << 31) - 1 || Hq > 4096 ||
+  if (B > (1ll << 24) || T > kMostTokens || Tk > kMostTokens || Hq > 4096 ||
       tile_slots(T, B) * Hq >= kMostGroups)
     return FAGQ_E_TOO_LARGE;
   return FAGQ_OK;

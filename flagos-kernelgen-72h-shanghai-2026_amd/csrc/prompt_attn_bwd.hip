@@ -478,12 +478,13 @@ int check_bwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int
   const int st = check_sizes(B, T, Tk, Hq, H, D);
   if (st != FAGQ_OK) return st;
   // With all the parts there may be, and the joining kernel's workgroups.
-  const bool large = tile_slots(Tk, B) * H * kMostParts + 16384 + B * Hq >= kMostGroups || Tk * H * D / 1024 >= kMostGroups - 1;
+  const bool large = tile_slots(Tk, B) * H * kMostParts + 16384 + B * Hq >= kMostGroups ||
+                     Tk * H * D / 1024 >= kMostGroups - 1;
   return large ? FAGQ_E_TOO_LARGE : FAGQ_OK;
 }
 
-// Calls of few rows: both passes in one launch, with one team and two terms (32 + 8 heads of 128, us, in one
-// launch / in two: 1 token 15 / 17, 200 tokens 26 / 36, 4 x 128 30 / 34, 4 x 200 58 / 41).
+// Calls of few rows: both passes in one launch, with one team and two terms (32 + 8 heads of 128, us,
+// in one launch / in two: 1 token 15 / 17, 200 tokens 26 / 36, 4 x 128 30 / 34, 4 x 200 58 / 41).
 bool small(int64_t T, int64_t Hq) { return T * Hq <= 16384; }
 
 // Parts of a key tile's steps: as many as let the tile with most of them, twice the average, not take

@@ -8,8 +8,8 @@ Layout (contiguous tensors, ``empty_kv_cache`` allocates them):
 A value is ``code * scale``, one scale for each group of G values of a token's head row, in the
 formats of ``fused_add_rmsnorm_group_quant``.  ``kv_cache_write`` quantises keys and values into
 slots (page * page_size + offset), ``kv_cache_read`` gathers the pages of a ragged batch, and
-``paged_attention`` and, for drafted trees, ``paged_tree_attention`` attend over them.  The kernels are libfagq.so's (include/fagq_cache.h);
-there is no fallback.
+``paged_attention`` and, for drafted trees, ``paged_tree_attention`` attend over them.  The kernels
+are libfagq.so's (include/fagq_cache.h); there is no fallback.
 
 No counterpart in the reference repository; the page tables are those that
 ``dsa_topk_page_table_transform`` reads

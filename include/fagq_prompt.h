@@ -49,8 +49,8 @@ enum fagq_prompt_bwd_fill { FAGQ_FILL_DQ = 1, FAGQ_FILL_DK = 2, FAGQ_FILL_DV = 4
  * [T, Hq, D] contiguous; lse fp32 [Hq, T], or null.  k and v may be null where Tk
  * is 0.  16-byte aligned, but lse and the lengths 4.  Workspace: 16-byte aligned,
  * of fagq_prompt_attention_workspace_bytes (0: may be null); calls that may overlap
- * need one each.  FAGQ_E_TOO_LARGE (workspace: -1) for 2^24 workgroups and more:
- * (T / 128 + B) Hq of them at least. */
+ * need one each.  FAGQ_E_TOO_LARGE (workspace: -1) for more than 2^31 - 1024 tokens,
+ * and for 2^24 workgroups and more: (T / 128 + B) Hq of them at least. */
 FAGQ_API int64_t fagq_prompt_attention_workspace_bytes(int64_t B, int64_t T, int64_t Tk,
                                                        int64_t Hq, int64_t H, int64_t D);
 FAGQ_API int fagq_prompt_attention_launch(const void* q, const void* k, const void* v,

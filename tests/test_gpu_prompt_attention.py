@@ -192,6 +192,19 @@ def test_lengths_of_any_value(pkg, gpu, cu):
         assert all(bool((t[:32] == 3.0).all()) and bool((t[122:] == 3.0).all()) for t in buf)
 
 
+def test_lengths_that_add_up_to_any_number(pkg, gpu):
+    """65536 sequences of which every second one claims all of 2^24 rows: 2^32 tiles."""
+    T, B = 1 << 24, 1 << 16
+    note("overlapping sequences")
+    buf = torch.full((T + 64, 1, 64), 3.0, dtype=BF16, device=gpu)
+    q, k = torch.zeros(T, 1, 64, dtype=BF16, device=gpu), torch.zeros(8, 1, 64, dtype=BF16, device=gpu)
+    cu = torch.tensor([0, T], dtype=torch.int32, device=gpu).repeat(B // 2 + 1)[:B + 1].contiguous()
+    pkg.prompt_attention(q, k, k, cu, 0.1, cu_seqlens_k=torch.zeros_like(cu), out=buf[32:T + 32])
+    torch.cuda.synchronize()
+    assert bool((buf[:32] == 3.0).all()) and bool((buf[T + 32:] == 3.0).all())
+    assert bool(((buf == 0.0) | (buf == 3.0)).all()) and bool((buf == 0.0).any())
+
+
 @pytest.mark.parametrize("lens,Hq,H,D", [([300, 20, 0], 4, 1, 128), ([900], 8, 2, 64), ([64], 2, 2, 256)])
 def test_workspaces(pkg, gpu, lens, Hq, H, D):
     """Nothing is written past the bytes a caller is told, and what they held does not matter."""

@@ -37,6 +37,7 @@ SIZES = [
     (dict(k=None), 1), (dict(v=None), 1), (dict(out=None), 1), (dict(cu=fake(3, 2)), 4), (dict(cu_k=fake(4, 2)), 4),
     (dict(q=fake(0, 8)), 4), (dict(v=fake(2, 8)), 4), (dict(out=fake(5, 8)), 4), (dict(lse=fake(6, 2)), 4),
     (dict(ws=fake(7, 8)), 4), (dict(cu_k=None), 2),
+    (dict(T=(1 << 31) - 1023, Hq=1, H=1), 7), (dict(Tk=(1 << 31) - 1023, Hq=1, H=1), 7),
 ]
 
 
