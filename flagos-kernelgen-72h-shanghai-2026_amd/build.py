@@ -25,9 +25,6 @@ PROBE_LIB_PATH = PKG_DIR / "libfagq_probe.so"
 LIB_UNITS = ("fagq_api", "fagq_device", "fagq_gemm", "dsa_topk", "mla_bwd", "qk_rope", "kv_cache",
              "paged_attn", "prompt_attn", "prompt_attn_bwd", "batch_tables")
 PROBE_UNITS = ("fagq_probe", "fagq_device")
-# The register pressure that the scheduler of prompt_attn_bwd.hip works with is the target's own count:
-# by the generic one it moves so many LDS reads ahead that 34 registers are spilled.
-UNIT_FLAGS = {"prompt_attn_bwd": ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"]}
 
 ARCH = "gfx950"
 # (code format, scale format) pairs compiled from fagq_inst.hip:
@@ -116,7 +113,7 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
         units.append((CSRC / "paged_attn_inst.hip", OBJ_DIR / f"paged_attn_inst_e{e}_q{q}_s{s}.o",
                       [f"-DFAGQ_ATTN_E={e}", f"-DFAGQ_ATTN_QF={q}", f"-DFAGQ_ATTN_SF={s}"]))
     for unit in sorted(set(LIB_UNITS) | set(PROBE_UNITS)):
-        units.append((CSRC / f"{unit}.hip", OBJ_DIR / f"{unit}.o", UNIT_FLAGS.get(unit, [])))
+        units.append((CSRC / f"{unit}.hip", OBJ_DIR / f"{unit}.o", []))
     jobs = jobs or min(len(units) + 1, max(1, min(16, os.cpu_count() or 1)))
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         futs = [ex.submit(_run, [cc, *flags, *defs, "-c", str(src), "-o", str(obj)], verbose)
@@ -178,7 +175,7 @@ def build_variant(name: str, *, defines: tuple[str, ...] = (), sanitize: bool = 
         units.append((CSRC / "paged_attn_inst.hip", out_dir / f"paged_attn_inst_e{e}_q{q}_s{s}.o",
                       [f"-DFAGQ_ATTN_E={e}", f"-DFAGQ_ATTN_QF={q}", f"-DFAGQ_ATTN_SF={s}"]))
     for unit in sorted(set(LIB_UNITS) | set(PROBE_UNITS)):
-        units.append((CSRC / f"{unit}.hip", out_dir / f"{unit}.o", UNIT_FLAGS.get(unit, [])))
+        units.append((CSRC / f"{unit}.hip", out_dir / f"{unit}.o", []))
     with ThreadPoolExecutor(max_workers=min(len(units), max(1, min(16, os.cpu_count() or 1)))) as ex:
         futs = [ex.submit(_run, [cc, *flags, *san, *defs, "-c", str(src), "-o", str(obj)], verbose)
                 for src, obj, defs in units]

@@ -278,7 +278,8 @@ def _attention(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, tree_
     """Either attention from its checks on; tree_mask: None without a tree."""
     P, H, page, D, G, qf, sf = _check_cache(k_cache, v_cache, k_scale, v_scale)
     if v_cache is None:
-        raise ValueError("attention needs a cache of keys and values")
+        name = "paged_attention" if tree_mask is None else "paged_tree_attention"
+        raise ValueError(f"{name} needs a cache of keys and values")
     dev = k_cache.device
     if q.dim() != 4 or q.shape[3] != D:
         raise ValueError(f"q must be [B, S, Hq, {D}], got {tuple(q.shape)}")
