@@ -211,24 +211,20 @@ __global__ __launch_bounds__(256) void prompt_attention_join(Args a) {
         l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * (1.0f / kLog2e) : -INFINITY;
 }
 
-// Parts of a workgroup's keys: as many as fill the GPU's places for two workgroups on each CU, but at
-// least 16 steps for each, which take about as long as the join.
+// Two workgroups run on a CU (us, so / in parts of 16 steps at least: 8 + 8 heads of 128, 100 tokens
+// behind 1500 17 / 31; 4 + 4, 200 behind 2000 19 / 27; 4 + 1, prompts of 3000 and 500 tokens 33 / 53;
+// 16 + 8 of 256, 20 behind 1800 23 / 34; 8 + 1 of 256, 2048 tokens 58 / 53).
 constexpr int64_t kSlots = 512;
-constexpr int64_t kMostParts = 16;
-int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t D) {
-  const int64_t groups = std::max<int64_t>(1, (T + kTile - 1) / kTile * Hq);
-  const int64_t steps = Tk / std::max<int64_t>(1, B) / (D == 256 ? 32 : 64);
-  return std::max<int64_t>(1, std::min<int64_t>({kSlots / groups, steps / 16, kMostParts}));
-}
+int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq) { return key_parts(B, T, Tk, Hq, kSlots); }
 
 int check_fwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
   const int st = check_sizes(B, T, Tk, Hq, H, D);
   if (st != FAGQ_OK) return st;
-  return tile_slots(T, B) * Hq * parts_for(B, T, Tk, Hq, D) >= kMostGroups ? FAGQ_E_TOO_LARGE : FAGQ_OK;
+  return tile_slots(T, B) * Hq * parts_for(B, T, Tk, Hq) >= kMostGroups ? FAGQ_E_TOO_LARGE : FAGQ_OK;
 }
 
 int64_t bytes_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t D) {
-  const int64_t parts = parts_for(B, T, Tk, Hq, D);
+  const int64_t parts = parts_for(B, T, Tk, Hq);
   return parts > 1 ? parts * T * Hq * (D + 2) * 4 : 0;
 }
 
@@ -309,7 +305,7 @@ FAGQ_API int fagq_prompt_attention_launch(const void* q, const void* k, const vo
   // What a query does not see has the score -inf, which times 0 would be no number.
   a.scale2 = std::fmax(std::fabs(sm_scale) * kLog2e, 0x1p-126f);
   a.flip = sm_scale < 0.0f ? 0x80008000u : 0u;
-  a.parts = (int32_t)parts_for(B, T, Tk, Hq, D), a.part = static_cast<float*>(workspace);
+  a.parts = (int32_t)parts_for(B, T, Tk, Hq), a.part = static_cast<float*>(workspace);
   void* args[] = {&a};
   const bool bf16 = dtype == FAGQ_DT_BF16;
   hipStream_t to = static_cast<hipStream_t>(stream);

@@ -14,6 +14,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 #include "fagq.h"
@@ -363,6 +365,19 @@ inline bool aligned(const void* p, uintptr_t a) {
 inline bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
+// Parts that a query tile's keys are cut into, each a workgroup's: as many as let `slots` workgroups run
+// at once, but four steps of 64 keys for each, on average.  What a part costs the join goes by the rows,
+// what it saves by the steps: with time a steps / n + b rows n, n = sqrt(a / b steps / rows) is best
+// (a / b = 8192, fitted).
+constexpr int64_t kMostParts = 16;
+inline int64_t key_parts(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t slots) {
+  if (B < 1 || T < 1) return 1;
+  const int64_t groups = B * ((T + B * kTile - 1) / (B * kTile)) * Hq;
+  const int64_t steps = std::max(Tk - T / 2, Tk / 2) / B / kStep;    // of a tile
+  const int64_t best = std::lround(std::sqrt(8192.0 * (double)steps / ((double)T * (double)Hq)));
+  return std::max<int64_t>(1, std::min<int64_t>({slots / groups, steps / 4, best, kMostParts}));
 }
 
 // T tokens of H rows of D elements of 16 bits, at token and head strides.

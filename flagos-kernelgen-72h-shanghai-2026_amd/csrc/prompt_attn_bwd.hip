@@ -4,12 +4,14 @@
 // atomics): seven products for the five of the formulas.
 //   prompt_dq     A workgroup takes 128 queries of one head, keys and values come through LDS.
 //                 S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.  It also leaves what the other
-//                 pass needs of each query: lse in units of log 2, and -delta.
+//                 pass needs of each query: lse in units of log 2, and -delta.  Where there are
+//                 few workgroups, the keys are cut into parts of their own sums.
 //   prompt_dkdv   A workgroup takes 128 keys of one head of k and v, the queries of all heads of
 //                 the group come through LDS.  S = Q K^T, dP = dO V^T, dV^T += dO^T P,
 //                 dK^T += Q^T dS.  Two teams of four waves share the steps of a tile and join
 //                 their sums through LDS; where there are few workgroups, the steps are cut into
-//                 parts of their own sums besides, which prompt_join adds up in order.
+//                 parts besides.
+//   prompt_join   adds the parts up, in order.
 // Calls of few rows, where a launch is what counts, take both passes in one (prompt_bwd_small): the
 // second then works out lse and delta of its queries by itself.
 #include <hip/hip_runtime.h>
@@ -41,8 +43,9 @@ struct Args {
   float* lse2;                       // [Hq, T]; +inf for a query without keys.  Null: small calls
   float* delta;                      // [Hq, T], negative
   float* part;                       // [parts][Tk][H][D] of dk, then of dv
+  float* dq_part;                    // [dq_parts][T][Hq][D]
   int64_t dos[2], qs[2], ks[2], vs[2], dqs[2], dks[2], dvs[2];   // {token, head} strides, elements
-  int32_t Hq, H, group, fill, parts;
+  int32_t Hq, H, group, fill, parts, dq_parts;
   int32_t dq_items;                  // small calls: workgroups of the first pass
   float scale, scale2;               // sm_scale, and times log2(e)
 };
@@ -72,11 +75,11 @@ __device__ __forceinline__ void run_dq(const Args& a, int item, DqLds<D>& shared
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int wave = scalar((int)(threadIdx.x >> 6));
   // Workgroup b runs on XCD b % 8: heads that share keys stay on one.
-  const int kvh = item % a.H, rest = item / a.H;
-  const int hq = kvh * a.group + rest % a.group;
-  const Place p = place_of<true>(a.queries, rest / a.group);
+  const int kvh = item % a.H, heads = item / a.H;
+  const int hq = kvh * a.group + heads % a.group, rest = heads / a.group, part = rest % a.dq_parts;
+  const Place p = place_of<true>(a.queries, rest / a.dq_parts);
   if (p.b < 0) {
-    if (a.fill & FAGQ_FILL_DQ) fill_tail<D>(a.dq, a.dqs, hq, a.queries.T, p);
+    if (part == 0 && (a.fill & FAGQ_FILL_DQ)) fill_tail<D>(a.dq, a.dqs, hq, a.queries.T, p);
     return;
   }
   const int32_t ahead = p.m - p.n;               // query i sees the keys up to i + ahead
@@ -90,14 +93,17 @@ __device__ __forceinline__ void run_dq(const Args& a, int item, DqLds<D>& shared
   const int32_t all = seen_by(mine);             // keys that every query of the wave sees
   const int32_t last = mine + kRows <= p.n ? mine + kRows - 1 : p.n - 1;
   const int32_t end = mine < p.n ? seen_by(last) : 0;                    // that one of them sees
-  const int32_t stop = seen_by(q0 + kTile <= p.n ? q0 + kTile - 1 : p.n - 1);
+  // Steps of the workgroup, this part's share of them.
+  const int32_t steps = (seen_by(q0 + kTile <= p.n ? q0 + kTile - 1 : p.n - 1) + kStep - 1) / kStep;
+  const int32_t from = (int32_t)((int64_t)steps * part / a.dq_parts) * kStep;
+  const int32_t stop = (int32_t)((int64_t)steps * (part + 1) / a.dq_parts) * kStep;
 
   Copier<D> ck, cv;
   ck.init(a.k, (int64_t)p.other * a.ks[0] + (int64_t)kvh * a.ks[1], a.ks[0], lane, wave);
   cv.init(a.v, (int64_t)p.other * a.vs[0] + (int64_t)kvh * a.vs[1], a.vs[0], lane, wave);
-  if (stop > 0) {
-    ck.issue(lds[0][0], wave, 0, p.m - 1);
-    cv.issue(lds[0][1], wave, 0, p.m - 1);
+  if (from < stop) {
+    ck.issue(lds[0][0], wave, from, p.m - 1);
+    cv.issue(lds[0][1], wave, from, p.m - 1);
   }
   u32x4 q[D / 16], g[D / 16];
   load_row<D>(a.q + (int64_t)row * a.qs[0] + (int64_t)hq * a.qs[1], h, q);
@@ -117,7 +123,7 @@ __device__ __forceinline__ void run_dq(const Args& a, int item, DqLds<D>& shared
   delta = cross_sum(delta);
   const float lse = a.lse[(int64_t)hq * a.queries.T + row];
   const float lse2 = lse_in_2(lse);
-  if (a.lse2 && h == 0 && i < p.n) {
+  if (a.lse2 && part == 0 && h == 0 && i < p.n) {
     a.lse2[(int64_t)hq * a.queries.T + row] = lse2;
     a.delta[(int64_t)hq * a.queries.T + row] = delta;
   }
@@ -126,7 +132,7 @@ __device__ __forceinline__ void run_dq(const Args& a, int item, DqLds<D>& shared
   for (int d = 0; d < D / 32; ++d) dq[d] = splat(0.0f);
 
   int buf = 0;
-  for (int32_t tok = 0; tok < stop; tok += kStep, buf ^= 1) {
+  for (int32_t tok = from; tok < stop; tok += kStep, buf ^= 1) {
     __builtin_amdgcn_s_waitcnt(kVmcnt0);         // this step's tiles have landed, of this wave
     lds_barrier();                               // of all; the last step's are done with
     if (tok + kStep < stop) {
@@ -163,7 +169,17 @@ __device__ __forceinline__ void run_dq(const Args& a, int item, DqLds<D>& shared
       }
     }
   }
-  store_row<E, D>(a.dq + (int64_t)row * a.dqs[0] + (int64_t)hq * a.dqs[1], h, dq, a.scale, i < p.n);
+  if (a.dq_parts == 1) {
+    store_row<E, D>(a.dq + (int64_t)row * a.dqs[0] + (int64_t)hq * a.dqs[1], h, dq, a.scale, i < p.n);
+  } else if (i < p.n) {
+    float* to = a.dq_part + (((int64_t)part * a.queries.T + row) * a.Hq + hq) * D;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<f32x4*>(to + 32 * d + row_of(r, h)) =
+            f32x4{dq[d][r], dq[d][r + 1], dq[d][r + 2], dq[d][r + 3]};
+  }
 }
 
 template <int E, int D>
@@ -443,49 +459,48 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_bwd_smal
   else run_dkdv<E, D, true>(a, (int)blockIdx.x - a.dq_items, lds.dkdv);
 }
 
-// Sums of the parts.  A thread has 8 elements of dk or of dv.
+// Sums of the parts.  A thread has 8 elements of dk or dv, where they have parts, or of dq.
 template <int E>
 __global__ __launch_bounds__(256) void prompt_join(Args a, int32_t D) {
-  const int64_t plane = (int64_t)a.keys.T * a.H * D;
-  const int64_t each = plane / 8, item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (item >= 2 * each) return;
-  const bool values = item >= each;
-  const int64_t at = (values ? item - each : item) * 8;
-  const int64_t row = at / ((int64_t)a.H * D);
-  const int32_t rest = (int32_t)(at - row * a.H * D), head = rest / D, d = rest - head * D;
-  if (row >= clamped(a.keys.cu[a.keys.B], a.keys.T)) return;
-  const float* part = a.part + (values ? a.parts * plane : 0) + at;
-  f32x4 s[2] = {};
-  for (int i = 0; i < a.parts; ++i, part += plane) {
-    s[0] += *reinterpret_cast<const f32x4*>(part);
-    s[1] += *reinterpret_cast<const f32x4*>(part + 4);
+  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t keys = a.parts > 1 ? (int64_t)a.keys.T * a.H * D / 8 : 0;
+  const int64_t queries = a.dq_parts > 1 ? (int64_t)a.queries.T * a.Hq * D / 8 : 0;
+  if (item >= 2 * keys + queries) return;
+  const bool of_q = item >= 2 * keys, values = !of_q && item >= keys;
+  const Sequences& s = of_q ? a.queries : a.keys;
+  const int32_t heads = of_q ? a.Hq : a.H, parts = of_q ? a.dq_parts : a.parts;
+  const int64_t plane = (int64_t)s.T * heads * D;
+  const int64_t at = (item - (of_q ? 2 * keys : values ? keys : 0)) * 8;
+  const int64_t row = at / ((int64_t)heads * D);
+  const int32_t rest = (int32_t)(at - row * heads * D), head = rest / D, d = rest - head * D;
+  if (row >= clamped(s.cu[s.B], s.T)) return;
+  const float* part = (of_q ? a.dq_part : values ? a.part + parts * plane : a.part) + at;
+  f32x4 sum[2] = {};
+  for (int i = 0; i < parts; ++i, part += plane) {
+    sum[0] += *reinterpret_cast<const f32x4*>(part);
+    sum[1] += *reinterpret_cast<const f32x4*>(part + 4);
   }
   const float f = values ? 1.0f : a.scale;
-  uint16_t* to = values ? a.dv + row * a.dvs[0] + (int64_t)head * a.dvs[1]
-                        : a.dk + row * a.dks[0] + (int64_t)head * a.dks[1];
+  const int64_t* strides = of_q ? a.dqs : values ? a.dvs : a.dks;
+  uint16_t* to = (of_q ? a.dq : values ? a.dv : a.dk) + row * strides[0] + (int64_t)head * strides[1];
   u32x4 w;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack16<E>(s[i / 2][2 * i % 4] * f, s[i / 2][2 * i % 4 + 1] * f);
+  for (int i = 0; i < 4; ++i) w[i] = pack16<E>(sum[i / 2][2 * i % 4] * f, sum[i / 2][2 * i % 4 + 1] * f);
   *reinterpret_cast<u32x4*>(to + d) = w;
 }
 
 // ---------------------------------------------------------------------------------- host
 
 constexpr int64_t kCUs = 256;        // a workgroup on each
-constexpr int64_t kMostParts = 16;
 
-int check_bwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
-  const int st = check_sizes(B, T, Tk, Hq, H, D);
-  if (st != FAGQ_OK) return st;
-  // With all the parts there may be, and the joining kernel's workgroups.
-  const bool large = tile_slots(Tk, B) * H * kMostParts + 16384 + B * Hq >= kMostGroups ||
-                     Tk * H * D / 1024 >= kMostGroups - 1;
-  return large ? FAGQ_E_TOO_LARGE : FAGQ_OK;
+// Calls of few rows and few pairs of query and key: both passes in one launch, with one team and two
+// terms (32 + 8 heads of 128, us, in one launch / in two: 1 token 15 / 17, 200 tokens 26 / 36, 4 x 128
+// 30 / 34, 4 x 200 58 / 41; 16 heads of 64, 1000 tokens 39 / 51; 8 heads of 128, 100 tokens behind 3000
+// 32 / 41, 1024 behind 1024 88 / 79; 24 + 8 of 256, 5 and 70 behind 4000 200 / 177).  The more a head
+// has, the fewer of the one launch's waves run at once.
+bool small(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t D) {
+  return T * Hq <= 16384 && (double)(T * Hq * D * D) * (double)Tk <= 0x1p36 * (double)std::max<int64_t>(1, B);
 }
-
-// Calls of few rows: both passes in one launch, with one team and two terms (32 + 8 heads of 128, us,
-// in one launch / in two: 1 token 15 / 17, 200 tokens 26 / 36, 4 x 128 30 / 34, 4 x 200 58 / 41).
-bool small(int64_t T, int64_t Hq) { return T * Hq <= 16384; }
 
 // Parts of a key tile's steps: as many as let the tile with most of them, twice the average, not take
 // longer than all together, but four steps for each team.
@@ -493,12 +508,42 @@ int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64
   const int64_t groups = std::max<int64_t>(1, (Tk + kTile - 1) / kTile * H);
   const int64_t steps = Hq / H * ((T + queries(D) - 1) / queries(D)) / std::max<int64_t>(1, B);
   return std::max<int64_t>(
-      1, std::min<int64_t>({2 * kCUs / groups, steps / (4 * teams(D, small(T, Hq))), kMostParts}));
+      1, std::min<int64_t>({2 * kCUs / groups, steps / (4 * teams(D, small(B, T, Tk, Hq, D))), kMostParts}));
 }
 
-int64_t bytes_for(int64_t parts, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
-  const int64_t stats = small(T, Hq) ? 0 : (2 * Hq * T * 4 + 15) / 16 * 16;
-  return stats + (parts > 1 ? 2 * parts * Tk * H * D * 4 : 0);
+// Parts of a query tile's keys (us, with parts / without: 8 + 2 heads of 128, 10 tokens behind 8000
+// 31 / 247; 8 heads of 64, 64 behind 1000 16 / 24; 4 of 128, 200 behind 2000 29 / 74, of 64, 4 x 300
+// behind 3000 43 / 65; but 8 + 1 of 256, 2048 tokens 180 / 157).  In one launch the keys' workgroups
+// run at the same time: one on a CU for heads of 128 and 256, two for those of 64.
+int64_t dq_parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
+  const bool one_launch = small(B, T, Tk, Hq, D);
+  int64_t slots = D == 256 || (D == 128 && one_launch) ? kCUs : 2 * kCUs;
+  if (one_launch) {
+    const int64_t others = (Tk + kTile - 1) / kTile * H * parts_for(B, T, Tk, Hq, H, D);
+    slots = std::max(slots - others, slots / 4);
+  }
+  return key_parts(B, T, Tk, Hq, slots);
+}
+
+int check_bwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
+  const int st = check_sizes(B, T, Tk, Hq, H, D);
+  if (st != FAGQ_OK) return st;
+  // With all the parts there may be of the keys', and the joining kernel's workgroups.
+  const int64_t dq_items = tile_slots(T, B) * Hq * dq_parts_for(B, T, Tk, Hq, H, D);
+  const bool large = dq_items >= kMostGroups ||
+                     tile_slots(Tk, B) * H * kMostParts + (small(B, T, Tk, Hq, D) ? dq_items : 0) >= kMostGroups ||
+                     Tk * H * D / 1024 >= kMostGroups / 2;
+  return large ? FAGQ_E_TOO_LARGE : FAGQ_OK;
+}
+
+struct Space {                       // elements of fp32 in the workspace
+  int64_t stats, part, dq_part;
+  int64_t bytes() const { return (stats + part + dq_part) * 4; }
+};
+Space space_for(int64_t parts, int64_t dq_parts, int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H,
+                int64_t D) {
+  return {small(B, T, Tk, Hq, D) ? 0 : (2 * Hq * T + 3) / 4 * 4, parts > 1 ? 2 * parts * Tk * H * D : 0,
+          dq_parts > 1 ? dq_parts * T * Hq * D : 0};
 }
 
 template <int E>
@@ -530,7 +575,7 @@ FAGQ_API int64_t fagq_prompt_attention_bwd_workspace_bytes(int64_t B, int64_t T,
                                                            int64_t Hq, int64_t H, int64_t D) {
   using namespace fagq::prompt;
   if (check_bwd_sizes(B, T, Tk, Hq, H, D) != FAGQ_OK) return -1;
-  return bytes_for(parts_for(B, T, Tk, Hq, H, D), T, Tk, Hq, H, D);
+  return space_for(parts_for(B, T, Tk, Hq, H, D), dq_parts_for(B, T, Tk, Hq, H, D), B, T, Tk, Hq, H, D).bytes();
 }
 
 FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, const void* k,
@@ -558,7 +603,9 @@ FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, c
                         (const void*)workspace})
     if (!aligned(p, 16)) return FAGQ_E_ALIGN;
   if (!aligned(lse, 4) || !aligned(cu_seqlens, 4) || !aligned(cu_seqlens_k, 4)) return FAGQ_E_ALIGN;
-  const int64_t parts = parts_for(B, T, Tk, Hq, H, D), need = bytes_for(parts, T, Tk, Hq, H, D);
+  const int64_t parts = parts_for(B, T, Tk, Hq, H, D), dq_parts = dq_parts_for(B, T, Tk, Hq, H, D);
+  const Space space = space_for(parts, dq_parts, B, T, Tk, Hq, H, D);
+  const int64_t need = space.bytes();
   if (workspace_bytes < need) return FAGQ_E_SHAPE;
   if (need > 0 && !workspace) return FAGQ_E_NULL;
   if (T == 0 && Tk == 0) return FAGQ_OK;
@@ -591,36 +638,36 @@ FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, c
   a.queries = {cu_seqlens, cu_k, (int32_t)B, (int32_t)T, (int32_t)Tk};
   a.keys = {cu_k, cu_seqlens, (int32_t)B, (int32_t)Tk, (int32_t)T};
   a.dq = static_cast<uint16_t*>(dq), a.dk = static_cast<uint16_t*>(dk), a.dv = static_cast<uint16_t*>(dv);
-  const bool one_launch = small(T, Hq);
-  a.part = static_cast<float*>(workspace);
-  if (!one_launch) {
-    a.lse2 = a.part, a.delta = a.lse2 + Hq * T;
-    a.part += (2 * Hq * T + 3) / 4 * 4;
-  }
+  const bool one_launch = small(B, T, Tk, Hq, D);
+  float* const room = static_cast<float*>(workspace);
+  if (!one_launch) a.lse2 = room, a.delta = room + Hq * T;
+  a.part = room + space.stats, a.dq_part = a.part + space.part;
   int64_t(*to[7])[2] = {&a.dos, &a.qs, &a.ks, &a.vs, &a.dqs, &a.dks, &a.dvs};
   for (int i = 0; i < 7; ++i) (*to[i])[0] = strides[2 * i], (*to[i])[1] = strides[2 * i + 1];
   a.Hq = (int32_t)Hq, a.H = (int32_t)H, a.group = (int32_t)(Hq / H);
-  a.fill = fill, a.parts = (int32_t)parts;
+  a.fill = fill, a.parts = (int32_t)parts, a.dq_parts = (int32_t)dq_parts;
   a.scale = sm_scale, a.scale2 = sm_scale * kLog2e;
   int32_t dim = (int32_t)D;
   void* args[] = {&a, &dim};
   const bool bf16 = dtype == FAGQ_DT_BF16;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t dq_items = tile_slots(T, B) * Hq, dkdv_items = Tk > 0 ? tile_slots(Tk, B) * H * parts : 0;
+  const int64_t dq_items = T > 0 ? tile_slots(T, B) * Hq * dq_parts : 0;
+  const int64_t dkdv_items = Tk > 0 ? tile_slots(Tk, B) * H * parts : 0;
   if (one_launch) {
-    a.dq_items = T > 0 ? (int32_t)dq_items : 0;
+    a.dq_items = (int32_t)dq_items;
     const int ls = launch_kernel(bf16 ? small_for<ET_BF16>(D) : small_for<ET_F16>(D),
                                  dim3((unsigned)(a.dq_items + dkdv_items)), dim3(64 * kWaves), args, 0, st);
-    if (ls != FAGQ_OK || parts == 1) return ls;
+    if (ls != FAGQ_OK) return ls;
   } else {
     int ls = launch_kernel(bf16 ? dq_for<ET_BF16>(D) : dq_for<ET_F16>(D), dim3((unsigned)dq_items),
                            dim3(64 * kWaves), args, 0, st);
-    if (ls != FAGQ_OK || dkdv_items == 0) return ls;
-    ls = launch_kernel(bf16 ? dkdv_for<ET_BF16>(D) : dkdv_for<ET_F16>(D), dim3((unsigned)dkdv_items),
-                       dim3((unsigned)(64 * kWaves * teams(D, false))), args, 0, st);
-    if (ls != FAGQ_OK || parts == 1) return ls;
+    if (ls == FAGQ_OK && dkdv_items > 0)
+      ls = launch_kernel(bf16 ? dkdv_for<ET_BF16>(D) : dkdv_for<ET_F16>(D), dim3((unsigned)dkdv_items),
+                         dim3((unsigned)(64 * kWaves * teams(D, false))), args, 0, st);
+    if (ls != FAGQ_OK) return ls;
   }
-  const int64_t items = 2 * Tk * H * (D / 8);
+  const int64_t items = (parts > 1 ? 2 * Tk * H * (D / 8) : 0) + (dq_parts > 1 ? T * Hq * (D / 8) : 0);
+  if (items == 0) return FAGQ_OK;
   return launch_kernel(bf16 ? reinterpret_cast<const void*>(&prompt_join<ET_BF16>)
                             : reinterpret_cast<const void*>(&prompt_join<ET_F16>),
                        dim3((unsigned)((items + 255) / 256)), dim3(256), args, 0, st);

@@ -89,6 +89,19 @@ def test_prompts(pkg, gpu, case, dtype):
     check(pkg, gpu, make(len(lens) * 31 + D, lens, lens_k, Hq, H, D, dtype, spare))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("case", [
+    ([10], [1500], 4, 2, 64, 3), ([10, 0, 70], [1300, 9, 600], 3, 1, 128, 0), ([140], [2000], 4, 1, 256, 0),
+    ([600], [1900], 8, 4, 64, 0), ([1030, 70], [1500, 3], 16, 16, 64, 5), ([1100], None, 16, 4, 128, 0),
+    ([300, 200], [0, 2500], 4, 4, 128, 0), ([90], [700], 16, 2, 256, 1), ([400, 380], [1500, 1600], 4, 1, 256, 0),
+], ids=lambda c: f"{len(c[0])}x{max(c[0])}k{max(c[1] or [0])}_{'_'.join(map(str, c[2:]))}")
+def test_keys_in_parts(pkg, gpu, case, dtype):
+    """Few queries of many keys: both directions cut a query tile's keys."""
+    lens, lens_k, Hq, H, D, spare = case
+    note(f"parts {case} {dtype}")
+    check(pkg, gpu, make(len(lens) + D, lens, lens_k, Hq, H, D, dtype, spare))
+
+
 @pytest.mark.parametrize("seed", range(16))
 def test_random(pkg, gpu, seed):
     rng = random.Random(seed)
