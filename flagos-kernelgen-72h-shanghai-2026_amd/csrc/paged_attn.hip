@@ -285,6 +285,7 @@ Plan plan_for(int64_t B, int64_t S, int64_t Hq, int64_t H, int64_t D, int64_t pr
     p.prefix_items = H * p.prefix_tiles * p.prefix_chunks;
   }
   p.tiles = (per + height(p.R, D) - 1) / height(p.R, D);
+  // Drafts always in chunks, which more than 16 rows (5 drafts of 4 heads that share one) take anyway.
   if (tree || p.tiles > 1 || p.R > 1 || most_rounds(1, 1, most) < (D == 64 ? kLongUnit64 : kLongUnit) ||
       most_rounds(B, H, most) <= kFewRounds) {
     p.form = kStatic;
