@@ -54,7 +54,7 @@ struct Args {
 template <int D>
 __device__ __forceinline__ void fill_tail(const Args& a, const Place& p, int hq) {
   const int64_t first = (int64_t)p.end + (int64_t)p.tile * kTile;
-  for (int i = threadIdx.x; i < kTile * (D / 8); i += 64 * kWaves) {
+  for (int i = threadIdx.x % (64 * kWaves); i < kTile * (D / 8); i += 64 * kWaves) {
     const int64_t row = first + i / (D / 8);
     if (row >= a.seq.T) break;
     if (a.fill & FAGQ_FILL_OUT)
@@ -63,16 +63,17 @@ __device__ __forceinline__ void fill_tail(const Args& a, const Place& p, int hq)
   }
 }
 
-template <int E, int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention(Args a) {
+// TEAMS: of four waves, each with a head of its own, of those that share keys.
+template <int E, int D, int TEAMS>
+__global__ __launch_bounds__(64 * kWaves * TEAMS, 2) void prompt_attention(Args a) {
   constexpr int kKeys = D == 256 ? 32 : 64;      // in LDS at a time
   using L = Tile<D, kKeys>;
   __shared__ __align__(16) char lds[2][2][L::kBytes];
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
-  const int wave = scalar((int)(threadIdx.x >> 6));
+  const int waves = scalar((int)(threadIdx.x >> 6)), wave = waves % kWaves, team = waves / kWaves;
   // Workgroup b runs on XCD b % 8: heads that share keys stay on one.
-  const int item = (int)blockIdx.x, kvh = item % a.H, heads = item / a.H;
-  const int hq = kvh * a.group + heads % a.group, rest = heads / a.group, part = rest % a.parts;
+  const int item = (int)blockIdx.x, kvh = item % a.H, heads = item / a.H, sets = a.group / TEAMS;
+  const int hq = kvh * a.group + heads % sets * TEAMS + team, rest = heads / sets, part = rest % a.parts;
   const Place p = place_of<true>(a.seq, rest / a.parts);
   if (p.b < 0) {
     if (a.fill && part == 0) fill_tail<D>(a, p, hq);
@@ -97,10 +98,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention(Args a) {
   Copier<D, kKeys> ck, cv;
   ck.init(a.k, (int64_t)p.other * a.ks[0] + (int64_t)kvh * a.ks[1], a.ks[0], lane, wave);
   cv.init(a.v, (int64_t)p.other * a.vs[0] + (int64_t)kvh * a.vs[1], a.vs[0], lane, wave);
-  if (from < stop) {
-    ck.issue(lds[0][0], wave, from, p.m - 1);
-    cv.issue(lds[0][1], wave, from, p.m - 1);
-  }
+  auto issue = [&](int buf, int32_t tok) {       // two teams: keys, values
+    if (TEAMS == 1 || team == 0) ck.issue(lds[buf][0], wave, tok, p.m - 1);
+    if (TEAMS == 1 || team == 1) cv.issue(lds[buf][1], wave, tok, p.m - 1);
+  };
+  if (from < stop) issue(0, from);
   u32x4 q[D / 16];
   load_row<D>(a.q + (int64_t)(p.row + (i < p.n ? i : p.n - 1)) * a.qs[0] + (int64_t)hq * a.qs[1], h, q);
 #pragma unroll
@@ -114,10 +116,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention(Args a) {
   for (int32_t tok = from; tok < stop; tok += kKeys, buf ^= 1) {
     __builtin_amdgcn_s_waitcnt(kVmcnt0);         // this step's tiles have landed, of this wave
     lds_barrier();                               // of all; the last step's are done with
-    if (tok + kKeys < stop) {
-      ck.issue(lds[buf ^ 1][0], wave, tok + kKeys, p.m - 1);
-      cv.issue(lds[buf ^ 1][1], wave, tok + kKeys, p.m - 1);
-    }
+    if (tok + kKeys < stop) issue(buf ^ 1, tok + kKeys);
     if (tok >= end) continue;
     f32x16 x[kKeys / 32];
 #pragma unroll
@@ -225,6 +224,15 @@ __global__ __launch_bounds__(256) void prompt_attention_join(Args a) {
 constexpr int64_t kSlots = 512;
 int64_t parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq) { return key_parts(B, T, Tk, Hq, kSlots); }
 
+// Two teams, and half as many workgroups, read keys once for two heads: for long calls of heads of 128 (us,
+// two / one, 32 + 8 heads: 4096 tokens 148 / 159, 8192 503 / 511, 8 x 512 behind 4096 265 / 278; 16 + 2,
+// 8192 251 / 275; but 2048 tokens 59 / 51, 16 x 1024 198 / 187).  For heads of 256 they take longer
+// there too (4 x 512 behind 4096, 16 + 4 heads 164 / 157), for heads of 64 within 2 % of as long.
+int teams_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
+  return D == 128 && B > 0 && Hq / H % 2 == 0 && query_tiles(B, T, Hq) >= 2 * kSlots &&
+                 steps_of_tile(B, T, Tk) >= 32 ? 2 : 1;
+}
+
 int check_fwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
   const int st = check_sizes(B, T, Tk, Hq, H, D);
   if (st != FAGQ_OK) return st;
@@ -237,10 +245,11 @@ int64_t bytes_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t D) {
 }
 
 template <int E>
-const void* kernel_for(int64_t D) {
-  return D == 64    ? reinterpret_cast<const void*>(&prompt_attention<E, 64>)
-         : D == 128 ? reinterpret_cast<const void*>(&prompt_attention<E, 128>)
-                    : reinterpret_cast<const void*>(&prompt_attention<E, 256>);
+const void* kernel_for(int64_t D, int teams) {
+  return D == 64      ? reinterpret_cast<const void*>(&prompt_attention<E, 64, 1>)
+         : D == 256   ? reinterpret_cast<const void*>(&prompt_attention<E, 256, 1>)
+         : teams == 2 ? reinterpret_cast<const void*>(&prompt_attention<E, 128, 2>)
+                      : reinterpret_cast<const void*>(&prompt_attention<E, 128, 1>);
 }
 template <int E>
 const void* join_for(int64_t D) {
@@ -317,8 +326,10 @@ FAGQ_API int fagq_prompt_attention_launch(const void* q, const void* k, const vo
   void* args[] = {&a};
   const bool bf16 = dtype == FAGQ_DT_BF16;
   hipStream_t to = static_cast<hipStream_t>(stream);
-  const int ls = launch_kernel(bf16 ? kernel_for<ET_BF16>(D) : kernel_for<ET_F16>(D),
-                               dim3((unsigned)(tile_slots(T, B) * Hq * a.parts)), dim3(64 * kWaves), args, 0, to);
+  const int teams = teams_for(B, T, Tk, Hq, H, D);
+  const int ls = launch_kernel(bf16 ? kernel_for<ET_BF16>(D, teams) : kernel_for<ET_F16>(D, teams),
+                               dim3((unsigned)(tile_slots(T, B) * Hq / teams * a.parts)),
+                               dim3((unsigned)(64 * kWaves * teams)), args, 0, to);
   if (ls != FAGQ_OK || a.parts == 1) return ls;
   return launch_kernel(bf16 ? join_for<ET_BF16>(D) : join_for<ET_F16>(D),
                        dim3((unsigned)((T * Hq * (D / 8) + 255) / 256)), dim3(256), args, 0, to);

@@ -367,6 +367,14 @@ inline bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
   return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
 }
 
+// Tiles of queries of all heads, and a tile's steps of keys, for sequences of average length.
+inline int64_t query_tiles(int64_t B, int64_t T, int64_t Hq) {
+  return B * ((T + B * kTile - 1) / (B * kTile)) * Hq;
+}
+inline int64_t steps_of_tile(int64_t B, int64_t T, int64_t Tk) {
+  return std::max(Tk - T / 2, Tk / 2) / B / kStep;
+}
+
 // Parts that a query tile's keys are cut into, each a workgroup's: as many as let `slots` workgroups run
 // at once, but four steps of 64 keys for each, on average.  What a part costs the join goes by the rows,
 // what it saves by the steps: with time a steps / n + b rows n, n = sqrt(a / b steps / rows) is best
@@ -374,8 +382,7 @@ inline bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
 constexpr int64_t kMostParts = 16;
 inline int64_t key_parts(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t slots) {
   if (B < 1 || T < 1) return 1;
-  const int64_t groups = B * ((T + B * kTile - 1) / (B * kTile)) * Hq;
-  const int64_t steps = std::max(Tk - T / 2, Tk / 2) / B / kStep;    // of a tile
+  const int64_t groups = query_tiles(B, T, Hq), steps = steps_of_tile(B, T, Tk);
   const int64_t best = std::lround(std::sqrt(8192.0 * (double)steps / ((double)T * (double)Hq)));
   return std::max<int64_t>(1, std::min<int64_t>({slots / groups, steps / 4, best, kMostParts}));
 }

@@ -102,6 +102,24 @@ def test_keys_in_parts(pkg, gpu, case, dtype):
     check(pkg, gpu, make(len(lens) + D, lens, lens_k, Hq, H, D, dtype, spare))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("Hq,H", [(512, 256), (1024, 2)])
+def test_many_heads_of_long_keys(pkg, gpu, Hq, H, dtype):
+    """Workgroups of two heads: some heads against 64 bits, rows behind the last sequence filled."""
+    note(f"two heads {Hq} {H} {dtype}")
+    lens, lens_k = [130, 60], [2400, 2300]
+    q, k, v, _, cu, cu_k = made = make(Hq, lens, lens_k, Hq, H, 128, dtype, 140)
+    out, lse = forward(pkg, gpu, made, 0.09)
+    T, Tk, group = sum(lens), sum(lens_k), Hq // H
+    assert bool((out[T:] == 0).all()) and bool((lse[:, T:] == float("-inf")).all())
+    for h in (0, H // 2, H - 1):
+        for first in {0, group - 2}:
+            own = slice(h * group + first, h * group + first + 2)
+            o, o_off, s, s_off = ref.forward(q[:T, own], k[:Tk, h:h + 1], v[:Tk, h:h + 1], cu, 0.09, cu_k)
+            assert attention_ref.outside(out[:T, own], o, o_off, dtype) == 0
+            assert bool(((lse[own, :T].double().cpu() - s).abs() <= s_off).all())
+
+
 @pytest.mark.parametrize("seed", range(16))
 def test_random(pkg, gpu, seed):
     rng = random.Random(seed)
