@@ -271,13 +271,14 @@ __device__ __forceinline__ int32_t clamped(int32_t v, int32_t most) {
 // they are of, so that the last workgroups to start are the shortest (32 + 8 heads of 128, us, so /
 // sequence by sequence: dk and dv of 16 sequences of 166 to 1000 tokens 141 / 180, four prompts of 800
 // 36 / 42).  Of more, or longer ones, the tiles come sequence by sequence, each one's in that order.
-// Lane l counts the tiles of sequences l n .. (l + 1) n - 1; up to 64 sequences it has everything about
-// its own in registers, and one trip to memory is enough.
-constexpr int kLevels = 64;
+// Up to 64 sequences a lane has everything about its own in registers, and one trip to memory is
+// enough; more are looked through kAtOnce to a lane at a time, lane by lane next to each other (us, so /
+// a run of them to each lane: 256 of 100 tokens, 8 heads 46 / 49, 1000 of 60 146 / 201, 4096 of 30, 4 heads
+// 223 / 662).
+constexpr int kLevels = 64, kAtOnce = 4;
 template <bool LATE>
 __device__ __forceinline__ Place place_of(const Sequences& s, int32_t slot) {
   const int lane = threadIdx.x & 63;
-  const int each = (s.B + 63) / 64;
   struct Sequence {
     int32_t row, n, other, m;
   };
@@ -288,65 +289,92 @@ __device__ __forceinline__ Place place_of(const Sequences& s, int32_t slot) {
     return Sequence{lo, hi > lo ? hi - lo : 0, lo2, hi2 > lo2 ? hi2 - lo2 : 0};
   };
   auto tiles_of = [](int32_t n) { return (n + kTile - 1) / kTile; };
+  // Sums of this lane and those before it.
+  auto sums = [&](int32_t v) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int32_t o = __shfl_up(v, d);
+      v += lane >= d ? o : 0;
+    }
+    return v;
+  };
   Place p = {};
   p.end = scalar(clamped(s.cu[s.B], s.T));
-  const int first = lane * each, stop = first + each < s.B ? first + each : s.B;
-  Sequence mine = {};
-  int32_t count = 0;
-  for (int i = first; i < stop; ++i) {
-    mine = sequence(i);
-    // Lengths that overlap may add up to any number: cut, so that 64 lanes' do not pass 31 bits.  No
-    // grid has as many workgroups.
-    count = clamped(count + tiles_of(mine.n), (int32_t)kMostGroups);
-  }
-  int32_t upto = count;
+  int i = 0;
+  int32_t at = slot;                             // of those from sequence i on
+  if (s.B > 64) {
+    bool found = false;
+    for (; i < s.B && !found;) {
+      int32_t n[kAtOnce], mine = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int32_t o = __shfl_up(upto, d);
-    upto += lane >= d ? o : 0;
-  }
-  const int32_t total = __builtin_amdgcn_readlane(upto, 63);
-  if (slot >= total) {
-    p.b = -1;
-    p.tile = slot - total;
-    return p;
-  }
-  int l, i;
-  int32_t at;
-  const bool level = each == 1 && __ballot(count > kLevels) == 0 && __popcll(__ballot(count > 0)) > 1;
-  if (level) {
-    // Tile `at` counted from the one with most work: tiles with as many behind them in their sequence
-    // as a level says, from the highest level on.
-    int32_t left = slot, most = 0;
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int j = i + 64 * u + lane, jj = j < s.B ? j : s.B - 1, b = LATE ? s.B - 1 - jj : jj;
+        const int32_t lo = clamped(s.cu[b], s.T), hi = clamped(s.cu[b + 1], s.T);
+        n[u] = j < s.B && hi > lo ? tiles_of(hi - lo) : 0;
+        mine += n[u];
+      }
+      // Lengths that overlap may add up to any number: cut, so that 64 lanes' do not pass 31 bits.  No
+      // grid has as many workgroups.
+      const int32_t all = __builtin_amdgcn_readlane(sums(clamped(mine, (int32_t)kMostGroups)), 63);
+      if (at >= all) {
+        at -= all;
+        i += 64 * kAtOnce;
+        continue;
+      }
+      found = true;                              // these have more than `at`
 #pragma unroll
-    for (int bit = kLevels; bit > 0; bit /= 2)
-      if (__ballot(count >= most + bit)) most += bit;
-    uint64_t mask = 0;
-    for (at = most - 1; at >= 0; --at) {         // ends before: slot < total
-      mask = __ballot(count > at);
-      const int n = __popcll(mask);
-      if (left < n) break;
-      left -= n;
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int32_t upto = sums(n[u]);
+        const uint64_t here = __ballot(at >= upto - n[u] && at < upto);
+        if (here) {
+          const int l = (int)__builtin_ctzll(here);
+          at -= __builtin_amdgcn_readlane(upto - n[u], l);
+          i += l;
+          break;
+        }
+        at -= __builtin_amdgcn_readlane(upto, 63);
+        i += 64;
+      }
     }
-    const bool mine = (mask >> lane & 1) && __popcll(mask & ((1ull << lane) - 1)) == left;
-    l = i = (int)__builtin_ctzll(__ballot(mine));
-    at = __builtin_amdgcn_readlane(count, l) - 1 - at;
-  } else {
-    const uint64_t here = __ballot(slot >= upto - count && slot < upto);
-    l = (int)__builtin_ctzll(here);
-    at = slot - __builtin_amdgcn_readlane(upto - count, l);
-    i = l * each;
-  }
-  if (each == 1) {
-    p.row = __builtin_amdgcn_readlane(mine.row, l), p.n = __builtin_amdgcn_readlane(mine.n, l);
-    p.other = __builtin_amdgcn_readlane(mine.other, l), p.m = __builtin_amdgcn_readlane(mine.m, l);
-  } else {
-    Sequence q = sequence(i);
-    while (at >= tiles_of(scalar(q.n))) {        // ends: the lane's tiles are more than `at`
-      at -= tiles_of(scalar(q.n));
-      q = sequence(++i);
+    if (!found) {
+      p.b = -1;
+      p.tile = at;
+      return p;
     }
+    const Sequence q = sequence(i);
     p.row = scalar(q.row), p.n = scalar(q.n), p.other = scalar(q.other), p.m = scalar(q.m);
+  } else {
+    const Sequence mine = lane < s.B ? sequence(lane) : Sequence{};
+    const int32_t count = tiles_of(mine.n), upto = sums(count);
+    const int32_t total = __builtin_amdgcn_readlane(upto, 63);
+    if (slot >= total) {
+      p.b = -1;
+      p.tile = slot - total;
+      return p;
+    }
+    if (__ballot(count > kLevels) == 0 && __popcll(__ballot(count > 0)) > 1) {
+      // Tile `at` counted from the one with most work: tiles with as many behind them in their
+      // sequence as a level says, from the highest level on.
+      int32_t left = slot, most = 0;
+#pragma unroll
+      for (int bit = kLevels; bit > 0; bit /= 2)
+        if (__ballot(count >= most + bit)) most += bit;
+      uint64_t mask = 0;
+      for (at = most - 1; at >= 0; --at) {       // ends before: slot < total
+        mask = __ballot(count > at);
+        const int n = __popcll(mask);
+        if (left < n) break;
+        left -= n;
+      }
+      const bool here = (mask >> lane & 1) && __popcll(mask & ((1ull << lane) - 1)) == left;
+      i = (int)__builtin_ctzll(__ballot(here));
+      at = __builtin_amdgcn_readlane(count, i) - 1 - at;
+    } else {
+      i = (int)__builtin_ctzll(__ballot(slot >= upto - count && slot < upto));
+      at = slot - __builtin_amdgcn_readlane(upto - count, i);
+    }
+    p.row = __builtin_amdgcn_readlane(mine.row, i), p.n = __builtin_amdgcn_readlane(mine.n, i);
+    p.other = __builtin_amdgcn_readlane(mine.other, i), p.m = __builtin_amdgcn_readlane(mine.m, i);
   }
   p.b = LATE ? s.B - 1 - i : i;
   p.tile = LATE ? tiles_of(p.n) - 1 - at : at;

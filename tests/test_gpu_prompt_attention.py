@@ -120,6 +120,25 @@ def test_many_heads_of_long_keys(pkg, gpu, Hq, H, dtype):
             assert bool(((lse[own, :T].double().cpu() - s).abs() <= s_off).all())
 
 
+@pytest.mark.parametrize("B", [64, 65, 255, 256, 257, 513, 1025])
+def test_places_among_many_sequences(pkg, gpu, B):
+    """Sequences of none to three tiles, the longest last or first, empty ones at either end."""
+    note(f"places {B}")
+    lens = [[0, 3, 1, 140, 0, 260][(i * 5 + i // 7) % 6] if 2 < i < B - 2 else 0 for i in range(B)]
+    for order in (lens, lens[::-1]):
+        q, k, v, do, cu, _ = made = make(B, order, None, 2, 1, 64, spare=200)
+        T = sum(order)
+        out, lse = forward(pkg, gpu, made, 0.2)
+        assert bool((out[T:] == 0).all()) and bool((lse[:, T:] == float("-inf")).all())
+        o, o_off, s, s_off = ref.forward(q[:T], k[:T], v[:T], cu, 0.2, None)
+        assert attention_ref.outside(out[:T], o, o_off, BF16) == 0
+        assert bool(((lse[:, :T].double().cpu() - s).abs() <= s_off).all())
+        grads = pkg.prompt_attention_bwd(do.to(gpu), q.to(gpu), k.to(gpu), v.to(gpu), out, lse, cu.to(gpu), 0.2)
+        want = ref.backward(do[:T], q[:T], k[:T], v[:T], out[:T].cpu(), lse[:, :T].cpu(), cu, 0.2, None)
+        for t, (r, off) in zip(grads, want):
+            assert bool((t[T:] == 0).all()) and attention_ref.outside(t[:T], r, off, BF16) == 0
+
+
 @pytest.mark.parametrize("seed", range(16))
 def test_random(pkg, gpu, seed):
     rng = random.Random(seed)
