@@ -355,6 +355,17 @@ struct Tree {
   const uint8_t* mask;
   int32_t context, len;
 };
+// A draft that none of a wave's rows sees may hold anything, NaN among it, which a weight of 0 does not
+// take away: its value scale and its values become zeros.  Element i of a lane's operand of values is
+// key i of the lane's eight.
+struct Kept {
+  u32x4 bits = {~0u, ~0u, ~0u, ~0u};
+  __device__ __forceinline__ void drop(int lane, int i, bool seen, float& scale) {
+    if ((__ballot(seen) >> (lane & 48)) & 0xffffu) return;       // by one of the 16 rows of some tile
+    scale = 0.0f;
+    bits[i / 2] &= i % 2 ? 0x0000ffffu : 0xffff0000u;
+  }
+};
 template <bool TREE>
 __device__ __forceinline__ bool sees(int32_t seen, const Tree& tree, int32_t at) {
   if constexpr (TREE)
@@ -400,8 +411,9 @@ __device__ __forceinline__ void scores(int lane, const RawKeys<D, SF>& raw, cons
 // and l may not: it takes the factor in two.
 template <int E, int D, int R, bool TREE>
 __device__ __forceinline__ void softmax(int lane, int32_t tok, int32_t all, const Pages& pages,
-                                        f32x4 (&x)[R][2], float (&ks)[8], const float (&vs)[8],
-                                        const Tree& tree, Rows<E, D, R>& s, u32x4 (&p)[R]) {
+                                        f32x4 (&x)[R][2], float (&ks)[8], float (&vs)[8],
+                                        const Tree& tree, Rows<E, D, R>& s, u32x4 (&p)[R],
+                                        Kept& kept) {
   constexpr int NT = D / 16;
   const int g = lane >> 4;
   if (tok + kStep > all || pages.p[0] < 0 || pages.p[1] < 0) {
@@ -409,11 +421,15 @@ __device__ __forceinline__ void softmax(int lane, int32_t tok, int32_t all, cons
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int32_t at = tok + 16 * (i / 4) + 4 * g + i % 4;
+      bool any = false;
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        x[r][i / 4][i % 4] =
-            sees<TREE>(s.seen[r], tree, at) && pages.p[i / 4] >= 0 ? x[r][i / 4][i % 4] * ks[i] : -INFINITY;
+      for (int r = 0; r < R; ++r) {
+        const bool seen = sees<TREE>(s.seen[r], tree, at) && pages.p[i / 4] >= 0;
+        x[r][i / 4][i % 4] = seen ? x[r][i / 4][i % 4] * ks[i] : -INFINITY;
+        any |= seen;
+      }
       ks[i] = 1.0f;
+      if constexpr (TREE) kept.drop(lane, i, any, vs[i]);
     }
   }
   const float most = fmaxf(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])),
@@ -473,7 +489,8 @@ __device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t
     }
   }
   u32x4 p[R];
-  softmax<E, D, R, TREE>(lane, tok, all, pages, x, ks, vs, tree, s, p);
+  Kept kept;
+  softmax<E, D, R, TREE>(lane, tok, all, pages, x, ks, vs, tree, s, p, kept);
 #pragma unroll
   for (int w = 0; w < NT / 4; ++w) {
     uint32_t d[2][4];
@@ -482,7 +499,9 @@ __device__ __forceinline__ void join(int lane, int32_t tok, int32_t all, int32_t
       transpose4(raw.v[4 * t][w], raw.v[4 * t + 1][w], raw.v[4 * t + 2][w], raw.v[4 * t + 3][w], d[t]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const u32x4 v = widen8<ET_F16, QF>(d[0][i], d[1][i]);
+      u32x4 v = widen8<ET_F16, QF>(d[0][i], d[1][i]);
+      if constexpr (TREE)
+        if (tok + kStep > all) v &= kept.bits;
 #pragma unroll
       for (int r = 0; r < R; ++r) s.o[r][4 * w + i] = mfma<ET_F16>(v, p[r], s.o[r][4 * w + i]);
     }
@@ -932,16 +951,27 @@ __device__ __forceinline__ void run_tall(const Args& a, const Segment& seg,
           vs[i] = sh.vs[buf][u][16 * (i / 4) + 4 * g + i % 4];
         }
         u32x4 p[R];
-        softmax<E, D, R, TREE>(lane, tok + u * kStep, all, now[u], x, ks, vs, tree, s, p);
+        Kept kept;
+        softmax<E, D, R, TREE>(lane, tok + u * kStep, all, now[u], x, ks, vs, tree, s, p, kept);
         if (u == kSteps - 1) {
 #pragma unroll
           for (int w = 0; w < kSteps; ++w) ahead[w] = entries(tok + 3 * kKeys + w * kStep);
         }
+        // Two loops: with a branch in one, 32 x 32 drafts over 8192 tokens take 385 us, so 364.
+        if (TREE && tok + (u + 1) * kStep > all) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const u32x4 v = sh.v[buf][u][j][lane];
+          for (int j = 0; j < NT; ++j) {
+            const u32x4 v = sh.v[buf][u][j][lane] & kept.bits;
 #pragma unroll
-          for (int r = 0; r < R; ++r) s.o[r][j] = mfma<ET_F16>(v, p[r], s.o[r][j]);
+            for (int r = 0; r < R; ++r) s.o[r][j] = mfma<ET_F16>(v, p[r], s.o[r][j]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const u32x4 v = sh.v[buf][u][j][lane];
+#pragma unroll
+            for (int r = 0; r < R; ++r) s.o[r][j] = mfma<ET_F16>(v, p[r], s.o[r][j]);
+          }
         }
       }
       if (!more) break;

@@ -253,7 +253,8 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     s sees the shared prefix, all tokens before the drafts, and the drafts t with
     ``tree_mask[b, s, t]`` (bool or uint8, [B, S, S], or [S, S] for all sequences; contiguous):
     itself only if the mask says so.  Where a sequence has fewer than S tokens, its first drafts do
-    not exist.  Any mask will do; a query that sees nothing gets zeros.
+    not exist.  Any mask will do; a query that sees nothing gets zeros, and the slots of drafts that no
+    row of the mask names (a padded tree's) may hold anything.
 
     S is at most 4096.  The other arguments, and what is returned, as in ``paged_attention``;
     ``workspace`` has ``tree_attention_workspace_bytes(...)`` bytes.  Asynchronous on the current

@@ -111,7 +111,8 @@ FAGQ_API int fagq_paged_attention_launch(const void* q, const void* k_cache, con
  * the drafts of a tree.  With len = min(kv_lens[b], max_kv_len, the table's room),
  * query s sees the prefix, the tokens j < len - S, and of the drafts t (token
  * len - S + t, if that is not negative) those whose byte [s][t] of the mask is not 0;
- * itself only if its own byte says so.  Any mask will do.
+ * itself only if its own byte says so.  Any mask will do; the slots of drafts that no
+ * row of a sequence's mask names may hold anything.
  * tree_mask: uint8 [B][S][S], or [S][S] for all sequences (shared_mask not 0).
  * S <= FAGQ_TREE_MAX_S.  The workspace has a size of its own. */
 #define FAGQ_TREE_MAX_S 4096

@@ -87,6 +87,34 @@ def test_a_chain_is_the_causal_attention(pkg, gpu):
         assert torch.equal(run(pkg, gpu, made, chain.to(torch.uint8) * 200, prefix), got)
 
 
+@pytest.mark.parametrize("qdt,ue8m0,dtype", [(FP8, False, BF16), (INT8, False, F16), (FP8, True, F16)])
+@pytest.mark.parametrize("case", [c for c in CASES if c[1] > 3], ids=lambda c: f"{len(c[0])}x{max(c[0])}_{'_'.join(map(str, c[1:]))}")
+def test_drafts_that_nobody_sees_may_hold_anything(pkg, gpu, case, qdt, ue8m0, dtype):
+    """A padded tree: some drafts are in no row of the mask, and their slots were never written."""
+    lens, S, Hq, H, D, page, prefix = case
+    note(f"unseen drafts {case} {qdt} {ue8m0} {dtype}")
+    made = make(len(lens) * 41 + S, lens, S, Hq, H, D, page, prefix, qdt, ue8m0, dtype)
+    q, caches, table, kv, pp = made
+    mask = masks(S + 1, len(lens), S)
+    dead = [t for t in range(S) if t % 3 == 1 or t >= S - 2]
+    mask[:, :, dead] = False
+    want = run(pkg, gpu, made, mask, prefix)
+    worse = []
+    for c, s in caches:
+        c, s = c.clone(), s.clone()
+        for b, n in enumerate(kv.tolist()):
+            for t in dead:
+                if n - S + t >= 0:
+                    slot = n - S + t
+                    at, off = int(table[b, slot // page]), slot % page
+                    c.view(torch.uint8)[at, :, off] = 0x7F
+                    s[at, :, :, off] = 255 if ue8m0 else float("nan") if t % 2 else float("inf")
+        worse.append((c, s))
+    got = run(pkg, gpu, (q, worse, table, kv, pp), mask, prefix)
+    assert bool(torch.isfinite(got).all()) and torch.equal(got, want)
+    check(pkg, gpu, made, mask, prefix)
+
+
 def test_masks_that_leave_nothing(pkg, gpu):
     note("empty masks")
     made = make(6, [4, 12, 0], 4, 8, 2, 64, 16)
