@@ -68,6 +68,69 @@ __device__ __forceinline__ void fill_tail(uint16_t* out, const int64_t (&s)[2], 
 // An lse in units of log 2, as the exponentials take it.
 __device__ __forceinline__ float lse_in_2(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
+// fp16 has neither the range nor the small values for dS, whose size is that of dout, nor for the weights
+// of long sequences: dS goes into its product times a power of two (Scaled), P for dv times 2^kShift,
+// which the dq pass takes off the lse2 that it leaves (P is at most 1 and a rounding of the exponent, so
+// 2^14 keeps a factor of four to infinity, and weights above 2^-28 keep all their bits).
+template <int E>
+constexpr float kShift = E == ET_F16 ? 14.0f : 0.0f;
+
+// What a lane's column of dS is multiplied by before it is packed: as much as leaves its largest element
+// below 2^15.  It falls as that element rises, to put it in 2^8 to 2^9, as a softmax's running maximum does,
+// and the column's sums with it: elements above 2^-22 of the largest keep all their bits.  A power of two,
+// so nothing is rounded.  bf16 has fp32's range, and none of this.  (fp16, us, with / without: 4096 tokens,
+// 32 + 8 heads of 64 327 / 304, of 128 565 / 532, 16 + 4 of 256 684 / 654; 100 tokens, 16 + 4 of 256 51 / 44.)
+struct Scaled {
+  float f = 0x1p60f;
+  __device__ __forceinline__ float inverse() const {
+    return __uint_as_float((2u * 127u << 23) - __float_as_uint(f));
+  }
+  // Multiplies a column's elements, half of which are in each of two lanes.  Whether the sums of some
+  // column are to be multiplied too, and by what in this lane.
+  __device__ __forceinline__ bool operator()(f32x16& x, float* change) {
+    float top = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
+    top *= f;
+    const bool falls = __any(top > 0x1p15f);
+    if (falls) {
+      top = cross_max(top);
+      const uint32_t exponent = __float_as_uint(top) >> 23;         // top is 2^(exponent - 127) and up
+      *change = top > 0x1p15f ? __uint_as_float((2 * 127 + 8 - exponent) << 23) : 1.0f;
+      f *= *change;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] *= f;
+    return falls;
+  }
+};
+// Sums times f.
+template <int N>
+__device__ __forceinline__ void rescale(f32x16 (&sum)[N], float f) {
+#pragma unroll
+  for (int d = 0; d < N; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[d][r] *= f;
+}
+// 16 of them by way of LDS, for sums in the accumulation half of the register file: multiplied in place they
+// cost dk and dv of heads of 256 134 spilled registers (fp16, 4096 tokens, 16 + 4 heads: 1512 us in all).
+using Room = f32x4[4][64];           // of a wave
+__device__ __forceinline__ void rescale_through(Room& room, int lane, f32x16& x, float f) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) room[r][lane] = f32x4{x[4 * r], x[4 * r + 1], x[4 * r + 2], x[4 * r + 3]};
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int r = 0; r < 4; ++r) room[r][lane] *= f;
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const f32x4 v = room[r][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * r + e] = v[e];
+  }
+  asm volatile("" ::: "memory");
+}
+
 template <int D>
 struct DqLds {
   char tile[2][2][Tile<D>::kBytes];
@@ -128,12 +191,13 @@ __device__ __forceinline__ void run_dq(const Args& a, int item, DqLds<D>& shared
   const float lse = a.lse[(int64_t)hq * a.queries.T + row];
   const float lse2 = lse_in_2(lse);
   if (a.lse2 && part == 0 && h == 0 && i < p.n) {
-    a.lse2[(int64_t)hq * a.queries.T + row] = lse2;
+    a.lse2[(int64_t)hq * a.queries.T + row] = lse2 - kShift<E>;
     a.delta[(int64_t)hq * a.queries.T + row] = delta;
   }
   f32x16 dq[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) dq[d] = splat(0.0f);
+  Scaled scaled;
 
   int buf = 0;
   for (int32_t tok = from; tok < stop; tok += kStep, buf ^= 1) {
@@ -161,6 +225,8 @@ __device__ __forceinline__ void run_dq(const Args& a, int item, DqLds<D>& shared
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] *= y[r];
+      if constexpr (E == ET_F16)
+        if (float f; scaled(x, &f)) rescale(dq, f);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const u32x4 w = pack8<E>(x, u), rest = pack_rest8<E>(x, u, w);
@@ -173,6 +239,7 @@ __device__ __forceinline__ void run_dq(const Args& a, int item, DqLds<D>& shared
       }
     }
   }
+  if constexpr (E == ET_F16) rescale(dq, scaled.inverse());
   if (a.dq_parts == 1) {
     store_row<E, D>(a.dq + (int64_t)row * a.dqs[0] + (int64_t)hq * a.dqs[1], h, dq, a.scale, i < p.n);
   } else if (i < p.n) {
@@ -202,6 +269,7 @@ struct DkdvLds {
   char tile[teams(D, SMALL)][2][2][Tile<D, queries(D)>::kBytes];
   char kv[2][kInLds ? Tile<D, kTile>::kBytes : 16];
   float stats[teams(D, SMALL)][2][2][queries(D)];         // lse2, -delta
+  char room[kInLds ? 16 : kWaves * sizeof(Room)];         // of rescale_through
 };
 
 // SMALL: one team, lse2 and delta worked out here, and two terms (of 16 bits each) of P and dS, as dq
@@ -286,7 +354,7 @@ __device__ __forceinline__ void run_dkdv(const Args& a, int item, DkdvLds<D, SMA
 #pragma unroll
     for (int d = 1; d < kThreads; d *= 2) delta += __shfl_xor(delta, d);
     if (own_at == 0) {
-      stats[buf][0][own_row] = lse_in_2(own_lse);
+      stats[buf][0][own_row] = lse_in_2(own_lse) - kShift<E>;
       stats[buf][1][own_row] = delta;
     }
   };
@@ -316,6 +384,7 @@ __device__ __forceinline__ void run_dkdv(const Args& a, int item, DkdvLds<D, SMA
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) dk[d] = dv[d] = splat(0.0f);
+  Scaled scaled;
 
   int buf = 0;
   for (int32_t round = 0; round < rounds; ++round, buf ^= 1, i0 += kQueries) {
@@ -380,6 +449,17 @@ __device__ __forceinline__ void run_dkdv(const Args& a, int item, DkdvLds<D, SMA
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] *= y[r];
+      if constexpr (E == ET_F16) {
+        if (float f; scaled(x, &f)) {
+          if constexpr (kInLds) {
+            rescale(dk, f);
+          } else {
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+              rescale_through(reinterpret_cast<Room*>(shared.room)[wave], lane, dk[d], f);
+          }
+        }
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const u32x4 w = pack8<E>(x, u);
@@ -397,6 +477,15 @@ __device__ __forceinline__ void run_dkdv(const Args& a, int item, DkdvLds<D, SMA
     if (SMALL && it + 1 < to) {
       if constexpr (SMALL && !kInLds) load_stats(head, step);   // no registers to hold them that long
       store_stats(buf ^ 1);
+    }
+  }
+  float fk = 1.0f, fv = 1.0f;                    // what the sums still have to be multiplied by
+  if constexpr (E == ET_F16) {
+    fv = 0x1p-14f, fk = fv * scaled.inverse();
+    if constexpr (kTeams > 1) {
+      rescale(dk, fk);
+      rescale(dv, fv);
+      fk = fv = 1.0f;
     }
   }
   if constexpr (kTeams > 1) {
@@ -429,8 +518,8 @@ __device__ __forceinline__ void run_dkdv(const Args& a, int item, DkdvLds<D, SMA
   }
   const int64_t row = p.row + j0;
   if (a.parts == 1) {
-    store_row<E, D>(a.dk + row * a.dks[0] + (int64_t)kvh * a.dks[1], h, dk, a.scale, j0 < p.n);
-    store_row<E, D>(a.dv + row * a.dvs[0] + (int64_t)kvh * a.dvs[1], h, dv, 1.0f, j0 < p.n);
+    store_row<E, D>(a.dk + row * a.dks[0] + (int64_t)kvh * a.dks[1], h, dk, a.scale * fk, j0 < p.n);
+    store_row<E, D>(a.dv + row * a.dvs[0] + (int64_t)kvh * a.dvs[1], h, dv, fv, j0 < p.n);
   } else if (j0 < p.n) {
     const int64_t plane = (int64_t)a.keys.T * a.H * D;
     float* to_k = a.part + part * plane + (row * a.H + kvh) * D;
@@ -440,9 +529,9 @@ __device__ __forceinline__ void run_dkdv(const Args& a, int item, DkdvLds<D, SMA
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         *reinterpret_cast<f32x4*>(to_k + 32 * d + row_of(r, h)) =
-            f32x4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+            f32x4{dk[d][r] * fk, dk[d][r + 1] * fk, dk[d][r + 2] * fk, dk[d][r + 3] * fk};
         *reinterpret_cast<f32x4*>(to_v + 32 * d + row_of(r, h)) =
-            f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+            f32x4{dv[d][r] * fv, dv[d][r + 1] * fv, dv[d][r + 2] * fv, dv[d][r + 3] * fv};
       }
   }
 }

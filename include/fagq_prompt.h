@@ -19,7 +19,8 @@
  *   dk_j = sm_scale sum dS_ij q_i,  dv_j = sum P_ij dout_i   (over i and the heads of the group)
  *
  * Sums, maxima and exponentials are in fp32; P and dS are rounded to the element
- * type for the products that they enter.
+ * type for the products that they enter, in fp16 times powers of two that keep dS
+ * in its range whatever dout's size: gradients that fp16 holds are right.
  *
  * Same conventions as fagq.h: device pointers, stream-ordered, no allocation, no
  * synchronization; returns 0, a FAGQ_E_* code or -hipError_t.  cu_seqlens and
