@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kThreads) void batch_tables(Args a) {
   __shared__ int32_t row[kRequests + 1], context[kRequests], have[kRequests];
   __shared__ int64_t page[kRequests + 1];       // new pages of the requests before
   const int tid = threadIdx.x, groups = gridDim.x, me = blockIdx.x;
-  const int64_t each = ((a.rows + groups - 1) / groups + kRun - 1) / kRun * kRun;
+  const int64_t each = (((int64_t)a.rows + groups - 1) / groups + kRun - 1) / kRun * kRun;
   const int64_t lo = me * each < a.rows ? me * each : a.rows, hi = lo + each < a.rows ? lo + each : a.rows;
   const int64_t start = a.free_start ? (a.free_start[0] > 0 ? a.free_start[0] : 0) : 0;
   const int64_t unit = 1ll << a.shift;
