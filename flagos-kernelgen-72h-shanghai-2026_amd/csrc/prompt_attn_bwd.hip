@@ -51,6 +51,7 @@ struct Args {
   int64_t dos[2], qs[2], ks[2], vs[2], dqs[2], dks[2], dvs[2];   // {token, head} strides, elements
   int32_t Hq, H, group, fill, parts, dq_parts;
   int32_t dq_items;                  // small calls: workgroups of the first pass
+  int32_t first;                     // of the second pass in this launch
   float scale, scale2;               // sm_scale, and times log2(e)
 };
 
@@ -539,7 +540,7 @@ __device__ __forceinline__ void run_dkdv(const Args& a, int item, DkdvLds<D, SMA
 template <int E, int D>
 __global__ __launch_bounds__(64 * kWaves * teams(D, false), teams(D, false)) void prompt_dkdv(Args a) {
   __shared__ __align__(16) DkdvLds<D, false> lds;
-  run_dkdv<E, D, false>(a, (int)blockIdx.x, lds);
+  run_dkdv<E, D, false>(a, a.first + (int)blockIdx.x, lds);
 }
 
 template <int E, int D>
@@ -590,9 +591,10 @@ constexpr int64_t kCUs = 256;        // a workgroup on each
 // terms (32 + 8 heads of 128, us, in one launch / in two: 1 token 15 / 17, 200 tokens 26 / 36, 4 x 128
 // 30 / 34, 4 x 200 58 / 41; 16 heads of 64, 1000 tokens 39 / 51; 8 heads of 128, 100 tokens behind 3000
 // 32 / 41, 1024 behind 1024 88 / 79; 24 + 8 of 256, 5 and 70 behind 4000 200 / 177).  The more a head
-// has, the fewer of the one launch's waves run at once.
+// has, the fewer of the one launch's waves run at once.  Not with more tiles than a grid may hold of both
+// passes, which few rows have in many empty sequences only.
 bool small(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t D) {
-  return T * Hq <= 16384 && (double)(T * Hq * D * D) * (double)Tk <= 0x1p36 * (double)std::max<int64_t>(1, B);
+  return T * Hq <= 16384 && B * Hq <= kMostGroups / 64 && (double)(T * Hq * D * D) * (double)Tk <= 0x1p36 * (double)std::max<int64_t>(1, B);
 }
 
 // Parts of a key tile's steps: as many as let the tile with most of them, twice the average, not take
@@ -621,11 +623,11 @@ int64_t dq_parts_for(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, in
 int check_bwd_sizes(int64_t B, int64_t T, int64_t Tk, int64_t Hq, int64_t H, int64_t D) {
   const int st = check_sizes(B, T, Tk, Hq, H, D);
   if (st != FAGQ_OK) return st;
-  // With all the parts there may be of the keys', and the joining kernel's workgroups.
+  // There are parts, and a joining kernel, where workgroups are few only.
   const int64_t dq_items = tile_slots(T, B) * Hq * dq_parts_for(B, T, Tk, Hq, H, D);
-  const bool large = dq_items >= kMostGroups ||
-                     tile_slots(Tk, B) * H * kMostParts + (small(B, T, Tk, Hq, D) ? dq_items : 0) >= kMostGroups ||
-                     Tk * H * D / 1024 >= kMostGroups / 2;
+  const int64_t dkdv_items = tile_slots(Tk, B) * H * parts_for(B, T, Tk, Hq, H, D);
+  const bool large =
+      dq_items >= kMostGroups || dkdv_items + (small(B, T, Tk, Hq, D) ? dq_items : 0) >= kMostGroups;
   return large ? FAGQ_E_TOO_LARGE : FAGQ_OK;
 }
 
@@ -752,11 +754,17 @@ FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, c
                                  dim3((unsigned)(a.dq_items + dkdv_items)), dim3(64 * kWaves), args, 0, st);
     if (ls != FAGQ_OK) return ls;
   } else {
-    int ls = launch_kernel(bf16 ? dq_for<ET_BF16>(D) : dq_for<ET_F16>(D), dim3((unsigned)dq_items),
-                           dim3(64 * kWaves), args, 0, st);
-    if (ls == FAGQ_OK && dkdv_items > 0)
-      ls = launch_kernel(bf16 ? dkdv_for<ET_BF16>(D) : dkdv_for<ET_F16>(D), dim3((unsigned)dkdv_items),
+    int ls = FAGQ_OK;
+    if (dq_items > 0)
+      ls = launch_kernel(bf16 ? dq_for<ET_BF16>(D) : dq_for<ET_F16>(D), dim3((unsigned)dq_items),
+                         dim3(64 * kWaves), args, 0, st);
+    // With two teams a grid of kMostGroups would be too large.
+    for (int64_t first = 0; first < dkdv_items && ls == FAGQ_OK; first += kMostGroups / 4) {
+      a.first = (int32_t)first;
+      ls = launch_kernel(bf16 ? dkdv_for<ET_BF16>(D) : dkdv_for<ET_F16>(D),
+                         dim3((unsigned)std::min(dkdv_items - first, kMostGroups / 4)),
                          dim3((unsigned)(64 * kWaves * teams(D, false))), args, 0, st);
+    }
     if (ls != FAGQ_OK) return ls;
   }
   const int64_t items = (parts > 1 ? 2 * Tk * H * (D / 8) : 0) + (dq_parts > 1 ? T * Hq * (D / 8) : 0);

@@ -65,7 +65,9 @@ FAGQ_API int fagq_prompt_attention_launch(const void* q, const void* k, const vo
 /* out, lse: of the call above.  dout [T, Hq, D], dq, dk, dv: dtype.  strides:
  * {token, head} of dout, q, k, v, dq, dk, dv, as above; out and lse are contiguous.
  * Gradients are written, not added to.  The sums are added in an order that depends
- * on the sizes alone: equal calls give equal bits. */
+ * on the sizes alone: equal calls give equal bits.  FAGQ_E_TOO_LARGE where the forward
+ * has it, and for 2^24 tiles of keys and more, (Tk / 128 + B) H, which Tk above T only
+ * can have. */
 FAGQ_API int64_t fagq_prompt_attention_bwd_workspace_bytes(int64_t B, int64_t T, int64_t Tk,
                                                            int64_t Hq, int64_t H, int64_t D);
 FAGQ_API int fagq_prompt_attention_bwd_launch(const void* dout, const void* q, const void* k,
