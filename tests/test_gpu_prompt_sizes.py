@@ -55,3 +55,20 @@ def test_hundreds_of_thousands_of_empty_sequences(pkg, gpu, T, Tk):
     assert attention_ref.outside(out, o, off, BF16) == 0
     for x, (r, off) in zip(grads, ref.backward(do, q, k, v, out.cpu(), lse.cpu(), two(T), 0.125, two(Tk))):
         assert attention_ref.outside(x, r, off, BF16) == 0
+
+
+@pytest.mark.parametrize("B,H", [(1000, 2), (5000, 1)])
+def test_gradients_of_many_sequences(pkg, gpu, B, H):
+    """One workgroup for each sequence and more, empty ones and some of several tiles among them."""
+    note(f"gradients of {B} sequences")
+    lens = [[1, 0, 5, 17, 2, 40, 0][(b * 3 + b // 11) % 7] + (300 if b % 997 == 5 else 0) for b in range(B)]
+    T, D = sum(lens), 64
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    g = torch.Generator().manual_seed(3)
+    q, do = (torch.randn(T, 2 * H, D, generator=g).to(BF16) for _ in range(2))
+    k, v = (torch.randn(T, H, D, generator=g).to(BF16) for _ in range(2))
+    up = [t.to(gpu) for t in (q, k, v, cu)]
+    out, lse = pkg.prompt_attention(*up, 0.125, return_lse=True)
+    grads = pkg.prompt_attention_bwd(do.to(gpu), *up[:3], out, lse, up[3], 0.125)
+    for x, (r, off) in zip(grads, ref.backward(do, q, k, v, out.cpu(), lse.cpu(), cu, 0.125)):
+        assert attention_ref.outside(x, r, off, BF16) == 0
