@@ -9,13 +9,13 @@
 // Where there are few workgroups, each one's keys are cut into parts with m, l and o of their own,
 // which prompt_attention_join puts together: o = sum 2^(m_i - m) o_i.
 //
-// Bound by power where calls are long: 16384 tokens, 64 + 8 heads of 128, 3.95 ms, 1.11 PFLOP/s, the
-// matrix units busy 63 % of the cycles at 1.7 GHz.  Tiles of 128 queries: a CU then reads 32 KB of keys
+// Bound by power where calls are long: 16384 tokens, 64 + 8 heads of 128, 3.87 ms, 1.14 PFLOP/s, the
+// matrix units busy 59 % of the cycles at 1.75 GHz.  Tiles of 128 queries: a CU then reads 32 KB of keys
 // and values in the time of 4.2 MFLOP from its L2.  Two workgroups a CU, so that one's softmax runs under
 // the other's products; three, with steps of 32 keys, take as long.  P is rounded to the element type
 // for its product: the output is 1.1 to 1.4 times as far off as its own rounding makes it.
 // Heads of 256 have their keys in tiles of 32: of 64, one workgroup fills a CU's LDS (4 chunks of 512
-// tokens over 4096, 16 + 4 heads, 170 us).
+// tokens over 4096, 16 + 4 heads, 175 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -12,8 +12,8 @@
 //                 their sums through LDS; where there are few workgroups, the steps are cut into
 //                 parts besides.
 //   prompt_join   adds the parts up, in order.
-// 8192 tokens, 32 + 8 heads of 128, in 1.87 ms: dq 880 us, bound by power (the matrix units busy 74 % of
-// the cycles at 1.65 GHz), dk and dv 1010 (58 %): what is between their products are LDS reads, the
+// 8192 tokens, 32 + 8 heads of 128, in 1.87 ms: dq 860 us, bound by power (the matrix units busy 73 % of
+// the cycles at 1.8 GHz), dk and dv 1000 (59 %): what is between their products are LDS reads, the
 // exponentials and the steps' barriers.  dS enters dq's product in two terms of 16 bits, without which dq
 // would be 1.7 times as far off as its own rounding makes it.
 // Calls of few rows, where a launch is what counts, take both passes in one (prompt_bwd_small): the
