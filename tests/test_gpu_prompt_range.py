@@ -124,3 +124,43 @@ def test_gradients_of_nothing(pkg, gpu):
     for x, r in zip(got, want):
         assert bool(torch.isfinite(x).all()) and bool((x[171:] == 0).all())
         assert excess(x, r) <= TWICE
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,Hq,H,D", [(200, 4, 2, 64), (1300, 16, 4, 64), (150, 2, 1, 256), (1200, 16, 16, 128)])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_an_overflow_is_not_hidden(pkg, gpu, n, Hq, H, D, dtype, bad):
+    """A dout that a scaled loss has driven to infinity shows in every gradient that it enters, and in no
+    other sequence's."""
+    note(f"dout of {bad} {n} {Hq} {H} {D} {dtype}")
+    g = torch.Generator().manual_seed(10)
+    q, do = (torch.randn(n, Hq, D, generator=g).to(dtype).to(gpu) for _ in range(2))
+    k, v = (torch.randn(n, H, D, generator=g).to(dtype).to(gpu) for _ in range(2))
+    cu = torch.tensor([0, n - 70, n], dtype=torch.int32, device=gpu)
+    out, lse = pkg.prompt_attention(q, k, v, cu, D ** -0.5, return_lse=True)
+    clean = pkg.prompt_attention_bwd(do, q, k, v, out, lse, cu, D ** -0.5)
+    i, h = n - 100, Hq - 1
+    do[i, h, 3] = bad
+    dq, dk, dv = pkg.prompt_attention_bwd(do, q, k, v, out, lse, cu, D ** -0.5)
+    lost = lambda t: ~torch.isfinite(t)
+    assert bool(lost(dq[i, h]).any()) and bool(lost(dk[:i + 1, H - 1]).any(-1).all())
+    assert bool(lost(dv[:i + 1, H - 1, 3]).all())
+    for x, y in zip((dq, dk, dv), clean):
+        assert torch.equal(x[n - 70:], y[n - 70:])
+    assert torch.equal(dq[:, :h], clean[0][:, :h]) and torch.equal(dq[:i, h], clean[0][:i, h])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1.0])
+def test_fp16_scales_of_either_sign(pkg, gpu, scale):
+    note(f"fp16 gradients, scale {scale}")
+    g = torch.Generator().manual_seed(11)
+    q, do = (torch.randn(130, 4, 64, generator=g).to(F16).to(gpu) for _ in range(2))
+    k, v = (torch.randn(130, 2, 64, generator=g).to(F16).to(gpu) for _ in range(2))
+    cu = torch.tensor([0, 130], dtype=torch.int32, device=gpu)
+    out, lse = pkg.prompt_attention(q, k, v, cu, scale, return_lse=True)
+    got = pkg.prompt_attention_bwd(do, q, k, v, out, lse, cu, scale)
+    want = gradients(do, q, k, v, out, lse, scale)
+    if scale == 0.0:
+        assert bool((got[0] == 0).all()) and bool((got[1] == 0).all())
+        got, want = got[2:], want[2:]
+    assert all(excess(x, r) <= TWICE for x, r in zip(got, want))

@@ -25,13 +25,11 @@ def test_the_backward_takes_what_the_forward_takes(lib, B, T, Hq, H, D):
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("B", [1, 7, 1000, 1 << 20])
-@pytest.mark.parametrize("Hq,H", [(1, 1), (8, 8), (64, 64), (64, 8), (4096, 4096)])
+@pytest.mark.parametrize("B,Hq,H", [(B, Hq, H) for B in (1, 7, 1000, 1 << 20)
+                                    for Hq, H in ((1, 1), (8, 8), (64, 64), (64, 8), (4096, 4096)) if B * Hq < LIMIT])
 def test_up_to_the_limit(lib, B, Hq, H, D):
     """The last number of tokens below 2^24 workgroups, and the first above."""
     T = LIMIT // Hq * 128 - B * 127 - 127
-    if T < 0:
-        pytest.skip("so many sequences alone are past the limit")
     for rows in (T - 129, T - 128, T - 1, T, T + 128):
         if not 0 <= rows < (1 << 31) - 1024:
             continue
